@@ -35,6 +35,7 @@ extern "C" {
 
 #define XGB_BF16 0
 #define XGB_F16 1
+#define XGB_F32 2 /* only where an entry point says so */
 
 /* Library ABI version (major*100 + minor). */
 int xgb_version(void);
@@ -263,6 +264,91 @@ int xgb_norm_modulate_quant(const void* x, int64_t ldx, int64_t rows, int64_t wi
                             int norm_kind, const void* weight, float eps, const void* scale,
                             int64_t lds, const void* shift, int64_t ldsh, const int64_t* indices,
                             uint8_t* out, float* out_scale, void* out_bf16, void* stream);
+
+/* ---- Operators of a conditioned DiT block (no counterpart in the reference) ---- */
+
+/* Rotary positions with several axes, and the per-head RMSNorm before them:
+ *   x <- x * rsqrt(mean(x^2) + eps) * weight   (q_weight / k_weight; NULL: no norm)
+ *   (a, b) <- (a cos t - b sin t, b cos t + a sin t),
+ *   t = position[axis] * theta[axis]^(-2 i / d)   for pair i of an axis of d channels
+ * Q/K [batch, seq, heads, width] views of `dtype` (XGB_BF16, XGB_F16, XGB_F32;
+ * element strides of batch, seq, head; channel stride 1; k may be NULL);
+ * outputs contiguous, rounded once. The axes' pairs follow one another;
+ * R = the sum of axis_channels (each even) <= width <= 512, at most 8 axes;
+ * channels from R on are not rotated. Pair i is (i, i + R/2), or with
+ * `interleaved` (2i, 2i + 1). positions [batch, seq, axes] (element strides
+ * position_batch_stride, 0 when shared, and position_stride; axis stride 1),
+ * position_type 0 int32, 1 int64, 2 float, 3 double; angles are formed in 64
+ * bits. axis_channels and thetas are host arrays of `axes` entries. */
+int xgb_rope_axes(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                  int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t width,
+                  const void* positions, int position_type, int64_t position_batch_stride,
+                  int64_t position_stride, int64_t axes, const int64_t* axis_channels, const double* thetas,
+                  int interleaved, const void* q_weight, const void* k_weight, float q_eps, float k_eps,
+                  void* q_out, void* k_out, void* stream);
+
+/* The norm after a block, its gate and residual, and the norm before the next:
+ *   x_out = x + residual_scale * gate[idx] * post(y)
+ *   h     = pre(x_out) * (1 + scale[idx]) + shift[idx]     (x_out before its rounding)
+ * y/x [batch, seq, width] of `dtype` (XGB_BF16, XGB_F16, XGB_F32; element
+ * strides of batch and seq, channel stride 1), width <= 16384; post_norm and
+ * pre_norm 0 none, 1 LayerNorm, 2 RMSNorm, times an optional weight [width];
+ * gate, scale and shift (any may be NULL, scale and shift together) rows of
+ * AdaLN tables of table_rows rows; idx = indices[batch * index_batch_stride +
+ * seq], where an index outside the table makes its row NaN. x_out contiguous;
+ * h to h_out (may be NULL), or as codes with one scale a row: quant 1 int8
+ * (scale max(amax/127, FLT_MIN)), 2 e4m3 (amax/448). */
+int xgb_sandwich_norm(const void* y, const int64_t* y_strides, const void* x, const int64_t* x_strides, int dtype,
+                      int64_t batch, int64_t seq, int64_t width, int post_norm, const void* post_weight,
+                      int pre_norm, const void* pre_weight, float eps, const void* gate, int64_t ldg,
+                      float residual_scale, const void* scale, int64_t lds, const void* shift, int64_t ldsh,
+                      const int64_t* indices, int64_t index_batch_stride, int64_t table_rows, void* x_out,
+                      void* h_out, int quant, uint8_t* codes, float* code_scale, void* stream);
+
+/* Per-row dynamic int8 of x [rows, cols] (bf16/fp16, rows row_stride apart):
+ * scales[r] = max(amax(|x[r,:]|)/127, FLT_MIN), out = the nearest integers to
+ * x / scale, ties to even, within +-127; out contiguous. */
+int xgb_int8_quantize_per_token(const void* x, int dtype, int64_t rows, int64_t cols, int64_t row_stride,
+                                int8_t* out, float* scales, void* stream);
+
+/* Linear layer in 8-bit integers (tcgen05 kind::i8, exact 32-bit sums):
+ *   y[m, n] = (sum_k a[m, k] w[n, k]) * (scale_a[m] * scale_w[n]) + bias[n]
+ *   out     = y (activation 0), gelu(y) (1 erf, 2 tanh),
+ *             silu(y[:, :N/2]) * y[:, N/2:] (3, N/2 columns), or
+ *             residual + gate[idx] * y (gate != NULL, activation 0)
+ * a [M, K], w [N, K] int8 contiguous, 16-byte aligned, K and N multiples of
+ * 16, K <= 131056; `dtype` (XGB_BF16 or XGB_F16) is that of bias [N], gate
+ * rows, residual and out (rows ldo apart, a multiple of 8, 16-byte aligned).
+ * idx = gate_index[m % index_rows] (M a multiple of index_rows); an index
+ * outside the table_rows rows makes its row NaN. 32-bit epilogue, one
+ * rounding. error_flag as for the attention kernels. */
+int xgb_int8_gemm(const int8_t* a, const int8_t* w, int64_t M, int64_t N, int64_t K, const float* scale_a,
+                  const float* scale_w, int dtype, const void* bias, int activation, void* out, int64_t ldo,
+                  const void* gate, int64_t ldg, const int64_t* gate_index, int64_t index_rows, int64_t table_rows,
+                  const void* residual, int64_t ldr, int* error_flag, void* stream);
+
+/* Attention of q [batch, heads, seq_q, head_dim] to k/v [batch, kv_heads,
+ * seq_kv, head_dim] views (bf16 or fp16, head_dim 64 or 128, strides in
+ * elements, multiples of 8; 0 where the batch or the heads are broadcast),
+ * heads a multiple of kv_heads. kv_lens (device, [batch], may be NULL): keys
+ * that each sample has, clamped to [0, seq_kv]; what lies behind them has no
+ * influence, NaN included, and a sample without keys gives zeros. workspace:
+ * xgb_cross_attention_workspace() bytes (0 for most sizes), 16-byte aligned,
+ * its contents need no initialisation. */
+int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim);
+int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides, int dtype, int64_t batch, int64_t heads,
+                        int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int* kv_lens,
+                        float sm_scale, void* out, const int64_t* out_strides, void* workspace,
+                        int64_t workspace_bytes, int* error_flag, void* stream);
+
+/* The keys and values that `mask` (bytes [batch, seq], 0 = left out) keeps, in
+ * order, at the front of contiguous k_out/v_out [batch, heads, seq, head_dim],
+ * and their number per sample: what xgb_cross_attention takes as kv_lens.
+ * 16-bit elements, head_dim 64 or 128, strides multiples of 8. */
+int xgb_pack_keys(const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, const void* k,
+                  const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t batch, int64_t heads,
+                  int64_t seq, int64_t head_dim, void* k_out, void* v_out, int* counts, void* stream);
 
 /* ---- Attention (tcgen05 / TMEM / TMA kernels) ---- */
 

@@ -1,0 +1,281 @@
+"""cross_attention against softmax attention in 64 bits over the keys that are
+there.
+
+Tolerance, with P rounded to the inputs' type (half a step e = eps/2 relative):
+  the output's rounding                        e |o|
+  P's rounding                                 e A,  A = sum p |v| / sum p
+  a score's 32-bit error, which p carries as its own relative error: a sum of
+  D products, each step within 2^-23 (the tensor core may truncate) of the sum
+  of magnitudes, in numerator and denominator  2 scale D 2^-23 max sum |q k| / 8
+  the two products' accumulation and exp2      2^-16 A
+and for fp16 the p below its smallest number: 2^-25 for each key (sum p >= 1).
+D/8: the tensor core adds at least 16 products in one step, D/16 steps, doubled."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def reference(q, k, v, valid, scale):
+    """(o, A, largest sum |q k|) in 64 bits; valid bool [B, Skv]."""
+    b, h, sq, d = q.shape
+    group = h // k.shape[1]
+    q, k, v = (t.double().cpu() for t in (q, k, v))
+    o, a, top = torch.zeros(b, h, sq, d).double(), torch.zeros(b, h, sq, d).double(), 0.0
+    for n in range(b):
+        at = valid[n].nonzero()[:, 0]
+        if not len(at):
+            continue
+        for j in range(h):
+            kk, vv = k[n, j // group, at], v[n, j // group, at]
+            p = torch.softmax(q[n, j] @ kk.t() * scale, -1)
+            o[n, j], a[n, j] = p @ vv, p @ vv.abs()
+            top = max(top, (q[n, j].abs() @ kk.abs().t()).max().item())
+    return o, a, top
+
+
+def check(got, q, k, v, valid, scale=None):
+    scale = scale or 1 / math.sqrt(q.shape[-1])
+    o, a, top = reference(q, k, v, valid, scale)
+    info = torch.finfo(q.dtype)
+    e = info.eps / 2
+    slack = (e + 2 * scale * (q.shape[-1] / 8) * 2.0 ** -23 * top + 2.0 ** -16) * a
+    if q.dtype == torch.float16:
+        slack = slack + 2.0 ** -25 * k.shape[2] * torch.nan_to_num(v.double().cpu()).abs().max() * (a > 0)
+    bound = e * (o.abs() + slack) + slack + info.smallest_normal * e
+    assert got.shape == q.shape and got.dtype == q.dtype
+    worst = ((got.double().cpu() - o).abs() / bound).max().item()
+    assert worst <= 1.0, worst
+
+
+def inputs(b, h, hk, sq, skv, d, dtype, dev, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(b, sq, h, d, generator=g).to(dev, dtype).transpose(1, 2)
+    kv = torch.randn(b, skv, 2, hk, d, generator=g)
+    kv[:, :, 0] += torch.randn(hk, d, generator=g)
+    kv = kv.to(dev, dtype)
+    return q, kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+
+
+@pytest.fixture(autouse=True)
+def no_timeouts(cuda_device):
+    yield
+    from xgen_b200.attention import kernel_errors
+
+    assert kernel_errors(cuda_device) == 0
+
+
+@pytest.mark.parametrize("b,h,hk,sq,skv", [
+    (1, 1, 1, 1, 1), (1, 2, 2, 128, 64), (1, 2, 1, 129, 65), (2, 3, 3, 300, 77), (1, 4, 2, 257, 512), (2, 2, 2, 1000, 333),
+    (1, 1, 1, 5, 1000), (3, 2, 1, 64, 63), (1, 24, 24, 700, 226), (1, 6, 2, 1, 4099), (1, 1, 1, 3000, 2), (5, 8, 8, 17, 129)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_matches_softmax(cuda_device, b, h, hk, sq, skv, d, dtype):
+    from xgen_b200.attention import cross_attention
+
+    q, k, v = inputs(b, h, hk, sq, skv, d, dtype, cuda_device, seed=sq + skv)
+    got = cross_attention(q, k, v)
+    check(got, q, k, v, torch.ones(b, skv, dtype=torch.bool))
+
+
+@pytest.mark.parametrize("sq", [1, 40, 300])
+@pytest.mark.parametrize("skv", [1, 64, 200, 1025])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_lengths(cuda_device, sq, skv, d, kind):
+    """Every sample its own count: none, one, ends inside, at and over a tile's
+    and the states' end; NaN and infinities behind it."""
+    from xgen_b200.attention import cross_attention
+
+    lens = [0, 1, min(63, skv), min(64, skv), min(65, skv), skv - 1, skv, skv + 100, -3]
+    q, k, v = inputs(len(lens), 4, 2, sq, skv, d, torch.bfloat16, cuda_device, seed=skv)
+    n = torch.tensor(lens, device=cuda_device, dtype=kind)
+    valid = torch.arange(skv, device=cuda_device)[None] < n[:, None]
+    for fill in (float("nan"), float("inf"), -3e38):
+        k = k.masked_fill(~valid[:, None, :, None], fill)
+        v = v.masked_fill(~valid[:, None, :, None], fill)
+        got = cross_attention(q, k, v, kv_lens=n)
+        check(got, q, k, v, valid.cpu())
+    assert not got[0].any() and not got[-1].any()
+
+
+@pytest.mark.parametrize("sq", [1, 300])
+@pytest.mark.parametrize("skv", [1, 65, 333, 1500])
+@pytest.mark.parametrize("d", [64, 128])
+def test_masks(cuda_device, sq, skv, d):
+    from xgen_b200.attention import cross_attention
+
+    g = torch.Generator().manual_seed(skv)
+    valid = torch.rand(5, skv, generator=g) < 0.6
+    valid[0] = False
+    valid[1] = True
+    valid[2] = False
+    valid[2, -1] = True  # the last key alone
+    q, k, v = inputs(5, 4, 2, sq, skv, d, torch.float16, cuda_device, seed=skv)
+    mask = valid.to(cuda_device)
+    k, v = (t.masked_fill(~mask[:, None, :, None], float("nan")) for t in (k, v))
+    got = cross_attention(q, k, v, key_mask=mask)
+    check(got, q, k, v, valid)
+    assert not got[0].any()
+    assert torch.equal(got, cross_attention(q, k, v, key_mask=mask[:, None, None]))
+    one = mask[3:4]
+    kk, vv = (t[3:4].expand(5, -1, -1, -1) for t in (k, v))
+    got = cross_attention(q, kk, vv, key_mask=one)
+    check(got, q, kk, vv, valid[3:4].expand(5, -1))
+
+
+def test_large_scores_and_infinities(cuda_device):
+    """Scores far apart (the running maximum rises many times), rows of -inf
+    scores, and a value of infinity where it is attended to."""
+    from xgen_b200.attention import cross_attention
+
+    q, k, v = inputs(1, 2, 2, 200, 700, 128, torch.bfloat16, cuda_device, seed=9)
+    ramp = torch.linspace(0.02, 6, 700, device=cuda_device).to(torch.bfloat16)[:, None]
+    got = cross_attention(q, k * ramp, v)
+    check(got, q, k * ramp, v, torch.ones(1, 700, dtype=torch.bool))
+    got = cross_attention(q, k, v, sm_scale=1e-4)
+    check(got, q, k, v, torch.ones(1, 700, dtype=torch.bool), 1e-4)
+    q2 = torch.full_like(q, 1.0)
+    k2 = k.clone()
+    k2[:, :, 100:] = float("-inf")  # scores of -inf: as if the keys were not there
+    got = cross_attention(q2, k2, v)
+    check(got, q2, k[:, :, :100], v[:, :, :100], torch.ones(1, 100, dtype=torch.bool))
+    assert not cross_attention(q2, torch.full_like(k, float("-inf")), v).any()
+    v2 = v.clone()
+    v2[0, 0, 3, 7] = float("inf")
+    got = cross_attention(q, k, v2)
+    assert torch.isinf(got[0, 0, :, 7]).all() and torch.isfinite(got[0, 1]).all()
+    q3 = q.clone()
+    q3[0, 1, 5] = float("nan")
+    got, clean = cross_attention(q3, k, v), cross_attention(q, k, v)
+    bad = torch.zeros(1, 2, 200, dtype=torch.bool, device=cuda_device)
+    bad[0, 1, 5] = True
+    assert torch.isnan(got[bad]).all() and torch.equal(got[~bad], clean[~bad])
+
+
+def test_strides_broadcast_and_output(cuda_device):
+    from xgen_b200.attention import cross_attention
+
+    b, h, sq, skv, d = 3, 4, 150, 130, 64
+    q, k, v = inputs(b, h, h, sq, skv, d, torch.bfloat16, cuda_device, seed=1)
+    every = torch.ones(b, skv, dtype=torch.bool)
+    hnd = [t.contiguous() for t in (q, k, v)]
+    base = cross_attention(*hnd)
+    check(base, q, k, v, every)
+    assert torch.equal(base, cross_attention(q, k, v))
+    # rows of a wider projection; every second token
+    wide = torch.randn(b, sq, h, 2 * d, device=cuda_device).bfloat16()[..., d:].transpose(1, 2)
+    check(cross_attention(wide, k, v), wide, k, v, every)
+    half = cross_attention(q, k[:, :, ::2], v[:, :, 1::2])
+    check(half, q, k[:, :, ::2], v[:, :, 1::2], every[:, :65])
+    # states shared by the batch, and by the heads
+    kb, vb = k[:1].expand(b, -1, -1, -1), v[:, :1].expand(-1, h, -1, -1)
+    check(cross_attention(q, kb, vb), q, kb, vb, every)
+    # into the layout of the next projection; what lies beside the view stays
+    frame = torch.full((b, sq + 2, h, d), 5.0, device=cuda_device).bfloat16()
+    out = frame[:, 1:-1].transpose(1, 2)
+    assert cross_attention(q, k, v, out=out) is out
+    assert torch.equal(out, base) and (frame[:, 0] == 5).all() and (frame[:, -1] == 5).all()
+
+
+def test_empty(cuda_device):
+    from xgen_b200.attention import cross_attention
+
+    q, k, v = inputs(2, 2, 2, 10, 20, 64, torch.bfloat16, cuda_device)
+    assert cross_attention(q[:, :, :0], k, v).shape == (2, 2, 0, 64)
+    assert not cross_attention(q, k[:, :, :0], v[:, :, :0]).any()
+    assert cross_attention(q[:0], k[:0], v[:0]).shape == (0, 2, 10, 64)
+
+
+@pytest.mark.parametrize("sq,skv", [(1, 2000), (700, 200)])
+def test_two_streams_and_graphs(cuda_device, sq, skv):
+    """Calls on two streams at once, and two captured graphs replayed in turn
+    and at once, give what single calls give: nothing is shared."""
+    from xgen_b200.attention import cross_attention
+
+    sets = [inputs(2, 4, 2, sq, skv, 128, torch.bfloat16, cuda_device, seed=n) for n in range(2)]
+    lens = [torch.tensor([skv, skv // 3], device=cuda_device, dtype=torch.int32),
+            torch.tensor([7, skv], device=cuda_device, dtype=torch.int32)]
+    single = [cross_attention(*s, kv_lens=n) for s, n in zip(sets, lens)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        outs = []
+        for st, s, n in zip(streams, sets, lens):
+            with torch.cuda.stream(st):
+                outs.append(cross_attention(*s, kv_lens=n))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, single))
+    graphs, results = [], []
+    for s, n in zip(sets, lens):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results.append(cross_attention(*s, kv_lens=n))
+        graphs.append(graph)
+    for _ in range(3):
+        for r in results:
+            r.zero_()
+        torch.cuda.synchronize()
+        for st, graph in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(results, single))
+    lens[0].copy_(torch.tensor([3, 0]))  # a replay reads the lengths of its time
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(results[0], cross_attention(*sets[0], kv_lens=lens[0]))
+
+
+def test_same_call_gives_the_same_bits(cuda_device):
+    from xgen_b200.attention import cross_attention
+
+    for sq, skv in ((1, 4099), (3000, 300)):
+        q, k, v = inputs(1, 4, 4, sq, skv, 128, torch.bfloat16, cuda_device)
+        first = cross_attention(q, k, v)
+        assert all(torch.equal(first, cross_attention(q, k, v)) for _ in range(5))
+
+
+def test_long_caches(cuda_device):
+    """Element offsets beyond 32 bits: 2^31 elements of K before the last head."""
+    from xgen_b200.attention import cross_attention
+
+    skv, h, d = 70000, 160, 128
+    assert h * skv * d > 2 ** 30 and 2 * h * skv * d > 2 ** 31
+    kv = torch.zeros(2, h, skv, d, device=cuda_device, dtype=torch.bfloat16)  # rows of one tensor: K, V
+    g = torch.Generator().manual_seed(0)
+    last = torch.randn(2, 1, 200, d, generator=g).to(cuda_device, torch.bfloat16)
+    wide = kv.view(1, 2 * h, skv, d)
+    wide[0, 2 * h - 1, -200:], wide[0, 2 * h - 2, -200:] = last[1, 0], last[0, 0]
+    q = torch.randn(1, 1, 30, d, generator=g).to(cuda_device, torch.bfloat16)
+    k, v = wide[:, 2 * h - 2:2 * h - 1, -200:], wide[:, 2 * h - 1:, -200:]
+    check(cross_attention(q, k, v), q, k, v, torch.ones(1, 200, dtype=torch.bool))
+    q2 = q.expand(1, 2 * h, 30, d)
+    got = cross_attention(q2, wide[:, :, -200:], wide[:, :, -200:])
+    check(got[:, -1:], q, wide[:, -1:, -200:], wide[:, -1:, -200:], torch.ones(1, 200, dtype=torch.bool))
+
+
+def test_refusals(cuda_device):
+    from xgen_b200.attention import cross_attention
+
+    q, k, v = inputs(2, 4, 2, 10, 20, 64, torch.bfloat16, cuda_device)
+    lens = torch.ones(2, dtype=torch.int32, device=cuda_device)
+    mask = torch.ones(2, 20, dtype=torch.bool, device=cuda_device)
+    for bad in (dict(kv_lens=lens, key_mask=mask), dict(kv_lens=lens[:1]), dict(kv_lens=lens.float()), dict(key_mask=mask.int()),
+                dict(key_mask=mask[:, :10]), dict(sm_scale=0.0), dict(sm_scale=float("nan")), dict(out=q[:, :, :5]),
+                dict(out=torch.empty_like(q).float()), dict(key_mask=mask[:, None].expand(2, 4, 20)[:, :, None])):
+        with pytest.raises(ValueError):
+            cross_attention(q, k, v, **bad)
+    for bad in ((q.float(), k.float(), v.float()), (q, k.half(), v), (q[..., :32], k[..., :32], v[..., :32]), (q, k, v[:, :, :10]),
+                (q[:, :3], k, v), (q[:1], k, v), (q, k[:, :, :, ::1].transpose(2, 3), v), (q.cpu(), k, v)):
+        with pytest.raises(ValueError):
+            cross_attention(*bad)
+    odd = torch.zeros(2, 10, 4, 68, device=cuda_device, dtype=torch.bfloat16)[..., :64].transpose(1, 2)  # rows of 136 bytes
+    with pytest.raises(ValueError):
+        cross_attention(odd, k, v)
+    with pytest.raises(ValueError):
+        cross_attention(q, k[:, :, :1].expand(-1, -1, 20, -1), v)  # one key for all places
+    with pytest.raises(ValueError, match="autograd"):
+        cross_attention(q.clone().requires_grad_(), k, v)

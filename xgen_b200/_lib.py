@@ -22,10 +22,12 @@ XGB_ERR_WORKSPACE = -7
 
 XGB_BF16 = 0
 XGB_F16 = 1
+XGB_F32 = 2
 
 c_i64 = ctypes.c_int64
 c_int = ctypes.c_int
 c_float = ctypes.c_float
+c_f64p = ctypes.POINTER(ctypes.c_double)
 c_vp = ctypes.c_void_p
 c_i64p = ctypes.POINTER(ctypes.c_int64)
 
@@ -84,6 +86,21 @@ SIGNATURES = {
                                            c_vp, c_i64p, c_vp, c_i64, c_vp, c_vp]),
     "xgb_attention_sage": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp,
                                    c_i64p, c_vp, c_i64, c_vp, c_vp]),
+    "xgb_rope_axes": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_int, c_i64, c_i64, c_i64, c_i64, c_i64, c_vp,
+                              c_int, c_i64, c_i64, c_i64, c_i64p, c_f64p, c_int, c_vp, c_vp, c_float,
+                              c_float, c_vp, c_vp, c_vp]),
+    "xgb_sandwich_norm": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_int, c_i64, c_i64, c_i64, c_int, c_vp,
+                                  c_int, c_vp, c_float, c_vp, c_i64, c_float, c_vp, c_i64, c_vp, c_i64,
+                                  c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_vp, c_vp]),
+    "xgb_int8_quantize_per_token": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
+    "xgb_int8_gemm": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_int, c_vp, c_i64,
+                              c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
+    "xgb_cross_attention_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "xgb_cross_attention": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_int, c_i64, c_i64, c_i64,
+                                    c_i64, c_i64, c_i64, c_vp, c_float, c_vp, c_i64p, c_vp, c_i64, c_vp,
+                                    c_vp]),
+    "xgb_pack_keys": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64p, c_vp, c_i64p, c_i64, c_i64, c_i64, c_i64,
+                              c_vp, c_vp, c_vp, c_vp]),
     "xgb_attention_bf16": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_i64, c_i64, c_i64,
                                    c_i64, c_float, c_vp, c_i64p, c_vp, c_i64, c_vp, c_vp]),
 }
@@ -135,6 +152,11 @@ def check(fn: str, status: int) -> None:
 
 def call(name: str, *args) -> None:
     check(name, getattr(lib(), name)(*args))
+
+
+def f64_array(values) -> ctypes.Array:
+    values = list(values)
+    return (ctypes.c_double * len(values))(*values)
 
 
 def i64_array(values) -> ctypes.Array:

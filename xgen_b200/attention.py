@@ -34,6 +34,15 @@ def _err_flag(device: torch.device) -> torch.Tensor:
     return flag
 
 
+def _err_ptr(device: torch.device):
+    """The error word's address; None when the first call on a device is being
+    captured (the word would then live in the graph's own memory)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if idx not in _err_flags and torch.cuda.is_current_stream_capturing():
+        return None
+    return _err_flag(device).data_ptr()
+
+
 _split_workspaces: dict[int, torch.Tensor] = {}
 
 
@@ -196,6 +205,87 @@ def dense_attention(q, k, v, sm_scale: float | None = None, out=None) -> torch.T
          i64_array(k.stride()), v.data_ptr(), i64_array(v.stride()), b, h, sq, skv, sm_scale,
          out.data_ptr(), i64_array(out.stride()), *_ws_args(q.device), _err_flag(q.device).data_ptr(),
          _stream(q))
+    return out
+
+
+CROSS_HEAD_DIMS = (64, 128)
+
+
+def _steps(t: torch.Tensor):
+    """Element strides with 0 for dimensions of one entry (never stepped over)."""
+    return i64_array([st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])] + [1])
+
+
+def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, kv_lens=None, key_mask=None,
+                    sm_scale: float | None = None, out=None) -> torch.Tensor:
+    """Attention of query [B, H, Sq, D] to an encoder's states, key and value
+    [B, H', Skv, D] with H a multiple of H' (query heads h * H/H' .. share key
+    head h): bf16 or fp16 views, D 64 or 128, 16-byte aligned strides (the
+    batch and the heads may be broadcast). Which keys a sample has:
+
+        kv_lens   int32/int64 [B]: the first kv_lens[b] (clamped to [0, Skv])
+        key_mask  bool [B, Skv], [1, Skv] or [B, 1, 1, Skv]: True = attend
+
+    Other keys and values have no influence, whatever they hold; a sample
+    without keys gives zeros. out: a [B, H, Sq, D] view of the query's type,
+    which must not overlap the inputs. Nothing is shared between calls: the
+    workspace of a call comes from the caching allocator."""
+    from .ops import _DTYPE_CODE, _on_device_of, _refuse_autograd, _same_device
+
+    what = "cross attention"
+    extra = [t for t in (kv_lens, key_mask, out) if t is not None]
+    for t in (query, key, value, *extra):
+        if not t.is_cuda:
+            raise ValueError(f"{what} requires CUDA tensors")
+    _refuse_autograd(query, key, value, what=what)
+    _same_device(query, key, value, *extra, what=what)
+    for t in (query, key, value):
+        if t.ndim != 4 or t.dtype not in _DTYPE_CODE or t.dtype != query.dtype or t.shape[-1] != query.shape[-1] or (
+                t.shape[-1] not in CROSS_HEAD_DIMS) or t.stride(-1) != 1:
+            raise ValueError(f"{what} requires bf16/fp16 [B, H, S, D] views of one type, D 64 or 128, unit channel stride")
+    b, h, sq, d = query.shape
+    hk, skv = key.shape[1:3]
+    if key.shape != value.shape or key.shape[0] != b or hk == 0 or h % hk:
+        raise ValueError(f"{what}: key and value must match, have the query's batch and divide its heads")
+    sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
+    if not 0.0 < sm_scale < math.inf:
+        raise ValueError(f"{what} requires a positive scale")
+    if kv_lens is not None and key_mask is not None:
+        raise ValueError(f"{what} takes kv_lens or key_mask, not both")
+    if kv_lens is not None and (kv_lens.shape != (b,) or kv_lens.dtype not in (torch.int32, torch.int64)):
+        raise ValueError(f"{what}: kv_lens must be int32 or int64 [B]")
+    if key_mask is not None:
+        if key_mask.ndim == 4 and key_mask.shape[1:3] == (1, 1):
+            key_mask = key_mask[:, 0, 0]
+        if key_mask.dtype != torch.bool or key_mask.ndim != 2 or key_mask.shape[0] not in (1, b) or key_mask.shape[1] != skv:
+            raise ValueError(f"{what}: key_mask must be bool [B, Skv], [1, Skv] or [B, 1, 1, Skv]")
+        key_mask = key_mask.expand(b, skv)
+    if out is None:
+        out = torch.empty((b, h, sq, d), dtype=query.dtype, device=query.device)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
+        raise ValueError(f"{what} output must be a [B, H, Sq, D] view of the query's type with unit channel stride")
+    if not out.numel():
+        return out
+    if not skv:
+        return out.zero_()
+    with _on_device_of(query):
+        if kv_lens is not None and kv_lens.dtype != torch.int32:
+            kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
+        if key_mask is not None:
+            kv_lens = torch.empty((b,), dtype=torch.int32, device=key.device)
+            packed = torch.empty((2, b, hk, skv, d), dtype=key.dtype, device=key.device)
+            call("xgb_pack_keys", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), key.data_ptr(), _steps(key),
+                 value.data_ptr(), _steps(value), b, hk, skv, d, packed[0].data_ptr(), packed[1].data_ptr(),
+                 kv_lens.data_ptr(), _stream(query))
+            key, value = packed[0], packed[1]
+        elif kv_lens is not None:
+            kv_lens = kv_lens.contiguous()
+        ws_bytes = _lib.lib().xgb_cross_attention_workspace(b, h, sq, skv, d)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
+        call("xgb_cross_attention", query.data_ptr(), _steps(query), key.data_ptr(), _steps(key), value.data_ptr(),
+             _steps(value), _DTYPE_CODE[query.dtype], b, h, hk, sq, skv, d,
+             kv_lens.data_ptr() if kv_lens is not None else None, sm_scale, out.data_ptr(), _steps(out),
+             ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(query.device), _stream(query))
     return out
 
 

@@ -1,0 +1,697 @@
+// Cross attention on sm_100a tensor cores: queries of one sequence against the
+// keys and values of another (an encoder's states), with a key count for each
+// sample, shared key heads, head dims 64 and 128, bf16 or fp16:
+//
+//   o[b, h, s] = sum_j p_j v[b, h', j] / sum_j p_j,  j < len[b],  h' = h / (H / H')
+//   p_j = 2^(scale log2(e) q.k_j - m),  m >= the row's largest score - 8
+//
+// A sample without keys gives rows of zeros. Keys and values at j >= len[b]
+// are not read as numbers: their scores are overwritten with -inf and their
+// value rows with zeros (a NaN times a probability of zero would be NaN).
+//
+// Encoder sequences are short (64 to a few hundred keys), so a query tile is
+// done after 4 to 8 key tiles, and what an own CTA for each would spend on
+// starting and ending (TMEM, barriers, first loads, last stores) is a large
+// part of its time. The kernel is therefore persistent, one CTA per SM over a
+// list of units; a unit is 256 query rows (two tiles of 128) of one (batch,
+// head) and, when there are fewer of those than SMs, one part of its keys. All
+// roles run through the list on their own, coupled by mbarriers only, so the
+// loads and first scores of the next unit overlap the last tiles and the
+// epilogue of this one:
+//   warps 0-3, 4-7  softmax and epilogue of query tile 0, 1 (a thread a row)
+//   warp 8          TMA producer: Q tiles, a ring of 64-key K/V tiles
+//   warps 9, 10     MMA issuers of query tile 0, 1
+//   warp 11         clears the value rows behind the last key of a sample
+// TMEM (512 columns): two S buffers of 64 fp32 columns for each query tile
+// (P overwrites its S), O0, O1. Softmax as in the self-attention kernel: exp2
+// domain, 32-bit statistics, O rescaled only when the running maximum rises by
+// more than 8, P rounded to the type of V for the second product.
+//
+// Parts of a unit leave 32-bit O, m and l rows in a workspace of the call;
+// a second small kernel joins them.
+#include <algorithm>
+#include <type_traits>
+
+#include "sm100.cuh"
+#include "tma_host.h"
+
+namespace xgb {
+namespace cross {
+
+using namespace sm100;
+
+constexpr int kBM = 128;   // rows per query tile
+constexpr int kRows = 256;  // rows per unit
+constexpr int kBN = 64;    // keys per tile
+constexpr int kThreads = 384;
+constexpr int kTmaWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kFixWarp = 11;
+constexpr float kTau = 8.0f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+template <typename T, int kD>
+struct Cfg {
+  static constexpr int kSubs = kD / 64;                // 128-byte-wide sub-tiles of a row
+  static constexpr int kQSub = kBM * 128;
+  static constexpr int kQBytes = kSubs * kQSub;
+  static constexpr int kKVSub = kBN * 128;
+  static constexpr int kKVBytes = kSubs * kKVSub;
+  static constexpr int kStages = kD == 128 ? 5 : 8;
+  static constexpr int kKOff = 2 * kQBytes;
+  static constexpr int kVOff = kKOff + kStages * kKVBytes;
+  static constexpr int kBarOff = kVOff + kStages * kKVBytes;
+  static constexpr int kSmem = kBarOff + 512 + 1024;  // + barriers + alignment slack
+  static constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  static constexpr uint32_t kIdescQK = instr_desc(1, kFmt, kFmt, false, false, kBM, kBN);
+  static constexpr uint32_t kIdescPV = instr_desc(1, kFmt, kFmt, false, true, kBM, kD);
+};
+
+struct Params {
+  int heads, group;  // query heads, query heads of one key head
+  int seq_q, seq_kv;
+  const int* lens;  // [batch], null: seq_kv
+  float scale_log2;
+  void* out;
+  int64_t osb, osh, oss;
+  // coordinate factors: 0 for a dimension that is broadcast
+  int qb, qh, kb, kh, vb, vh;
+  int n_qt;      // units of 256 rows of a (batch, head)
+  int splits;    // parts of a unit's keys
+  int64_t units;  // batch * heads * n_qt * splits
+  int part_rows;  // rows of a part in the workspace
+  float* part_o;  // [units][part_rows][D]
+  float2* part_ml;  // [units][part_rows]
+  int* err;
+};
+
+struct Barriers {
+  uint64_t q_full[2], q_empty[2];
+  uint64_t k_full[8], v_full[8], v_ready[8], kv_empty[8];
+  uint64_t s_full[2][2], p_full[2][2];
+  uint64_t pv_done[2];
+  uint64_t o_full[2], o_empty[2];
+  uint64_t end[2];
+  uint32_t tmem_base;
+};
+
+// A CTA's walk over its non-empty units. Units without keys are visited by the
+// softmax warps only.
+struct Unit {
+  int64_t id;
+  int b, h, m0;
+  int kv0, n_kv;  // key tiles [kv0, kv0 + n_kv)
+  int len;
+};
+
+__device__ __forceinline__ Unit unit_at(const Params& p, int64_t id) {
+  Unit u;
+  u.id = id;
+  const int64_t item = id / p.splits;
+  const int part = static_cast<int>(id - item * p.splits);
+  const int64_t bh = item / p.n_qt;
+  u.m0 = static_cast<int>(item - bh * p.n_qt) * kRows;
+  u.b = static_cast<int>(bh / p.heads);
+  u.h = static_cast<int>(bh - static_cast<int64_t>(u.b) * p.heads);
+  u.len = p.lens ? min(max(__ldg(p.lens + u.b), 0), p.seq_kv) : p.seq_kv;
+  const int n_all = (u.len + kBN - 1) / kBN;
+  const int per = (n_all + p.splits - 1) / p.splits;
+  u.kv0 = min(part * per, n_all);
+  u.n_kv = min(per, n_all - u.kv0);
+  return u;
+}
+
+// Position in the stream of key tiles that the CTA's non-empty units make up.
+struct Cursor {
+  Unit u;
+  int t;      // tile within the unit
+  int g;      // tile within the stream
+  int n;      // non-empty units before this one
+  bool more;
+  __device__ __forceinline__ void seek(const Params& p, int64_t id) {
+    more = false;
+    for (; id < p.units; id += gridDim.x) {
+      u = unit_at(p, id);
+      if (u.n_kv > 0) {
+        more = true;
+        break;
+      }
+    }
+    t = 0;
+  }
+  __device__ __forceinline__ void start(const Params& p) {
+    g = n = 0;
+    seek(p, blockIdx.x);
+  }
+  __device__ __forceinline__ void next(const Params& p) {
+    ++g;
+    if (++t == u.n_kv) {
+      ++n;
+      seek(p, u.id + gridDim.x);
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t s_col(int i, int b) { return static_cast<uint32_t>(i * 128 + b * 64); }
+__device__ __forceinline__ uint32_t o_col(int i) { return static_cast<uint32_t>(256 + i * 128); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kThreads, 1)
+    cross_attention_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                           const __grid_constant__ CUtensorMap v_map, const Params p) {
+  using C = Cfg<T, kD>;
+  constexpr int kStages = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_ready[s], 1);
+      mbar_init(&bars->kv_empty[s], 2);  // released by both issuers
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->q_full[i], 1);
+      mbar_init(&bars->q_empty[i], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->s_full[i][b], 1);
+        mbar_init(&bars->p_full[i][b], kBM);
+      }
+      mbar_init(&bars->pv_done[i], 1);
+      mbar_init(&bars->o_full[i], 1);
+      mbar_init(&bars->o_empty[i], kBM);
+      mbar_init(&bars->end[i], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) tmem_alloc<512>(&bars->tmem_base);
+  if (warp == kTmaWarp && lane == 0) {
+    prefetch_tmap(&q_map);
+    prefetch_tmap(&k_map);
+    prefetch_tmap(&v_map);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars->tmem_base;
+
+  if (warp == kTmaWarp) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      bool ok = true;
+      Cursor c;
+      int q_loaded[2] = {0, 0};
+      for (c.start(p); c.more && ok; c.next(p)) {
+        if (c.t == 0) {
+          for (int i = 0; i < 2 && ok; ++i) {
+            if (c.n > 0) ok = mbar_wait(&bars->q_empty[i], (c.n - 1) & 1, p.err);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&bars->q_full[i], C::kQBytes);
+            for (int j = 0; j < C::kSubs; ++j)
+              tma_load_4d(smem + i * C::kQBytes + j * C::kQSub, &q_map, &bars->q_full[i], j * 64, c.u.m0 + i * kBM,
+                          c.u.h * p.qh, c.u.b * p.qb);
+            ++q_loaded[i];
+          }
+          if (!ok) break;
+        }
+        const int s = c.g % kStages, row = (c.u.kv0 + c.t) * kBN, kvh = c.u.h / p.group;
+        if (c.g >= kStages) ok = mbar_wait(&bars->kv_empty[s], ((c.g / kStages) - 1) & 1, p.err);
+        if (!ok) break;
+        mbar_arrive_expect_tx(&bars->k_full[s], C::kKVBytes);
+        for (int j = 0; j < C::kSubs; ++j)
+          tma_load_4d(smem + C::kKOff + s * C::kKVBytes + j * C::kKVSub, &k_map, &bars->k_full[s], j * 64, row, kvh * p.kh,
+                      c.u.b * p.kb);
+        mbar_arrive_expect_tx(&bars->v_full[s], C::kKVBytes);
+        for (int j = 0; j < C::kSubs; ++j)
+          tma_load_4d(smem + C::kVOff + s * C::kKVBytes + j * C::kKVSub, &v_map, &bars->v_full[s], j * 64, row, kvh * p.vh,
+                      c.u.b * p.vb);
+      }
+      // Never leave with copies in flight: wait (bounded) for the last ones.
+      for (int g = max(0, c.g - kStages); g < c.g; ++g) {
+        mbar_wait(&bars->k_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
+        mbar_wait(&bars->v_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
+      }
+      for (int i = 0; i < 2; ++i)
+        if (q_loaded[i]) mbar_wait(&bars->q_full[i], (q_loaded[i] - 1) & 1, p.err, 100000000ull);
+    }
+  } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+    // ------------------------------------------------------------ MMA issuers
+    const int i = warp - kMmaWarp;
+    if (lane == 0) {
+      const uint32_t qa = smem_u32(smem) + i * C::kQBytes;
+      const uint32_t k_saddr = smem_u32(smem + C::kKOff), v_saddr = smem_u32(smem + C::kVOff);
+      uint64_t* v_bar = p.lens ? bars->v_ready : bars->v_full;
+      bool ok = true;
+      Cursor sc, pc;  // scores run two tiles ahead of the second product
+      sc.start(p);
+      pc = sc;
+      auto issue_s = [&]() {
+        const int s = sc.g % kStages;
+        if (sc.t == 0) ok = mbar_wait(&bars->q_full[i], sc.n & 1, p.err);
+        ok = ok && mbar_wait(&bars->k_full[s], (sc.g / kStages) & 1, p.err);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t ka = k_saddr + s * C::kKVBytes;
+#pragma unroll
+        for (int k = 0; k < kD / 16; ++k)
+          mma_ss<Kind::kF16>(tmem + s_col(i, sc.g & 1), smem_desc_sw128(qa + (k >> 2) * C::kQSub + (k & 3) * 32, 16, 1024),
+                             smem_desc_sw128(ka + (k >> 2) * C::kKVSub + (k & 3) * 32, 16, 1024), C::kIdescQK, k > 0);
+        tc_commit(&bars->s_full[i][sc.g & 1]);
+        if (sc.t == sc.u.n_kv - 1) tc_commit(&bars->q_empty[i]);
+        sc.next(p);
+      };
+      for (int k = 0; k < 2 && sc.more && ok; ++k) issue_s();
+      for (; pc.more && ok; pc.next(p)) {
+        const int s = pc.g % kStages;
+        ok = mbar_wait(&v_bar[s], (pc.g / kStages) & 1, p.err) &&
+             mbar_wait(&bars->p_full[i][pc.g & 1], (pc.g >> 1) & 1, p.err);
+        if (ok && pc.t == 0 && pc.n > 0) ok = mbar_wait(&bars->o_empty[i], (pc.n - 1) & 1, p.err);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = v_saddr + s * C::kKVBytes;
+#pragma unroll
+        for (int k = 0; k < kBN / 16; ++k)
+          mma_ts<Kind::kF16>(tmem + o_col(i), tmem + s_col(i, pc.g & 1) + k * 8,
+                             smem_desc_sw128(va + k * 16 * 128, C::kKVSub, 1024), C::kIdescPV, pc.t > 0 || k > 0);
+        tc_commit(&bars->pv_done[i]);
+        tc_commit(&bars->kv_empty[s]);
+        if (pc.t == pc.u.n_kv - 1) tc_commit(&bars->o_full[i]);
+        if (sc.more) issue_s();
+      }
+      tc_commit(&bars->end[i]);
+      mbar_wait(&bars->end[i], 0, p.err, 100000000ull);
+    }
+  } else if (warp == kFixWarp) {
+    // ------------------------------------------------------------ value rows behind the last key
+    if (p.lens) {
+      Cursor c;
+      for (c.start(p); c.more; c.next(p)) {
+        const int s = c.g % kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->v_full[s], (c.g / kStages) & 1, p.err))) break;
+        const int valid = c.u.len - (c.u.kv0 + c.t) * kBN;
+        if (valid < kBN) {
+          // rows of 128 bytes; the swizzle moves 16-byte pieces within a row
+          for (int j = 0; j < C::kSubs; ++j) {
+            uint4* rows = reinterpret_cast<uint4*>(smem + C::kVOff + s * C::kKVBytes + j * C::kKVSub);
+            for (int e = valid * 8 + lane; e < kBN * 8; e += 32) rows[e] = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->v_ready[s]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int i = warp >> 2;
+    const int lane_base = (warp & 3) * 32;
+    const uint32_t lane_addr = tmem + (static_cast<uint32_t>(lane_base) << 16);
+    const uint32_t o_addr = lane_addr + o_col(i);
+    const int r = i * kBM + lane_base + lane;  // row within the unit
+    const float comb = p.scale_log2;
+    bool ok = true;
+    int g = 0, n = 0;
+    for (int64_t id = blockIdx.x; id < p.units && ok; id += gridDim.x) {
+      const Unit u = unit_at(p, id);
+      const int row = u.m0 + r;
+      T* dst = static_cast<T*>(p.out) + u.b * p.osb + u.h * p.osh + row * p.oss;
+      const int64_t part = id * p.part_rows + r;
+      if (u.n_kv == 0) {
+        if (row < p.seq_q) {
+          if (p.splits > 1) {
+            p.part_ml[part] = make_float2(kNegInf, 0.f);
+          } else {
+#pragma unroll
+            for (int c = 0; c < kD / 8; ++c) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        continue;
+      }
+      float m_used = kNegInf;
+      float rsa[4] = {0.f, 0.f, 0.f, 0.f}, rsb[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < u.n_kv; ++t, ++g) {
+        const uint32_t s_addr = lane_addr + s_col(i, g & 1);
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[i][g & 1], (g >> 1) & 1, p.err));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t x[2][32];
+        tmem_ld64(s_addr, x);
+        tmem_ld_wait();
+        const int valid = u.len - (u.kv0 + t) * kBN;
+        if (valid < kBN) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= valid) x[c][e] = 0xFF800000u;
+        }
+        float m4[4];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          m4[2 * c] = fmax3(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+          m4[2 * c + 1] = fmax3(__uint_as_float(x[c][3]), __uint_as_float(x[c][4]), __uint_as_float(x[c][5]));
+#pragma unroll
+          for (int e = 6; e < 30; e += 4) {
+            m4[2 * c] = fmax3(m4[2 * c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+            m4[2 * c + 1] = fmax3(m4[2 * c + 1], __uint_as_float(x[c][e + 2]), __uint_as_float(x[c][e + 3]));
+          }
+          m4[2 * c] = fmax3(m4[2 * c], __uint_as_float(x[c][30]), __uint_as_float(x[c][31]));
+        }
+        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * comb;
+        const float m_new = fmaxf(m_used, mt);
+        const bool need = m_new > m_used + kTau;
+        if (t == 0) {
+          m_used = m_new;
+        } else if (__any_sync(0xffffffffu, need)) {
+          // O must hold the second product of the tile before this one
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->pv_done[i], (g - 1) & 1, p.err));
+          if (!ok) break;
+          tc_fence_after();
+          const float alpha = need ? ex2_approx(m_used - m_new) : 1.0f;
+          if (need) m_used = m_new;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            rsa[j] *= alpha;
+            rsb[j] *= alpha;
+          }
+#pragma unroll 1
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(o_addr + c * 32, o);
+          }
+          tmem_st_wait();
+        }
+        // a row whose scores are all -inf keeps its maximum there: p = 2^-inf
+        const float off = m_used == kNegInf ? 0.f : -m_used;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t packed[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float xa, xb;
+            ffma2(xa, xb, __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]), comb, comb, off, off);
+            const float a = ex2_approx(xa), b = ex2_approx(xb);
+            const int ch = (e / 2) & 3;
+            fadd2(rsa[ch], rsb[ch], rsa[ch], rsb[ch], a, b);
+            packed[e / 2] = pack2<T>(a, b);
+          }
+          tmem_st16(s_addr + c * 16, packed);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[i][g & 1]);
+      }
+      if (!ok) break;
+      const float l = ((rsa[0] + rsb[0]) + (rsa[1] + rsb[1])) + ((rsa[2] + rsb[2]) + (rsa[3] + rsb[3]));
+      // ------------------------------------------------------------ epilogue
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[i], n & 1, p.err));
+      ++n;
+      if (!ok) break;
+      tc_fence_after();
+      const float inv_l = l != 0.f ? 1.0f / l : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(o_addr + c * 32, o);
+        tmem_ld_wait();
+        if (row >= p.seq_q) continue;
+        if (p.splits > 1) {
+          float4* po = reinterpret_cast<float4*>(p.part_o + part * kD) + c * 8;
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            po[v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]), __uint_as_float(o[4 * v + 2]),
+                                __uint_as_float(o[4 * v + 3]));
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2)
+            w[e / 2] = pack2<T>(__uint_as_float(o[e]) * inv_l, __uint_as_float(o[e + 1]) * inv_l);
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            reinterpret_cast<uint4*>(dst + c * 32)[v] = make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
+        }
+      }
+      if (p.splits > 1 && row < p.seq_q) p.part_ml[part] = make_float2(m_used, l);
+      tc_fence_before();
+      mbar_arrive(&bars->o_empty[i]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc<512>(tmem);
+  }
+}
+
+// Joins the parts of a row: M = max m, o = sum 2^(m - M) O / sum 2^(m - M) l.
+// One warp a row; a part without keys (l = 0) left no O.
+template <typename T, int kD>
+__global__ void __launch_bounds__(256) join_kernel(const Params p, int64_t rows) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (batch, head, row)
+  if (at >= rows) return;
+  const int64_t bh = at / p.seq_q;
+  const int row = static_cast<int>(at - bh * p.seq_q);
+  const int64_t item = bh * p.n_qt + row / kRows;
+  const int r = row % kRows;
+  const int64_t first = item * p.splits * p.part_rows + r;
+  float mx = kNegInf;
+  for (int q = 0; q < p.splits; ++q) mx = fmaxf(mx, __ldg(&p.part_ml[first + static_cast<int64_t>(q) * p.part_rows]).x);
+  const float base = mx == kNegInf ? 0.f : mx;
+  float l = 0.f, o[kD / 32] = {};
+  for (int q = 0; q < p.splits; ++q) {
+    const int64_t at_q = first + static_cast<int64_t>(q) * p.part_rows;
+    const float2 ml = __ldg(&p.part_ml[at_q]);
+    if (ml.y == 0.f) continue;
+    const float w = ex2_approx(ml.x - base);
+    l = fmaf(w, ml.y, l);
+#pragma unroll
+    for (int c = 0; c < kD / 32; ++c) o[c] = fmaf(w, __ldg(p.part_o + at_q * kD + c * 32 + lane), o[c]);
+  }
+  const float inv_l = l != 0.f ? 1.0f / l : 0.f;
+  const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<int64_t>(b) * p.heads);
+  T* dst = static_cast<T*>(p.out) + b * p.osb + h * p.osh + row * p.oss;
+#pragma unroll
+  for (int c = 0; c < kD / 32; ++c) {
+    if constexpr (std::is_same<T, __half>::value) dst[c * 32 + lane] = __float2half_rn(o[c] * inv_l);
+    else dst[c * 32 + lane] = __float2bfloat16_rn(o[c] * inv_l);
+  }
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 148;
+}
+
+// Parts of a unit's keys: 1 unless whole units would leave more than half of
+// the SMs without work, then as many as fill them, each at least one tile.
+int parts(int64_t items, int64_t seq_kv, int sms) {
+  if (items * 2 > sms) return 1;
+  return static_cast<int>(std::min<int64_t>(sms / std::max<int64_t>(items, 1), cdiv(seq_kv, kBN)));
+}
+
+template <typename T, int kD>
+int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int64_t batch, int sms,
+           cudaStream_t st) {
+  using C = Cfg<T, kD>;
+  auto kernel = cross_attention_kernel<T, kD>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+    return XGB_ERR_LAUNCH;
+  const int grid = static_cast<int>(std::min<int64_t>(p.units, sms));
+  kernel<<<grid, kThreads, C::kSmem, st>>>(qm, km, vm, p);
+  const int rc = launch_status();
+  if (rc || p.splits == 1) return rc;
+  const int64_t rows = batch * p.heads * p.seq_q;
+  join_kernel<T, kD><<<static_cast<unsigned>(cdiv(rows, 8)), 256, 0, st>>>(p, rows);
+  return launch_status();
+}
+
+// ---------------------------------------------------------------- masked keys
+// Gathers the keys and values that a mask keeps to the front of packed
+// [batch, heads, seq_kv, D] tensors, in order, and counts them; what lies
+// behind the count is not written. A block takes 64 keys of one sample and
+// counts the kept ones before its own.
+__global__ void __launch_bounds__(256) pack_keys_kernel(const uint8_t* __restrict__ mask, int64_t msb, int64_t mss,
+                                                        const uint4* __restrict__ k, int64_t ksb, int64_t ksh, int64_t kss,
+                                                        const uint4* __restrict__ v, int64_t vsb, int64_t vsh, int64_t vss,
+                                                        int heads, int seq, int words, uint4* __restrict__ k_out,
+                                                        uint4* __restrict__ v_out, int* __restrict__ counts) {
+  __shared__ int red[8];
+  __shared__ int place[kBN];
+  const int b = blockIdx.y, first = blockIdx.x * kBN;
+  const uint8_t* row = mask + b * msb;
+  int before = 0;
+  for (int j = threadIdx.x; j < first; j += 256) before += row[j * mss] != 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = before;
+  __syncthreads();
+  before = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) before += red[w];
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int at = before;
+    for (int c = 0; c < kBN / 32; ++c) {
+      const int j = first + c * 32 + lane;
+      const bool keep = j < seq && row[j * mss] != 0;
+      const uint32_t kept = __ballot_sync(0xffffffffu, keep);
+      place[c * 32 + lane] = keep ? at + __popc(kept & ((1u << lane) - 1)) : -1;
+      at += __popc(kept);
+    }
+    if (lane == 0 && first + kBN >= seq) counts[b] = at;
+  }
+  __syncthreads();
+  const int per_head = kBN * words;
+  for (int e = threadIdx.x; e < heads * per_head; e += 256) {
+    const int h = e / per_head, j = (e - h * per_head) / words, w = e % words;
+    const int to = place[j];
+    if (to < 0) continue;
+    const int64_t dst = ((static_cast<int64_t>(b) * heads + h) * seq + to) * words + w;
+    k_out[dst] = __ldg(k + b * ksb + h * ksh + (first + j) * kss + w);
+    v_out[dst] = __ldg(v + b * vsb + h * vsh + (first + j) * vss + w);
+  }
+}
+
+inline bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
+
+}  // namespace cross
+}  // namespace xgb
+
+using namespace xgb;
+
+XGB_API int xgb_pack_keys(const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, const void* k,
+                          const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t batch, int64_t heads,
+                          int64_t seq, int64_t head_dim, void* k_out, void* v_out, int* counts, void* stream) {
+  if (!mask || !k || !v || !k_strides || !v_strides || !k_out || !v_out || !counts) return XGB_ERR_ARG;
+  if (batch <= 0 || batch > 65535 || heads <= 0 || heads > 65535 || seq <= 0 || seq > (1 << 30) ||
+      (head_dim != 64 && head_dim != 128))
+    return XGB_ERR_SHAPE;
+  for (int d = 0; d < 3; ++d)
+    if (k_strides[d] % 8 || v_strides[d] % 8) return XGB_ERR_STRIDE;
+  if (k_strides[3] != 1 || v_strides[3] != 1) return XGB_ERR_STRIDE;
+  if (!cross::aligned16(k) || !cross::aligned16(v) || !cross::aligned16(k_out) || !cross::aligned16(v_out))
+    return XGB_ERR_ALIGN;
+  const dim3 grid(static_cast<unsigned>(cdiv(seq, cross::kBN)), static_cast<unsigned>(batch));
+  cross::pack_keys_kernel<<<grid, 256, 0, as_stream(stream)>>>(
+      mask, mask_batch_stride, mask_stride, static_cast<const uint4*>(k), k_strides[0] / 8, k_strides[1] / 8,
+      k_strides[2] / 8, static_cast<const uint4*>(v), v_strides[0] / 8, v_strides[1] / 8, v_strides[2] / 8,
+      static_cast<int>(heads), static_cast<int>(seq), static_cast<int>(head_dim / 8), static_cast<uint4*>(k_out),
+      static_cast<uint4*>(v_out), counts);
+  return launch_status();
+}
+
+XGB_API int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim) {
+  if (batch <= 0 || heads <= 0 || seq_q <= 0 || seq_kv <= 0) return 0;
+  const int64_t items = batch * heads * cdiv(seq_q, cross::kRows);
+  const int splits = cross::parts(items, seq_kv, cross::sm_count());
+  if (splits <= 1) return 0;
+  return items * splits * std::min<int64_t>(seq_q, cross::kRows) * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                const void* v, const int64_t* v_strides, int dtype, int64_t batch, int64_t heads,
+                                int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int* kv_lens,
+                                float sm_scale, void* out, const int64_t* out_strides, void* workspace,
+                                int64_t workspace_bytes, int* error_flag, void* stream) {
+  if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides || !out_strides) return XGB_ERR_ARG;
+  if (dtype != XGB_BF16 && dtype != XGB_F16) return XGB_ERR_ARG;
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq_q <= 0 || seq_kv <= 0 || seq_q > (1 << 30) ||
+      seq_kv > (1 << 30) || batch > 65535 || heads > 65535 || (head_dim != 64 && head_dim != 128))
+    return XGB_ERR_SHAPE;
+  if (!(sm_scale > 0.f)) return XGB_ERR_ARG;
+  const int64_t* all[4] = {q_strides, k_strides, v_strides, out_strides};
+  for (int n = 0; n < 4; ++n) {
+    const int64_t extent[3] = {batch, n == 1 || n == 2 ? kv_heads : heads, n == 1 || n == 2 ? seq_kv : seq_q};
+    if (all[n][3] != 1) return XGB_ERR_STRIDE;
+    for (int d = 0; d < 3; ++d) {
+      if (extent[d] == 1) continue;  // never stepped over
+      // inputs may be broadcast over the batch and the heads
+      if (all[n][d] % 8 || all[n][d] < 0 || (all[n][d] == 0 && (n == 3 || d == 2))) return XGB_ERR_STRIDE;
+    }
+  }
+  if (!cross::aligned16(q) || !cross::aligned16(k) || !cross::aligned16(v) || !cross::aligned16(out)) return XGB_ERR_ALIGN;
+  const int64_t need = xgb_cross_attention_workspace(batch, heads, seq_q, seq_kv, head_dim);
+  if (need && (!workspace || workspace_bytes < need)) return XGB_ERR_WORKSPACE;
+  if (need && !cross::aligned16(workspace)) return XGB_ERR_ALIGN;
+  int dev = 0, major = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10)
+    return XGB_ERR_DEVICE;
+  cross::Params p{};
+  CUtensorMap map[3];
+  const void* base[3] = {q, k, v};
+  int factor[3][2];  // batch, head
+  for (int n = 0; n < 3; ++n) {
+    const int64_t* s = all[n];
+    const int64_t seq = n == 0 ? seq_q : seq_kv, hh = n == 0 ? heads : kv_heads;
+    // a dimension of one entry, or a broadcast one, is one entry of the map
+    const int64_t ext[3] = {seq, hh > 1 && s[1] ? hh : 1, batch > 1 && s[0] ? batch : 1};
+    factor[n][0] = ext[2] > 1;
+    factor[n][1] = ext[1] > 1;
+    const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(ext[0]), static_cast<uint64_t>(ext[1]),
+                              static_cast<uint64_t>(ext[2])};
+    const uint64_t row = static_cast<uint64_t>(head_dim) * 2;
+    const uint64_t strides[3] = {ext[0] > 1 ? static_cast<uint64_t>(s[2]) * 2 : row,
+                                 ext[1] > 1 ? static_cast<uint64_t>(s[1]) * 2 : row,
+                                 ext[2] > 1 ? static_cast<uint64_t>(s[0]) * 2 : row};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(n == 0 ? cross::kBM : cross::kBN), 1, 1};
+    if (!make_tensor_map(&map[n], dtype == XGB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         base[n], dims, strides, box))
+      return XGB_ERR_ALIGN;
+  }
+  p.qb = factor[0][0];
+  p.qh = factor[0][1];
+  p.kb = factor[1][0];
+  p.kh = factor[1][1];
+  p.vb = factor[2][0];
+  p.vh = factor[2][1];
+  const int sms = cross::sm_count();
+  p.heads = static_cast<int>(heads);
+  p.group = static_cast<int>(heads / kv_heads);
+  p.seq_q = static_cast<int>(seq_q);
+  p.seq_kv = static_cast<int>(seq_kv);
+  p.lens = kv_lens;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.out = out;
+  p.osb = out_strides[0];
+  p.osh = out_strides[1];
+  p.oss = out_strides[2];
+  p.n_qt = static_cast<int>(cdiv(seq_q, cross::kRows));
+  const int64_t items = batch * heads * p.n_qt;
+  p.splits = cross::parts(items, seq_kv, sms);
+  p.units = items * p.splits;
+  p.part_rows = static_cast<int>(std::min<int64_t>(seq_q, cross::kRows));
+  if (p.splits > 1) {
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + p.units * p.part_rows * head_dim);
+  }
+  p.err = error_flag;
+  cudaStream_t st = as_stream(stream);
+  if (dtype == XGB_BF16)
+    return head_dim == 128 ? cross::launch<__nv_bfloat16, 128>(map[0], map[1], map[2], p, batch, sms, st)
+                           : cross::launch<__nv_bfloat16, 64>(map[0], map[1], map[2], p, batch, sms, st);
+  return head_dim == 128 ? cross::launch<__half, 128>(map[0], map[1], map[2], p, batch, sms, st)
+                         : cross::launch<__half, 64>(map[0], map[1], map[2], p, batch, sms, st);
+}

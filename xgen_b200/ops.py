@@ -8,12 +8,15 @@ non-CUDA tensors raise ValueError (or return None where the reference's
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
-from ._lib import call, i64_array
+from ._lib import call, f64_array, i64_array
 
 _DTYPE_CODE = {torch.bfloat16: _lib.XGB_BF16, torch.float16: _lib.XGB_F16}
+_DTYPE_CODE_F32 = {**_DTYPE_CODE, torch.float32: _lib.XGB_F32}
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -24,6 +27,24 @@ def _require_cuda(*tensors: torch.Tensor, what: str) -> None:
     for t in tensors:
         if not t.is_cuda:
             raise ValueError(f"{what} requires CUDA tensors")
+
+
+def _refuse_autograd(*tensors, what: str) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
+
+
+def _on_device_of(t: torch.Tensor):
+    """Context in which `t`'s device is the current one: launches go to the
+    current device, whatever the stream they are given."""
+    if t.device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(t.device)
+
+
+def _same_device(first: torch.Tensor, *others, what: str) -> None:
+    if any(t is not None and t.device != first.device for t in others):
+        raise ValueError(f"{what} needs its tensors on one device")
 
 
 def try_h3_partial_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
@@ -227,4 +248,176 @@ def quantize_per_token(x: torch.Tensor):
     scales = torch.empty((rows,), device=x.device, dtype=torch.float32)
     call("xgb_fp8_quantize_per_token", x.data_ptr(), _DTYPE_CODE[x.dtype], rows, cols,
          x.stride(0), out.data_ptr(), scales.data_ptr(), _stream(x))
+    return out, scales
+
+
+_POSITION_CODE = {torch.int32: 0, torch.int64: 1, torch.float32: 2, torch.float64: 3}
+
+
+def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor, *, axes,
+              theta=10000.0, interleaved: bool = False, norm_q=None, norm_k=None):
+    """Rotary positions with several axes (time, height, width), taken from
+    the positions themselves rather than from a table, and the per-head Q/K
+    RMSNorm before them.
+
+    query [B, S, H, D], key [B, S, H', D] (or None): bf16, fp16 or fp32 views
+    with unit channel stride, D <= 512. positions [S, A] or [B, S, A]: int32,
+    int64, float32 or float64 (grid indices, or fractions of them where a
+    model rescales its grid). axes: even channel counts of the A axes, whose
+    pairs follow one another; channels behind their sum R pass through.
+    theta: one base, or one for each axis. Pair i turns by position *
+    theta ** (-2 i / d) within its axis of d channels (angles in 64 bits) and
+    is made of channels (i, i + R/2), the convention of the cos/sin tables of
+    h3.rope, or of (2i, 2i + 1) with interleaved=True. norm_q / norm_k: the
+    torch.nn.RMSNorm modules of a model with Q/K norms, applied first.
+
+    32-bit arithmetic, one rounding at the end (the try_h3_* operators round
+    after every step, as the reference does). Returns contiguous (query, key)."""
+    what = "rotary positions"
+    _require_cuda(query, positions, *(() if key is None else (key,)), what=what)
+    _refuse_autograd(query, key, what=what)
+    axes = tuple(int(a) for a in axes)
+    thetas = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(axes)
+    if query.dtype not in _DTYPE_CODE_F32:
+        raise ValueError(f"{what} need bf16, fp16 or fp32 queries")
+    for t in (query,) if key is None else (query, key):
+        if t.ndim != 4 or t.dtype != query.dtype or (t.stride(-1) != 1 and t.shape[-1] > 1):
+            raise ValueError(f"{what} need [B, S, H, D] views of one type with unit channel stride")
+    b, s, h, d = query.shape
+    if key is not None and (key.shape[:2] != query.shape[:2] or key.shape[-1] != d):
+        raise ValueError(f"{what}: query and key differ in batch, sequence or head dim")
+    if not axes or any(a <= 0 or a % 2 for a in axes) or sum(axes) > d or len(thetas) != len(axes) or not all(
+            0 < t < float("inf") for t in thetas):
+        raise ValueError(f"{what} need positive even axis channels within the head dim and a positive theta for each axis")
+    if positions.dtype not in _POSITION_CODE or positions.shape not in ((s, len(axes)), (b, s, len(axes))):
+        raise ValueError(f"{what}: positions must be integers or 32/64-bit floats of shape [S, A] or [B, S, A]")
+    if positions.stride(-1) != 1 and len(axes) > 1:
+        positions = positions.contiguous()
+    weights, eps = [], []
+    for norm in (norm_q, norm_k if key is not None else None):
+        if norm is None:
+            weights.append(None)
+            eps.append(0.0)
+            continue
+        if type(norm) is not torch.nn.RMSNorm or tuple(norm.normalized_shape) != (d,) or norm.weight is None or (
+                norm.weight.dtype != query.dtype) or not norm.weight.is_contiguous():
+            raise ValueError(f"{what}: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
+        _require_cuda(norm.weight, what=what)
+        weights.append(norm.weight)
+        eps.append(float(norm.eps if norm.eps is not None else torch.finfo(query.dtype).eps))
+    _refuse_autograd(*weights, what=what)
+    _same_device(query, key, positions, *weights, what=what)
+    q_out = torch.empty(query.shape, device=query.device, dtype=query.dtype)
+    k_out = torch.empty(key.shape, device=key.device, dtype=key.dtype) if key is not None else None
+    if not b * s * h * d:
+        if key is None or not key.numel():
+            return q_out, k_out
+        raise ValueError(f"{what} need at least one query head")
+    with _on_device_of(query):
+        call("xgb_rope_axes", query.data_ptr(), i64_array(query.stride()[:3]),
+             key.data_ptr() if key is not None else None,
+             i64_array(key.stride()[:3]) if key is not None else None, _DTYPE_CODE_F32[query.dtype], b, s, h,
+             key.shape[2] if key is not None else 0, d, positions.data_ptr(), _POSITION_CODE[positions.dtype],
+             positions.stride(0) if positions.ndim == 3 else 0, positions.stride(-2), len(axes), i64_array(axes),
+             f64_array(thetas), int(interleaved), *(w.data_ptr() if w is not None else None for w in weights), *eps,
+             q_out.data_ptr(), k_out.data_ptr() if key is not None else None, _stream(query))
+    return q_out, k_out
+
+
+_NORM_CODE = {None: 0, "layernorm": 1, "rmsnorm": 2}
+_QUANT_CODE = {None: (0, None), "int8": (1, torch.int8), "e4m3": (2, torch.float8_e4m3fn)}
+
+
+def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: str | None = "rmsnorm",
+                  pre_norm: str | None = "rmsnorm", post_weight=None, pre_weight=None, eps: float = 1e-6,
+                  gate=None, residual_scale: float = 1.0, scale=None, shift=None, indices=None,
+                  quant: str | None = None):
+    """The norm after a block, its gate and residual, and the norm and
+    modulation before the next block, in one pass:
+
+        x = residual + residual_scale * gate[idx] * post(branch)
+        h = pre(x) * (1 + scale[idx]) + shift[idx]
+
+    branch, residual [B, S, W]: bf16, fp16 or fp32 views of one type with unit
+    channel stride, W <= 16384. post_norm / pre_norm: "layernorm", "rmsnorm" or
+    None, times an optional weight [W]; pre_norm=None returns x alone. gate,
+    scale, shift: rows [M, W] of AdaLN tables (row-strided views; scale and
+    shift come together); indices: int64 [S], shared by the batch, or [B, S];
+    an index outside the tables makes its row NaN. Returns (x, h), or with
+    quant="int8" / "e4m3" (x, codes, scales [B, S]): the per-token codes that
+    int8_linear_quantized / H3FP8Linear.forward_quantized take.
+
+    32-bit arithmetic; x and h are rounded once each, h from the x before its
+    rounding."""
+    what = "sandwich norm"
+    tables = [t for t in (gate, scale, shift) if t is not None]
+    weights = [t for t in (post_weight, pre_weight) if t is not None]
+    extra = [indices] if indices is not None else []
+    _require_cuda(branch, residual, *tables, *weights, *extra, what=what)
+    _refuse_autograd(branch, residual, *tables, *weights, what=what)
+    _same_device(branch, residual, *tables, *weights, *extra, what=what)
+    if (branch.ndim != 3 or branch.shape != residual.shape or branch.dtype not in _DTYPE_CODE_F32
+            or residual.dtype != branch.dtype or any(t.stride(-1) != 1 and t.shape[-1] > 1 for t in (branch, residual))):
+        raise ValueError(f"{what} needs [B, S, W] branch and residual of one 16- or 32-bit float type with unit channel stride")
+    if post_norm not in _NORM_CODE or pre_norm not in _NORM_CODE or quant not in _QUANT_CODE:
+        raise ValueError(f"{what}: norms are 'layernorm', 'rmsnorm' or None, quant 'int8', 'e4m3' or None")
+    b, s, w = branch.shape
+    if w > 16384 or w == 0:
+        raise ValueError(f"{what} takes rows of 1 to 16384 channels")
+    if (scale is None) != (shift is None):
+        raise ValueError(f"{what} needs scale and shift together")
+    if pre_norm is None and (quant is not None or scale is not None or pre_weight is not None):
+        raise ValueError(f"{what} without a norm before the next block has no modulation and no codes")
+    if post_norm is None and post_weight is not None:
+        raise ValueError(f"{what} without a norm after the block has no weight for it")
+    if any(t.ndim != 2 or t.shape[1] != w or t.dtype != branch.dtype or (t.stride(1) != 1 and w > 1)
+           or t.shape[0] != tables[0].shape[0] or t.shape[0] == 0 for t in tables):
+        raise ValueError(f"{what}: gate, scale and shift must be [M, W] rows of the branch's type")
+    if any(t.shape != (w,) or t.dtype != branch.dtype or not t.is_contiguous() for t in weights):
+        raise ValueError(f"{what}: weights must be contiguous [W] of the branch's type")
+    if bool(tables) != (indices is not None):
+        raise ValueError(f"{what}: indices come with gate or scale and shift")
+    if indices is not None:
+        if indices.dtype != torch.int64 or indices.shape not in ((s,), (b, s)):
+            raise ValueError(f"{what}: indices must be int64 [S] or [B, S]")
+        indices = indices.contiguous()
+    x_out = torch.empty((b, s, w), device=branch.device, dtype=branch.dtype)
+    code, code_type = _QUANT_CODE[quant]
+    h_out = torch.empty_like(x_out) if pre_norm is not None and code == 0 else None
+    codes = torch.empty((b, s, w), device=branch.device, dtype=code_type) if code else None
+    scales = torch.empty((b, s), device=branch.device, dtype=torch.float32) if code else None
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    # one row's stride is never stepped over
+    row = lambda t: (t.stride(0) if t.shape[0] > 1 else w) if t is not None else 0  # noqa: E731
+    if b * s:
+        with _on_device_of(branch):
+            call("xgb_sandwich_norm", branch.data_ptr(), i64_array(branch.stride()[:2]), residual.data_ptr(),
+                 i64_array(residual.stride()[:2]), _DTYPE_CODE_F32[branch.dtype], b, s, w, _NORM_CODE[post_norm],
+                 ptr(post_weight), _NORM_CODE[pre_norm], ptr(pre_weight), float(eps), ptr(gate), row(gate),
+                 float(residual_scale), ptr(scale), row(scale), ptr(shift), row(shift), ptr(indices),
+                 s if indices is not None and indices.ndim == 2 else 0, tables[0].shape[0] if tables else 0,
+                 x_out.data_ptr(), ptr(h_out), code, ptr(codes), ptr(scales), _stream(branch))
+    if pre_norm is None:
+        return x_out
+    return (x_out, codes, scales) if code else (x_out, h_out)
+
+
+def quantize_per_token_int8(x: torch.Tensor):
+    """Per-row dynamic int8 of a bf16/fp16 matrix (rows may be strided):
+    (codes, scales[rows]) with scale = max(amax/127, FLT_MIN) and codes the
+    nearest integers to x / scale, ties to even."""
+    what = "H3 INT8 quantization"
+    _require_cuda(x, what=what)
+    _refuse_autograd(x, what=what)
+    if x.dtype not in _DTYPE_CODE or x.ndim != 2 or (x.stride(-1) != 1 and x.shape[1] > 1) or x.shape[1] == 0 or (
+            x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        raise ValueError(f"{what} requires a row-major 2-D bf16/fp16 matrix")
+    rows, cols = x.shape
+    out = torch.empty((rows, cols), device=x.device, dtype=torch.int8)
+    scales = torch.empty((rows,), device=x.device, dtype=torch.float32)
+    if not rows:
+        return out, scales
+    with _on_device_of(x):
+        call("xgb_int8_quantize_per_token", x.data_ptr(), _DTYPE_CODE[x.dtype], rows, cols, x.stride(0),
+             out.data_ptr(), scales.data_ptr(), _stream(x))
     return out, scales
