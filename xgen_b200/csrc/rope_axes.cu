@@ -11,9 +11,10 @@
 // and only the fraction is rounded to 32 bits for sincospif. Everything after
 // that is 32-bit, rounded once to the tensor's type.
 //
-// Bound by HBM: Q and K once in, once out. A token's cos/sin (R/2 pairs) are
-// computed once into shared memory and used by all of its heads, so the 64-bit
-// work is 1/96th of the elements at 48 heads of 128.
+// Bound by HBM: Q and K once in, once out. In the vector form a thread owns 16
+// channels (two 16-byte pieces holding 8 whole pairs) of one token and keeps
+// their cos/sin in registers while it walks over the token's heads of Q and K,
+// so a token's angles are computed once, not once a head.
 #include <algorithm>
 
 #include "xgb_common.cuh"
@@ -47,7 +48,6 @@ struct Params {
   int64_t tokens;  // batch * seq
   int64_t seq;
   int width, rotary;
-  int per_block;  // tokens of one step of a block
 };
 
 __device__ __forceinline__ double load_position(const Params& p, int64_t at) {
@@ -121,12 +121,195 @@ __global__ void __launch_bounds__(kThreads) rope_axes_scalar_kernel(const Params
   }
 }
 
+// Eight consecutive channels.
+__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
+  unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(p)), f);
+}
+__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
+  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(round_bf16x2(f[0], f[1]), round_bf16x2(f[2], f[3]), round_bf16x2(f[4], f[5]),
+                                            round_bf16x2(f[6], f[7]));
+}
+__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Vector form: width and rotary multiples of 16, 16-byte aligned rows. Threads
+// are (token, head step, lane): 2^lane_bits lanes a head, 2^head_bits heads at
+// a time, the rest of the 256 threads tokens. A block walks over groups of
+// tokens; a group's cos/sin go through one of two shared buffers, so one
+// barrier a group is enough.
+template <typename T, bool kInterleaved, bool kNorm>
+__global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const Params p, const __grid_constant__ Turns turns,
+                                                                 int lane_bits, int head_bits) {
+  __shared__ double per_unit[kMaxPairs];
+  __shared__ uint8_t axis[kMaxPairs];
+  // at most 256 / lanes tokens of 8 * lanes pairs each
+  __shared__ __align__(16) float cos_buf[2][kThreads * 8];
+  __shared__ __align__(16) float sin_buf[2][kThreads * 8];
+  const int pairs = p.rotary / 2;
+  for (int i = threadIdx.x; i < pairs; i += kThreads) {
+    per_unit[i] = turns.per_unit[i];
+    axis[i] = turns.axis[i];
+  }
+  __syncthreads();
+  const int j = threadIdx.x & ((1 << lane_bits) - 1);
+  const int first_head = (threadIdx.x >> lane_bits) & ((1 << head_bits) - 1);
+  const int t = threadIdx.x >> (lane_bits + head_bits);
+  const int per_group = kThreads >> (lane_bits + head_bits);
+  const int heads = p.heads[0] + p.heads[1];
+  const bool active = j < p.width / 16, turned = j < p.rotary / 16;
+  const int ca = kInterleaved || !turned ? 16 * j : 8 * j;
+  const int cb = kInterleaved || !turned ? ca + 8 : ca + pairs;
+  const int64_t groups = (p.tokens + per_group - 1) / per_group;
+  int buf = 0;
+  for (int64_t group = blockIdx.x; group < groups; group += gridDim.x, buf ^= 1) {
+    const int64_t first = group * per_group;
+    for (int i = threadIdx.x; i < per_group * pairs; i += kThreads) {
+      const int tt = i / pairs, pair = i - tt * pairs;
+      if (first + tt < p.tokens) {
+        const float2 cs = cos_sin(p, first + tt, per_unit[pair], axis[pair]);
+        cos_buf[buf][i] = cs.x;
+        sin_buf[buf][i] = cs.y;
+      }
+    }
+    __syncthreads();
+    const int64_t token = first + t;
+    const bool here = active && token < p.tokens;
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = 1.f;
+      s[i] = 0.f;
+    }
+    if (here && turned) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        const float4 cv = *reinterpret_cast<const float4*>(&cos_buf[buf][t * pairs + 8 * j + i]);
+        const float4 sv = *reinterpret_cast<const float4*>(&sin_buf[buf][t * pairs + 8 * j + i]);
+        c[i] = cv.x; c[i + 1] = cv.y; c[i + 2] = cv.z; c[i + 3] = cv.w;
+        s[i] = sv.x; s[i + 1] = sv.y; s[i + 2] = sv.z; s[i + 3] = sv.w;
+      }
+    }
+    const int64_t b = token / p.seq, at = token - b * p.seq;
+#pragma unroll 2
+    for (int h0 = 0; h0 < heads; h0 += 1 << head_bits) {
+      int h = h0 + first_head;
+      const bool go = here && h < heads;
+      const int which = h >= p.heads[0];
+      if (which) h -= p.heads[0];
+      float x[8], y[8];
+      if (go) {
+        const T* src = static_cast<const T*>(p.src[which]) + b * p.sb[which] + at * p.ss[which] + h * p.sh[which];
+        load8(src + ca, x);
+        load8(src + cb, y);
+      }
+      if constexpr (kNorm) {
+        // every lane takes part; a tensor without a norm keeps its values
+        float sq = 0.f;
+        if (go) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], fmaf(y[i], y[i], sq));
+        }
+        for (int o = (1 << lane_bits) >> 1; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+        const T* w = static_cast<const T*>(p.weight[which]);
+        if (go && w) {
+          const float rstd = rsqrtf(sq / p.width + p.eps[which]);
+          float wa[8], wb[8];
+          load8(w + ca, wa);
+          load8(w + cb, wb);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            x[i] *= rstd * wa[i];
+            y[i] *= rstd * wb[i];
+          }
+        }
+      }
+      if (go) {
+        T* dst = static_cast<T*>(p.dst[which]) + (token * p.heads[which] + h) * p.width;
+        if constexpr (kInterleaved) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float a = x[2 * i], d = y[2 * i];
+            x[2 * i] = a * c[i] - x[2 * i + 1] * s[i];
+            x[2 * i + 1] = x[2 * i + 1] * c[i] + a * s[i];
+            y[2 * i] = d * c[4 + i] - y[2 * i + 1] * s[4 + i];
+            y[2 * i + 1] = y[2 * i + 1] * c[4 + i] + d * s[4 + i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float a = x[i];
+            x[i] = a * c[i] - y[i] * s[i];
+            y[i] = y[i] * c[i] + a * s[i];
+          }
+        }
+        store8(dst + ca, x);
+        store8(dst + cb, y);
+      }
+    }
+  }
+}
+
+int bits_for(int n) {  // smallest b with 2^b >= n
+  int b = 0;
+  while ((1 << b) < n) ++b;
+  return b;
+}
+
 template <typename T>
 int launch(const Params& p, const Turns& turns, bool interleaved, cudaStream_t st) {
-  const int64_t rows = p.tokens * (p.heads[0] + p.heads[1]);
-  const int64_t blocks = std::min<int64_t>(cdiv(rows, kThreads / 32), 148 * 64);
-  rope_axes_scalar_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p, turns, interleaved);
-  return launch_status();
+  const int heads = p.heads[0] + p.heads[1];
+  bool vec = p.width % 16 == 0 && p.rotary % 16 == 0;
+  for (int i = 0; i < 2 && vec; ++i) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p.src[i]) | reinterpret_cast<uintptr_t>(p.dst[i]) |
+                         reinterpret_cast<uintptr_t>(p.weight[i]);
+    const int64_t strides = p.sb[i] | p.ss[i] | p.sh[i];
+    vec = at % 16 == 0 && strides * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+  }
+  if (!vec) {
+    const int64_t blocks = std::min<int64_t>(cdiv(p.tokens * heads, kThreads / 32), 148 * 64);
+    rope_axes_scalar_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p, turns, interleaved);
+    return launch_status();
+  }
+  const int lane_bits = bits_for(p.width / 16);
+  // Few tokens: all heads of a token at once, so that more blocks have work.
+  // Many: 8 heads at a time, so that a group has enough angles for its threads.
+  const int most = p.tokens <= 2 * 148 ? 8 - lane_bits : std::min(3, 8 - lane_bits);
+  const int head_bits = std::min(bits_for(heads), most);
+  const int64_t groups = cdiv(p.tokens, kThreads >> (lane_bits + head_bits));
+  const int64_t blocks = std::min<int64_t>(groups, 148 * 8);
+  const bool norm = p.weight[0] || p.weight[1];
+  auto run = [&](auto kernel) {
+    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p, turns, lane_bits, head_bits);
+    return launch_status();
+  };
+  if (interleaved) return norm ? run(rope_axes_vec_kernel<T, true, true>) : run(rope_axes_vec_kernel<T, true, false>);
+  return norm ? run(rope_axes_vec_kernel<T, false, true>) : run(rope_axes_vec_kernel<T, false, false>);
 }
 
 }  // namespace

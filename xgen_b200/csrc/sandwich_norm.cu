@@ -167,8 +167,223 @@ __global__ void __launch_bounds__(kScalarThreads) sandwich_norm_scalar_kernel(co
   for (int c = threadIdx.x; c < p.width; c += kScalarThreads) p.codes[r * p.width + c] = code_of(row[c], sc, p.quant);
 }
 
+// Eight channels as they lie in memory.
+template <typename T>
+struct Raw {
+  uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p) {
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+  return r;
+}
+__device__ __forceinline__ void unpack(const Raw<float>& r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f[4 * i] = __uint_as_float(r.w[i].x);
+    f[4 * i + 1] = __uint_as_float(r.w[i].y);
+    f[4 * i + 2] = __uint_as_float(r.w[i].z);
+    f[4 * i + 3] = __uint_as_float(r.w[i].w);
+  }
+}
+__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16>& r, float (&f)[8]) { unpack_bf16x8(r.w[0], f); }
+__device__ __forceinline__ void unpack(const Raw<__half>& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(round_bf16x2(f[0], f[1]), round_bf16x2(f[2], f[3]), round_bf16x2(f[4], f[5]),
+                                            round_bf16x2(f[6], f[7]));
+}
+__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Vector form: 16-byte aligned rows of a multiple of 8 channels. One block a
+// row, each thread kChunks pieces of 8 channels in registers; both inputs are
+// requested before anything waits for them.
+constexpr int kVecThreads = 512;
+
+template <typename T, int kChunks>
+__global__ void __launch_bounds__(kVecThreads) sandwich_norm_vec_kernel(const Params p) {
+  __shared__ float red[5][kVecThreads / 32];
+  const int64_t r = blockIdx.x, b = r / p.seq, s = r - b * p.seq;
+  const T* y = static_cast<const T*>(p.y) + b * p.yb + s * p.ys;
+  const T* x = static_cast<const T*>(p.x) + b * p.xb + s * p.xs;
+  const int chunks = p.width >> 3, warps = blockDim.x >> 5;
+  auto at = [&](int j) { return static_cast<int>(threadIdx.x) + j * static_cast<int>(blockDim.x); };
+  Raw<T> yr[kChunks], xr[kChunks];
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j)
+    if (at(j) < chunks) {
+      yr[j] = load_raw(y + at(j) * 8);
+      xr[j] = load_raw(x + at(j) * 8);
+    }
+  int64_t t = 0;
+  bool known = true;
+  if (p.idx) {
+    t = __ldg(p.idx + b * p.idx_batch + s);
+    known = t >= 0 && t < p.table_rows;
+    if (!known) t = 0;
+  }
+  // every reduction has its own slots, so one barrier each is enough
+  auto sum = [&](float v, int slot) {
+    v = warp_sum(v);
+    if (warps == 1) return v;
+    if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = 0.f;
+    for (int i = 0; i < warps; ++i) v += red[slot][i];
+    return v;
+  };
+  float v[kChunks][8];
+  auto stats = [&](int kind, int slot, float& mean, float& rstd) {
+    mean = 0.f;
+    rstd = 1.f;
+    if (kind == kNone) return;
+    if (kind == kLayer) {
+      float acc = 0.f;
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+        if (at(j) < chunks)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc += v[j][e];
+      mean = sum(acc, slot) / p.width;
+    }
+    float acc = 0.f;
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+      if (at(j) < chunks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float d = v[j][e] - mean;
+          acc = fmaf(d, d, acc);
+        }
+    rstd = rsqrtf(sum(acc, slot + 1) / p.width + p.eps);
+  };
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j)
+    if (at(j) < chunks) unpack(yr[j], v[j]);
+  float mean, rstd;
+  stats(p.post, 0, mean, rstd);
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    if (at(j) >= chunks) continue;
+    const int c = at(j) * 8;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[j][e] = (v[j][e] - mean) * rstd;
+    if (p.post_weight) {
+      unpack(load_raw(static_cast<const T*>(p.post_weight) + c), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] *= f[e];
+    }
+    if (p.gate) {
+      unpack(load_raw(static_cast<const T*>(p.gate) + t * p.ldg + c), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] *= known ? f[e] : CUDART_NAN_F;
+    }
+    unpack(xr[j], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[j][e] = fmaf(p.residual_scale, v[j][e], f[e]);
+    store8(static_cast<T*>(p.x_out) + r * p.width + c, v[j]);
+  }
+  if (!p.h_out && !p.codes) return;
+  stats(p.pre, 2, mean, rstd);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    if (at(j) >= chunks) continue;
+    const int c = at(j) * 8;
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[j][e] = (v[j][e] - mean) * rstd;
+    if (p.pre_weight) {
+      unpack(load_raw(static_cast<const T*>(p.pre_weight) + c), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] *= f[e];
+    }
+    if (p.scale) {
+      float g[8];
+      unpack(load_raw(static_cast<const T*>(p.scale) + t * p.lds + c), f);
+      unpack(load_raw(static_cast<const T*>(p.shift) + t * p.ldsh + c), g);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], 1.0f + (known ? f[e] : CUDART_NAN_F), g[e]);
+    }
+    if (p.h_out) store8(static_cast<T*>(p.h_out) + r * p.width + c, v[j]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
+  }
+  if (!p.codes) return;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (warps > 1) {
+    if ((threadIdx.x & 31) == 0) red[4][threadIdx.x >> 5] = __uint_as_float(top);
+    __syncthreads();
+    for (int i = 0; i < warps; ++i) top = max(top, __float_as_uint(red[4][i]));
+  }
+  const float sc = code_scale_of(__uint_as_float(top), p.quant);
+  const float inv = __frcp_rn(sc);
+  if (threadIdx.x == 0) p.code_scale[r] = sc;
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    if (at(j) >= chunks) continue;
+    uint32_t q[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float d = div_by(v[j][e], sc, inv);
+      q[e] = p.quant == kInt8 ? static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(d, -127.f), 127.f))) & 0xFFu
+                              : f32_to_e4m3(fminf(fmaxf(d, -448.f), 448.f));
+    }
+    *reinterpret_cast<uint2*>(p.codes + r * p.width + at(j) * 8) =
+        make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+  }
+}
+
 template <typename T>
 int launch(const Params& p, int64_t rows, cudaStream_t st) {
+  const auto whole = [](const void* q, int64_t strides) {  // 16-byte pieces
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && strides * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+  };
+  if (p.width % 8 == 0 && whole(p.y, p.yb | p.ys) && whole(p.x, p.xb | p.xs) && whole(p.post_weight, 0) &&
+      whole(p.pre_weight, 0) && whole(p.gate, p.ldg) && whole(p.scale, p.lds) && whole(p.shift, p.ldsh) &&
+      whole(p.x_out, 0) && whole(p.h_out, 0) && whole(p.codes, 0)) {
+    // Pieces of a thread: the count that leaves the fewest lanes idle, the
+    // larger of equals (more bytes requested by a thread, fewer warps to join).
+    const int chunks = p.width / 8;
+    int best = 4, lanes = 1 << 30;
+    for (int k = 4; k >= 1; --k) {
+      const int threads = static_cast<int>(cdiv(cdiv(chunks, k), 32) * 32);
+      if (threads <= kVecThreads && threads * k < lanes) {
+        best = k;
+        lanes = threads * k;
+      }
+    }
+    const unsigned threads = static_cast<unsigned>(lanes / best), grid = static_cast<unsigned>(rows);
+    switch (best) {
+      case 1: sandwich_norm_vec_kernel<T, 1><<<grid, threads, 0, st>>>(p); break;
+      case 2: sandwich_norm_vec_kernel<T, 2><<<grid, threads, 0, st>>>(p); break;
+      case 3: sandwich_norm_vec_kernel<T, 3><<<grid, threads, 0, st>>>(p); break;
+      default: sandwich_norm_vec_kernel<T, 4><<<grid, threads, 0, st>>>(p); break;
+    }
+    return launch_status();
+  }
   auto kernel = sandwich_norm_scalar_kernel<T>;
   const size_t smem = static_cast<size_t>(p.width) * sizeof(float);
   if (smem > 40 * 1024 &&
