@@ -332,14 +332,18 @@ int xgb_int8_gemm(const int8_t* a, const int8_t* w, int64_t M, int64_t N, int64_
  * elements, multiples of 8; 0 where the batch or the heads are broadcast),
  * heads a multiple of kv_heads. kv_lens (device, [batch], may be NULL): keys
  * that each sample has, clamped to [0, seq_kv]; what lies behind them has no
- * influence, NaN included, and a sample without keys gives zeros. workspace:
- * xgb_cross_attention_workspace() bytes (0 for most sizes), 16-byte aligned,
- * its contents need no initialisation. */
-int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim);
+ * influence, NaN included, and a sample without keys gives zeros. mask (device
+ * bytes [batch, seq_kv], may be NULL): 0 leaves a key out as well; taken where
+ * xgb_cross_attention_takes_mask() says so (few query rows), elsewhere
+ * xgb_pack_keys comes before. workspace: xgb_cross_attention_workspace() bytes
+ * (0 for most sizes), 16-byte aligned, its contents need no initialisation. */
+int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv,
+                                      int64_t head_dim);
+int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int64_t seq_q);
 int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                         const void* v, const int64_t* v_strides, int dtype, int64_t batch, int64_t heads,
                         int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int* kv_lens,
-                        float sm_scale, void* out, const int64_t* out_strides, void* workspace,
+                        const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, float sm_scale, void* out, const int64_t* out_strides, void* workspace,
                         int64_t workspace_bytes, int* error_flag, void* stream);
 
 /* The keys and values that `mask` (bytes [batch, seq], 0 = left out) keeps, in

@@ -88,8 +88,8 @@ def test_cross_attention_arguments():
     h, i64, _ = lib()
     qs, ks = i64([4 * 64 * 2, 64, 2 * 64, 1]), i64([8 * 64 * 2, 64, 2 * 64, 1])
 
-    def call(q=D, qst=qs, kst=ks, dtype=0, b=2, heads=2, kvh=2, sq=4, skv=8, d=64, scale=0.1, ost=qs, ws=None, wsb=0):
-        return h.xgb_cross_attention(q, qst, D, kst, D, ks, dtype, b, heads, kvh, sq, skv, d, None, F(scale), D, ost, ws, wsb, None,
+    def call(q=D, qst=qs, kst=ks, dtype=0, b=2, heads=2, kvh=2, sq=4, skv=8, d=64, scale=0.1, ost=qs, ws=None, wsb=0, mask=None):
+        return h.xgb_cross_attention(q, qst, D, kst, D, ks, dtype, b, heads, kvh, sq, skv, d, None, mask, 0, 1, F(scale), D, ost, ws, wsb, None,
                                      None)
 
     assert call(q=None) == -1 and call(dtype=2) == -1 and call(scale=0.0) == -1 and call(scale=float("nan")) == -1
@@ -97,10 +97,11 @@ def test_cross_attention_arguments():
     assert call(qst=i64([512, 64, 128, 2])) == -3 and call(qst=i64([512, 64, 132, 1])) == -3
     assert call(kst=i64([1024, 64, 0, 1])) == -3 and call(ost=i64([0, 64, 128, 1])) == -3 and call(qst=i64([512, 64, -128, 1])) == -3
     assert call(q=ODD) == -4
-    need = h.xgb_cross_attention_workspace(1, 2, 1, 4096, 64)  # few rows, many keys: split
+    assert call(sq=33, mask=D) == -2 and h.xgb_cross_attention_takes_mask(2, 2, 32) and not h.xgb_cross_attention_takes_mask(4, 2, 17)
+    need = h.xgb_cross_attention_workspace(1, 2, 2, 1, 4096, 64)  # few rows, many keys: split
     assert need > 0
     assert call(b=1, sq=1, skv=4096) == -7 and call(b=1, sq=1, skv=4096, ws=D, wsb=need - 1) == -7
-    assert h.xgb_cross_attention_workspace(1, 2, 1, 64, 64) == 0 and h.xgb_cross_attention_workspace(4, 24, 4096, 512, 64) == 0
+    assert h.xgb_cross_attention_workspace(1, 2, 2, 1, 64, 64) == 0 and h.xgb_cross_attention_workspace(4, 24, 24, 4096, 512, 64) == 0
     assert h.xgb_pack_keys(None, 0, 1, D, ks, D, ks, 1, 2, 8, 64, D, D, D, None) == -1
     assert h.xgb_pack_keys(D, 0, 1, D, ks, D, ks, 1, 2, 8, 96, D, D, D, None) == -2
     assert h.xgb_pack_keys(D, 0, 1, D, i64([1024, 64, 12, 1]), D, ks, 1, 2, 8, 64, D, D, D, None) == -3

@@ -95,10 +95,11 @@ SIGNATURES = {
     "xgb_int8_quantize_per_token": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "xgb_int8_gemm": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_int, c_vp, c_i64,
                               c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
-    "xgb_cross_attention_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "xgb_cross_attention_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "xgb_cross_attention_takes_mask": (c_int, [c_i64, c_i64, c_i64]),
     "xgb_cross_attention": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_int, c_i64, c_i64, c_i64,
-                                    c_i64, c_i64, c_i64, c_vp, c_float, c_vp, c_i64p, c_vp, c_i64, c_vp,
-                                    c_vp]),
+                                    c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_float, c_vp,
+                                    c_i64p, c_vp, c_i64, c_vp, c_vp]),
     "xgb_pack_keys": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64p, c_vp, c_i64p, c_i64, c_i64, c_i64, c_i64,
                               c_vp, c_vp, c_vp, c_vp]),
     "xgb_attention_bf16": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_i64, c_i64, c_i64,

@@ -271,20 +271,21 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     with _on_device_of(query):
         if kv_lens is not None and kv_lens.dtype != torch.int32:
             kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
-        if key_mask is not None:
+        if key_mask is not None and not _lib.lib().xgb_cross_attention_takes_mask(h, hk, sq):
             kv_lens = torch.empty((b,), dtype=torch.int32, device=key.device)
             packed = torch.empty((2, b, hk, skv, d), dtype=key.dtype, device=key.device)
             call("xgb_pack_keys", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), key.data_ptr(), _steps(key),
                  value.data_ptr(), _steps(value), b, hk, skv, d, packed[0].data_ptr(), packed[1].data_ptr(),
                  kv_lens.data_ptr(), _stream(query))
-            key, value = packed[0], packed[1]
+            key, value, key_mask = packed[0], packed[1], None
         elif kv_lens is not None:
             kv_lens = kv_lens.contiguous()
-        ws_bytes = _lib.lib().xgb_cross_attention_workspace(b, h, sq, skv, d)
+        ws_bytes = _lib.lib().xgb_cross_attention_workspace(b, h, hk, sq, skv, d)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
         call("xgb_cross_attention", query.data_ptr(), _steps(query), key.data_ptr(), _steps(key), value.data_ptr(),
              _steps(value), _DTYPE_CODE[query.dtype], b, h, hk, sq, skv, d,
-             kv_lens.data_ptr() if kv_lens is not None else None, sm_scale, out.data_ptr(), _steps(out),
+             kv_lens.data_ptr() if kv_lens is not None else None,
+             *((key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1)) if key_mask is not None else (None, 0, 0)), sm_scale, out.data_ptr(), _steps(out),
              ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(query.device), _stream(query))
     return out
 

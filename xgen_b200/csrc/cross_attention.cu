@@ -462,17 +462,207 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- few query rows
+// One token, or a few, for each sample: the query rows of one key head (its
+// H/H' query heads times Sq) fit a tile of 8, a 128-row tensor-core tile would
+// be empty, and the time is that of reading K and V once. Warps take 16 keys
+// at a time straight from global memory into the fragments of the warp-level
+// 16x8x16 products, with no shared memory on the way:
+//   S^T [16 keys x 8 rows] = K Q^T: a lane loads 16-byte pieces of the rows of
+//     keys g and g + 8 (g = lane / 4); the products' inner index is any order
+//     of d as long as Q's is the same one, so the pieces are the fragments.
+//   O^T [D x 8 rows] += V^T P^T: the same pieces of V, transposed 8 x 8 by
+//     movmatrix; the order of d that comes out is undone when O is written.
+// Each warp keeps its own running maximum and O; the warps of a CTA join in
+// shared memory, the CTAs of a unit (parts of its keys) in the second kernel.
+// Keys that are not there are not loaded: zeros, with scores of -inf.
+constexpr int kFewRows = 8;
+constexpr int kFewWarps = 4;
+constexpr int kFewKeys = 16;  // keys of a warp's step
+
+struct FewParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t qsb, qsh, qss, ksb, ksh, kss, vsb, vsh, vss;
+  const uint8_t* mask;  // [batch, seq_kv] bytes, null: none
+  int64_t msb, mss;
+  int kv_heads, tiles;  // row tiles of 8 of a key head
+};
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Transpose of an 8 x 8 tile of 16-bit values spread over the warp.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// The 16-byte pieces 8c.. of every 32 channels of one row.
+template <int kChunks>
+__device__ __forceinline__ void load_row(const void* base, int64_t at, bool go, uint4 (&r)[kChunks]) {
+  const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at);
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) r[j] = go ? __ldg(src + 4 * j) : make_uint4(0, 0, 0, 0);
+}
+
+template <typename T, int kD>
+__global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params p, const FewParams f) {
+  constexpr int kChunks = kD / 32;
+  __shared__ float so[kFewWarps][kFewRows][kD];
+  __shared__ float2 sml[kFewWarps][kFewRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int64_t unit = blockIdx.x / p.splits;  // (batch, key head, row tile)
+  const int part = static_cast<int>(blockIdx.x - unit * p.splits);
+  const int64_t bh = unit / f.tiles;
+  const int first_row = static_cast<int>(unit - bh * f.tiles) * kFewRows;
+  const int b = static_cast<int>(bh / f.kv_heads), hk = static_cast<int>(bh - static_cast<int64_t>(b) * f.kv_heads);
+  const int rows = p.group * p.seq_q;
+  const int len = p.lens ? min(max(__ldg(p.lens + b), 0), p.seq_kv) : p.seq_kv;
+  const int steps_all = (len + kFewKeys - 1) / kFewKeys;
+  const int per = (steps_all + p.splits - 1) / p.splits;
+  const int step0 = min(part * per, steps_all), step1 = min(step0 + per, steps_all);
+
+  // query row g of the tile, as the second operand of S^T
+  uint4 q[kChunks];
+  {
+    const int r = first_row + g;
+    const int h = hk * p.group + r / p.seq_q, s = r % p.seq_q;
+    load_row<kChunks>(f.q, b * f.qsb + h * f.qsh + s * f.qss + 8 * c, r < rows, q);
+  }
+  const int64_t kbase = b * f.ksb + hk * f.ksh + 8 * c, vbase = b * f.vsb + hk * f.vsh + 8 * c;
+  auto there = [&](int key) { return key < len && (!f.mask || __ldg(f.mask + b * f.msb + key * f.mss) != 0); };
+
+  float o[2 * kChunks][4] = {};
+  float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};  // rows 2c, 2c + 1
+  uint4 k0[kChunks], k1[kChunks], v0[kChunks], v1[kChunks];
+  int step = step0 + warp;
+  bool go0 = false, go1 = false;
+  if (step < step1) {
+    go0 = there(step * kFewKeys + g);
+    go1 = there(step * kFewKeys + g + 8);
+    load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(step) * kFewKeys + g) * f.kss, go0, k0);
+    load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(step) * kFewKeys + g + 8) * f.kss, go1, k1);
+  }
+  for (; step < step1; step += kFewWarps) {
+    const int64_t key = static_cast<int64_t>(step) * kFewKeys + g;
+    load_row<kChunks>(f.v, vbase + key * f.vss, go0, v0);
+    load_row<kChunks>(f.v, vbase + (key + 8) * f.vss, go1, v1);
+    float st[4] = {0.f, 0.f, 0.f, 0.f};  // keys g (0, 1) and g + 8 (2, 3), rows 2c, 2c + 1
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      mma16816<T>(st, k0[j].x, k1[j].x, k0[j].y, k1[j].y, q[j].x, q[j].y);
+      mma16816<T>(st, k0[j].z, k1[j].z, k0[j].w, k1[j].w, q[j].z, q[j].w);
+    }
+    const bool was0 = go0, was1 = go1;
+    const int next = step + kFewWarps;
+    if (next < step1) {
+      go0 = there(next * kFewKeys + g);
+      go1 = there(next * kFewKeys + g + 8);
+      load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(next) * kFewKeys + g) * f.kss, go0, k0);
+      load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(next) * kFewKeys + g + 8) * f.kss, go1, k1);
+    }
+    float pr[4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float a = was0 ? st[e] * p.scale_log2 : kNegInf, d = was1 ? st[e + 2] * p.scale_log2 : kNegInf;
+      float top = fmaxf(a, d);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+      const float m_new = fmaxf(m[e], top);
+      const float base = m_new == kNegInf ? 0.f : m_new;
+      const float alpha = ex2_approx(m[e] - base);
+      m[e] = m_new;
+      pr[e] = ex2_approx(a - base);
+      pr[e + 2] = ex2_approx(d - base);
+      l[e] = fmaf(l[e], alpha, pr[e] + pr[e + 2]);
+#pragma unroll
+      for (int n = 0; n < 2 * kChunks; ++n) {
+        o[n][e] *= alpha;
+        o[n][e + 2] *= alpha;
+      }
+    }
+    // P^T: keys (2c, 2c + 1) of row g, for the two halves of the 16 keys
+    const uint32_t p0 = transpose8x8(pack2<T>(pr[0], pr[1])), p1 = transpose8x8(pack2<T>(pr[2], pr[3]));
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+      mma16816<T>(o[2 * j], transpose8x8(v0[j].x), transpose8x8(v0[j].y), transpose8x8(v1[j].x), transpose8x8(v1[j].y), p0, p1);
+      mma16816<T>(o[2 * j + 1], transpose8x8(v0[j].z), transpose8x8(v0[j].w), transpose8x8(v1[j].z), transpose8x8(v1[j].w), p0,
+                  p1);
+    }
+  }
+  // l over the keys of the warp
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+    for (int x = 4; x <= 16; x <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], x);
+    if (g == 0) sml[warp][2 * c + e] = make_float2(m[e], l[e]);
+  }
+  // o[2j + u]: channels 32 j + 8 (g / 2) + g % 2 + 4 u (values 0, 1) and + 2 (values 2, 3)
+#pragma unroll
+  for (int n = 0; n < 2 * kChunks; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      so[warp][2 * c + (e & 1)][32 * (n >> 1) + 8 * (g >> 1) + (g & 1) + 4 * (n & 1) + 2 * (e >> 1)] = o[n][e];
+  __syncthreads();
+  for (int at = threadIdx.x; at < kFewRows * kD; at += kFewWarps * 32) {
+    const int r = at / kD, d = at % kD, row = first_row + r;
+    if (row >= rows) break;
+    float mx = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) mx = fmaxf(mx, sml[w][r].x);
+    const float base = mx == kNegInf ? 0.f : mx;
+    float lsum = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      const float wt = ex2_approx(sml[w][r].x - base);
+      lsum = fmaf(wt, sml[w][r].y, lsum);
+      sum = fmaf(wt, so[w][r][d], sum);
+    }
+    if (p.splits > 1) {
+      const int64_t slot = (unit * p.splits + part) * kFewRows + r;
+      p.part_o[slot * kD + d] = sum;
+      if (d == 0) p.part_ml[slot] = make_float2(mx, lsum);
+    } else {
+      const int h = hk * p.group + row / p.seq_q, s = row % p.seq_q;
+      const float v = lsum != 0.f ? sum / lsum : 0.f;
+      T* dst = static_cast<T*>(p.out) + b * p.osb + h * p.osh + s * p.oss + d;
+      if constexpr (std::is_same<T, __half>::value) *dst = __float2half_rn(v);
+      else *dst = __float2bfloat16_rn(v);
+    }
+  }
+}
+
 // Joins the parts of a row: M = max m, o = sum 2^(m - M) O / sum 2^(m - M) l.
 // One warp a row; a part without keys (l = 0) left no O.
 template <typename T, int kD>
-__global__ void __launch_bounds__(256) join_kernel(const Params p, int64_t rows) {
+__global__ void __launch_bounds__(256) join_kernel(const Params p, int64_t rows, int few_tiles) {
   const int lane = threadIdx.x & 31;
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (batch, head, row)
   if (at >= rows) return;
   const int64_t bh = at / p.seq_q;
   const int row = static_cast<int>(at - bh * p.seq_q);
-  const int64_t item = bh * p.n_qt + row / kRows;
-  const int r = row % kRows;
+  const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<int64_t>(b) * p.heads);
+  int64_t item = bh * p.n_qt + row / kRows;
+  int r = row % kRows;
+  if (few_tiles) {  // rows of a key head in tiles of 8
+    const int in_head = h % p.group * p.seq_q + row;
+    item = (static_cast<int64_t>(b) * (p.heads / p.group) + h / p.group) * few_tiles + in_head / kFewRows;
+    r = in_head % kFewRows;
+  }
   const int64_t first = item * p.splits * p.part_rows + r;
   float mx = kNegInf;
   for (int q = 0; q < p.splits; ++q) mx = fmaxf(mx, __ldg(&p.part_ml[first + static_cast<int64_t>(q) * p.part_rows]).x);
@@ -488,7 +678,6 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int64_t rows)
     for (int c = 0; c < kD / 32; ++c) o[c] = fmaf(w, __ldg(p.part_o + at_q * kD + c * 32 + lane), o[c]);
   }
   const float inv_l = l != 0.f ? 1.0f / l : 0.f;
-  const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<int64_t>(b) * p.heads);
   T* dst = static_cast<T*>(p.out) + b * p.osb + h * p.osh + row * p.oss;
 #pragma unroll
   for (int c = 0; c < kD / 32; ++c) {
@@ -504,11 +693,35 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
-// Parts of a unit's keys: 1 unless whole units would leave more than half of
-// the SMs without work, then as many as fill them, each at least one tile.
-int parts(int64_t items, int64_t seq_kv, int sms) {
-  if (items * 2 > sms) return 1;
-  return static_cast<int>(std::min<int64_t>(sms / std::max<int64_t>(items, 1), cdiv(seq_kv, kBN)));
+// How a call is laid out: the few-row form for up to kFewMost query rows of a
+// key head, and the parts of a unit's keys.
+constexpr int64_t kFewMost = 32;
+struct Plan {
+  bool few;
+  int tiles;  // few: row tiles of a key head
+  int64_t items;
+  int splits;
+  int64_t part_rows;
+};
+inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int sms) {
+  Plan n{};
+  const int64_t rows = heads / kv_heads * seq_q;
+  n.few = rows <= kFewMost;
+  if (n.few) {
+    n.tiles = static_cast<int>(cdiv(rows, kFewRows));
+    n.items = batch * kv_heads * n.tiles;
+    // three CTAs an SM, each at least one step for each of its warps
+    n.splits = static_cast<int>(std::max<int64_t>(
+        1, std::min<int64_t>(3 * sms / n.items, cdiv(seq_kv, kFewKeys * kFewWarps))));
+    n.part_rows = kFewRows;
+    return n;
+  }
+  n.items = batch * heads * cdiv(seq_q, kRows);
+  n.splits = 1;
+  // parts only where whole units would leave more than half of the SMs idle
+  if (n.items * 2 <= sms) n.splits = static_cast<int>(std::min<int64_t>(sms / n.items, cdiv(seq_kv, kBN)));
+  n.part_rows = std::min<int64_t>(seq_q, kRows);
+  return n;
 }
 
 template <typename T, int kD>
@@ -523,7 +736,19 @@ int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, 
   const int rc = launch_status();
   if (rc || p.splits == 1) return rc;
   const int64_t rows = batch * p.heads * p.seq_q;
-  join_kernel<T, kD><<<static_cast<unsigned>(cdiv(rows, 8)), 256, 0, st>>>(p, rows);
+  join_kernel<T, kD><<<static_cast<unsigned>(cdiv(rows, 8)), 256, 0, st>>>(p, rows, 0);
+  return launch_status();
+}
+
+template <typename T, int kD>
+int launch_few(const Params& p, const FewParams& f, int64_t items, int64_t batch, cudaStream_t st) {
+  const int64_t grid = items * p.splits;
+  if (grid > INT32_MAX) return XGB_ERR_SHAPE;
+  cross_few_kernel<T, kD><<<static_cast<unsigned>(grid), kFewWarps * 32, 0, st>>>(p, f);
+  const int rc = launch_status();
+  if (rc || p.splits == 1) return rc;
+  const int64_t rows = batch * p.heads * p.seq_q;
+  join_kernel<T, kD><<<static_cast<unsigned>(cdiv(rows, 8)), 256, 0, st>>>(p, rows, f.tiles);
   return launch_status();
 }
 
@@ -602,18 +827,22 @@ XGB_API int xgb_pack_keys(const uint8_t* mask, int64_t mask_batch_stride, int64_
   return launch_status();
 }
 
-XGB_API int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim) {
-  if (batch <= 0 || heads <= 0 || seq_q <= 0 || seq_kv <= 0) return 0;
-  const int64_t items = batch * heads * cdiv(seq_q, cross::kRows);
-  const int splits = cross::parts(items, seq_kv, cross::sm_count());
-  if (splits <= 1) return 0;
-  return items * splits * std::min<int64_t>(seq_q, cross::kRows) * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+XGB_API int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv,
+                                              int64_t head_dim) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq_q <= 0 || seq_kv <= 0) return 0;
+  const cross::Plan n = cross::plan(batch, heads, kv_heads, seq_q, seq_kv, cross::sm_count());
+  if (n.splits <= 1) return 0;
+  return n.items * n.splits * n.part_rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+XGB_API int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int64_t seq_q) {
+  return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads * seq_q <= cross::kFewMost;
 }
 
 XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                 const void* v, const int64_t* v_strides, int dtype, int64_t batch, int64_t heads,
                                 int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int* kv_lens,
-                                float sm_scale, void* out, const int64_t* out_strides, void* workspace,
+                                const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, float sm_scale, void* out, const int64_t* out_strides, void* workspace,
                                 int64_t workspace_bytes, int* error_flag, void* stream) {
   if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides || !out_strides) return XGB_ERR_ARG;
   if (dtype != XGB_BF16 && dtype != XGB_F16) return XGB_ERR_ARG;
@@ -622,17 +851,20 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
     return XGB_ERR_SHAPE;
   if (!(sm_scale > 0.f)) return XGB_ERR_ARG;
   const int64_t* all[4] = {q_strides, k_strides, v_strides, out_strides};
-  for (int n = 0; n < 4; ++n) {
-    const int64_t extent[3] = {batch, n == 1 || n == 2 ? kv_heads : heads, n == 1 || n == 2 ? seq_kv : seq_q};
-    if (all[n][3] != 1) return XGB_ERR_STRIDE;
+  for (int t = 0; t < 4; ++t) {
+    const int64_t extent[3] = {batch, t == 1 || t == 2 ? kv_heads : heads, t == 1 || t == 2 ? seq_kv : seq_q};
+    if (all[t][3] != 1) return XGB_ERR_STRIDE;
     for (int d = 0; d < 3; ++d) {
       if (extent[d] == 1) continue;  // never stepped over
       // inputs may be broadcast over the batch and the heads
-      if (all[n][d] % 8 || all[n][d] < 0 || (all[n][d] == 0 && (n == 3 || d == 2))) return XGB_ERR_STRIDE;
+      if (all[t][d] % 8 || all[t][d] < 0 || (all[t][d] == 0 && (t == 3 || d == 2))) return XGB_ERR_STRIDE;
     }
   }
   if (!cross::aligned16(q) || !cross::aligned16(k) || !cross::aligned16(v) || !cross::aligned16(out)) return XGB_ERR_ALIGN;
-  const int64_t need = xgb_cross_attention_workspace(batch, heads, seq_q, seq_kv, head_dim);
+  if (mask && !xgb_cross_attention_takes_mask(heads, kv_heads, seq_q)) return XGB_ERR_SHAPE;
+  const int sms = cross::sm_count();
+  const cross::Plan n = cross::plan(batch, heads, kv_heads, seq_q, seq_kv, sms);
+  const int64_t need = xgb_cross_attention_workspace(batch, heads, kv_heads, seq_q, seq_kv, head_dim);
   if (need && (!workspace || workspace_bytes < need)) return XGB_ERR_WORKSPACE;
   if (need && !cross::aligned16(workspace)) return XGB_ERR_ALIGN;
   int dev = 0, major = 0;
@@ -640,34 +872,6 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
       cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10)
     return XGB_ERR_DEVICE;
   cross::Params p{};
-  CUtensorMap map[3];
-  const void* base[3] = {q, k, v};
-  int factor[3][2];  // batch, head
-  for (int n = 0; n < 3; ++n) {
-    const int64_t* s = all[n];
-    const int64_t seq = n == 0 ? seq_q : seq_kv, hh = n == 0 ? heads : kv_heads;
-    // a dimension of one entry, or a broadcast one, is one entry of the map
-    const int64_t ext[3] = {seq, hh > 1 && s[1] ? hh : 1, batch > 1 && s[0] ? batch : 1};
-    factor[n][0] = ext[2] > 1;
-    factor[n][1] = ext[1] > 1;
-    const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(ext[0]), static_cast<uint64_t>(ext[1]),
-                              static_cast<uint64_t>(ext[2])};
-    const uint64_t row = static_cast<uint64_t>(head_dim) * 2;
-    const uint64_t strides[3] = {ext[0] > 1 ? static_cast<uint64_t>(s[2]) * 2 : row,
-                                 ext[1] > 1 ? static_cast<uint64_t>(s[1]) * 2 : row,
-                                 ext[2] > 1 ? static_cast<uint64_t>(s[0]) * 2 : row};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(n == 0 ? cross::kBM : cross::kBN), 1, 1};
-    if (!make_tensor_map(&map[n], dtype == XGB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                         base[n], dims, strides, box))
-      return XGB_ERR_ALIGN;
-  }
-  p.qb = factor[0][0];
-  p.qh = factor[0][1];
-  p.kb = factor[1][0];
-  p.kh = factor[1][1];
-  p.vb = factor[2][0];
-  p.vh = factor[2][1];
-  const int sms = cross::sm_count();
   p.heads = static_cast<int>(heads);
   p.group = static_cast<int>(heads / kv_heads);
   p.seq_q = static_cast<int>(seq_q);
@@ -679,17 +883,69 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
   p.osh = out_strides[1];
   p.oss = out_strides[2];
   p.n_qt = static_cast<int>(cdiv(seq_q, cross::kRows));
-  const int64_t items = batch * heads * p.n_qt;
-  p.splits = cross::parts(items, seq_kv, sms);
-  p.units = items * p.splits;
-  p.part_rows = static_cast<int>(std::min<int64_t>(seq_q, cross::kRows));
+  p.splits = n.splits;
+  p.units = n.items * n.splits;
+  p.part_rows = static_cast<int>(n.part_rows);
   if (p.splits > 1) {
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + p.units * p.part_rows * head_dim);
   }
   p.err = error_flag;
   cudaStream_t st = as_stream(stream);
-  if (dtype == XGB_BF16)
+  const bool bf16 = dtype == XGB_BF16;
+  if (n.few) {
+    cross::FewParams f{};
+    f.q = q;
+    f.k = k;
+    f.v = v;
+    f.qsb = q_strides[0];
+    f.qsh = q_strides[1];
+    f.qss = q_strides[2];
+    f.ksb = k_strides[0];
+    f.ksh = k_strides[1];
+    f.kss = k_strides[2];
+    f.vsb = v_strides[0];
+    f.vsh = v_strides[1];
+    f.vss = v_strides[2];
+    f.mask = mask;
+    f.msb = mask_batch_stride;
+    f.mss = mask_stride;
+    f.kv_heads = static_cast<int>(kv_heads);
+    f.tiles = n.tiles;
+    if (bf16)
+      return head_dim == 128 ? cross::launch_few<__nv_bfloat16, 128>(p, f, n.items, batch, st)
+                             : cross::launch_few<__nv_bfloat16, 64>(p, f, n.items, batch, st);
+    return head_dim == 128 ? cross::launch_few<__half, 128>(p, f, n.items, batch, st)
+                           : cross::launch_few<__half, 64>(p, f, n.items, batch, st);
+  }
+  CUtensorMap map[3];
+  const void* base[3] = {q, k, v};
+  int factor[3][2];  // batch, head
+  for (int t = 0; t < 3; ++t) {
+    const int64_t* s = all[t];
+    const int64_t seq = t == 0 ? seq_q : seq_kv, hh = t == 0 ? heads : kv_heads;
+    // a dimension of one entry, or a broadcast one, is one entry of the map
+    const int64_t ext[3] = {seq, hh > 1 && s[1] ? hh : 1, batch > 1 && s[0] ? batch : 1};
+    factor[t][0] = ext[2] > 1;
+    factor[t][1] = ext[1] > 1;
+    const uint64_t dims[4] = {static_cast<uint64_t>(head_dim), static_cast<uint64_t>(ext[0]), static_cast<uint64_t>(ext[1]),
+                              static_cast<uint64_t>(ext[2])};
+    const uint64_t row = static_cast<uint64_t>(head_dim) * 2;
+    const uint64_t strides[3] = {ext[0] > 1 ? static_cast<uint64_t>(s[2]) * 2 : row,
+                                 ext[1] > 1 ? static_cast<uint64_t>(s[1]) * 2 : row,
+                                 ext[2] > 1 ? static_cast<uint64_t>(s[0]) * 2 : row};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(t == 0 ? cross::kBM : cross::kBN), 1, 1};
+    if (!make_tensor_map(&map[t], bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                         base[t], dims, strides, box))
+      return XGB_ERR_ALIGN;
+  }
+  p.qb = factor[0][0];
+  p.qh = factor[0][1];
+  p.kb = factor[1][0];
+  p.kh = factor[1][1];
+  p.vb = factor[2][0];
+  p.vh = factor[2][1];
+  if (bf16)
     return head_dim == 128 ? cross::launch<__nv_bfloat16, 128>(map[0], map[1], map[2], p, batch, sms, st)
                            : cross::launch<__nv_bfloat16, 64>(map[0], map[1], map[2], p, batch, sms, st);
   return head_dim == 128 ? cross::launch<__half, 128>(map[0], map[1], map[2], p, batch, sms, st)

@@ -358,7 +358,22 @@ int pick(int epilogue, const void* a, const void* w, const Params<T>& p, cudaStr
 // ---------------------------------------------------------------- quantiser
 // One block per row; the scale is max(amax / 127, FLT_MIN) and the codes the
 // correctly rounded quotients, rounded to the nearest even integer. A row with
-// a NaN or an infinity gets a scale that is not finite.
+// a NaN or an infinity gets a scale that is not finite. The largest magnitude
+// is the largest bit pattern without its sign, so a NaN is found too.
+__device__ __forceinline__ float scale_of(uint32_t top) {
+  const float s = __fdiv_rn(__uint_as_float(top), 127.0f);
+  return s < FLT_MIN ? FLT_MIN : s;
+}
+__device__ __forceinline__ uint32_t code_of(float v, float s, float inv) {
+  return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(div_by(v, s, inv), -127.f), 127.f))) & 0xFFu;
+}
+__device__ __forceinline__ uint2 codes8(const float (&f)[8], float s, float inv) {
+  uint32_t q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) q[e] = code_of(f[e], s, inv);
+  return make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+}
+
 constexpr int kQuantThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* __restrict__ x, int64_t ldx, int cols,
@@ -374,12 +389,71 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_int8_kernel(const T* _
   top = 0;
 #pragma unroll
   for (int i = 0; i < kQuantThreads / 32; ++i) top = max(top, red[i]);
-  float s = __fdiv_rn(__uint_as_float(top), 127.0f);
-  if (s < FLT_MIN) s = FLT_MIN;
+  const float s = scale_of(top), inv = __frcp_rn(s);
   if (threadIdx.x == 0) scales[row] = s;
   for (int c = threadIdx.x; c < cols; c += kQuantThreads)
-    out[row * cols + c] =
-        static_cast<int8_t>(__float2int_rn(fminf(fmaxf(__fdiv_rn(load_as_float(xr + c), s), -127.f), 127.f)));
+    out[row * cols + c] = static_cast<int8_t>(code_of(load_as_float(xr + c), s, inv));
+}
+
+// Rows of 16-byte pieces that fit a block's registers (kChunks a thread): one
+// read.
+constexpr int kQuantVecThreads = 512;
+template <typename T, int kChunks>
+__global__ void __launch_bounds__(kQuantVecThreads) quantize_int8_vec_kernel(const T* __restrict__ x, int64_t ldx, int cols,
+                                                                             int8_t* __restrict__ out,
+                                                                             float* __restrict__ scales) {
+  __shared__ uint32_t red[kQuantVecThreads / 32];
+  const int64_t row = blockIdx.x;
+  const uint4* xr = reinterpret_cast<const uint4*>(x + row * ldx);
+  const int chunks = cols >> 3, warps = blockDim.x >> 5;
+  uint4 raw[kChunks];
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    const int c = threadIdx.x + j * blockDim.x;
+    raw[j] = c < chunks ? __ldg(xr + c) : make_uint4(0, 0, 0, 0);
+  }
+  // both types order their magnitudes as their bits
+  uint32_t top2 = 0;
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    const uint32_t w[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top2 = __vmaxu2(top2, w[i] & 0x7FFF7FFFu);
+  }
+  uint32_t top = __reduce_max_sync(0xffffffffu, max(top2 & 0xFFFFu, top2 >> 16));
+  if (warps > 1) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+    __syncthreads();
+    for (int i = 0; i < warps; ++i) top = max(top, red[i]);
+  }
+  const uint16_t bits = static_cast<uint16_t>(top);
+  const float s = scale_of(__float_as_uint(load_as_float(reinterpret_cast<const T*>(&bits)))), inv = __frcp_rn(s);
+  if (threadIdx.x == 0) scales[row] = s;
+#pragma unroll
+  for (int j = 0; j < kChunks; ++j) {
+    const int c = threadIdx.x + j * blockDim.x;
+    if (c >= chunks) continue;
+    float f[8];
+    unpack8(static_cast<const T*>(nullptr), raw[j], f);
+    reinterpret_cast<uint2*>(out + row * cols)[c] = codes8(f, s, inv);
+  }
+}
+
+template <typename T>
+int quantize(const T* x, int64_t ldx, int64_t rows, int64_t cols, int8_t* out, float* scales, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>(rows);
+  const int n = static_cast<int>(cols);
+  if (cols % 8 == 0 && cols <= kQuantVecThreads * 8 * 4 && ldx % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 &&
+      reinterpret_cast<uintptr_t>(out) % 8 == 0) {
+    const int chunks = n / 8, k = chunks > 1024 ? 4 : chunks > 32 ? 2 : 1;
+    const unsigned threads = static_cast<unsigned>(cdiv(cdiv(chunks, k), 32) * 32);
+    if (k == 4) quantize_int8_vec_kernel<T, 4><<<grid, threads, 0, st>>>(x, ldx, n, out, scales);
+    else if (k == 2) quantize_int8_vec_kernel<T, 2><<<grid, threads, 0, st>>>(x, ldx, n, out, scales);
+    else quantize_int8_vec_kernel<T, 1><<<grid, threads, 0, st>>>(x, ldx, n, out, scales);
+  } else {
+    quantize_int8_kernel<<<grid, kQuantThreads, 0, st>>>(x, ldx, n, out, scales);
+  }
+  return launch_status();
 }
 
 }  // namespace int8
@@ -395,14 +469,9 @@ XGB_API int xgb_int8_quantize_per_token(const void* x, int dtype, int64_t rows, 
   if (rows > 1 && row_stride < cols) return XGB_ERR_STRIDE;
   if (rows == 0) return XGB_OK;
   cudaStream_t st = as_stream(stream);
-  const unsigned grid = static_cast<unsigned>(rows);
-  if (dtype == XGB_BF16)
-    int8::quantize_int8_kernel<<<grid, int8::kQuantThreads, 0, st>>>(static_cast<const __nv_bfloat16*>(x), row_stride,
-                                                                     static_cast<int>(cols), out, scales);
-  else
-    int8::quantize_int8_kernel<<<grid, int8::kQuantThreads, 0, st>>>(static_cast<const __half*>(x), row_stride,
-                                                                     static_cast<int>(cols), out, scales);
-  return launch_status();
+  return dtype == XGB_BF16
+             ? int8::quantize(static_cast<const __nv_bfloat16*>(x), row_stride, rows, cols, out, scales, st)
+             : int8::quantize(static_cast<const __half*>(x), row_stride, rows, cols, out, scales, st);
 }
 
 template <typename T>
