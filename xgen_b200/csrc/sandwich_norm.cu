@@ -167,7 +167,9 @@ __global__ void __launch_bounds__(kScalarThreads) sandwich_norm_scalar_kernel(co
   for (int c = threadIdx.x; c < p.width; c += kScalarThreads) p.codes[r * p.width + c] = code_of(row[c], sc, p.quant);
 }
 
-// Eight channels as they lie in memory.
+// Eight channels as they lie in memory, and as four pairs of 32-bit values:
+// the arithmetic below is packed (two values an instruction), because at two
+// bytes a value the instructions are as near to their limit as the bytes.
 template <typename T>
 struct Raw {
   uint4 w[sizeof(T) / 2];
@@ -179,62 +181,69 @@ __device__ __forceinline__ Raw<T> load_raw(const T* p) {
   for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
   return r;
 }
-__device__ __forceinline__ void unpack(const Raw<float>& r, float (&f)[8]) {
+__device__ __forceinline__ void unpack(const Raw<float>& r, float2 (&f)[4]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    f[4 * i] = __uint_as_float(r.w[i].x);
-    f[4 * i + 1] = __uint_as_float(r.w[i].y);
-    f[4 * i + 2] = __uint_as_float(r.w[i].z);
-    f[4 * i + 3] = __uint_as_float(r.w[i].w);
+    f[2 * i] = make_float2(__uint_as_float(r.w[i].x), __uint_as_float(r.w[i].y));
+    f[2 * i + 1] = make_float2(__uint_as_float(r.w[i].z), __uint_as_float(r.w[i].w));
   }
 }
-__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16>& r, float (&f)[8]) { unpack_bf16x8(r.w[0], f); }
-__device__ __forceinline__ void unpack(const Raw<__half>& r, float (&f)[8]) {
+__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16>& r, float2 (&f)[4]) {
   const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    f[2 * i] = v.x;
-    f[2 * i + 1] = v.y;
-  }
+  for (int i = 0; i < 4; ++i) f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
 }
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+__device__ __forceinline__ void unpack(const Raw<__half>& r, float2 (&f)[4]) {
+  const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(round_bf16x2(f[0], f[1]), round_bf16x2(f[2], f[3]), round_bf16x2(f[4], f[5]),
-                                            round_bf16x2(f[6], f[7]));
+__device__ __forceinline__ void store8(float* p, const float2 (&f)[4]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+  reinterpret_cast<float4*>(p)[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
 }
-__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float2 (&f)[4]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(round_bf16x2(f[0].x, f[0].y), round_bf16x2(f[1].x, f[1].y), round_bf16x2(f[2].x, f[2].y), round_bf16x2(f[3].x, f[3].y));
+}
+__device__ __forceinline__ void store8(__half* p, const float2 (&f)[4]) {
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    const __half2 v = __floats2half2_rn(f[i].x, f[i].y);
     w[i] = *reinterpret_cast<const uint32_t*>(&v);
   }
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// Vector form: 16-byte aligned rows of a multiple of 8 channels. One block a
-// row, each thread kChunks pieces of 8 channels in registers; both inputs are
-// requested before anything waits for them.
-constexpr int kVecThreads = 512;
+// Vector form: 16-byte aligned rows of a multiple of 8 channels. kThreads
+// threads hold a row, kChunks pieces of 8 channels each, so that its sums are
+// short and, up to 1024 channels, need no barrier. The thread count is a
+// constant because every address is then a base and an immediate: with both
+// as run-time values the addresses, index divisions and joins of the sums took
+// more instructions than the arithmetic (55 a channel at width 5120).
+template <int kThreads>
+constexpr int kRowsOf = kThreads == 32 ? 4 : 1;  // rows of a block
 
-template <typename T, int kChunks>
-__global__ void __launch_bounds__(kVecThreads) sandwich_norm_vec_kernel(const Params p) {
-  __shared__ float red[5][kVecThreads / 32];
-  const int64_t r = blockIdx.x, b = r / p.seq, s = r - b * p.seq;
-  const T* y = static_cast<const T*>(p.y) + b * p.yb + s * p.ys;
-  const T* x = static_cast<const T*>(p.x) + b * p.xb + s * p.xs;
-  const int chunks = p.width >> 3, warps = blockDim.x >> 5;
-  auto at = [&](int j) { return static_cast<int>(threadIdx.x) + j * static_cast<int>(blockDim.x); };
+template <typename T, int kThreads, int kChunks>
+__global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>) sandwich_norm_vec_kernel(const Params p, uint32_t rows,
+                                                                                         FastDiv div_seq) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ float red[5][kWarps];
+  const uint32_t r = kWarps == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (kWarps == 1 && r >= rows) return;
+  const uint32_t b = fast_div(r, div_seq), s = r - b * div_seq.d;
+  const int lane = kWarps == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int left = (p.width >> 3) - lane;  // piece j exists while j * kThreads < left
+  const T* y = static_cast<const T*>(p.y) + b * p.yb + s * p.ys + lane * 8;
+  const T* x = static_cast<const T*>(p.x) + b * p.xb + s * p.xs + lane * 8;
   Raw<T> yr[kChunks], xr[kChunks];
 #pragma unroll
   for (int j = 0; j < kChunks; ++j)
-    if (at(j) < chunks) {
-      yr[j] = load_raw(y + at(j) * 8);
-      xr[j] = load_raw(x + at(j) * 8);
+    if (j * kThreads < left) {
+      yr[j] = load_raw(y + j * kThreads * 8);
+      xr[j] = load_raw(x + j * kThreads * 8);
     }
   int64_t t = 0;
   bool known = true;
@@ -243,117 +252,182 @@ __global__ void __launch_bounds__(kVecThreads) sandwich_norm_vec_kernel(const Pa
     known = t >= 0 && t < p.table_rows;
     if (!known) t = 0;
   }
+  const T* gate = static_cast<const T*>(p.gate) + t * p.ldg + lane * 8;
+  const T* post_weight = static_cast<const T*>(p.post_weight) + lane * 8;
+  const float inv_width = 1.0f / p.width;
   // every reduction has its own slots, so one barrier each is enough
   auto sum = [&](float v, int slot) {
     v = warp_sum(v);
-    if (warps == 1) return v;
-    if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-    for (int i = 0; i < warps; ++i) v += red[slot][i];
+    if constexpr (kWarps > 1) {
+      if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = v;
+      __syncthreads();
+      v = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) v += red[slot][i];
+    }
     return v;
   };
-  float v[kChunks][8];
-  auto stats = [&](int kind, int slot, float& mean, float& rstd) {
-    mean = 0.f;
+  float2 v[kChunks][4];
+  // The norm as v * rstd + shift.
+  auto stats = [&](int kind, int slot, float& rstd, float& shift) {
     rstd = 1.f;
+    shift = 0.f;
     if (kind == kNone) return;
+    float2 acc = both(0.f);
     if (kind == kLayer) {
-      float acc = 0.f;
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
-        if (at(j) < chunks)
+        if (j * kThreads < left)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc += v[j][e];
-      mean = sum(acc, slot) / p.width;
+          for (int e = 0; e < 4; ++e) acc = __fadd2_rn(acc, v[j][e]);
+      const float mean = sum(acc.x + acc.y, slot) * inv_width;
+      const float2 minus = both(-mean);
+      acc = both(0.f);
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+        if (j * kThreads < left)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 d = __fadd2_rn(v[j][e], minus);
+            acc = __ffma2_rn(d, d, acc);
+          }
+      rstd = rsqrtf(fmaf(sum(acc.x + acc.y, slot + 1), inv_width, p.eps));
+      shift = -mean * rstd;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kChunks; ++j)
+        if (j * kThreads < left)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc = __ffma2_rn(v[j][e], v[j][e], acc);
+      rstd = rsqrtf(fmaf(sum(acc.x + acc.y, slot + 1), inv_width, p.eps));
     }
-    float acc = 0.f;
-#pragma unroll
-    for (int j = 0; j < kChunks; ++j)
-      if (at(j) < chunks)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float d = v[j][e] - mean;
-          acc = fmaf(d, d, acc);
-        }
-    rstd = rsqrtf(sum(acc, slot + 1) / p.width + p.eps);
   };
 #pragma unroll
   for (int j = 0; j < kChunks; ++j)
-    if (at(j) < chunks) unpack(yr[j], v[j]);
-  float mean, rstd;
-  stats(p.post, 0, mean, rstd);
+    if (j * kThreads < left) unpack(yr[j], v[j]);
+  float rstd, shift;
+  stats(p.post, 0, rstd, shift);
+  // a row whose index is outside the table becomes NaN through its factor
+  if (p.gate && !known) rstd = CUDART_NAN_F;
+  T* x_out = static_cast<T*>(p.x_out) + static_cast<int64_t>(r) * p.width + lane * 8;
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    if (at(j) >= chunks) continue;
-    const int c = at(j) * 8;
-    float f[8];
+    if (j * kThreads >= left) continue;
+    float2 f[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[j][e] = (v[j][e] - mean) * rstd;
+    for (int e = 0; e < 4; ++e) v[j][e] = __ffma2_rn(v[j][e], both(rstd), both(shift));
     if (p.post_weight) {
-      unpack(load_raw(static_cast<const T*>(p.post_weight) + c), f);
+      unpack(load_raw(post_weight + j * kThreads * 8), f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= f[e];
+      for (int e = 0; e < 4; ++e) v[j][e] = __fmul2_rn(v[j][e], f[e]);
     }
     if (p.gate) {
-      unpack(load_raw(static_cast<const T*>(p.gate) + t * p.ldg + c), f);
+      unpack(load_raw(gate + j * kThreads * 8), f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= known ? f[e] : CUDART_NAN_F;
+      for (int e = 0; e < 4; ++e) v[j][e] = __fmul2_rn(v[j][e], f[e]);
     }
     unpack(xr[j], f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[j][e] = fmaf(p.residual_scale, v[j][e], f[e]);
-    store8(static_cast<T*>(p.x_out) + r * p.width + c, v[j]);
+    for (int e = 0; e < 4; ++e) v[j][e] = __ffma2_rn(v[j][e], both(p.residual_scale), f[e]);
+    store8(x_out + j * kThreads * 8, v[j]);
   }
   if (!p.h_out && !p.codes) return;
-  stats(p.pre, 2, mean, rstd);
+  stats(p.pre, 2, rstd, shift);
+  if (p.scale && !known) rstd = CUDART_NAN_F;
+  const T* pre_weight = static_cast<const T*>(p.pre_weight) + lane * 8;
+  const T* mod_scale = static_cast<const T*>(p.scale) + t * p.lds + lane * 8;
+  const T* mod_shift = static_cast<const T*>(p.shift) + t * p.ldsh + lane * 8;
+  T* h_out = static_cast<T*>(p.h_out) + static_cast<int64_t>(r) * p.width + lane * 8;
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    if (at(j) >= chunks) continue;
-    const int c = at(j) * 8;
-    float f[8];
+    if (j * kThreads >= left) continue;
+    float2 f[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[j][e] = (v[j][e] - mean) * rstd;
+    for (int e = 0; e < 4; ++e) v[j][e] = __ffma2_rn(v[j][e], both(rstd), both(shift));
     if (p.pre_weight) {
-      unpack(load_raw(static_cast<const T*>(p.pre_weight) + c), f);
+      unpack(load_raw(pre_weight + j * kThreads * 8), f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] *= f[e];
+      for (int e = 0; e < 4; ++e) v[j][e] = __fmul2_rn(v[j][e], f[e]);
     }
     if (p.scale) {
-      float g[8];
-      unpack(load_raw(static_cast<const T*>(p.scale) + t * p.lds + c), f);
-      unpack(load_raw(static_cast<const T*>(p.shift) + t * p.ldsh + c), g);
+      float2 g[4];
+      unpack(load_raw(mod_scale + j * kThreads * 8), f);
+      unpack(load_raw(mod_shift + j * kThreads * 8), g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[j][e] = fmaf(v[j][e], 1.0f + (known ? f[e] : CUDART_NAN_F), g[e]);
+      for (int e = 0; e < 4; ++e) v[j][e] = __ffma2_rn(v[j][e], __fadd2_rn(f[e], both(1.f)), g[e]);
     }
-    if (p.h_out) store8(static_cast<T*>(p.h_out) + r * p.width + c, v[j]);
+    if (p.h_out) {
+      store8(h_out + j * kThreads * 8, v[j]);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[j][e]) & 0x7FFFFFFFu);
+      for (int e = 0; e < 4; ++e)
+        top = max(max(top, __float_as_uint(v[j][e].x) & 0x7FFFFFFFu), __float_as_uint(v[j][e].y) & 0x7FFFFFFFu);
+    }
   }
   if (!p.codes) return;
   top = __reduce_max_sync(0xffffffffu, top);
-  if (warps > 1) {
+  if constexpr (kWarps > 1) {
     if ((threadIdx.x & 31) == 0) red[4][threadIdx.x >> 5] = __uint_as_float(top);
     __syncthreads();
-    for (int i = 0; i < warps; ++i) top = max(top, __float_as_uint(red[4][i]));
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) top = max(top, __float_as_uint(red[4][i]));
   }
   const float sc = code_scale_of(__uint_as_float(top), p.quant);
   const float inv = __frcp_rn(sc);
-  if (threadIdx.x == 0) p.code_scale[r] = sc;
+  if (lane == 0) p.code_scale[r] = sc;
+  uint8_t* codes = p.codes + static_cast<int64_t>(r) * p.width + lane * 8;
 #pragma unroll
   for (int j = 0; j < kChunks; ++j) {
-    if (at(j) >= chunks) continue;
-    uint32_t q[8];
+    if (j * kThreads >= left) continue;
+    uint32_t lo, hi;
+    // the correctly rounded quotient (div_by, two at a time)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float d = div_by(v[j][e], sc, inv);
-      q[e] = p.quant == kInt8 ? static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(d, -127.f), 127.f))) & 0xFFu
-                              : f32_to_e4m3(fminf(fmaxf(d, -448.f), 448.f));
+    for (int e = 0; e < 4; ++e) {
+      const float2 q = __fmul2_rn(v[j][e], both(inv));
+      v[j][e] = __ffma2_rn(__ffma2_rn(q, both(-sc), v[j][e]), both(inv), q);
     }
-    *reinterpret_cast<uint2*>(p.codes + r * p.width + at(j) * 8) =
-        make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+    if (p.quant == kInt8) {
+      // |q| <= 127 and a rounding: 1.5 * 2^23 + q has the nearest even integer
+      // in its low bits
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[j][e] = __fadd2_rn(v[j][e], both(12582912.0f));
+      lo = __byte_perm(__byte_perm(__float_as_uint(v[j][0].x), __float_as_uint(v[j][0].y), 0x0040),
+                       __byte_perm(__float_as_uint(v[j][1].x), __float_as_uint(v[j][1].y), 0x0040), 0x5410);
+      hi = __byte_perm(__byte_perm(__float_as_uint(v[j][2].x), __float_as_uint(v[j][2].y), 0x0040),
+                       __byte_perm(__float_as_uint(v[j][3].x), __float_as_uint(v[j][3].y), 0x0040), 0x5410);
+    } else {
+      lo = e4m3x2(v[j][0].x, v[j][0].y) | (e4m3x2(v[j][1].x, v[j][1].y) << 16);
+      hi = e4m3x2(v[j][2].x, v[j][2].y) | (e4m3x2(v[j][3].x, v[j][3].y) << 16);
+    }
+    *reinterpret_cast<uint2*>(codes + j * kThreads * 8) = make_uint2(lo, hi);
   }
+}
+
+template <typename T, int kThreads, int kChunks>
+int launch_vec(const Params& p, int64_t rows, cudaStream_t st) {
+  constexpr int kBlockRows = kRowsOf<kThreads>;
+  sandwich_norm_vec_kernel<T, kThreads, kChunks><<<static_cast<unsigned>(cdiv(rows, kBlockRows)), kThreads * kBlockRows, 0, st>>>(
+      p, static_cast<uint32_t>(rows), make_fastdiv(static_cast<uint32_t>(p.seq)));
+  return launch_status();
+}
+
+// The fewest threads that hold a row at up to four pieces a thread.
+template <typename T>
+int pick_vec(const Params& p, int64_t rows, cudaStream_t st) {
+  const int chunks = p.width / 8;
+  if (chunks <= 32) return launch_vec<T, 32, 1>(p, rows, st);
+  if (chunks <= 64) return launch_vec<T, 32, 2>(p, rows, st);
+  if (chunks <= 128) return launch_vec<T, 32, 4>(p, rows, st);
+  if (chunks <= 192) return launch_vec<T, 64, 3>(p, rows, st);
+  if (chunks <= 256) return launch_vec<T, 64, 4>(p, rows, st);
+  if (chunks <= 384) return launch_vec<T, 96, 4>(p, rows, st);
+  if (chunks <= 512) return launch_vec<T, 128, 4>(p, rows, st);
+  if (chunks <= 640) return launch_vec<T, 160, 4>(p, rows, st);
+  if (chunks <= 768) return launch_vec<T, 192, 4>(p, rows, st);
+  if (chunks <= 1024) return launch_vec<T, 256, 4>(p, rows, st);
+  if (chunks <= 1536) return launch_vec<T, 384, 4>(p, rows, st);
+  return launch_vec<T, 512, 4>(p, rows, st);
 }
 
 template <typename T>
@@ -363,27 +437,8 @@ int launch(const Params& p, int64_t rows, cudaStream_t st) {
   };
   if (p.width % 8 == 0 && whole(p.y, p.yb | p.ys) && whole(p.x, p.xb | p.xs) && whole(p.post_weight, 0) &&
       whole(p.pre_weight, 0) && whole(p.gate, p.ldg) && whole(p.scale, p.lds) && whole(p.shift, p.ldsh) &&
-      whole(p.x_out, 0) && whole(p.h_out, 0) && whole(p.codes, 0)) {
-    // Pieces of a thread: the count that leaves the fewest lanes idle, the
-    // larger of equals (more bytes requested by a thread, fewer warps to join).
-    const int chunks = p.width / 8;
-    int best = 4, lanes = 1 << 30;
-    for (int k = 4; k >= 1; --k) {
-      const int threads = static_cast<int>(cdiv(cdiv(chunks, k), 32) * 32);
-      if (threads <= kVecThreads && threads * k < lanes) {
-        best = k;
-        lanes = threads * k;
-      }
-    }
-    const unsigned threads = static_cast<unsigned>(lanes / best), grid = static_cast<unsigned>(rows);
-    switch (best) {
-      case 1: sandwich_norm_vec_kernel<T, 1><<<grid, threads, 0, st>>>(p); break;
-      case 2: sandwich_norm_vec_kernel<T, 2><<<grid, threads, 0, st>>>(p); break;
-      case 3: sandwich_norm_vec_kernel<T, 3><<<grid, threads, 0, st>>>(p); break;
-      default: sandwich_norm_vec_kernel<T, 4><<<grid, threads, 0, st>>>(p); break;
-    }
-    return launch_status();
-  }
+      whole(p.x_out, 0) && whole(p.h_out, 0) && whole(p.codes, 0))
+    return pick_vec<T>(p, rows, st);
   auto kernel = sandwich_norm_scalar_kernel<T>;
   const size_t smem = static_cast<size_t>(p.width) * sizeof(float);
   if (smem > 40 * 1024 &&
