@@ -327,6 +327,17 @@ int xgb_int8_gemm(const int8_t* a, const int8_t* w, int64_t M, int64_t N, int64_
                   const void* gate, int64_t ldg, const int64_t* gate_index, int64_t index_rows, int64_t table_rows,
                   const void* residual, int64_t ldr, int* error_flag, void* stream);
 
+/* xgb_int8_quantize_per_token of x [M, K] (`dtype`, rows ldx apart) and
+ * xgb_int8_gemm in one call; few tokens take one launch. workspace:
+ * xgb_int8_linear_workspace(M, K) bytes, 16-byte aligned, its contents need
+ * no initialisation. */
+int64_t xgb_int8_linear_workspace(int64_t M, int64_t K);
+int xgb_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t M, int64_t N, int64_t K,
+                    const float* scale_w, int dtype, const void* bias, int activation, void* out, int64_t ldo,
+                    const void* gate, int64_t ldg, const int64_t* gate_index, int64_t index_rows,
+                    int64_t table_rows, const void* residual, int64_t ldr, void* workspace, int64_t workspace_bytes,
+                    int* error_flag, void* stream);
+
 /* Attention of q [batch, heads, seq_q, head_dim] to k/v [batch, kv_heads,
  * seq_kv, head_dim] views (bf16 or fp16, head_dim 64 or 128, strides in
  * elements, multiples of 8; 0 where the batch or the heads are broadcast),

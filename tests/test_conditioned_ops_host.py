@@ -78,6 +78,14 @@ def test_int8_arguments():
     assert gemm(gate=D) == -1 and gemm(gate=D, idx=D, res=D, act=1) == -1 and gemm(gate=D, idx=D, res=D, m=3, irows=2) == -1
     assert gemm(ldo=31) == -3 and gemm(gate=D, idx=D, res=D, ldg=16) == -3
     assert gemm(a=ODD) == -4 and gemm(out=ODD) == -4
+    need = h.xgb_int8_linear_workspace(3, 32)
+    assert need == 96 + 12
+
+    def linear(x=D, ldx=32, m=3, k=32, ws=D, bytes_=need):
+        return h.xgb_int8_linear(x, ldx, D, m, 32, k, D, 0, None, 0, D, 32, None, 0, None, 1, 0, None, 0, ws, bytes_, None, None)
+
+    assert linear(x=None) == -1 and linear(ldx=31) == -3 and linear(k=24) == -2
+    assert linear(ws=None) == -7 and linear(bytes_=need - 1) == -7 and linear(ws=ODD) == -4
     assert h.xgb_int8_quantize_per_token(None, 0, 1, 16, 16, D, D, None) == -1
     assert h.xgb_int8_quantize_per_token(D, 2, 1, 16, 16, D, D, None) == -1
     assert h.xgb_int8_quantize_per_token(D, 0, 2, 16, 8, D, D, None) == -3

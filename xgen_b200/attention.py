@@ -211,9 +211,13 @@ def dense_attention(q, k, v, sm_scale: float | None = None, out=None) -> torch.T
 CROSS_HEAD_DIMS = (64, 128)
 
 
+_I64x4 = _lib.c_i64 * 4
+
+
 def _steps(t: torch.Tensor):
     """Element strides with 0 for dimensions of one entry (never stepped over)."""
-    return i64_array([st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])] + [1])
+    n, st = t.shape, t.stride()
+    return _I64x4(st[0] if n[0] > 1 else 0, st[1] if n[1] > 1 else 0, st[2] if n[2] > 1 else 0, 1)
 
 
 def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, kv_lens=None, key_mask=None,
@@ -230,30 +234,29 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     without keys gives zeros. out: a [B, H, Sq, D] view of the query's type,
     which must not overlap the inputs. Nothing is shared between calls: the
     workspace of a call comes from the caching allocator."""
-    from .ops import _DTYPE_CODE, _on_device_of, _refuse_autograd, _same_device
+    from .ops import _DTYPE_CODE, _call_on, _device_of, _refuse_autograd
 
     what = "cross attention"
-    extra = [t for t in (kv_lens, key_mask, out) if t is not None]
-    for t in (query, key, value, *extra):
-        if not t.is_cuda:
-            raise ValueError(f"{what} requires CUDA tensors")
-    _refuse_autograd(query, key, value, what=what)
-    _same_device(query, key, value, *extra, what=what)
-    for t in (query, key, value):
-        if t.ndim != 4 or t.dtype not in _DTYPE_CODE or t.dtype != query.dtype or t.shape[-1] != query.shape[-1] or (
-                t.shape[-1] not in CROSS_HEAD_DIMS) or t.stride(-1) != 1:
-            raise ValueError(f"{what} requires bf16/fp16 [B, H, S, D] views of one type, D 64 or 128, unit channel stride")
+    index = _device_of(what, query, key, value, kv_lens, key_mask, out)
+    _refuse_autograd(what, query, key, value)
+    code = _DTYPE_CODE.get(query.dtype)
+    if (code is None or query.ndim != 4 or key.ndim != 4 or value.ndim != 4 or key.dtype != query.dtype
+            or value.dtype != query.dtype or query.stride(3) != 1 or key.stride(3) != 1 or value.stride(3) != 1):
+        raise ValueError(f"{what} requires bf16/fp16 [B, H, S, D] views of one type with unit channel stride")
     b, h, sq, d = query.shape
-    hk, skv = key.shape[1:3]
-    if key.shape != value.shape or key.shape[0] != b or hk == 0 or h % hk:
-        raise ValueError(f"{what}: key and value must match, have the query's batch and divide its heads")
+    hk, skv = key.shape[1], key.shape[2]
+    if d not in CROSS_HEAD_DIMS:
+        raise ValueError(f"{what} requires head dim 64 or 128")
+    if key.shape != value.shape or key.shape[0] != b or key.shape[3] != d or hk == 0 or h % hk:
+        raise ValueError(f"{what}: key and value must match, have the query's batch and head dim and divide its heads")
     sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
     if not 0.0 < sm_scale < math.inf:
         raise ValueError(f"{what} requires a positive scale")
-    if kv_lens is not None and key_mask is not None:
-        raise ValueError(f"{what} takes kv_lens or key_mask, not both")
-    if kv_lens is not None and (kv_lens.shape != (b,) or kv_lens.dtype not in (torch.int32, torch.int64)):
-        raise ValueError(f"{what}: kv_lens must be int32 or int64 [B]")
+    if kv_lens is not None:
+        if key_mask is not None:
+            raise ValueError(f"{what} takes kv_lens or key_mask, not both")
+        if kv_lens.shape != (b,) or kv_lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{what}: kv_lens must be int32 or int64 [B]")
     if key_mask is not None:
         if key_mask.ndim == 4 and key_mask.shape[1:3] == (1, 1):
             key_mask = key_mask[:, 0, 0]
@@ -264,29 +267,31 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
         out = torch.empty((b, h, sq, d), dtype=query.dtype, device=query.device)
     elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
         raise ValueError(f"{what} output must be a [B, H, Sq, D] view of the query's type with unit channel stride")
-    if not out.numel():
+    if not b * h * sq:
         return out
     if not skv:
         return out.zero_()
-    with _on_device_of(query):
-        if kv_lens is not None and kv_lens.dtype != torch.int32:
-            kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
-        if key_mask is not None and not _lib.lib().xgb_cross_attention_takes_mask(h, hk, sq):
+    lib = _lib.lib()
+    mask = (None, 0, 0)
+    if key_mask is not None:
+        if lib.xgb_cross_attention_takes_mask(h, hk, sq):
+            mask = (key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1))
+        else:
             kv_lens = torch.empty((b,), dtype=torch.int32, device=key.device)
             packed = torch.empty((2, b, hk, skv, d), dtype=key.dtype, device=key.device)
-            call("xgb_pack_keys", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), key.data_ptr(), _steps(key),
-                 value.data_ptr(), _steps(value), b, hk, skv, d, packed[0].data_ptr(), packed[1].data_ptr(),
-                 kv_lens.data_ptr(), _stream(query))
-            key, value, key_mask = packed[0], packed[1], None
-        elif kv_lens is not None:
-            kv_lens = kv_lens.contiguous()
-        ws_bytes = _lib.lib().xgb_cross_attention_workspace(b, h, hk, sq, skv, d)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
-        call("xgb_cross_attention", query.data_ptr(), _steps(query), key.data_ptr(), _steps(key), value.data_ptr(),
-             _steps(value), _DTYPE_CODE[query.dtype], b, h, hk, sq, skv, d,
-             kv_lens.data_ptr() if kv_lens is not None else None,
-             *((key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1)) if key_mask is not None else (None, 0, 0)), sm_scale, out.data_ptr(), _steps(out),
-             ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(query.device), _stream(query))
+            _call_on(index, "xgb_pack_keys", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), key.data_ptr(),
+                     _steps(key), value.data_ptr(), _steps(value), b, hk, skv, d, packed[0].data_ptr(), packed[1].data_ptr(),
+                     kv_lens.data_ptr())
+            key, value = packed[0], packed[1]
+    elif kv_lens is not None:
+        if kv_lens.dtype != torch.int32:
+            kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
+        kv_lens = kv_lens.contiguous()
+    ws_bytes = lib.xgb_cross_attention_workspace(b, h, hk, sq, skv, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
+    _call_on(index, "xgb_cross_attention", query.data_ptr(), _steps(query), key.data_ptr(), _steps(key), value.data_ptr(),
+             _steps(value), code, b, h, hk, sq, skv, d, kv_lens.data_ptr() if kv_lens is not None else None, *mask, sm_scale,
+             out.data_ptr(), _steps(out), ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(query.device))
     return out
 
 

@@ -4,19 +4,21 @@
 //   y[m, n]  = (sum_k a[m, k] w[n, k]) * (sa[m] * sw[n]) + bias[n]
 //   out      = y | gelu(y) | silu(y[:, :N/2]) * y[:, N/2:] | residual + gate[idx[m]] * y
 //
-// a [M, K] and w [N, K] int8 row-major. The sum is exact (tcgen05 kind::i8,
-// 32-bit integers: K <= 131056 keeps 128 * 128 * K below 2^31); it becomes a
-// 32-bit float once, the epilogue stays in 32 bits and the output is rounded
-// once to bf16 or fp16.
+// a [M, K] and w [N, K] int8 row-major. The sum is exact (32-bit integers:
+// K <= 131056 keeps 128 * 128 * K below 2^31); it becomes a 32-bit float once,
+// the epilogue stays in 32 bits and the output is rounded once to bf16 or fp16.
 //
-// Persistent kernel, one CTA per SM, tiles of 128 x 256 (M x N), K blocks of
-// 128 bytes:
-//   warp 0     TMA producer (A 16 KB + W 32 KB per stage, 4 stages)
-//   warp 1     TMEM allocator + MMA issuer (4 x M128 N256 K32 per stage)
+// Three forms, picked by sizes (see pick_form and run_few):
+//   few tokens   bound by reading w once: warp-level products, below
+//   CTA pairs    bound by the tensor cores: tcgen05 kind::i8, 256 x kBN tiles
+//   single CTAs  tiles of 128 x kBN, where they fill the SMs better
+// The tiled kernels are persistent, K blocks of 128 bytes:
+//   warp 0     TMA producer
+//   warp 1     TMEM allocator + MMA issuer (of rank 0 in a pair)
 //   warps 2-9  epilogue: one thread per output row (TMEM lane) and column half
-// Two TMEM accumulators (2 x 256 columns) let the epilogue of one tile run
-// under the MMAs of the next. A W tile is loaded as two boxes of 128 rows, so
-// the gate and value rows of one SwiGLU tile come from their two places in a
+// Two TMEM accumulators let the epilogue of one tile run under the MMAs of the
+// next. A W tile is two boxes of kBN/2 rows (in a pair, one of each CTA), so
+// the gate and value rows of a SwiGLU tile come from their two places in a
 // plain [gate | value] weight. Every mbarrier wait is bounded.
 //
 // The quantiser reads a row once into registers, takes its largest magnitude
@@ -24,6 +26,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cfloat>
 
 #include "sm100.cuh"
@@ -34,19 +37,27 @@ namespace int8 {
 
 using namespace sm100;
 
-constexpr int kBM = 128;
-constexpr int kBN = 256;
+constexpr int kBM = 128;  // A rows of a CTA
 constexpr int kBK = 128;  // bytes of K per stage
-constexpr int kStages = 4;
 constexpr int kThreads = 320;
 constexpr int kEpiThreads = 256;
 constexpr int kABytes = kBM * kBK;
-constexpr int kBBytes = kBN * kBK;
-constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kBarOff = kStages * kStageBytes;
-constexpr int kSmem = kBarOff + 256 + 1024;
-constexpr uint32_t kIdesc = instr_desc(2, 1, 1, false, false, kBM, kBN);
 constexpr int64_t kMaxK = 131056;
+constexpr int kRaster = 8;  // row tiles that a group of consecutive tiles shares
+
+// Shared memory of a CTA: per stage 128 rows of A and kBN (single) or kBN/2
+// (pair) rows of W; as many stages as fit.
+template <int kBN, bool kPair>
+struct Cfg {
+  static constexpr int kBoxRows = kBN / 2;
+  static constexpr int kBoxBytes = kBoxRows * kBK;
+  static constexpr int kStageBytes = kABytes + (kPair ? 1 : 2) * kBoxBytes;
+  static constexpr int kStages = 224 * 1024 / kStageBytes < 8 ? 224 * 1024 / kStageBytes : 8;
+  static constexpr int kBarOff = kStages * kStageBytes;
+  static constexpr int kSmem = kBarOff + 256 + 1024;
+  static constexpr uint32_t kIdesc = instr_desc(2, 1, 1, false, false, kPair ? 2 * kBM : kBM, kBN);
+  static constexpr uint32_t kTmemCols = 2 * kBN;
+};
 
 enum Epilogue : int { kPlain = 0, kGeluErf = 1, kGeluTanh = 2, kSwiGLU = 3, kGated = 4 };
 
@@ -73,12 +84,13 @@ struct Params {
   const T* residual;
   int64_t ldr;
   int* err;
-  bool vec;  // bias, gate and residual may be read 16 bytes at a time (host-checked)
+  bool vec;        // bias, gate and residual may be read 16 bytes at a time (host-checked)
+  bool vec_scale;  // and sw
 };
 
 struct Barriers {
-  uint64_t full[kStages];
-  uint64_t empty[kStages];
+  uint64_t full[8];
+  uint64_t empty[8];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t end;
@@ -104,27 +116,32 @@ __device__ __forceinline__ void unpack8(const __half*, const uint4& raw, float (
     f[2 * i + 1] = v.y;
   }
 }
-// Eight entries of a row of the tensor's type; `vec` says that the place is
-// 16-byte aligned, `left` how many exist.
+// Eight entries of a row of the tensor's type (widths are multiples of 8);
+// `vec` says that the place is 16-byte aligned.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int left, float (&f)[8]) {
-  if (vec && left >= 8) {
-    unpack8(p, __ldg(reinterpret_cast<const uint4*>(p)), f);
+__device__ __forceinline__ uint4 load_raw8(const T* p, bool vec) {
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = __ldg(reinterpret_cast<const uint16_t*>(p) + 2 * i);
+    w[i] = lo | static_cast<uint32_t>(__ldg(reinterpret_cast<const uint16_t*>(p) + 2 * i + 1)) << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void scaled8(const Params<T>& p, const uint32_t* acc, float sa, int n, float (&y)[8]) {
+  float sw[8], bias[8];
+  if (p.vec_scale) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p.sw + n)), b = __ldg(reinterpret_cast<const float4*>(p.sw + n) + 1);
+    sw[0] = a.x; sw[1] = a.y; sw[2] = a.z; sw[3] = a.w;
+    sw[4] = b.x; sw[5] = b.y; sw[6] = b.z; sw[7] = b.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < left ? load_as_float(p + i) : 0.f;
+    for (int i = 0; i < 8; ++i) sw[i] = __ldg(p.sw + n + i);
   }
-}
-__device__ __forceinline__ void load8(const float* p, int left, float (&f)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = i < left ? __ldg(p + i) : 0.f;
-}
-template <typename T>
-__device__ __forceinline__ void scaled8(const Params<T>& p, const uint32_t* acc, float sa, int n, int left, float (&y)[8]) {
-  float sw[8], bias[8];
-  load8(p.sw + n, left, sw);
   if (p.bias) {
-    load8(p.bias + n, p.vec, left, bias);
+    unpack8(p.bias, load_raw8(p.bias + n, p.vec), bias);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) bias[i] = 0.f;
@@ -133,86 +150,135 @@ __device__ __forceinline__ void scaled8(const Params<T>& p, const uint32_t* acc,
   for (int i = 0; i < 8; ++i) y[i] = fmaf(__int2float_rn(static_cast<int>(acc[i])), sa * sw[i], bias[i]);
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* dst, int left, const float (&y)[8]) {
-  const uint32_t w[4] = {pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7])};
-  if (left >= 8) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-    const T* wb = reinterpret_cast<const T*>(w);
-    for (int i = 0; i < left; ++i) dst[i] = wb[i];
-  }
+__device__ __forceinline__ void store8(T* dst, const float (&y)[8]) {
+  *reinterpret_cast<uint4*>(dst) =
+      make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
 }
 
-// One accumulator tile's epilogue for the output row `m` this thread owns and
-// the column half `half`; n0 = first W row of the tile (SwiGLU: first gate row
-// and output column, its values N/2 further).
+// What an output row needs besides the accumulators.
+template <typename T>
+struct Row {
+  float sa;
+  const T* gate;  // null factor row: outside the table
+  const T* residual;
+  T* out;
+  bool ok;     // the row exists
+  bool known;  // its index is inside the table
+};
 template <typename T, int kEpi>
-__device__ __forceinline__ void epilogue_tile(const Params<T>& p, uint32_t acc, int m, int n0, int half) {
-  const bool row_ok = m < p.M;
-  const float sa = row_ok ? p.sa[m] : 0.f;
-  const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
-  int64_t grow = 0;
-  bool known = true;
-  if (kEpi == kGated && row_ok) {
-    grow = p.idx[m % p.idx_rows];
-    known = grow >= 0 && grow < p.table_rows;
-    if (!known) grow = 0;
+__device__ __forceinline__ Row<T> row_of(const Params<T>& p, int m) {
+  Row<T> r{};
+  r.ok = m < p.M;
+  r.known = true;
+  if (!r.ok) return r;
+  r.sa = __ldg(p.sa + m);
+  r.out = p.out + static_cast<int64_t>(m) * p.ldo;
+  if constexpr (kEpi == kGated) {
+    const int64_t at = __ldg(p.idx + m % p.idx_rows);
+    r.known = at >= 0 && at < p.table_rows;
+    r.gate = p.gate + (r.known ? at : 0) * p.ldg;
+    r.residual = p.residual + static_cast<int64_t>(m) * p.ldr;
   }
-  T* dst = p.out + static_cast<int64_t>(m) * p.ldo;
-  constexpr int kChunks = kEpi == kSwiGLU ? 2 : 4;  // 32 output columns each
-#pragma unroll 1
-  for (int c = half * kChunks; c < (half + 1) * kChunks; ++c) {
-    uint32_t r[32], rv[kEpi == kSwiGLU ? 32 : 1];
-    tmem_ld32(acc + c * 32, r);
-    if constexpr (kEpi == kSwiGLU) tmem_ld32(acc + kBN / 2 + c * 32, rv);
-    tmem_ld_wait();
-    if (!row_ok) continue;
+  return r;
+}
+
+// Gate and residual of 32 columns, requested before they are needed.
+template <int kEpi>
+struct Ahead {
+  uint4 gate[kEpi == kGated ? 4 : 1], res[kEpi == kGated ? 4 : 1];
+};
+template <typename T, int kEpi>
+__device__ __forceinline__ void fetch(const Params<T>& p, const Row<T>& r, int n, Ahead<kEpi>& a) {
+  if constexpr (kEpi == kGated) {
+    if (!r.ok) return;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int n = n0 + c * 32 + g * 8;
-      const int left = width - n;
-      if (left <= 0) break;
-      float y[8];
-      scaled8(p, r + 8 * g, sa, n, left, y);
-      if constexpr (kEpi == kSwiGLU) {
-        float v[8];
-        scaled8(p, rv + 8 * g, sa, n + width, left, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = swiglu(y[i], v[i]);
-      }
-      if constexpr (kEpi == kGated) {
-        float gt[8], res[8];
-        load8(p.gate + grow * p.ldg + n, p.vec, left, gt);
-        load8(p.residual + static_cast<int64_t>(m) * p.ldr + n, p.vec, left, res);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = fmaf(known ? gt[i] : CUDART_NAN_F, y[i], res[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (kEpi == kGeluErf) y[i] = gelu_erf(y[i]);
-        if constexpr (kEpi == kGeluTanh) y[i] = gelu_tanh(y[i]);
-      }
-      store8(dst + n, left, y);
+      if (n + 8 * g >= p.N) break;
+      a.gate[g] = load_raw8(r.gate + n + 8 * g, p.vec);
+      a.res[g] = load_raw8(r.residual + n + 8 * g, p.vec);
     }
   }
 }
 
-template <typename T, int kEpi>
+// One accumulator tile's epilogue for the output row this thread owns and the
+// column half `half`; n0 = the tile's first output column. `ahead` holds the
+// first 32 columns' gate and residual on entry.
+template <typename T, int kBN, int kEpi>
+__device__ __forceinline__ void epilogue_tile(const Params<T>& p, uint32_t acc, const Row<T>& row, int n0, int half,
+                                              Ahead<kEpi>& ahead) {
+  const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
+  constexpr int kChunks = (kEpi == kSwiGLU ? kBN / 2 : kBN) / 64;  // of 32 output columns, for each half
+#pragma unroll 1
+  for (int i = 0; i < kChunks; ++i) {
+    const int c = half * kChunks + i, n1 = n0 + c * 32;
+    uint32_t r[32], rv[kEpi == kSwiGLU ? 32 : 1];
+    tmem_ld32(acc + c * 32, r);
+    if constexpr (kEpi == kSwiGLU) tmem_ld32(acc + kBN / 2 + c * 32, rv);
+    Ahead<kEpi> now = ahead;
+    if (i + 1 < kChunks) fetch<T, kEpi>(p, row, n1 + 32, ahead);
+    tmem_ld_wait();
+    if (!row.ok) continue;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int n = n1 + g * 8;
+      if (n >= width) break;
+      float y[8];
+      scaled8(p, r + 8 * g, row.sa, n, y);
+      if constexpr (kEpi == kSwiGLU) {
+        float v[8];
+        scaled8(p, rv + 8 * g, row.sa, n + width, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = swiglu(y[e], v[e]);
+      }
+      if constexpr (kEpi == kGated) {
+        float gt[8], res[8];
+        unpack8(p.gate, now.gate[g], gt);
+        unpack8(p.gate, now.res[g], res);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(row.known ? gt[e] : CUDART_NAN_F, y[e], res[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (kEpi == kGeluErf) y[e] = gelu_erf(y[e]);
+        if constexpr (kEpi == kGeluTanh) y[e] = gelu_tanh(y[e]);
+      }
+      store8(row.out + n, y);
+    }
+  }
+}
+
+// Tile t of the walk: groups of kRaster row tiles, columns within a group, so
+// that tiles in flight share rows of A and of W in L2.
+struct Walk {
+  int m_tiles, n_tiles;
+  __device__ __forceinline__ void at(int64_t t, int& m, int& n) const {
+    const int64_t per_group = static_cast<int64_t>(kRaster) * n_tiles;
+    const int64_t g = t / per_group;
+    const int in = static_cast<int>(t - g * per_group);
+    const int rows = min(kRaster, m_tiles - static_cast<int>(g) * kRaster);
+    m = static_cast<int>(g) * kRaster + in % rows;
+    n = in / rows;
+  }
+};
+
+template <typename T, int kBN, int kEpi, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_int8_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const Params<T> p) {
+  using C = Cfg<kBN, kPair>;
+  constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  Barriers* bars = reinterpret_cast<Barriers*>(smem + kBarOff);
+  Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // W rows of a tile: two boxes of 128; SwiGLU tiles cover 128 gate rows and
-  // their 128 value rows.
-  constexpr int kCols = kEpi == kSwiGLU ? kBN / 2 : kBN;
+  const int rank = kPair ? static_cast<int>(cluster_rank()) : 0;
+  const int64_t first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
+  constexpr int kCols = kEpi == kSwiGLU ? kBN / 2 : kBN;  // output columns of a tile
+  constexpr int kRowsOfTile = kPair ? 2 * kBM : kBM;
   const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
-  const int second = kEpi == kSwiGLU ? width : kBN / 2;
-  const int m_tiles = (p.M + kBM - 1) / kBM;
-  const int n_tiles = (width + kCols - 1) / kCols;
-  const int64_t tiles = static_cast<int64_t>(m_tiles) * n_tiles;
+  const int second = kEpi == kSwiGLU ? width : kBN / 2;  // W rows from the first box to the second
+  const Walk walk{(p.M + kRowsOfTile - 1) / kRowsOfTile, (width + kCols - 1) / kCols};
+  const int64_t tiles = static_cast<int64_t>(walk.m_tiles) * walk.n_tiles;
   const int k_blocks = (p.K + kBK - 1) / kBK;
 
   if (threadIdx.x == 0) {
@@ -222,50 +288,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&bars->acc_full[a], 1);
-      mbar_init(&bars->acc_empty[a], kEpiThreads);
+      mbar_init(&bars->acc_empty[a], (kPair ? 2 : 1) * kEpiThreads / 32);
     }
     mbar_init(&bars->end, 1);
     fence_barrier_init();
   }
-  if (warp == 1) tmem_alloc<512>(&bars->tmem_base);
+  if (warp == 1) {
+    if constexpr (kPair) tmem_alloc_pair<C::kTmemCols>(&bars->tmem_base);
+    else tmem_alloc<C::kTmemCols>(&bars->tmem_base);
+  }
   if (warp == 0 && lane == 0) {
     prefetch_tmap(&a_map);
     prefetch_tmap(&b_map);
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (kPair) cluster_sync();  // both CTAs' barriers exist
   tc_fence_after();
   const uint32_t tmem = bars->tmem_base;
 
   if (warp == 0) {
-    // ------------------------------------------------------------ producer
+    // ------------------------------------------------------------ producer (each CTA its own rows)
     if (lane == 0) {
       bool ok = true;
       int it = 0;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-        const int m0 = static_cast<int>(t / n_tiles) * kBM;
-        const int n0 = static_cast<int>(t % n_tiles) * kCols;
+      for (int64_t t = first; t < tiles && ok; t += step) {
+        int mt, nt;
+        walk.at(t, mt, nt);
+        const int m0 = mt * kRowsOfTile + rank * kBM, n0 = nt * kCols;
         for (int kb = 0; kb < k_blocks; ++kb, ++it) {
           const int s = it % kStages;
           if (it >= kStages) ok = mbar_wait(&bars->empty[s], ((it / kStages) - 1) & 1, p.err);
           if (!ok) break;
-          uint8_t* st = smem + s * kStageBytes;
-          mbar_arrive_expect_tx(&bars->full[s], kStageBytes);
-          tma_load_2d(st, &a_map, &bars->full[s], kb * kBK, m0);
-          tma_load_2d(st + kABytes, &b_map, &bars->full[s], kb * kBK, n0);
-          tma_load_2d(st + kABytes + kBBytes / 2, &b_map, &bars->full[s], kb * kBK, n0 + second);
+          uint8_t* st = smem + s * C::kStageBytes;
+          if constexpr (kPair) {
+            // both CTAs' bytes are counted on rank 0's barrier
+            const uint32_t full0 = map_to_rank(&bars->full[s], 0);
+            if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], 2 * C::kStageBytes);
+            tma_load_2d_pair(st, &a_map, full0, kb * kBK, m0);
+            tma_load_2d_pair(st + kABytes, &b_map, full0, kb * kBK, n0 + rank * second);
+          } else {
+            mbar_arrive_expect_tx(&bars->full[s], C::kStageBytes);
+            tma_load_2d(st, &a_map, &bars->full[s], kb * kBK, m0);
+            tma_load_2d(st + kABytes, &b_map, &bars->full[s], kb * kBK, n0);
+            tma_load_2d(st + kABytes + C::kBoxBytes, &b_map, &bars->full[s], kb * kBK, n0 + second);
+          }
         }
       }
-      // the last stages' copies must land before the CTA exits
-      for (int j = max(0, it - kStages); j < it; ++j)
-        mbar_wait(&bars->full[j % kStages], (j / kStages) & 1, p.err, 100000000ull);
+      // The armed stages' copies must land before the CTA (the pair: rank 0's
+      // barrier counts both CTAs' loads) exits.
+      if (!kPair || rank == 0)
+        for (int j = max(0, it - kStages); j < it; ++j)
+          mbar_wait(&bars->full[j % kStages], (j / kStages) & 1, p.err, 100000000ull);
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    // ------------------------------------------------------------ MMA issuer (rank 0)
+    if (lane == 0 && rank == 0) {
+      auto commit = [&](uint64_t* bar) {
+        if constexpr (kPair) {
+          tc_commit_pair(map_to_rank(bar, 0));
+          tc_commit_pair(map_to_rank(bar, 1));
+        } else {
+          tc_commit(bar);
+        }
+      };
       bool ok = true;
       int it = 0, lt = 0;
-      for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++lt) {
+      for (int64_t t = first; t < tiles && ok; t += step, ++lt) {
         const int a = lt & 1;
         if (lt >= 2) ok = mbar_wait(&bars->acc_empty[a], ((lt >> 1) - 1) & 1, p.err);
         if (!ok) break;
@@ -276,19 +365,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = mbar_wait(&bars->full[s], (it / kStages) & 1, p.err);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t as = smem_u32(smem + s * kStageBytes);
-          const uint32_t bs = as + kABytes;
+          const uint32_t as = smem_u32(smem + s * C::kStageBytes), bs = as + kABytes;
 #pragma unroll
-          for (int k = 0; k < kBK / 32; ++k)
-            mma_ss<Kind::kI8>(d, smem_desc_sw128(as + k * 32, 16, 1024), smem_desc_sw128(bs + k * 32, 16, 1024), kIdesc,
-                              kb > 0 || k > 0);
-          tc_commit(&bars->empty[s]);
+          for (int k = 0; k < kBK / 32; ++k) {
+            const uint64_t da = smem_desc_sw128(as + k * 32, 16, 1024), db = smem_desc_sw128(bs + k * 32, 16, 1024);
+            if constexpr (kPair) mma_pair_i8(d, da, db, C::kIdesc, kb > 0 || k > 0);
+            else mma_ss<Kind::kI8>(d, da, db, C::kIdesc, kb > 0 || k > 0);
+          }
+          commit(&bars->empty[s]);
         }
         if (!ok) break;
-        tc_commit(&bars->acc_full[a]);
+        commit(&bars->acc_full[a]);
       }
-      tc_commit(&bars->end);
-      mbar_wait(&bars->end, 0, p.err, 100000000ull);
+      commit(&bars->end);
     }
   } else {
     // ------------------------------------------------------------ epilogue
@@ -296,24 +385,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int half = (warp - 2) >> 2;  // column half of the tile
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
     int lt = 0;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x, ++lt) {
+    for (int64_t t = first; t < tiles; t += step, ++lt) {
       const int a = lt & 1;
-      const bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[a], (lt >> 1) & 1, p.err));
-      if (!ok) break;
+      int mt, nt;
+      walk.at(t, mt, nt);
+      const int n0 = nt * kCols;
+      const Row<T> row = row_of<T, kEpi>(p, mt * kRowsOfTile + rank * kBM + quarter * 32 + lane);
+      Ahead<kEpi> ahead;
+      fetch<T, kEpi>(p, row, n0 + half * (kCols / 2), ahead);
+      if (!__all_sync(0xffffffffu, mbar_wait(&bars->acc_full[a], (lt >> 1) & 1, p.err))) break;
       tc_fence_after();
-      const int m = static_cast<int>(t / n_tiles) * kBM + quarter * 32 + lane;
-      const int n0 = static_cast<int>(t % n_tiles) * kCols;
-      epilogue_tile<T, kEpi>(p, lane_addr + a * kBN, m, n0, half);
+      epilogue_tile<T, kBN, kEpi>(p, lane_addr + a * kBN, row, n0, half, ahead);
       tc_fence_before();
-      mbar_arrive(&bars->acc_empty[a]);
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (kPair) mbar_arrive_cluster(map_to_rank(&bars->acc_empty[a], 0));
+        else mbar_arrive(&bars->acc_empty[a]);
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
+    // every MMA, which in a pair reads both CTAs' shared memory, has ended
+    mbar_wait(&bars->end, 0, p.err, 100000000ull);
     tc_fence_after();
-    tmem_dealloc<512>(tmem);
+    if constexpr (kPair) tmem_dealloc_pair<C::kTmemCols>(tmem);
+    else tmem_dealloc<C::kTmemCols>(tmem);
   }
+  if constexpr (kPair) cluster_sync();
 }
 
 int sm_count() {
@@ -323,36 +423,105 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
-template <typename T, int kEpi>
+// Pairs that can be resident at once, measured once per kernel and device
+// (stored as pairs + 1): a walk over more of them would wait for another pair
+// to end.
+template <typename Kernel>
+int pair_slots(Kernel kernel, std::atomic<int>* cached, const cudaLaunchConfig_t& like, int sms) {
+  constexpr int kMaxDevices = 64;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sms / 2;
+  const int known = cached[dev].load(std::memory_order_relaxed);
+  if (known > 0) return known - 1;
+  cudaLaunchConfig_t cfg = like;
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(sms));
+  int pairs = 0;
+  if (cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg) != cudaSuccess || pairs <= 0) {
+    cudaGetLastError();
+    return sms / 2;
+  }
+  pairs = std::min(pairs, sms / 2);
+  cached[dev].store(pairs + 1, std::memory_order_relaxed);
+  return pairs;
+}
+
+template <typename T, int kBN, int kEpi, bool kPair>
 int launch(const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
+  using C = Cfg<kBN, kPair>;
   CUtensorMap am, bm;
   const uint64_t adims[2] = {static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.M)};
   const uint64_t str[1] = {static_cast<uint64_t>(p.K)};
-  const uint32_t box[2] = {kBK, 128};
+  const uint32_t abox[2] = {kBK, kBM}, bbox[2] = {kBK, C::kBoxRows};
   const uint64_t bdims[2] = {static_cast<uint64_t>(p.K), static_cast<uint64_t>(p.N)};
-  if (!make_tensor_map(&am, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, str, box) ||
-      !make_tensor_map(&bm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, bdims, str, box))
+  if (!make_tensor_map(&am, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, str, abox) ||
+      !make_tensor_map(&bm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, bdims, str, bbox))
     return XGB_ERR_ALIGN;
-  auto kernel = gemm_int8_kernel<T, kEpi>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess)
+  auto kernel = gemm_int8_kernel<T, kBN, kEpi, kPair>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
     return XGB_ERR_LAUNCH;
-  const int cols = kEpi == kSwiGLU ? kBN / 2 : kBN;
-  const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
-  const int64_t tiles = cdiv(p.M, kBM) * cdiv(width, cols);
-  const int grid = static_cast<int>(std::min<int64_t>(tiles, sm_count()));
-  kernel<<<grid, kThreads, kSmem, st>>>(am, bm, p);
+  const int cols = kEpi == kSwiGLU ? kBN / 2 : kBN, rows = kPair ? 2 * kBM : kBM;
+  const int64_t tiles = cdiv(p.M, rows) * cdiv(kEpi == kSwiGLU ? p.N / 2 : p.N, cols);
+  const int sms = sm_count();
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  if constexpr (kPair) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    static std::atomic<int> cached[64];
+    cfg.gridDim = dim3(static_cast<unsigned>(2 * std::min<int64_t>(tiles, pair_slots(kernel, cached, cfg, sms))));
+  } else {
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sms)));
+  }
+  if (cudaLaunchKernelEx(&cfg, kernel, am, bm, p) != cudaSuccess) {
+    cudaGetLastError();
+    return XGB_ERR_LAUNCH;
+  }
   return launch_status();
 }
 
-template <typename T>
-int pick(int epilogue, const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
-  switch (epilogue) {
-    case kPlain: return launch<T, kPlain>(a, w, p, st);
-    case kGeluErf: return launch<T, kGeluErf>(a, w, p, st);
-    case kGeluTanh: return launch<T, kGeluTanh>(a, w, p, st);
-    case kSwiGLU: return launch<T, kSwiGLU>(a, w, p, st);
-    default: return launch<T, kGated>(a, w, p, st);
+// The tile shape: rounds of tiles over the SMs, each of k_blocks steps and an
+// epilogue that the last round does not hide.
+enum Form { kPair256, kPair128, kSingle128, kSingle64 };
+inline Form pick_form(int64_t m, int64_t width, int64_t k, bool swiglu, int sms) {
+  const int64_t blocks = cdiv(k, kBK);
+  struct Candidate {
+    Form form;
+    int rows, cols, slots;
+    double block, fixed;  // microseconds of a K block and of a tile's start and end
+  };
+  const int half = swiglu ? 2 : 1;
+  const Candidate all[4] = {{kPair256, 256, 256 / half, sms / 2, 0.40, 5.0},
+                            {kPair128, 256, 128 / half, sms / 2, 0.25, 4.0},
+                            {kSingle128, 128, 128 / half, sms, 0.25, 4.0},
+                            {kSingle64, 128, 64, sms, 0.20, 3.0}};
+  Form best = kPair256;
+  double least = 1e300;
+  for (const Candidate& c : all) {
+    if ((c.form == kSingle64 && swiglu) || (c.rows == 256 && m <= 128)) continue;
+    const double rounds = static_cast<double>(cdiv(cdiv(m, c.rows) * cdiv(width, c.cols), c.slots));
+    const double cost = rounds * blocks * c.block + c.fixed;
+    if (cost < least) {
+      least = cost;
+      best = c.form;
+    }
   }
+  return best;
+}
+
+template <typename T, int kEpi>
+int launch_form(const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
+  const Form f = pick_form(p.M, kEpi == kSwiGLU ? p.N / 2 : p.N, p.K, kEpi == kSwiGLU, sm_count());
+  if (f == kPair256) return launch<T, 256, kEpi, true>(a, w, p, st);
+  if (f == kPair128) return launch<T, 128, kEpi, true>(a, w, p, st);
+  if constexpr (kEpi != kSwiGLU)
+    if (f == kSingle64) return launch<T, 64, kEpi, false>(a, w, p, st);
+  return launch<T, 128, kEpi, false>(a, w, p, st);
 }
 
 // ---------------------------------------------------------------- quantiser
@@ -367,11 +536,186 @@ __device__ __forceinline__ float scale_of(uint32_t top) {
 __device__ __forceinline__ uint32_t code_of(float v, float s, float inv) {
   return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(div_by(v, s, inv), -127.f), 127.f))) & 0xFFu;
 }
+// Eight codes, two values an instruction; |q| <= 127 and a rounding, and
+// 1.5 * 2^23 + q has the nearest even integer in its low bits.
 __device__ __forceinline__ uint2 codes8(const float (&f)[8], float s, float inv) {
-  uint32_t q[8];
+  const float2 inv2 = make_float2(inv, inv), minus = make_float2(-s, -s), shift = make_float2(12582912.0f, 12582912.0f);
+  uint32_t h[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = code_of(f[e], s, inv);
-  return make_uint2(q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24), q[4] | (q[5] << 8) | (q[6] << 16) | (q[7] << 24));
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = make_float2(f[2 * i], f[2 * i + 1]), q = __fmul2_rn(v, inv2);
+    const float2 d = __fadd2_rn(__ffma2_rn(__ffma2_rn(q, minus, v), inv2, q), shift);
+    h[i] = __byte_perm(__float_as_uint(d.x), __float_as_uint(d.y), 0x0040);
+  }
+  return make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410));
+}
+
+// ---------------------------------------------------------------- few tokens
+// Up to 32 tokens: the time is that of reading w once, and a 128-row tile would
+// be mostly empty. A CTA takes 16 rows of w (SwiGLU: 8 gate and their 8 value
+// rows) for all tokens, its 8 warps share K in pieces of 64 bytes. A lane loads
+// 16-byte pieces of rows g and g + 8 (g = lane / 4) straight into the fragments
+// of the warp-level 16 x 8 x 32 products; their inner index is any order of k
+// as long as the tokens' codes follow the same one, so the pieces need no
+// rearranging. The integer sums of the warps meet in shared memory: the result
+// does not depend on how K is shared. With kFused every CTA first quantises
+// the tokens itself, a few thousand values, while its first rows of w are on
+// their way: one launch instead of two.
+constexpr int kFewThreads = 256;
+constexpr int kFewWarps = kFewThreads / 32;
+constexpr int kFewAhead = 3;        // pieces of a warp in flight
+constexpr int kFewMost = 32;        // tokens
+constexpr int64_t kFusedMost = 16384;  // values that every CTA quantises for itself
+
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// x: the tokens of a fused launch (rows ldx apart, 16-byte aligned pieces).
+template <typename T, int kEpi, int kTokenTiles, bool kFused>
+__global__ void __launch_bounds__(kFewThreads) few_int8_kernel(const int8_t* __restrict__ a, const int8_t* __restrict__ w,
+                                                               const Params<T> p, const T* __restrict__ x, int64_t ldx) {
+  constexpr int kTokens = 8 * kTokenTiles;
+  __shared__ int part[kFewWarps][16][kTokens + 1];
+  __shared__ uint32_t red[kFewWarps];
+  __shared__ float scales[kTokens];
+  extern __shared__ __align__(16) int8_t codes[];  // fused: [M][K + 64]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
+  const int n0 = blockIdx.x * (kEpi == kSwiGLU ? 8 : 16);
+  // w rows of this lane; the last tile's missing ones read a row that exists
+  const int8_t* w0 = w + static_cast<int64_t>(min(n0 + g, width - 1)) * p.K + 16 * c;
+  const int8_t* w1 = w + static_cast<int64_t>(kEpi == kSwiGLU ? width + min(n0 + g, width - 1) : min(n0 + g + 8, width - 1)) * p.K + 16 * c;
+  const int pieces = (p.K + 63) / 64;
+  auto piece = [&](const int8_t* row, int j) {
+    return 64 * j + 16 * c < p.K ? __ldg(reinterpret_cast<const uint4*>(row + 64 * j)) : make_uint4(0, 0, 0, 0);
+  };
+  uint4 r0[kFewAhead], r1[kFewAhead];
+#pragma unroll
+  for (int i = 0; i < kFewAhead; ++i) {
+    const int j = warp + i * kFewWarps;
+    r0[i] = j < pieces ? piece(w0, j) : make_uint4(0, 0, 0, 0);
+    r1[i] = j < pieces ? piece(w1, j) : make_uint4(0, 0, 0, 0);
+  }
+  const int stride = p.K + 64;
+  if constexpr (kFused) {
+    for (int m = 0; m < p.M; ++m) {
+      const T* xr = x + m * ldx;
+      uint32_t top = 0;
+      for (int k = threadIdx.x; k < p.K / 8; k += kFewThreads) {
+        float f[8];
+        unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) red[warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kFewWarps; ++i) top = max(top, red[i]);
+      const float s = scale_of(top), inv = __frcp_rn(s);
+      if (threadIdx.x == 0) scales[m] = s;
+      for (int k = threadIdx.x; k < p.K / 8; k += kFewThreads) {
+        float f[8];
+        unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
+        *reinterpret_cast<uint2*>(codes + m * stride + 8 * k) = codes8(f, s, inv);
+      }
+      __syncthreads();
+    }
+  }
+  int acc[kTokenTiles][4] = {};
+  for (int j0 = warp; j0 < pieces; j0 += kFewAhead * kFewWarps) {
+#pragma unroll
+    for (int i = 0; i < kFewAhead; ++i) {
+      const int j = j0 + i * kFewWarps;
+      if (j >= pieces) break;
+      const uint4 u = r0[i], v = r1[i];
+      const int next = j + kFewAhead * kFewWarps;
+      if (next < pieces) {
+        r0[i] = piece(w0, next);
+        r1[i] = piece(w1, next);
+      }
+#pragma unroll
+      for (int t = 0; t < kTokenTiles; ++t) {
+        const int m = 8 * t + g;
+        uint4 b = make_uint4(0, 0, 0, 0);
+        if (m < p.M && 64 * j + 16 * c < p.K) {
+          if constexpr (kFused) b = *reinterpret_cast<const uint4*>(codes + m * stride + 64 * j + 16 * c);
+          else b = __ldg(reinterpret_cast<const uint4*>(a + static_cast<int64_t>(m) * p.K + 64 * j + 16 * c));
+        }
+        mma16832(acc[t], u.x, v.x, u.y, v.y, b.x, b.y);
+        mma16832(acc[t], u.z, v.z, u.w, v.w, b.z, b.w);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < kTokenTiles; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) part[warp][g + 8 * (e >> 1)][8 * t + 2 * c + (e & 1)] = acc[t][e];
+  __syncthreads();
+  constexpr int kOut = kEpi == kSwiGLU ? 8 : 16;  // output columns of the CTA
+  for (int e = threadIdx.x; e < kOut * kTokens; e += kFewThreads) {
+    const int m = e / kOut, r = e % kOut, n = n0 + r;
+    if (m >= p.M || n >= width) continue;
+    const float sa = kFused ? scales[m] : __ldg(p.sa + m);
+    auto value = [&](int row, int col) {
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < kFewWarps; ++i) sum += part[i][row][m];
+      return fmaf(__int2float_rn(sum), sa * __ldg(p.sw + col), p.bias ? load_as_float(p.bias + col) : 0.f);
+    };
+    float y = value(r, n);
+    if constexpr (kEpi == kGeluErf) y = gelu_erf(y);
+    if constexpr (kEpi == kGeluTanh) y = gelu_tanh(y);
+    if constexpr (kEpi == kSwiGLU) y = swiglu(y, value(r + 8, n + width));
+    if constexpr (kEpi == kGated) {
+      const int64_t at = __ldg(p.idx + m % p.idx_rows);
+      const bool known = at >= 0 && at < p.table_rows;
+      const float gt = known ? load_as_float(p.gate + at * p.ldg + n) : CUDART_NAN_F;
+      y = fmaf(gt, y, load_as_float(p.residual + m * p.ldr + n));
+    }
+    const uint32_t packed = pack2<T>(y, 0.f);
+    p.out[m * p.ldo + n] = *reinterpret_cast<const T*>(&packed);
+  }
+}
+
+template <typename T, int kEpi, bool kFused>
+int launch_few(const void* a, const void* w, const Params<T>& p, const T* x, int64_t ldx, cudaStream_t st) {
+  const int8_t* ap = static_cast<const int8_t*>(a);
+  const int8_t* wp = static_cast<const int8_t*>(w);
+  const unsigned grid = static_cast<unsigned>(kEpi == kSwiGLU ? cdiv(p.N / 2, 8) : cdiv(p.N, 16));
+  const size_t smem = kFused ? static_cast<size_t>(p.M) * (p.K + 64) : 0;
+  if (p.M <= 8) few_int8_kernel<T, kEpi, 1, kFused><<<grid, kFewThreads, smem, st>>>(ap, wp, p, x, ldx);
+  else if (p.M <= 16) few_int8_kernel<T, kEpi, 2, kFused><<<grid, kFewThreads, smem, st>>>(ap, wp, p, x, ldx);
+  else few_int8_kernel<T, kEpi, 4, kFused><<<grid, kFewThreads, smem, st>>>(ap, wp, p, x, ldx);
+  return launch_status();
+}
+
+// Tokens that a call may quantise within the product: codes of all of them in
+// the 32 KB of shared memory that need no opting in, and little work.
+inline bool fuses(int64_t m, int64_t k) { return m <= kFewMost && m * k <= kFusedMost && m * (k + 64) <= 32 * 1024; }
+
+// x: the tokens to quantise within the product (null: `a` and p.sa hold their
+// codes and scales).
+template <typename T, int kEpi>
+int run(const void* a, const void* w, const Params<T>& p, const T* x, int64_t ldx, cudaStream_t st) {
+  if (x) return launch_few<T, kEpi, true>(a, w, p, x, ldx, st);
+  if (p.M <= kFewMost) return launch_few<T, kEpi, false>(a, w, p, x, ldx, st);
+  return launch_form<T, kEpi>(a, w, p, st);
+}
+
+template <typename T>
+int pick(int epilogue, const void* a, const void* w, const Params<T>& p, const T* x, int64_t ldx, cudaStream_t st) {
+  switch (epilogue) {
+    case kPlain: return run<T, kPlain>(a, w, p, x, ldx, st);
+    case kGeluErf: return run<T, kGeluErf>(a, w, p, x, ldx, st);
+    case kGeluTanh: return run<T, kGeluTanh>(a, w, p, x, ldx, st);
+    case kSwiGLU: return run<T, kSwiGLU>(a, w, p, x, ldx, st);
+    default: return run<T, kGated>(a, w, p, x, ldx, st);
+  }
 }
 
 constexpr int kQuantThreads = 256;
@@ -474,55 +818,124 @@ XGB_API int xgb_int8_quantize_per_token(const void* x, int dtype, int64_t rows, 
              : int8::quantize(static_cast<const __half*>(x), row_stride, rows, cols, out, scales, st);
 }
 
-template <typename T>
-static int run_int8_gemm(const int8_t* a, const int8_t* w, int64_t M, int64_t N, int64_t K, const float* scale_a,
-                         const float* scale_w, const void* bias, int epilogue, void* out, int64_t ldo, const void* gate,
-                         int64_t ldg, const int64_t* gate_index, int64_t index_rows, int64_t table_rows,
-                         const void* residual, int64_t ldr, int* error_flag, cudaStream_t st) {
-  int8::Params<T> p{};
-  p.M = static_cast<int>(M);
-  p.N = static_cast<int>(N);
-  p.K = static_cast<int>(K);
-  p.sa = scale_a;
-  p.sw = scale_w;
-  p.bias = static_cast<const T*>(bias);
-  p.out = static_cast<T*>(out);
-  p.ldo = ldo;
-  p.gate = static_cast<const T*>(gate);
-  p.ldg = ldg;
-  p.idx = gate_index;
-  p.idx_rows = static_cast<int>(index_rows);
-  p.table_rows = table_rows;
-  p.residual = static_cast<const T*>(residual);
-  p.ldr = ldr;
-  p.err = error_flag;
-  const auto a16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; };
-  p.vec = (!bias || a16(bias)) && (!gate || (a16(gate) && a16(residual) && ldg % 8 == 0 && ldr % 8 == 0));
-  return int8::pick<T>(epilogue, a, w, p, st);
+namespace {
+
+struct Call {
+  const int8_t* a;
+  const int8_t* w;
+  int64_t M, N, K;
+  const float* scale_a;
+  const float* scale_w;
+  int dtype;
+  const void* bias;
+  int activation;
+  void* out;
+  int64_t ldo;
+  const void* gate;
+  int64_t ldg;
+  const int64_t* gate_index;
+  int64_t index_rows, table_rows;
+  const void* residual;
+  int64_t ldr;
+  int* error_flag;
+  cudaStream_t st;
+};
+
+inline bool a16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0; }
+
+int check(const Call& c) {
+  if (!c.w || !c.scale_w || !c.out) return XGB_ERR_ARG;
+  if (c.dtype != XGB_BF16 && c.dtype != XGB_F16) return XGB_ERR_ARG;
+  if (c.M <= 0 || c.N <= 0 || c.K <= 0 || c.M > INT32_MAX - 256 || c.N > INT32_MAX - 512 || c.K > int8::kMaxK)
+    return XGB_ERR_SHAPE;
+  if (c.K % 16 || c.N % 16) return XGB_ERR_SHAPE;  // 16-byte TMA rows and output vectors
+  if (c.activation < 0 || c.activation > 3) return XGB_ERR_ARG;
+  const bool gated = c.gate != nullptr;
+  if (gated && (c.activation != 0 || !c.gate_index || !c.residual || c.index_rows <= 0 || c.index_rows > INT32_MAX ||
+                c.M % c.index_rows || c.table_rows <= 0))
+    return XGB_ERR_ARG;
+  if (c.ldo < (c.activation == 3 ? c.N / 2 : c.N) || c.ldo % 8 || (gated && (c.ldg < c.N || c.ldr < c.N)))
+    return XGB_ERR_STRIDE;
+  if (!a16(c.w) || !a16(c.out)) return XGB_ERR_ALIGN;
+  return XGB_OK;
 }
+
+int check_device() {
+  int dev = 0, major = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10)
+    return XGB_ERR_DEVICE;
+  return XGB_OK;
+}
+
+template <typename T>
+int product(const Call& c, const void* x, int64_t ldx) {
+  int8::Params<T> p{};
+  p.M = static_cast<int>(c.M);
+  p.N = static_cast<int>(c.N);
+  p.K = static_cast<int>(c.K);
+  p.sa = c.scale_a;
+  p.sw = c.scale_w;
+  p.bias = static_cast<const T*>(c.bias);
+  p.out = static_cast<T*>(c.out);
+  p.ldo = c.ldo;
+  p.gate = static_cast<const T*>(c.gate);
+  p.ldg = c.ldg;
+  p.idx = c.gate_index;
+  p.idx_rows = static_cast<int>(c.index_rows);
+  p.table_rows = c.table_rows;
+  p.residual = static_cast<const T*>(c.residual);
+  p.ldr = c.ldr;
+  p.err = c.error_flag;
+  p.vec = (!c.bias || a16(c.bias)) && (!c.gate || (a16(c.gate) && a16(c.residual) && c.ldg % 8 == 0 && c.ldr % 8 == 0));
+  p.vec_scale = a16(c.scale_w);
+  return int8::pick<T>(c.gate ? int8::kGated : c.activation, c.a, c.w, p, static_cast<const T*>(x), ldx, c.st);
+}
+
+}  // namespace
 
 XGB_API int xgb_int8_gemm(const int8_t* a, const int8_t* w, int64_t M, int64_t N, int64_t K, const float* scale_a,
                           const float* scale_w, int dtype, const void* bias, int activation, void* out, int64_t ldo,
                           const void* gate, int64_t ldg, const int64_t* gate_index, int64_t index_rows, int64_t table_rows,
                           const void* residual, int64_t ldr, int* error_flag, void* stream) {
-  if (!a || !w || !scale_a || !scale_w || !out) return XGB_ERR_ARG;
-  if (dtype != XGB_BF16 && dtype != XGB_F16) return XGB_ERR_ARG;
-  if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX - 256 || N > INT32_MAX - 512 || K > int8::kMaxK) return XGB_ERR_SHAPE;
-  if (K % 16 || N % 16) return XGB_ERR_SHAPE;  // 16-byte TMA rows and output vectors
-  if (activation < 0 || activation > 3) return XGB_ERR_ARG;
-  const bool swiglu = activation == 3, gated = gate != nullptr;
-  if (gated && (activation != 0 || !gate_index || !residual || index_rows <= 0 || index_rows > INT32_MAX ||
-                M % index_rows || table_rows <= 0))
-    return XGB_ERR_ARG;
-  if (ldo < (swiglu ? N / 2 : N) || ldo % 8 || (gated && (ldg < N || ldr < N))) return XGB_ERR_STRIDE;
-  if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(out)) & 15u)
-    return XGB_ERR_ALIGN;
-  int dev = 0, major = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10)
-    return XGB_ERR_DEVICE;
-  const int epilogue = gated ? int8::kGated : activation;
-  const auto run = dtype == XGB_BF16 ? run_int8_gemm<__nv_bfloat16> : run_int8_gemm<__half>;
-  return run(a, w, M, N, K, scale_a, scale_w, bias, epilogue, out, ldo, gate, ldg, gate_index, index_rows, table_rows,
-             residual, ldr, error_flag, as_stream(stream));
+  const Call c{a, w, M, N, K, scale_a, scale_w, dtype, bias, activation, out, ldo, gate, ldg, gate_index, index_rows,
+               table_rows, residual, ldr, error_flag, as_stream(stream)};
+  if (!a || !scale_a) return XGB_ERR_ARG;
+  int rc = check(c);
+  if (rc) return rc;
+  if (!a16(a)) return XGB_ERR_ALIGN;
+  if ((rc = check_device())) return rc;
+  return dtype == XGB_BF16 ? product<__nv_bfloat16>(c, nullptr, 0) : product<__half>(c, nullptr, 0);
+}
+
+XGB_API int64_t xgb_int8_linear_workspace(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  return cdiv(M * K, 16) * 16 + M * static_cast<int64_t>(sizeof(float));
+}
+
+XGB_API int xgb_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t M, int64_t N, int64_t K,
+                            const float* scale_w, int dtype, const void* bias, int activation, void* out, int64_t ldo,
+                            const void* gate, int64_t ldg, const int64_t* gate_index, int64_t index_rows,
+                            int64_t table_rows, const void* residual, int64_t ldr, void* workspace, int64_t workspace_bytes,
+                            int* error_flag, void* stream) {
+  Call c{nullptr, w, M, N, K, nullptr, scale_w, dtype, bias, activation, out, ldo, gate, ldg, gate_index, index_rows,
+         table_rows, residual, ldr, error_flag, as_stream(stream)};
+  if (!x) return XGB_ERR_ARG;
+  int rc = check(c);
+  if (rc) return rc;
+  if (M > 1 && ldx < K) return XGB_ERR_STRIDE;
+  if (!workspace || workspace_bytes < xgb_int8_linear_workspace(M, K)) return XGB_ERR_WORKSPACE;
+  if (!a16(workspace)) return XGB_ERR_ALIGN;
+  if ((rc = check_device())) return rc;
+  const bool bf16 = dtype == XGB_BF16;
+  if (int8::fuses(M, K) && a16(x) && (M == 1 || ldx % 8 == 0))
+    return bf16 ? product<__nv_bfloat16>(c, x, ldx) : product<__half>(c, x, ldx);
+  int8_t* codes = static_cast<int8_t*>(workspace);
+  float* scales = reinterpret_cast<float*>(codes + cdiv(M * K, 16) * 16);
+  rc = bf16 ? int8::quantize(static_cast<const __nv_bfloat16*>(x), ldx, M, K, codes, scales, c.st)
+            : int8::quantize(static_cast<const __half*>(x), ldx, M, K, codes, scales, c.st);
+  if (rc) return rc;
+  c.a = codes;
+  c.scale_a = scales;
+  return bf16 ? product<__nv_bfloat16>(c, nullptr, 0) : product<__half>(c, nullptr, 0);
 }

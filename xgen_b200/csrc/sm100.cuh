@@ -236,6 +236,16 @@ __device__ __forceinline__ void mma_pair_f8f6f4(uint32_t d_tmem, uint64_t a_desc
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc));
 }
 
+// The same for int8 operands and 32-bit integer sums.
+__device__ __forceinline__ void mma_pair_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            bool accumulate) {
+  const uint32_t acc = accumulate ? 1u : 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc));
+}
+
 // ---------------------------------------------------------------- UMMA
 enum class Kind { kF16, kI8, kF8F6F4 };
 

@@ -12,10 +12,8 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ._lib import call
 from .attention import _err_ptr
-from .ops import (_DTYPE_CODE, _on_device_of, _refuse_autograd, _require_cuda, _same_device, _stream,
-                  quantize_per_token_int8)
+from .ops import _DTYPE_CODE, _call_on, _device_of, _refuse_autograd, _row_stride
 
 ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "swiglu": 3}
 MAX_IN_FEATURES = 131056  # sums of 128 * 128 * K stay within 32-bit integers
@@ -29,39 +27,33 @@ def quantize_per_channel_int8(value: torch.Tensor):
     return (value.float() / scale[:, None]).round().clamp(-127, 127).to(torch.int8), scale
 
 
-def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
-                          weight_scale: torch.Tensor, bias=None, *, activation: str | None = None, gate=None,
-                          gate_index=None, residual=None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """int8_linear on activations that are already int8: codes [..., in] and
-    scales [...] (quantize_per_token_int8, or sandwich_norm with
-    quant="int8"). dtype: bf16 or fp16, the type of the result and of bias,
-    gate and residual."""
+def _arguments(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index, residual):
+    """Checks what int8_linear and int8_linear_quantized share; `lead` is the
+    input's shape without its channels. Returns (rows, weight, weight_scale,
+    arguments of the epilogue, output [rows, width])."""
     what = "H3 INT8 Linear"
-    given = [t for t in (bias, gate, gate_index, residual) if t is not None]
-    _require_cuda(codes, scales, weight, weight_scale, *given, what=what)
-    _refuse_autograd(bias, gate, residual, weight_scale, scales, what=what)
-    _same_device(codes, scales, weight, weight_scale, *given, what=what)
-    if codes.dtype != torch.int8 or weight.dtype != torch.int8 or weight.ndim != 2 or dtype not in _DTYPE_CODE:
-        raise ValueError(f"{what} requires int8 codes, an int8 [out, in] weight and a bf16/fp16 result")
+    if weight.dtype != torch.int8 or weight.ndim != 2 or dtype not in _DTYPE_CODE:
+        raise ValueError(f"{what} requires an int8 [out, in] weight and a bf16/fp16 result")
     n, k = weight.shape
     if n % 16 or k % 16 or not n or not k or k > MAX_IN_FEATURES:
         raise ValueError(f"{what} requires projection dimensions divisible by 16 (in <= {MAX_IN_FEATURES})")
-    if codes.ndim < 1 or codes.shape[-1] != k or scales.shape != codes.shape[:-1]:
-        raise ValueError(f"{what} input width does not match its weight, or its scales do not match its rows")
-    if scales.dtype != torch.float32 or weight_scale.dtype != torch.float32 or weight_scale.shape != (n,):
-        raise ValueError(f"{what} requires fp32 scales, one for each row and output channel")
-    if activation not in ACTIVATIONS:
+    if weight_scale.dtype != torch.float32 or weight_scale.shape != (n,):
+        raise ValueError(f"{what} requires an fp32 scale for each output channel")
+    code = ACTIVATIONS.get(activation, -1)
+    if code < 0:
         raise ValueError(f"Unknown {what} activation: {activation}")
-    width = n // 2 if activation == "swiglu" else n
-    if bias is not None and (bias.shape != (n,) or bias.dtype != dtype):
-        raise ValueError(f"{what} requires a bias [out] of the result's type")
-    m = codes.numel() // k
+    width = n // 2 if code == 3 else n
+    if bias is not None:
+        if bias.shape != (n,) or bias.dtype != dtype:
+            raise ValueError(f"{what} requires a bias [out] of the result's type")
+        bias = bias.contiguous()
+    m = lead.numel()
     ldg = ldr = rows = index_rows = 0
     if gate is not None or gate_index is not None or residual is not None:
-        if gate is None or gate_index is None or residual is None or activation is not None:
+        if gate is None or gate_index is None or residual is None or code:
             raise ValueError(f"gated {what} needs gate rows, their index and a residual, and no activation")
         if (gate.ndim != 2 or gate.shape[1] != n or gate.shape[0] == 0 or gate.dtype != dtype or gate.stride(1) != 1
-                or residual.dtype != dtype or residual.shape != (*codes.shape[:-1], n) or residual.stride(-1) != 1):
+                or residual.dtype != dtype or residual.shape != (*lead, n) or residual.stride(-1) != 1):
             raise ValueError(f"gated {what} needs [M, out] gate rows and a residual of the result's shape and type")
         index_rows = gate_index.numel()
         if gate_index.dtype != torch.int64 or (m and (index_rows == 0 or m % index_rows)):
@@ -72,20 +64,39 @@ def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: tor
             gate = gate.contiguous()
         if m > 1 and residual.stride(0) < n:
             residual = residual.contiguous()
-        ldg = gate.stride(0) if rows > 1 else n
-        ldr = residual.stride(0) if m > 1 else n
-    out = torch.empty((m, width), device=codes.device, dtype=dtype)
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+        ldg, ldr = _row_stride(gate, n), residual.stride(0) if m > 1 else n
+    out = torch.empty((m, width), device=weight.device, dtype=dtype)
+    epilogue = (_DTYPE_CODE[dtype], bias, code, out, width, gate, ldg, gate_index, index_rows, rows, residual, ldr)
+    return m, weight.contiguous(), weight_scale.contiguous(), epilogue, out
+
+
+def _pointers(epilogue):
+    return [t.data_ptr() if isinstance(t, torch.Tensor) else t for t in epilogue]
+
+
+def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
+                          weight_scale: torch.Tensor, bias=None, *, activation: str | None = None, gate=None,
+                          gate_index=None, residual=None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """int8_linear on activations that are already int8: codes [..., in] and
+    scales [...] (quantize_per_token_int8, or sandwich_norm with
+    quant="int8"). dtype: bf16 or fp16, the type of the result and of bias,
+    gate and residual."""
+    what = "H3 INT8 Linear"
+    index = _device_of(what, codes, scales, weight, weight_scale, bias, gate, gate_index, residual)
+    _refuse_autograd(what, scales, weight_scale, bias, gate, residual)
+    if codes.dtype != torch.int8 or codes.ndim < 1 or weight.ndim != 2 or codes.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what} requires int8 codes of its weight's width")
+    lead = codes.shape[:-1]
+    if scales.dtype != torch.float32 or scales.shape != lead:
+        raise ValueError(f"{what} requires an fp32 scale for each row of codes")
+    m, weight, weight_scale, epilogue, out = _arguments(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index,
+                                                        residual)
+    n, k = weight.shape
     if m:
         flat, scales = codes.reshape(m, k).contiguous(), scales.reshape(m).contiguous()
-        weight, weight_scale = weight.contiguous(), weight_scale.contiguous()
-        bias = bias.contiguous() if bias is not None else None
-        with _on_device_of(codes):
-            call("xgb_int8_gemm", flat.data_ptr(), weight.data_ptr(), m, n, k, scales.data_ptr(),
-                 weight_scale.data_ptr(), _DTYPE_CODE[dtype], ptr(bias), ACTIVATIONS[activation], out.data_ptr(), width,
-                 ptr(gate), ldg, ptr(gate_index), index_rows, rows, ptr(residual), ldr,
-                 _err_ptr(codes.device), _stream(codes))
-    return out.reshape(*codes.shape[:-1], width)
+        _call_on(index, "xgb_int8_gemm", flat.data_ptr(), weight.data_ptr(), m, n, k, scales.data_ptr(), weight_scale.data_ptr(),
+                 *_pointers(epilogue), _err_ptr(codes.device))
+    return out.view(*lead, out.shape[1])
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias=None, *,
@@ -101,16 +112,24 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
     Each token's largest magnitude becomes 127; sums are exact, one rounding."""
     what = "H3 INT8 Linear"
-    _require_cuda(x, what=what)
+    index = _device_of(what, x, weight, weight_scale, bias, gate, gate_index, residual)
+    _refuse_autograd(what, x, weight_scale, bias, gate, residual)
     if x.dtype not in _DTYPE_CODE or x.ndim < 1 or weight.ndim != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"{what} requires BF16/FP16 input of its weight's width")
-    matrix = x.reshape(-1, x.shape[-1])
-    if matrix.shape[0] > 1 and (matrix.stride(-1) != 1 or matrix.stride(0) < matrix.shape[1]):
-        matrix = matrix.contiguous()
-    codes, scales = quantize_per_token_int8(matrix)
-    return int8_linear_quantized(codes.view(x.shape), scales.view(x.shape[:-1]), weight, weight_scale, bias,
-                                 activation=activation, gate=gate, gate_index=gate_index, residual=residual,
-                                 dtype=x.dtype)
+    lead = x.shape[:-1]
+    m, weight, weight_scale, epilogue, out = _arguments(lead, x.dtype, weight, weight_scale, bias, activation, gate, gate_index,
+                                                        residual)
+    n, k = weight.shape
+    if m:
+        matrix = x.reshape(m, k)
+        if matrix.stride(1) != 1 or (m > 1 and matrix.stride(0) < k):
+            matrix = matrix.contiguous()
+        # codes and scales, laid out as xgb_int8_linear_workspace() says
+        ws_bytes = (m * k + 15) // 16 * 16 + 4 * m
+        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
+        _call_on(index, "xgb_int8_linear", matrix.data_ptr(), matrix.stride(0), weight.data_ptr(), m, n, k,
+                 weight_scale.data_ptr(), *_pointers(epilogue), ws.data_ptr(), ws_bytes, _err_ptr(x.device))
+    return out.view(*lead, out.shape[1])
 
 
 class H3Int8Linear(nn.Module):

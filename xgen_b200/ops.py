@@ -8,7 +8,7 @@ non-CUDA tensors raise ValueError (or return None where the reference's
 """
 from __future__ import annotations
 
-import contextlib
+import functools
 
 import torch
 
@@ -17,6 +17,8 @@ from ._lib import call, f64_array, i64_array
 
 _DTYPE_CODE = {torch.bfloat16: _lib.XGB_BF16, torch.float16: _lib.XGB_F16}
 _DTYPE_CODE_F32 = {**_DTYPE_CODE, torch.float32: _lib.XGB_F32}
+_raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
+_I64x2, _I64x3 = _lib.c_i64 * 2, _lib.c_i64 * 3
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -29,22 +31,32 @@ def _require_cuda(*tensors: torch.Tensor, what: str) -> None:
             raise ValueError(f"{what} requires CUDA tensors")
 
 
-def _refuse_autograd(*tensors, what: str) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
+def _device_of(what: str, *tensors) -> int:
+    """Index of the one GPU that all tensors (None: not given) are on."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != index or index < 0:
+            if any(x is not None and not x.is_cuda for x in tensors):
+                raise ValueError(f"{what} requires CUDA tensors")
+            raise ValueError(f"{what} needs its tensors on one device")
+    return index
 
 
-def _on_device_of(t: torch.Tensor):
-    """Context in which `t`'s device is the current one: launches go to the
-    current device, whatever the stream they are given."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _refuse_autograd(what: str, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
 
 
-def _same_device(first: torch.Tensor, *others, what: str) -> None:
-    if any(t is not None and t.device != first.device for t in others):
-        raise ValueError(f"{what} needs its tensors on one device")
+def _call_on(index: int, name: str, *args) -> None:
+    """call(name, *args, stream) with device `index` current (launches go to
+    the current device, whatever their stream) and on its current stream."""
+    if index == torch.cuda.current_device():
+        call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            call(name, *args, _raw_stream(index))
 
 
 def try_h3_partial_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
@@ -274,54 +286,68 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     32-bit arithmetic, one rounding at the end (the try_h3_* operators round
     after every step, as the reference does). Returns contiguous (query, key)."""
     what = "rotary positions"
-    _require_cuda(query, positions, *(() if key is None else (key,)), what=what)
-    _refuse_autograd(query, key, what=what)
-    axes = tuple(int(a) for a in axes)
-    thetas = tuple(float(t) for t in theta) if isinstance(theta, (tuple, list)) else (float(theta),) * len(axes)
-    if query.dtype not in _DTYPE_CODE_F32:
-        raise ValueError(f"{what} need bf16, fp16 or fp32 queries")
-    for t in (query,) if key is None else (query, key):
-        if t.ndim != 4 or t.dtype != query.dtype or (t.stride(-1) != 1 and t.shape[-1] > 1):
-            raise ValueError(f"{what} need [B, S, H, D] views of one type with unit channel stride")
+    w_q, eps_q = _norm_of(norm_q, query)
+    w_k, eps_k = _norm_of(norm_k, query) if key is not None else (None, 0.0)
+    index = _device_of(what, query, key, positions, w_q, w_k)
+    _refuse_autograd(what, query, key, w_q, w_k)
+    code = _DTYPE_CODE_F32.get(query.dtype)
+    if code is None or query.ndim != 4:
+        raise ValueError(f"{what} need bf16, fp16 or fp32 queries [B, S, H, D]")
     b, s, h, d = query.shape
-    if key is not None and (key.shape[:2] != query.shape[:2] or key.shape[-1] != d):
-        raise ValueError(f"{what}: query and key differ in batch, sequence or head dim")
-    if not axes or any(a <= 0 or a % 2 for a in axes) or sum(axes) > d or len(thetas) != len(axes) or not all(
-            0 < t < float("inf") for t in thetas):
-        raise ValueError(f"{what} need positive even axis channels within the head dim and a positive theta for each axis")
-    if positions.dtype not in _POSITION_CODE or positions.shape not in ((s, len(axes)), (b, s, len(axes))):
+    qs = query.stride()
+    if qs[3] != 1 and d > 1:
+        raise ValueError(f"{what} need views with unit channel stride")
+    axes, channels, thetas, rotary = _axes_of(axes if type(axes) is tuple else tuple(axes),
+                                              tuple(theta) if type(theta) is list else theta)
+    if rotary > d:
+        raise ValueError(f"{what} need axis channels within the head dim")
+    at = _POSITION_CODE.get(positions.dtype)
+    ps = positions.shape
+    if at is None or not (ps == (s, axes) or ps == (b, s, axes)):
         raise ValueError(f"{what}: positions must be integers or 32/64-bit floats of shape [S, A] or [B, S, A]")
-    if positions.stride(-1) != 1 and len(axes) > 1:
+    if axes > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    weights, eps = [], []
-    for norm in (norm_q, norm_k if key is not None else None):
-        if norm is None:
-            weights.append(None)
-            eps.append(0.0)
-            continue
-        if type(norm) is not torch.nn.RMSNorm or tuple(norm.normalized_shape) != (d,) or norm.weight is None or (
-                norm.weight.dtype != query.dtype) or not norm.weight.is_contiguous():
-            raise ValueError(f"{what}: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
-        _require_cuda(norm.weight, what=what)
-        weights.append(norm.weight)
-        eps.append(float(norm.eps if norm.eps is not None else torch.finfo(query.dtype).eps))
-    _refuse_autograd(*weights, what=what)
-    _same_device(query, key, positions, *weights, what=what)
-    q_out = torch.empty(query.shape, device=query.device, dtype=query.dtype)
-    k_out = torch.empty(key.shape, device=key.device, dtype=key.dtype) if key is not None else None
-    if not b * s * h * d:
-        if key is None or not key.numel():
-            return q_out, k_out
-        raise ValueError(f"{what} need at least one query head")
-    with _on_device_of(query):
-        call("xgb_rope_axes", query.data_ptr(), i64_array(query.stride()[:3]),
-             key.data_ptr() if key is not None else None,
-             i64_array(key.stride()[:3]) if key is not None else None, _DTYPE_CODE_F32[query.dtype], b, s, h,
-             key.shape[2] if key is not None else 0, d, positions.data_ptr(), _POSITION_CODE[positions.dtype],
-             positions.stride(0) if positions.ndim == 3 else 0, positions.stride(-2), len(axes), i64_array(axes),
-             f64_array(thetas), int(interleaved), *(w.data_ptr() if w is not None else None for w in weights), *eps,
-             q_out.data_ptr(), k_out.data_ptr() if key is not None else None, _stream(query))
+    q_out = torch.empty((b, s, h, d), device=query.device, dtype=query.dtype)
+    k_out = k_ptr = k_out_ptr = k_strides = None
+    kh = 0
+    if key is not None:
+        if key.ndim != 4 or key.dtype != query.dtype or (key.stride(-1) != 1 and d > 1):
+            raise ValueError(f"{what} need [B, S, H, D] views of one type with unit channel stride")
+        kh = key.shape[2]
+        if key.shape != (b, s, kh, d):
+            raise ValueError(f"{what}: query and key differ in batch, sequence or head dim")
+        k_out = torch.empty((b, s, kh, d), device=key.device, dtype=key.dtype)
+        k_ptr, k_out_ptr, k_strides = key.data_ptr(), k_out.data_ptr(), _I64x3(*key.stride()[:3])
+    if not b * s * d or not h or (key is not None and not kh):
+        if b * s * d and (h or kh):
+            raise ValueError(f"{what} need at least one head of query and key")
+        return q_out, k_out
+    _call_on(index, "xgb_rope_axes", query.data_ptr(), _I64x3(qs[0], qs[1], qs[2]), k_ptr, k_strides, code, b, s, h, kh, d,
+             positions.data_ptr(), at, positions.stride(0) if len(ps) == 3 else 0, positions.stride(-2), axes, channels,
+             thetas, int(interleaved), w_q.data_ptr() if w_q is not None else None,
+             w_k.data_ptr() if w_k is not None else None, eps_q, eps_k, q_out.data_ptr(), k_out_ptr)
     return q_out, k_out
+
+
+@functools.lru_cache(maxsize=256)
+def _axes_of(axes: tuple, theta):
+    """(number, channels and thetas as C arrays, sum) of the axes."""
+    axes = tuple(int(a) for a in axes)
+    thetas = tuple(float(t) for t in theta) if isinstance(theta, tuple) else (float(theta),) * len(axes)
+    if not axes or any(a <= 0 or a % 2 for a in axes) or len(thetas) != len(axes) or not all(
+            0 < t < float("inf") for t in thetas):
+        raise ValueError("rotary positions need positive even axis channels and a positive theta for each axis")
+    return len(axes), i64_array(axes), f64_array(thetas), sum(axes)
+
+
+def _norm_of(norm, query):
+    """(weight, eps) of a Q/K norm module, (None, 0) without one."""
+    if norm is None:
+        return None, 0.0
+    weight = norm.weight if type(norm) is torch.nn.RMSNorm else None
+    if weight is None or weight.shape != query.shape[-1:] or weight.dtype != query.dtype or not weight.is_contiguous():
+        raise ValueError("rotary positions: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
+    return weight, float(norm.eps if norm.eps is not None else torch.finfo(query.dtype).eps)
 
 
 _NORM_CODE = {None: 0, "layernorm": 1, "rmsnorm": 2}
@@ -350,56 +376,71 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
     32-bit arithmetic; x and h are rounded once each, h from the x before its
     rounding."""
     what = "sandwich norm"
-    tables = [t for t in (gate, scale, shift) if t is not None]
-    weights = [t for t in (post_weight, pre_weight) if t is not None]
-    extra = [indices] if indices is not None else []
-    _require_cuda(branch, residual, *tables, *weights, *extra, what=what)
-    _refuse_autograd(branch, residual, *tables, *weights, what=what)
-    _same_device(branch, residual, *tables, *weights, *extra, what=what)
-    if (branch.ndim != 3 or branch.shape != residual.shape or branch.dtype not in _DTYPE_CODE_F32
-            or residual.dtype != branch.dtype or any(t.stride(-1) != 1 and t.shape[-1] > 1 for t in (branch, residual))):
-        raise ValueError(f"{what} needs [B, S, W] branch and residual of one 16- or 32-bit float type with unit channel stride")
-    if post_norm not in _NORM_CODE or pre_norm not in _NORM_CODE or quant not in _QUANT_CODE:
-        raise ValueError(f"{what}: norms are 'layernorm', 'rmsnorm' or None, quant 'int8', 'e4m3' or None")
+    index = _device_of(what, branch, residual, post_weight, pre_weight, gate, scale, shift, indices)
+    _refuse_autograd(what, branch, residual, post_weight, pre_weight, gate, scale, shift)
+    dtype = branch.dtype
+    code = _DTYPE_CODE_F32.get(dtype)
+    if code is None or branch.ndim != 3 or branch.shape != residual.shape or residual.dtype != dtype:
+        raise ValueError(f"{what} needs [B, S, W] branch and residual of one 16- or 32-bit float type")
     b, s, w = branch.shape
+    bs, rs = branch.stride(), residual.stride()
+    if (bs[2] != 1 or rs[2] != 1) and w > 1:
+        raise ValueError(f"{what} needs views with unit channel stride")
     if w > 16384 or w == 0:
         raise ValueError(f"{what} takes rows of 1 to 16384 channels")
+    if post_norm not in _NORM_CODE or pre_norm not in _NORM_CODE or quant not in _QUANT_CODE:
+        raise ValueError(f"{what}: norms are 'layernorm', 'rmsnorm' or None, quant 'int8', 'e4m3' or None")
     if (scale is None) != (shift is None):
         raise ValueError(f"{what} needs scale and shift together")
     if pre_norm is None and (quant is not None or scale is not None or pre_weight is not None):
         raise ValueError(f"{what} without a norm before the next block has no modulation and no codes")
     if post_norm is None and post_weight is not None:
         raise ValueError(f"{what} without a norm after the block has no weight for it")
-    if any(t.ndim != 2 or t.shape[1] != w or t.dtype != branch.dtype or (t.stride(1) != 1 and w > 1)
-           or t.shape[0] != tables[0].shape[0] or t.shape[0] == 0 for t in tables):
-        raise ValueError(f"{what}: gate, scale and shift must be [M, W] rows of the branch's type")
-    if any(t.shape != (w,) or t.dtype != branch.dtype or not t.is_contiguous() for t in weights):
-        raise ValueError(f"{what}: weights must be contiguous [W] of the branch's type")
-    if bool(tables) != (indices is not None):
+    for t in (post_weight, pre_weight):
+        if t is not None and (t.shape != (w,) or t.dtype != dtype or not t.is_contiguous()):
+            raise ValueError(f"{what}: weights must be contiguous [W] of the branch's type")
+    table_rows = 0
+    for t in (gate, scale, shift):
+        if t is not None:
+            table_rows = table_rows or t.shape[0]
+            if t.ndim != 2 or t.shape != (table_rows, w) or t.dtype != dtype or (t.stride(1) != 1 and w > 1) or not table_rows:
+                raise ValueError(f"{what}: gate, scale and shift must be [M, W] rows of the branch's type")
+    if (table_rows > 0) != (indices is not None):
         raise ValueError(f"{what}: indices come with gate or scale and shift")
+    index_batch = 0
     if indices is not None:
-        if indices.dtype != torch.int64 or indices.shape not in ((s,), (b, s)):
+        if indices.dtype != torch.int64 or not (indices.shape == (s,) or indices.shape == (b, s)):
             raise ValueError(f"{what}: indices must be int64 [S] or [B, S]")
+        index_batch = s if indices.ndim == 2 else 0
         indices = indices.contiguous()
-    x_out = torch.empty((b, s, w), device=branch.device, dtype=branch.dtype)
-    code, code_type = _QUANT_CODE[quant]
-    h_out = torch.empty_like(x_out) if pre_norm is not None and code == 0 else None
-    codes = torch.empty((b, s, w), device=branch.device, dtype=code_type) if code else None
-    scales = torch.empty((b, s), device=branch.device, dtype=torch.float32) if code else None
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    # one row's stride is never stepped over
-    row = lambda t: (t.stride(0) if t.shape[0] > 1 else w) if t is not None else 0  # noqa: E731
+    x_out = torch.empty((b, s, w), device=branch.device, dtype=dtype)
+    quant_code, code_type = _QUANT_CODE[quant]
+    h_out = codes = scales = None
+    if quant_code:
+        codes = torch.empty((b, s, w), device=branch.device, dtype=code_type)
+        scales = torch.empty((b, s), device=branch.device, dtype=torch.float32)
+    elif pre_norm is not None:
+        h_out = torch.empty((b, s, w), device=branch.device, dtype=dtype)
     if b * s:
-        with _on_device_of(branch):
-            call("xgb_sandwich_norm", branch.data_ptr(), i64_array(branch.stride()[:2]), residual.data_ptr(),
-                 i64_array(residual.stride()[:2]), _DTYPE_CODE_F32[branch.dtype], b, s, w, _NORM_CODE[post_norm],
-                 ptr(post_weight), _NORM_CODE[pre_norm], ptr(pre_weight), float(eps), ptr(gate), row(gate),
-                 float(residual_scale), ptr(scale), row(scale), ptr(shift), row(shift), ptr(indices),
-                 s if indices is not None and indices.ndim == 2 else 0, tables[0].shape[0] if tables else 0,
-                 x_out.data_ptr(), ptr(h_out), code, ptr(codes), ptr(scales), _stream(branch))
+        _call_on(index, "xgb_sandwich_norm", branch.data_ptr(), _I64x2(bs[0], bs[1]), residual.data_ptr(), _I64x2(rs[0], rs[1]),
+                 code, b, s, w, _NORM_CODE[post_norm], _ptr(post_weight), _NORM_CODE[pre_norm], _ptr(pre_weight), eps,
+                 _ptr(gate), _row_stride(gate, w), residual_scale, _ptr(scale), _row_stride(scale, w), _ptr(shift),
+                 _row_stride(shift, w), _ptr(indices), index_batch, table_rows, x_out.data_ptr(), _ptr(h_out), quant_code,
+                 _ptr(codes), _ptr(scales))
     if pre_norm is None:
         return x_out
-    return (x_out, codes, scales) if code else (x_out, h_out)
+    return (x_out, codes, scales) if quant_code else (x_out, h_out)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _row_stride(t, width: int) -> int:
+    """Elements between the rows of a table; one row is never stepped over."""
+    if t is None:
+        return 0
+    return t.stride(0) if t.shape[0] > 1 else width
 
 
 def quantize_per_token_int8(x: torch.Tensor):
@@ -407,17 +448,15 @@ def quantize_per_token_int8(x: torch.Tensor):
     (codes, scales[rows]) with scale = max(amax/127, FLT_MIN) and codes the
     nearest integers to x / scale, ties to even."""
     what = "H3 INT8 quantization"
-    _require_cuda(x, what=what)
-    _refuse_autograd(x, what=what)
+    index = _device_of(what, x)
+    _refuse_autograd(what, x)
     if x.dtype not in _DTYPE_CODE or x.ndim != 2 or (x.stride(-1) != 1 and x.shape[1] > 1) or x.shape[1] == 0 or (
             x.shape[0] > 1 and x.stride(0) < x.shape[1]):
         raise ValueError(f"{what} requires a row-major 2-D bf16/fp16 matrix")
     rows, cols = x.shape
     out = torch.empty((rows, cols), device=x.device, dtype=torch.int8)
     scales = torch.empty((rows,), device=x.device, dtype=torch.float32)
-    if not rows:
-        return out, scales
-    with _on_device_of(x):
-        call("xgb_int8_quantize_per_token", x.data_ptr(), _DTYPE_CODE[x.dtype], rows, cols, x.stride(0),
-             out.data_ptr(), scales.data_ptr(), _stream(x))
+    if rows:
+        _call_on(index, "xgb_int8_quantize_per_token", x.data_ptr(), _DTYPE_CODE[x.dtype], rows, cols, x.stride(0),
+                 out.data_ptr(), scales.data_ptr())
     return out, scales
