@@ -15,9 +15,14 @@
 // The tiled kernels are persistent, K blocks of 128 bytes:
 //   warp 0     TMA producer
 //   warp 1     TMEM allocator + MMA issuer (of rank 0 in a pair)
-//   warps 2-9  epilogue: one thread per output row (TMEM lane) and column half
+//   warps 2-9  epilogue: one thread per output row (TMEM lane); warps 2-5 and
+//              6-9 each half of a tile's columns, or every other narrow tile
 // Two TMEM accumulators let the epilogue of one tile run under the MMAs of the
-// next. A W tile is two boxes of kBN/2 rows (in a pair, one of each CTA), so
+// next. A thread's row is 64 columns of shared memory at a time: the residual
+// comes in there by TMA ahead of the accumulators, the result takes its place
+// and leaves by TMA. (With rows read and written by their threads directly,
+// 32 lanes on 32 lines each, the gated epilogue took 98 us at 15845 x 2048 x
+// 2048 where the products need 40.) A W tile is two boxes of kBN/2 rows (in a pair, one of each CTA), so
 // the gate and value rows of a SwiGLU tile come from their two places in a
 // plain [gate | value] weight. Every mbarrier wait is bounded.
 //
@@ -28,6 +33,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
+#include <type_traits>
 
 #include "sm100.cuh"
 #include "tma_host.h"
@@ -45,6 +51,13 @@ constexpr int kABytes = kBM * kBK;
 constexpr int64_t kMaxK = 131056;
 constexpr int kRaster = 8;  // row tiles that a group of consecutive tiles shares
 
+constexpr int kChunk = 64;                    // output columns of a step of the epilogue
+constexpr int kChunkBytes = 32 * kChunk * 2;  // a warp's 32 rows of them
+constexpr int kOutBytes = kEpiThreads / 32 * 2 * kChunkBytes;  // two steps of every epilogue warp
+constexpr int kGroupCols = 128;                  // accumulator columns that a warpgroup takes of a tile, at most
+constexpr int kColBytes = kGroupCols * (4 + 2);  // their scales and biases
+constexpr int kGroupBar = 1;                     // named barriers 1, 2: an epilogue warpgroup
+
 // Shared memory of a CTA: per stage 128 rows of A and kBN (single) or kBN/2
 // (pair) rows of W; as many stages as fit.
 template <int kBN, bool kPair>
@@ -52,9 +65,11 @@ struct Cfg {
   static constexpr int kBoxRows = kBN / 2;
   static constexpr int kBoxBytes = kBoxRows * kBK;
   static constexpr int kStageBytes = kABytes + (kPair ? 1 : 2) * kBoxBytes;
-  static constexpr int kStages = 224 * 1024 / kStageBytes < 8 ? 224 * 1024 / kStageBytes : 8;
-  static constexpr int kBarOff = kStages * kStageBytes;
-  static constexpr int kSmem = kBarOff + 256 + 1024;
+  static constexpr int kStages = (224 * 1024 - kOutBytes) / kStageBytes < 8 ? (224 * 1024 - kOutBytes) / kStageBytes : 8;
+  static constexpr int kOutOff = kStages * kStageBytes;
+  static constexpr int kColOff = kOutOff + kOutBytes;
+  static constexpr int kBarOff = kColOff + 2 * kColBytes;
+  static constexpr int kSmem = kBarOff + 512 + 1024;
   static constexpr uint32_t kIdesc = instr_desc(2, 1, 1, false, false, kPair ? 2 * kBM : kBM, kBN);
   static constexpr uint32_t kTmemCols = 2 * kBN;
 };
@@ -62,8 +77,9 @@ struct Cfg {
 enum Epilogue : int { kPlain = 0, kGeluErf = 1, kGeluTanh = 2, kSwiGLU = 3, kGated = 4 };
 
 __device__ __forceinline__ float gelu_erf(float y) { return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f)); }
+// 0.5 (1 + tanh u) = 1 / (1 + e^-2u)
 __device__ __forceinline__ float gelu_tanh(float y) {
-  return 0.5f * y * (1.0f + tanhf(0.79788456080286536f * (y + 0.044715f * y * y * y)));
+  return __fdividef(y, 1.0f + __expf(-1.5957691216057308f * (y + 0.044715f * y * y * y)));
 }
 __device__ __forceinline__ float swiglu(float g, float v) { return __fdividef(g, 1.0f + __expf(-g)) * v; }
 
@@ -84,8 +100,7 @@ struct Params {
   const T* residual;
   int64_t ldr;
   int* err;
-  bool vec;        // bias, gate and residual may be read 16 bytes at a time (host-checked)
-  bool vec_scale;  // and sw
+  bool vec;  // gate and residual may be read 16 bytes at a time (host-checked)
 };
 
 struct Barriers {
@@ -94,6 +109,7 @@ struct Barriers {
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t end;
+  uint64_t residual[kEpiThreads / 32][2];
   uint32_t tmem_base;
 };
 
@@ -129,123 +145,152 @@ __device__ __forceinline__ uint4 load_raw8(const T* p, bool vec) {
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// Scaled and biased values of eight columns, whose scales and biases a
+// warpgroup keeps in shared memory (every thread reads the same ones).
 template <typename T>
-__device__ __forceinline__ void scaled8(const Params<T>& p, const uint32_t* acc, float sa, int n, float (&y)[8]) {
-  float sw[8], bias[8];
-  if (p.vec_scale) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p.sw + n)), b = __ldg(reinterpret_cast<const float4*>(p.sw + n) + 1);
-    sw[0] = a.x; sw[1] = a.y; sw[2] = a.z; sw[3] = a.w;
-    sw[4] = b.x; sw[5] = b.y; sw[6] = b.z; sw[7] = b.w;
-  } else {
+__device__ __forceinline__ void scaled8(const uint32_t* acc, float sa, const float* sw, const T* bias, float (&y)[8]) {
+  float s[8], b[8];
+  const float4 lo = reinterpret_cast<const float4*>(sw)[0], hi = reinterpret_cast<const float4*>(sw)[1];
+  s[0] = lo.x; s[1] = lo.y; s[2] = lo.z; s[3] = lo.w;
+  s[4] = hi.x; s[5] = hi.y; s[6] = hi.z; s[7] = hi.w;
+  unpack8(bias, *reinterpret_cast<const uint4*>(bias), b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sw[i] = __ldg(p.sw + n + i);
-  }
-  if (p.bias) {
-    unpack8(p.bias, load_raw8(p.bias + n, p.vec), bias);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bias[i] = 0.f;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = fmaf(__int2float_rn(static_cast<int>(acc[i])), sa * sw[i], bias[i]);
+  for (int i = 0; i < 8; ++i) y[i] = fmaf(__int2float_rn(static_cast<int>(acc[i])), sa * s[i], b[i]);
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* dst, const float (&y)[8]) {
-  *reinterpret_cast<uint4*>(dst) =
-      make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+__device__ __forceinline__ uint4 pack8(const float (&y)[8]) {
+  return make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
 }
 
-// What an output row needs besides the accumulators.
-template <typename T>
-struct Row {
-  float sa;
-  const T* gate;  // null factor row: outside the table
-  const T* residual;
-  T* out;
-  bool ok;     // the row exists
-  bool known;  // its index is inside the table
-};
-template <typename T, int kEpi>
-__device__ __forceinline__ Row<T> row_of(const Params<T>& p, int m) {
-  Row<T> r{};
-  r.ok = m < p.M;
-  r.known = true;
-  if (!r.ok) return r;
-  r.sa = __ldg(p.sa + m);
-  r.out = p.out + static_cast<int64_t>(m) * p.ldo;
-  if constexpr (kEpi == kGated) {
-    const int64_t at = __ldg(p.idx + m % p.idx_rows);
-    r.known = at >= 0 && at < p.table_rows;
-    r.gate = p.gate + (r.known ? at : 0) * p.ldg;
-    r.residual = p.residual + static_cast<int64_t>(m) * p.ldr;
-  }
-  return r;
-}
-
-// Gate and residual of 32 columns, requested before they are needed.
+// Gate values of a thread's row for one step, requested ahead of it.
 template <int kEpi>
-struct Ahead {
-  uint4 gate[kEpi == kGated ? 4 : 1], res[kEpi == kGated ? 4 : 1];
-};
-template <typename T, int kEpi>
-__device__ __forceinline__ void fetch(const Params<T>& p, const Row<T>& r, int n, Ahead<kEpi>& a) {
-  if constexpr (kEpi == kGated) {
-    if (!r.ok) return;
+struct Gates {
+  uint4 raw[kEpi == kGated ? kChunk / 8 : 1];
+  template <typename T>
+  __device__ __forceinline__ void load(const Params<T>& p, const T* gate, int n1, int width) {
+    if constexpr (kEpi == kGated) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      if (n + 8 * g >= p.N) break;
-      a.gate[g] = load_raw8(r.gate + n + 8 * g, p.vec);
-      a.res[g] = load_raw8(r.residual + n + 8 * g, p.vec);
+      for (int g = 0; g < kChunk / 8; ++g)
+        if (n1 + 8 * g < width) raw[g] = load_raw8(gate + n1 + 8 * g, p.vec);
     }
   }
-}
+};
 
-// One accumulator tile's epilogue for the output row this thread owns and the
-// column half `half`; n0 = the tile's first output column. `ahead` holds the
-// first 32 columns' gate and residual on entry.
+// An epilogue warp's walk over its steps of 32 rows x 64 columns.
 template <typename T, int kBN, int kEpi>
-__device__ __forceinline__ void epilogue_tile(const Params<T>& p, uint32_t acc, const Row<T>& row, int n0, int half,
-                                              Ahead<kEpi>& ahead) {
-  const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
-  constexpr int kChunks = (kEpi == kSwiGLU ? kBN / 2 : kBN) / 64;  // of 32 output columns, for each half
-#pragma unroll 1
-  for (int i = 0; i < kChunks; ++i) {
-    const int c = half * kChunks + i, n1 = n0 + c * 32;
-    uint32_t r[32], rv[kEpi == kSwiGLU ? 32 : 1];
-    tmem_ld32(acc + c * 32, r);
-    if constexpr (kEpi == kSwiGLU) tmem_ld32(acc + kBN / 2 + c * 32, rv);
-    Ahead<kEpi> now = ahead;
-    if (i + 1 < kChunks) fetch<T, kEpi>(p, row, n1 + 32, ahead);
+struct Steps {
+  static constexpr int kCols = kEpi == kSwiGLU ? kBN / 2 : kBN;
+  static constexpr bool kHalves = kCols >= 2 * kChunk;  // both warpgroups on each tile; else on every other one
+  static constexpr int kSteps = kHalves ? kCols / 2 / kChunk : 1;
+
+  const Params<T>& p;
+  const CUtensorMap* out_map;
+  const CUtensorMap* res_map;
+  uint8_t* buf;       // two steps
+  uint64_t* arrived;  // residual of each
+  const float* sw;    // scales and biases of the group's columns (SwiGLU: 64 gate, 64 value)
+  const T* bias;
+  int lane;
+  int used = 0;     // steps so far
+  int fetched = 0;  // of them requested
+
+  __device__ __forceinline__ int width() const { return kEpi == kSwiGLU ? p.N / 2 : p.N; }
+
+  // Requests the residual of a tile's steps, n1 = first column, m1 = first row.
+  __device__ __forceinline__ void fetch(int n1, int m1) {
+    if constexpr (kEpi == kGated) {
+      if (!p.vec || lane != 0) return;
+      bulk_wait_read<0>();  // earlier results have left the buffers
+      for (int i = 0; i < kSteps && n1 + i * kChunk < width(); ++i, ++fetched) {
+        const int b = fetched & 1;
+        mbar_arrive_expect_tx(&arrived[b], kChunkBytes);
+        tma_load_2d(buf + b * kChunkBytes, res_map, &arrived[b], n1 + i * kChunk, m1);
+      }
+    }
+  }
+
+  // After a failed wait: requested residuals still land before the CTA exits.
+  __device__ __forceinline__ void drain() {
+    for (; used < fetched; ++used) mbar_wait(&arrived[used & 1], (used >> 1) & 1, p.err, 100000000ull);
+  }
+
+  // One step: accumulators at `acc`, output columns n1.., rows m1 + lane.
+  // `free` is called when the accumulators have been read.
+  // `c` is the step's first column of the group, `gates` its gate values on
+  // entry and the next step's on return.
+  template <typename Free>
+  __device__ __forceinline__ bool step(uint32_t acc, int c, int n1, int m1, float sa, const T* gate, bool known,
+                                       Gates<kEpi>& gates, Free free) {
+    // SwiGLU takes its two accumulators 32 columns at a time, for registers
+    uint32_t r[2][32], rv[kEpi == kSwiGLU ? 32 : 1];
+    if constexpr (kEpi == kSwiGLU) {
+      tmem_ld32(acc, r[0]);
+      tmem_ld32(acc + kBN / 2, rv);
+    } else {
+      tmem_ld64(acc, r);
+    }
+    const int b = used & 1, m = m1 + lane;
+    uint8_t* row = buf + b * kChunkBytes + lane * kChunk * 2;
+    bool ok = true;
+    if constexpr (kEpi == kGated) {
+      if (p.vec) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&arrived[b], (used >> 1) & 1, p.err));
+      } else {
+        if (lane == 0) bulk_wait_read<1>();
+        __syncwarp();
+      }
+    } else {
+      if (lane == 0) bulk_wait_read<1>();
+      __syncwarp();
+    }
+    ++used;
     tmem_ld_wait();
-    if (!row.ok) continue;
+    if (kEpi != kSwiGLU) free();
+    if (!ok) return false;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < kChunk / 8; ++g) {
+      if (kEpi == kSwiGLU && g == 4) {
+        tmem_ld32(acc + 32, r[0]);
+        if constexpr (kEpi == kSwiGLU) tmem_ld32(acc + kBN / 2 + 32, rv);
+        tmem_ld_wait();
+        free();
+      }
       const int n = n1 + g * 8;
-      if (n >= width) break;
+      if (n >= width()) continue;
+      uint4* place = reinterpret_cast<uint4*>(row + ((g ^ (lane & 7)) << 4));  // 128-byte swizzle
       float y[8];
-      scaled8(p, r + 8 * g, row.sa, n, y);
+      scaled8<T>(&r[kEpi == kSwiGLU ? 0 : g >> 2][(g & 3) * 8], sa, sw + c + 8 * g, bias + c + 8 * g, y);
       if constexpr (kEpi == kSwiGLU) {
         float v[8];
-        scaled8(p, rv + 8 * g, row.sa, n + width, v);
+        scaled8<T>(&rv[(g & 3) * 8], sa, sw + kChunk + 8 * g, bias + kChunk + 8 * g, v);
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = swiglu(y[e], v[e]);
       }
       if constexpr (kEpi == kGated) {
         float gt[8], res[8];
-        unpack8(p.gate, now.gate[g], gt);
-        unpack8(p.gate, now.res[g], res);
+        unpack8(p.gate, gates.raw[g], gt);
+        if (p.vec) unpack8(p.gate, *place, res);
+        else unpack8(p.gate, load_raw8(p.residual + static_cast<int64_t>(min(m, p.M - 1)) * p.ldr + n, false), res);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = fmaf(row.known ? gt[e] : CUDART_NAN_F, y[e], res[e]);
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(known ? gt[e] : CUDART_NAN_F, y[e], res[e]);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         if constexpr (kEpi == kGeluErf) y[e] = gelu_erf(y[e]);
         if constexpr (kEpi == kGeluTanh) y[e] = gelu_tanh(y[e]);
       }
-      store8(row.out + n, y);
+      *place = pack8<T>(y);
     }
+    if (kSteps > 1) gates.load(p, gate, n1 + kChunk, width());
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(out_map, buf + b * kChunkBytes, n1, m1);
+      bulk_commit();
+    }
+    return true;
   }
-}
+};
 
 // Tile t of the walk: groups of kRaster row tiles, columns within a group, so
 // that tiles in flight share rows of A and of W in L2.
@@ -263,7 +308,9 @@ struct Walk {
 
 template <typename T, int kBN, int kEpi, bool kPair>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemm_int8_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map, const Params<T> p) {
+    gemm_int8_kernel(const __grid_constant__ CUtensorMap a_map, const __grid_constant__ CUtensorMap b_map,
+                     const __grid_constant__ CUtensorMap out_map, const __grid_constant__ CUtensorMap res_map,
+                     const Params<T> p) {
   using C = Cfg<kBN, kPair>;
   constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -273,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int lane = threadIdx.x & 31;
   const int rank = kPair ? static_cast<int>(cluster_rank()) : 0;
   const int64_t first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
-  constexpr int kCols = kEpi == kSwiGLU ? kBN / 2 : kBN;  // output columns of a tile
+  constexpr int kCols = Steps<T, kBN, kEpi>::kCols;  // output columns of a tile
   constexpr int kRowsOfTile = kPair ? 2 * kBM : kBM;
   const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
   const int second = kEpi == kSwiGLU ? width : kBN / 2;  // W rows from the first box to the second
@@ -288,8 +335,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&bars->acc_full[a], 1);
-      mbar_init(&bars->acc_empty[a], (kPair ? 2 : 1) * kEpiThreads / 32);
+      // every epilogue warp that reads the tile, of both CTAs of a pair
+      mbar_init(&bars->acc_empty[a], (kPair ? 2 : 1) * (Steps<T, kBN, kEpi>::kHalves ? 8 : 4));
     }
+    for (int e = 0; e < kEpiThreads / 32; ++e)
+      for (int b = 0; b < 2; ++b) mbar_init(&bars->residual[e][b], 1);
     mbar_init(&bars->end, 1);
     fence_barrier_init();
   }
@@ -381,27 +431,83 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ epilogue
-    const int quarter = warp & 3;      // TMEM lane quarter this warp may access
-    const int half = (warp - 2) >> 2;  // column half of the tile
+    using S = Steps<T, kBN, kEpi>;
+    const int quarter = warp & 3;       // TMEM lane quarter this warp may access
+    const int group = (warp - 2) >> 2;  // column half, or parity of the tiles
     const uint32_t lane_addr = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
-    int lt = 0;
-    for (int64_t t = first; t < tiles; t += step, ++lt) {
+    float* sw = reinterpret_cast<float*>(smem + C::kColOff + group * kColBytes);
+    T* bias = reinterpret_cast<T*>(sw + kGroupCols);
+    S steps{p, &out_map, &res_map, smem + C::kOutOff + (warp - 2) * 2 * kChunkBytes, bars->residual[warp - 2], sw, bias, lane};
+    // This thread's column of the group, of a tile; loaded a tile ahead.
+    const int mine = threadIdx.x - 64 - group * 128;
+    float next_sw = 0.f;
+    T next_bias = T(0.f);
+    auto load_column = [&](int64_t t) {
+      if (t >= tiles) return;
+      int mt, nt;
+      walk.at(t, mt, nt);
+      int n = nt * kCols + (S::kHalves ? group * (kCols / 2) : 0) + mine;
+      bool there = n < width;
+      if constexpr (kEpi == kSwiGLU) {  // 64 gate columns, then their values
+        n -= mine & kChunk;
+        there = n < width;
+        n += mine & kChunk ? width : 0;
+      }
+      next_sw = there ? __ldg(p.sw + n) : 0.f;
+      next_bias = there && p.bias ? p.bias[n] : T(0.f);
+    };
+    const int64_t skip = S::kHalves ? step : 2 * step, start = S::kHalves ? first : first + group * step;
+    load_column(start);
+    bool ok = true;
+    int lt = S::kHalves ? 0 : group;
+    for (int64_t t = start; t < tiles; t += skip, lt += S::kHalves ? 1 : 2) {
       const int a = lt & 1;
       int mt, nt;
       walk.at(t, mt, nt);
-      const int n0 = nt * kCols;
-      const Row<T> row = row_of<T, kEpi>(p, mt * kRowsOfTile + rank * kBM + quarter * 32 + lane);
-      Ahead<kEpi> ahead;
-      fetch<T, kEpi>(p, row, n0 + half * (kCols / 2), ahead);
-      if (!__all_sync(0xffffffffu, mbar_wait(&bars->acc_full[a], (lt >> 1) & 1, p.err))) break;
-      tc_fence_after();
-      epilogue_tile<T, kBN, kEpi>(p, lane_addr + a * kBN, row, n0, half, ahead);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (kPair) mbar_arrive_cluster(map_to_rank(&bars->acc_empty[a], 0));
-        else mbar_arrive(&bars->acc_empty[a]);
+      const int c0 = S::kHalves ? group * (kCols / 2) : 0;  // column of the tile
+      const int n1 = nt * kCols + c0, m1 = mt * kRowsOfTile + rank * kBM + quarter * 32, m = m1 + lane;
+      named_sync(kGroupBar + group, 128);  // the last tile's columns have been used
+      sw[mine] = next_sw;
+      bias[mine] = next_bias;
+      load_column(t + skip);
+      named_sync(kGroupBar + group, 128);
+      // After a failed wait the warps stay in step for these barriers and do
+      // nothing else.
+      if (!ok) continue;
+      steps.fetch(n1, m1);
+      const float sa = m < p.M ? __ldg(p.sa + m) : 0.f;
+      const T* gate = p.gate;
+      bool known = true;
+      Gates<kEpi> gates;
+      if constexpr (kEpi == kGated) {
+        const int64_t at = __ldg(p.idx + min(m, p.M - 1) % p.idx_rows);
+        known = at >= 0 && at < p.table_rows;
+        gate += (known ? at : 0) * p.ldg;
+        gates.load(p, gate, n1, width);
       }
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->acc_full[a], (lt >> 1) & 1, p.err));
+      if (!ok) continue;
+      tc_fence_after();
+      // the last step that has columns frees the accumulators
+      const int last = min(S::kSteps, (width - n1 + kChunk - 1) / kChunk) - 1;
+      auto release = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) mbar_arrive_cluster(map_to_rank(&bars->acc_empty[a], 0));
+          else mbar_arrive(&bars->acc_empty[a]);
+        }
+      };
+      if (last < 0) release();  // this half lies outside the matrix
+#pragma unroll 1
+      for (int i = 0; i <= last && ok; ++i)
+        ok = steps.step(lane_addr + a * kBN + c0 + i * kChunk, i * kChunk, n1 + i * kChunk, m1, sa, gate, known, gates, [&]() {
+          if (i == last) release();
+        });
+    }
+    if (lane == 0) {
+      steps.drain();
+      bulk_wait_all();  // the results have left
     }
   }
   tc_fence_before();
@@ -456,11 +562,24 @@ int launch(const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
   if (!make_tensor_map(&am, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, a, adims, str, abox) ||
       !make_tensor_map(&bm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, bdims, str, bbox))
     return XGB_ERR_ALIGN;
+  const int width = kEpi == kSwiGLU ? p.N / 2 : p.N;
+  constexpr auto kType = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                                 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap om, rm;
+  const uint64_t odims[2] = {static_cast<uint64_t>(width), static_cast<uint64_t>(p.M)};
+  const uint32_t obox[2] = {kChunk, 32};
+  const uint64_t ostr[1] = {static_cast<uint64_t>(p.ldo) * 2};
+  if (!make_tensor_map(&om, kType, 2, p.out, odims, ostr, obox)) return XGB_ERR_ALIGN;
+  rm = om;
+  if (kEpi == kGated && p.vec) {
+    const uint64_t rstr[1] = {static_cast<uint64_t>(p.ldr) * 2};
+    if (!make_tensor_map(&rm, kType, 2, p.residual, odims, rstr, obox)) return XGB_ERR_ALIGN;
+  }
   auto kernel = gemm_int8_kernel<T, kBN, kEpi, kPair>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
     return XGB_ERR_LAUNCH;
   const int cols = kEpi == kSwiGLU ? kBN / 2 : kBN, rows = kPair ? 2 * kBM : kBM;
-  const int64_t tiles = cdiv(p.M, rows) * cdiv(kEpi == kSwiGLU ? p.N / 2 : p.N, cols);
+  const int64_t tiles = cdiv(p.M, rows) * cdiv(width, cols);
   const int sms = sm_count();
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(kThreads);
@@ -478,34 +597,41 @@ int launch(const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
   } else {
     cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, sms)));
   }
-  if (cudaLaunchKernelEx(&cfg, kernel, am, bm, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, am, bm, om, rm, p) != cudaSuccess) {
     cudaGetLastError();
     return XGB_ERR_LAUNCH;
   }
   return launch_status();
 }
 
-// The tile shape: rounds of tiles over the SMs, each of k_blocks steps and an
-// epilogue that the last round does not hide.
-enum Form { kPair256, kPair128, kSingle128, kSingle64 };
+// The tile shape whose estimate is least: rounds of tiles over the SMs, each
+// K block of a round, and what a launch and every further round add. The
+// constants are fits to measured times on B200 (us; products alone), where
+// the shapes take turns by size:
+//                       pair 256x256   128x128   128x64
+//   300 x 1600 x 256         7.5          5.1       4.4
+//   1024 x 1536 x 1536      10.7          8.3      11.2
+//   4352 x 1536 x 1536      15.9         17.1      26.6
+//   128 x 16384 x 4096      17.5         14.5      22.6
+//   15845 x 2048 x 2048     52.2         75.3     132.3
+// (Pairs on 256 x 128 tiles were slower than one of these at every size.)
+enum Form { kPair256, kSingle128, kSingle64 };
 inline Form pick_form(int64_t m, int64_t width, int64_t k, bool swiglu, int sms) {
-  const int64_t blocks = cdiv(k, kBK);
   struct Candidate {
     Form form;
     int rows, cols, slots;
-    double block, fixed;  // microseconds of a K block and of a tile's start and end
+    double start, block, round;
   };
-  const int half = swiglu ? 2 : 1;
-  const Candidate all[4] = {{kPair256, 256, 256 / half, sms / 2, 0.40, 5.0},
-                            {kPair128, 256, 128 / half, sms / 2, 0.25, 4.0},
-                            {kSingle128, 128, 128 / half, sms, 0.25, 4.0},
-                            {kSingle64, 128, 64, sms, 0.20, 3.0}};
-  Form best = kPair256;
+  const int half = swiglu ? 2 : 1;  // a SwiGLU tile has half as many output columns
+  const Candidate all[3] = {{kPair256, 256, 256 / half, sms / 2, 6.9, 0.31, 1.6},
+                            {kSingle128, 128, 128 / half, sms, 4.5, 0.29, 1.0},
+                            {kSingle64, 128, 64, sms, 3.8, 0.276, 0.6}};
+  Form best = kSingle128;
   double least = 1e300;
   for (const Candidate& c : all) {
-    if ((c.form == kSingle64 && swiglu) || (c.rows == 256 && m <= 128)) continue;
+    if (c.form == kSingle64 && swiglu) continue;
     const double rounds = static_cast<double>(cdiv(cdiv(m, c.rows) * cdiv(width, c.cols), c.slots));
-    const double cost = rounds * blocks * c.block + c.fixed;
+    const double cost = c.start + rounds * cdiv(k, kBK) * c.block + (rounds - 1) * c.round;
     if (cost < least) {
       least = cost;
       best = c.form;
@@ -518,7 +644,6 @@ template <typename T, int kEpi>
 int launch_form(const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
   const Form f = pick_form(p.M, kEpi == kSwiGLU ? p.N / 2 : p.N, p.K, kEpi == kSwiGLU, sm_count());
   if (f == kPair256) return launch<T, 256, kEpi, true>(a, w, p, st);
-  if (f == kPair128) return launch<T, 128, kEpi, true>(a, w, p, st);
   if constexpr (kEpi != kSwiGLU)
     if (f == kSingle64) return launch<T, 64, kEpi, false>(a, w, p, st);
   return launch<T, 128, kEpi, false>(a, w, p, st);
@@ -887,8 +1012,7 @@ int product(const Call& c, const void* x, int64_t ldx) {
   p.residual = static_cast<const T*>(c.residual);
   p.ldr = c.ldr;
   p.err = c.error_flag;
-  p.vec = (!c.bias || a16(c.bias)) && (!c.gate || (a16(c.gate) && a16(c.residual) && c.ldg % 8 == 0 && c.ldr % 8 == 0));
-  p.vec_scale = a16(c.scale_w);
+  p.vec = c.gate && a16(c.gate) && a16(c.residual) && c.ldg % 8 == 0 && c.ldr % 8 == 0;
   return int8::pick<T>(c.gate ? int8::kGated : c.activation, c.a, c.w, p, static_cast<const T*>(x), ldx, c.st);
 }
 
