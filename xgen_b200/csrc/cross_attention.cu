@@ -50,6 +50,8 @@ constexpr int kFixWarp = 11;
 constexpr float kTau = 8.0f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
+constexpr int kOutBytes = 32 * 128;
+
 template <typename T, int kD>
 struct Cfg {
   static constexpr int kSubs = kD / 64;                // 128-byte-wide sub-tiles of a row
@@ -57,10 +59,11 @@ struct Cfg {
   static constexpr int kQBytes = kSubs * kQSub;
   static constexpr int kKVSub = kBN * 128;
   static constexpr int kKVBytes = kSubs * kKVSub;
-  static constexpr int kStages = kD == 128 ? 5 : 8;
+  static constexpr int kStages = kD == 128 ? 4 : 8;
   static constexpr int kKOff = 2 * kQBytes;
   static constexpr int kVOff = kKOff + kStages * kKVBytes;
-  static constexpr int kBarOff = kVOff + kStages * kKVBytes;
+  static constexpr int kOutOff = kVOff + kStages * kKVBytes;  // 32 rows x 64 channels of each softmax warp
+  static constexpr int kBarOff = kOutOff + 8 * kOutBytes;
   static constexpr int kSmem = kBarOff + 512 + 1024;  // + barriers + alignment slack
   static constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   static constexpr uint32_t kIdescQK = instr_desc(1, kFmt, kFmt, false, false, kBM, kBN);
@@ -168,7 +171,8 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
 template <typename T, int kD>
 __global__ void __launch_bounds__(kThreads, 1)
     cross_attention_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                           const __grid_constant__ CUtensorMap v_map, const Params p) {
+                           const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap o_map,
+                           const Params p) {
   using C = Cfg<T, kD>;
   constexpr int kStages = C::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -426,33 +430,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       ++n;
       if (!ok) break;
       tc_fence_after();
-      const float inv_l = l != 0.f ? 1.0f / l : 0.f;
+      if (p.splits > 1) {
 #pragma unroll 1
-      for (int c = 0; c < kD / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(o_addr + c * 32, o);
-        tmem_ld_wait();
-        if (row >= p.seq_q) continue;
-        if (p.splits > 1) {
+        for (int c = 0; c < kD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_ld_wait();
+          if (row >= p.seq_q) continue;
           float4* po = reinterpret_cast<float4*>(p.part_o + part * kD) + c * 8;
 #pragma unroll
           for (int v = 0; v < 8; ++v)
             po[v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]), __uint_as_float(o[4 * v + 2]),
                                 __uint_as_float(o[4 * v + 3]));
-        } else {
-          uint32_t w[16];
+        }
+        if (row < p.seq_q) p.part_ml[part] = make_float2(m_used, l);
+        tc_fence_before();
+        mbar_arrive(&bars->o_empty[i]);
+        continue;
+      }
+      // 64 channels at a time through shared memory, so that rows leave as whole
+      // lines; rows behind the last query are not written by the store.
+      const float inv_l = l != 0.f ? 1.0f / l : 0.f;
+      uint8_t* stage = smem + C::kOutOff + warp * kOutBytes;
+#pragma unroll 1
+      for (int c = 0; c < C::kSubs; ++c) {
+        uint32_t o[2][32];
+        tmem_ld64(o_addr + c * 64, o);
+        if (lane == 0) bulk_wait_read<0>();  // the store before this one has left the buffer
+        __syncwarp();
+        tmem_ld_wait();
+        if (c == C::kSubs - 1) {
+          tc_fence_before();
+          mbar_arrive(&bars->o_empty[i]);
+        }
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            w[e / 2] = pack2<T>(__uint_as_float(o[e]) * inv_l, __uint_as_float(o[e + 1]) * inv_l);
+        for (int v = 0; v < 8; ++v) {
+          const uint32_t* x = &o[v >> 2][(v & 3) * 8];
+          uint32_t w[4];
 #pragma unroll
-          for (int v = 0; v < 4; ++v)
-            reinterpret_cast<uint4*>(dst + c * 32)[v] = make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
+          for (int e = 0; e < 4; ++e) w[e] = pack2<T>(__uint_as_float(x[2 * e]) * inv_l, __uint_as_float(x[2 * e + 1]) * inv_l);
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_4d(&o_map, stage, c * 64, u.m0 + i * kBM + lane_base, u.h, u.b);
+          bulk_commit();
         }
       }
-      if (p.splits > 1 && row < p.seq_q) p.part_ml[part] = make_float2(m_used, l);
-      tc_fence_before();
-      mbar_arrive(&bars->o_empty[i]);
     }
+    if (lane == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -664,19 +691,32 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int64_t rows,
     r = in_head % kFewRows;
   }
   const int64_t first = item * p.splits * p.part_rows + r;
+  // m and l of 32 parts at a time, a lane each; then the O of the parts with
+  // keys, whose loads do not wait for one another
   float mx = kNegInf;
-  for (int q = 0; q < p.splits; ++q) mx = fmaxf(mx, __ldg(&p.part_ml[first + static_cast<int64_t>(q) * p.part_rows]).x);
+  for (int q = lane; q < p.splits; q += 32) mx = fmaxf(mx, __ldg(&p.part_ml[first + static_cast<int64_t>(q) * p.part_rows]).x);
+  mx = warp_max(mx);
   const float base = mx == kNegInf ? 0.f : mx;
   float l = 0.f, o[kD / 32] = {};
-  for (int q = 0; q < p.splits; ++q) {
-    const int64_t at_q = first + static_cast<int64_t>(q) * p.part_rows;
-    const float2 ml = __ldg(&p.part_ml[at_q]);
-    if (ml.y == 0.f) continue;
-    const float w = ex2_approx(ml.x - base);
-    l = fmaf(w, ml.y, l);
+  for (int q0 = 0; q0 < p.splits; q0 += 32) {
+    float w = 0.f, lq = 0.f;
+    if (q0 + lane < p.splits) {
+      const float2 ml = __ldg(&p.part_ml[first + static_cast<int64_t>(q0 + lane) * p.part_rows]);
+      lq = ml.y;
+      w = ex2_approx(ml.x - base);
+      l = fmaf(w, lq, l);
+    }
+    const int n = min(32, p.splits - q0);
+#pragma unroll 4
+    for (int q = 0; q < n; ++q) {
+      const float wq = __shfl_sync(0xffffffffu, w, q), has = __shfl_sync(0xffffffffu, lq, q);
+      if (has == 0.f) continue;
+      const float* po = p.part_o + (first + static_cast<int64_t>(q0 + q) * p.part_rows) * kD + lane;
 #pragma unroll
-    for (int c = 0; c < kD / 32; ++c) o[c] = fmaf(w, __ldg(p.part_o + at_q * kD + c * 32 + lane), o[c]);
+      for (int c = 0; c < kD / 32; ++c) o[c] = fmaf(wq, __ldg(po + c * 32), o[c]);
+    }
   }
+  l = warp_sum(l);
   const float inv_l = l != 0.f ? 1.0f / l : 0.f;
   T* dst = static_cast<T*>(p.out) + b * p.osb + h * p.osh + row * p.oss;
 #pragma unroll
@@ -725,14 +765,13 @@ inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, 
 }
 
 template <typename T, int kD>
-int launch(const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Params& p, int64_t batch, int sms,
-           cudaStream_t st) {
+int launch(const CUtensorMap (&map)[4], const Params& p, int64_t batch, int sms, cudaStream_t st) {
   using C = Cfg<T, kD>;
   auto kernel = cross_attention_kernel<T, kD>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
     return XGB_ERR_LAUNCH;
   const int grid = static_cast<int>(std::min<int64_t>(p.units, sms));
-  kernel<<<grid, kThreads, C::kSmem, st>>>(qm, km, vm, p);
+  kernel<<<grid, kThreads, C::kSmem, st>>>(map[0], map[1], map[2], map[3], p);
   const int rc = launch_status();
   if (rc || p.splits == 1) return rc;
   const int64_t rows = batch * p.heads * p.seq_q;
@@ -757,10 +796,11 @@ int launch_few(const Params& p, const FewParams& f, int64_t items, int64_t batch
 // [batch, heads, seq_kv, D] tensors, in order, and counts them; what lies
 // behind the count is not written. A block takes 64 keys of one sample and
 // counts the kept ones before its own.
+template <int kWords>
 __global__ void __launch_bounds__(256) pack_keys_kernel(const uint8_t* __restrict__ mask, int64_t msb, int64_t mss,
                                                         const uint4* __restrict__ k, int64_t ksb, int64_t ksh, int64_t kss,
                                                         const uint4* __restrict__ v, int64_t vsb, int64_t vsh, int64_t vss,
-                                                        int heads, int seq, int words, uint4* __restrict__ k_out,
+                                                        int heads, int seq, uint4* __restrict__ k_out,
                                                         uint4* __restrict__ v_out, int* __restrict__ counts) {
   __shared__ int red[8];
   __shared__ int place[kBN];
@@ -785,17 +825,22 @@ __global__ void __launch_bounds__(256) pack_keys_kernel(const uint8_t* __restric
       place[c * 32 + lane] = keep ? at + __popc(kept & ((1u << lane) - 1)) : -1;
       at += __popc(kept);
     }
-    if (lane == 0 && first + kBN >= seq) counts[b] = at;
+    if (lane == 0 && first + kBN >= seq && blockIdx.z == 0) counts[b] = at;
   }
   __syncthreads();
-  const int per_head = kBN * words;
-  for (int e = threadIdx.x; e < heads * per_head; e += 256) {
-    const int h = e / per_head, j = (e - h * per_head) / words, w = e % words;
-    const int to = place[j];
-    if (to < 0) continue;
-    const int64_t dst = ((static_cast<int64_t>(b) * heads + h) * seq + to) * words + w;
-    k_out[dst] = __ldg(k + b * ksb + h * ksh + (first + j) * kss + w);
-    v_out[dst] = __ldg(v + b * vsb + h * vsh + (first + j) * vss + w);
+  // kWords pieces of 16 bytes a row; a block's heads are blockIdx.z, + gridDim.z, ..
+  const int w = threadIdx.x % kWords;
+  for (int h = blockIdx.z; h < heads; h += gridDim.z) {
+#pragma unroll
+    for (int j = threadIdx.x / kWords; j < kBN; j += 256 / kWords) {
+      const int to = place[j];
+      if (to < 0) continue;
+      const int64_t dst = ((static_cast<int64_t>(b) * heads + h) * seq + to) * kWords + w;
+      const uint4 kw = __ldg(k + b * ksb + h * ksh + (first + j) * kss + w);
+      const uint4 vw = __ldg(v + b * vsb + h * vsh + (first + j) * vss + w);
+      k_out[dst] = kw;
+      v_out[dst] = vw;
+    }
   }
 }
 
@@ -818,13 +863,18 @@ XGB_API int xgb_pack_keys(const uint8_t* mask, int64_t mask_batch_stride, int64_
   if (k_strides[3] != 1 || v_strides[3] != 1) return XGB_ERR_STRIDE;
   if (!cross::aligned16(k) || !cross::aligned16(v) || !cross::aligned16(k_out) || !cross::aligned16(v_out))
     return XGB_ERR_ALIGN;
-  const dim3 grid(static_cast<unsigned>(cdiv(seq, cross::kBN)), static_cast<unsigned>(batch));
-  cross::pack_keys_kernel<<<grid, 256, 0, as_stream(stream)>>>(
-      mask, mask_batch_stride, mask_stride, static_cast<const uint4*>(k), k_strides[0] / 8, k_strides[1] / 8,
-      k_strides[2] / 8, static_cast<const uint4*>(v), v_strides[0] / 8, v_strides[1] / 8, v_strides[2] / 8,
-      static_cast<int>(heads), static_cast<int>(seq), static_cast<int>(head_dim / 8), static_cast<uint4*>(k_out),
-      static_cast<uint4*>(v_out), counts);
-  return launch_status();
+  // enough blocks to fill the GPU a few times; further heads in a loop
+  const int64_t tiles = cdiv(seq, cross::kBN) * batch;
+  const dim3 grid(static_cast<unsigned>(cdiv(seq, cross::kBN)), static_cast<unsigned>(batch),
+                  static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(heads, 148 * 8 / tiles))));
+  auto run = [&](auto kernel) {
+    kernel<<<grid, 256, 0, as_stream(stream)>>>(
+        mask, mask_batch_stride, mask_stride, static_cast<const uint4*>(k), k_strides[0] / 8, k_strides[1] / 8,
+        k_strides[2] / 8, static_cast<const uint4*>(v), v_strides[0] / 8, v_strides[1] / 8, v_strides[2] / 8,
+        static_cast<int>(heads), static_cast<int>(seq), static_cast<uint4*>(k_out), static_cast<uint4*>(v_out), counts);
+    return launch_status();
+  };
+  return head_dim == 64 ? run(cross::pack_keys_kernel<8>) : run(cross::pack_keys_kernel<16>);
 }
 
 XGB_API int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv,
@@ -918,12 +968,13 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
     return head_dim == 128 ? cross::launch_few<__half, 128>(p, f, n.items, batch, st)
                            : cross::launch_few<__half, 64>(p, f, n.items, batch, st);
   }
-  CUtensorMap map[3];
-  const void* base[3] = {q, k, v};
-  int factor[3][2];  // batch, head
-  for (int t = 0; t < 3; ++t) {
+  CUtensorMap map[4];
+  const void* base[4] = {q, k, v, out};
+  int factor[4][2];  // batch, head
+  for (int t = 0; t < 4; ++t) {
+    const bool rows = t == 0 || t == 3;
     const int64_t* s = all[t];
-    const int64_t seq = t == 0 ? seq_q : seq_kv, hh = t == 0 ? heads : kv_heads;
+    const int64_t seq = rows ? seq_q : seq_kv, hh = rows ? heads : kv_heads;
     // a dimension of one entry, or a broadcast one, is one entry of the map
     const int64_t ext[3] = {seq, hh > 1 && s[1] ? hh : 1, batch > 1 && s[0] ? batch : 1};
     factor[t][0] = ext[2] > 1;
@@ -934,7 +985,7 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
     const uint64_t strides[3] = {ext[0] > 1 ? static_cast<uint64_t>(s[2]) * 2 : row,
                                  ext[1] > 1 ? static_cast<uint64_t>(s[1]) * 2 : row,
                                  ext[2] > 1 ? static_cast<uint64_t>(s[0]) * 2 : row};
-    const uint32_t box[4] = {64, static_cast<uint32_t>(t == 0 ? cross::kBM : cross::kBN), 1, 1};
+    const uint32_t box[4] = {64, static_cast<uint32_t>(t == 0 ? cross::kBM : t == 3 ? 32 : cross::kBN), 1, 1};
     if (!make_tensor_map(&map[t], bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                          base[t], dims, strides, box))
       return XGB_ERR_ALIGN;
@@ -946,8 +997,8 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
   p.vb = factor[2][0];
   p.vh = factor[2][1];
   if (bf16)
-    return head_dim == 128 ? cross::launch<__nv_bfloat16, 128>(map[0], map[1], map[2], p, batch, sms, st)
-                           : cross::launch<__nv_bfloat16, 64>(map[0], map[1], map[2], p, batch, sms, st);
-  return head_dim == 128 ? cross::launch<__half, 128>(map[0], map[1], map[2], p, batch, sms, st)
-                         : cross::launch<__half, 64>(map[0], map[1], map[2], p, batch, sms, st);
+    return head_dim == 128 ? cross::launch<__nv_bfloat16, 128>(map, p, batch, sms, st)
+                           : cross::launch<__nv_bfloat16, 64>(map, p, batch, sms, st);
+  return head_dim == 128 ? cross::launch<__half, 128>(map, p, batch, sms, st)
+                         : cross::launch<__half, 64>(map, p, batch, sms, st);
 }
