@@ -329,9 +329,10 @@ int xgb_int8_gemm(const int8_t* a, const int8_t* w, int64_t M, int64_t N, int64_
 
 /* xgb_int8_quantize_per_token of x [M, K] (`dtype`, rows ldx apart) and
  * xgb_int8_gemm in one call; few tokens take one launch. workspace:
- * xgb_int8_linear_workspace(M, K) bytes, 16-byte aligned, its contents need
- * no initialisation. */
-int64_t xgb_int8_linear_workspace(int64_t M, int64_t K);
+ * xgb_int8_linear_workspace() bytes of the same x, ldx, M, K (0 where the
+ * call takes one launch), 16-byte aligned, its contents need no
+ * initialisation. */
+int64_t xgb_int8_linear_workspace(const void* x, int64_t ldx, int64_t M, int64_t K);
 int xgb_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t M, int64_t N, int64_t K,
                     const float* scale_w, int dtype, const void* bias, int activation, void* out, int64_t ldo,
                     const void* gate, int64_t ldg, const int64_t* gate_index, int64_t index_rows,

@@ -78,10 +78,12 @@ def test_int8_arguments():
     assert gemm(gate=D) == -1 and gemm(gate=D, idx=D, res=D, act=1) == -1 and gemm(gate=D, idx=D, res=D, m=3, irows=2) == -1
     assert gemm(ldo=31) == -3 and gemm(gate=D, idx=D, res=D, ldg=16) == -3
     assert gemm(a=ODD) == -4 and gemm(out=ODD) == -4
-    need = h.xgb_int8_linear_workspace(3, 32)
-    assert need == 96 + 12
+    assert h.xgb_int8_linear_workspace(D, 32, 3, 32) == 0  # one launch
+    assert h.xgb_int8_linear_workspace(ODD, 32, 3, 32) == 96 + 12
+    need = h.xgb_int8_linear_workspace(D, 32, 300, 32)
+    assert need == 9600 + 1200
 
-    def linear(x=D, ldx=32, m=3, k=32, ws=D, bytes_=need):
+    def linear(x=D, ldx=32, m=300, k=32, ws=D, bytes_=need):
         return h.xgb_int8_linear(x, ldx, D, m, 32, k, D, 0, None, 0, D, 32, None, 0, None, 1, 0, None, 0, ws, bytes_, None, None)
 
     assert linear(x=None) == -1 and linear(ldx=31) == -3 and linear(k=24) == -2

@@ -95,7 +95,7 @@ SIGNATURES = {
     "xgb_int8_quantize_per_token": (c_int, [c_vp, c_int, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp]),
     "xgb_int8_gemm": (c_int, [c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_vp, c_int, c_vp, c_int, c_vp, c_i64,
                               c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp]),
-    "xgb_int8_linear_workspace": (c_i64, [c_i64, c_i64]),
+    "xgb_int8_linear_workspace": (c_i64, [c_vp, c_i64, c_i64, c_i64]),
     "xgb_int8_linear": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_int, c_vp, c_i64,
                                 c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp]),
     "xgb_cross_attention_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),

@@ -264,7 +264,7 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
             raise ValueError(f"{what}: key_mask must be bool [B, Skv], [1, Skv] or [B, 1, 1, Skv]")
         key_mask = key_mask.expand(b, skv)
     if out is None:
-        out = torch.empty((b, h, sq, d), dtype=query.dtype, device=query.device)
+        out = query.new_empty((b, h, sq, d))
     elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
         raise ValueError(f"{what} output must be a [B, H, Sq, D] view of the query's type with unit channel stride")
     if not b * h * sq:
@@ -277,8 +277,8 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
         if lib.xgb_cross_attention_takes_mask(h, hk, sq):
             mask = (key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1))
         else:
-            kv_lens = torch.empty((b,), dtype=torch.int32, device=key.device)
-            packed = torch.empty((2, b, hk, skv, d), dtype=key.dtype, device=key.device)
+            kv_lens = key.new_empty((b,), dtype=torch.int32)
+            packed = key.new_empty((2, b, hk, skv, d))
             _call_on(index, "xgb_pack_keys", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), key.data_ptr(),
                      _steps(key), value.data_ptr(), _steps(value), b, hk, skv, d, packed[0].data_ptr(), packed[1].data_ptr(),
                      kv_lens.data_ptr())
@@ -288,7 +288,7 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
             kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
         kv_lens = kv_lens.contiguous()
     ws_bytes = lib.xgb_cross_attention_workspace(b, h, hk, sq, skv, d)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=query.device) if ws_bytes else None
+    ws = query.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
     _call_on(index, "xgb_cross_attention", query.data_ptr(), _steps(query), key.data_ptr(), _steps(key), value.data_ptr(),
              _steps(value), code, b, h, hk, sq, skv, d, kv_lens.data_ptr() if kv_lens is not None else None, *mask, sm_scale,
              out.data_ptr(), _steps(out), ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(query.device))

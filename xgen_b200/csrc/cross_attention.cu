@@ -501,7 +501,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 //   O^T [D x 8 rows] += V^T P^T: the same pieces of V, transposed 8 x 8 by
 //     movmatrix; the order of d that comes out is undone when O is written.
 // Each warp keeps its own running maximum and O; the warps of a CTA join in
-// shared memory, the CTAs of a unit (parts of its keys) in the second kernel.
+// shared memory. The CTAs of a unit (parts of its keys) are a cluster of up to
+// 8, whose members each join some of the rows over distributed shared memory;
+// only few units with many keys need more parts than that, and join in the
+// second kernel.
 // Keys that are not there are not loaded: zeros, with scores of -inf.
 constexpr int kFewRows = 8;
 constexpr int kFewWarps = 4;
@@ -515,6 +518,7 @@ struct FewParams {
   const uint8_t* mask;  // [batch, seq_kv] bytes, null: none
   int64_t msb, mss;
   int kv_heads, tiles;  // row tiles of 8 of a key head
+  int clustered;        // a unit's parts are a cluster
 };
 
 template <typename T>
@@ -550,6 +554,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
   constexpr int kChunks = kD / 32;
   __shared__ float so[kFewWarps][kFewRows][kD];
   __shared__ float2 sml[kFewWarps][kFewRows];
+  __shared__ float2 part_ml[kFewRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int64_t unit = blockIdx.x / p.splits;  // (batch, key head, row tile)
   const int part = static_cast<int>(blockIdx.x - unit * p.splits);
@@ -645,9 +650,10 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
     for (int e = 0; e < 4; ++e)
       so[warp][2 * c + (e & 1)][32 * (n >> 1) + 8 * (g >> 1) + (g & 1) + 4 * (n & 1) + 2 * (e >> 1)] = o[n][e];
   __syncthreads();
+  // The CTA's part of each value: thread t takes channels t of all rows, so it
+  // is the only one that touches them in the warps' tiles.
   for (int at = threadIdx.x; at < kFewRows * kD; at += kFewWarps * 32) {
-    const int r = at / kD, d = at % kD, row = first_row + r;
-    if (row >= rows) break;
+    const int r = at / kD, d = at % kD;
     float mx = kNegInf;
 #pragma unroll
     for (int w = 0; w < kFewWarps; ++w) mx = fmaxf(mx, sml[w][r].x);
@@ -659,18 +665,43 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
       lsum = fmaf(wt, sml[w][r].y, lsum);
       sum = fmaf(wt, so[w][r][d], sum);
     }
-    if (p.splits > 1) {
+    so[0][r][d] = sum;
+    if (d == 0) part_ml[r] = make_float2(mx, lsum);
+  }
+  __syncthreads();
+  const bool clustered = f.clustered != 0;
+  if (clustered) cluster_sync();
+  // Rows of this CTA: all of a unit's only part or of a part for the second
+  // kernel, every splits-th one in a cluster.
+  const int row_step = clustered ? p.splits : 1;
+  for (int e = threadIdx.x; e < kFewRows * kD; e += kFewWarps * 32) {
+    const int r = e / kD, d = e % kD, row = first_row + r;
+    if (row >= rows) break;
+    if (clustered && r % row_step != part) continue;
+    float sum = so[0][r][d], lsum = part_ml[r].y;
+    if (clustered) {
+      float mx = kNegInf;
+      for (int q = 0; q < p.splits; ++q) mx = fmaxf(mx, ld_cluster_f32(map_to_rank(&part_ml[r].x, q)));
+      const float base = mx == kNegInf ? 0.f : mx;
+      sum = lsum = 0.f;
+      for (int q = 0; q < p.splits; ++q) {
+        const float wt = ex2_approx(ld_cluster_f32(map_to_rank(&part_ml[r].x, q)) - base);
+        lsum = fmaf(wt, ld_cluster_f32(map_to_rank(&part_ml[r].y, q)), lsum);
+        sum = fmaf(wt, ld_cluster_f32(map_to_rank(&so[0][r][d], q)), sum);
+      }
+    } else if (p.splits > 1) {
       const int64_t slot = (unit * p.splits + part) * kFewRows + r;
       p.part_o[slot * kD + d] = sum;
-      if (d == 0) p.part_ml[slot] = make_float2(mx, lsum);
-    } else {
-      const int h = hk * p.group + row / p.seq_q, s = row % p.seq_q;
-      const float v = lsum != 0.f ? sum / lsum : 0.f;
-      T* dst = static_cast<T*>(p.out) + b * p.osb + h * p.osh + s * p.oss + d;
-      if constexpr (std::is_same<T, __half>::value) *dst = __float2half_rn(v);
-      else *dst = __float2bfloat16_rn(v);
+      if (d == 0) p.part_ml[slot] = part_ml[r];
+      continue;
     }
+    const int h = hk * p.group + row / p.seq_q, s = row % p.seq_q;
+    const float v = lsum != 0.f ? sum / lsum : 0.f;
+    T* dst = static_cast<T*>(p.out) + b * p.osb + h * p.osh + s * p.oss + d;
+    if constexpr (std::is_same<T, __half>::value) *dst = __float2half_rn(v);
+    else *dst = __float2bfloat16_rn(v);
   }
+  if (clustered) cluster_sync();  // nobody leaves while its part is read
 }
 
 // Joins the parts of a row: M = max m, o = sum 2^(m - M) O / sum 2^(m - M) l.
@@ -741,6 +772,7 @@ struct Plan {
   int tiles;  // few: row tiles of a key head
   int64_t items;
   int splits;
+  bool clustered;
   int64_t part_rows;
 };
 inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int sms) {
@@ -750,9 +782,13 @@ inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, 
   if (n.few) {
     n.tiles = static_cast<int>(cdiv(rows, kFewRows));
     n.items = batch * kv_heads * n.tiles;
-    // three CTAs an SM, each at least one step for each of its warps
-    n.splits = static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>(3 * sms / n.items, cdiv(seq_kv, kFewKeys * kFewWarps))));
+    // Three CTAs an SM are resident, each should have a step for each of its
+    // warps. A cluster of up to 8 parts needs no second kernel; it is taken as
+    // soon as it gives every SM a CTA.
+    const int64_t most = cdiv(seq_kv, kFewKeys * kFewWarps);
+    n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(3 * sms / n.items, most)));
+    n.clustered = n.splits > 1 && (n.splits <= 8 || n.items * 8 >= sms);
+    if (n.clustered) n.splits = std::min(n.splits, 8);
     n.part_rows = kFewRows;
     return n;
   }
@@ -783,9 +819,22 @@ template <typename T, int kD>
 int launch_few(const Params& p, const FewParams& f, int64_t items, int64_t batch, cudaStream_t st) {
   const int64_t grid = items * p.splits;
   if (grid > INT32_MAX) return XGB_ERR_SHAPE;
-  cross_few_kernel<T, kD><<<static_cast<unsigned>(grid), kFewWarps * 32, 0, st>>>(p, f);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kFewWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(f.clustered ? p.splits : 1);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, cross_few_kernel<T, kD>, p, f) != cudaSuccess) {
+    cudaGetLastError();
+    return XGB_ERR_LAUNCH;
+  }
   const int rc = launch_status();
-  if (rc || p.splits == 1) return rc;
+  if (rc || p.splits == 1 || f.clustered) return rc;
   const int64_t rows = batch * p.heads * p.seq_q;
   join_kernel<T, kD><<<static_cast<unsigned>(cdiv(rows, 8)), 256, 0, st>>>(p, rows, f.tiles);
   return launch_status();
@@ -881,7 +930,7 @@ XGB_API int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int6
                                               int64_t head_dim) {
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq_q <= 0 || seq_kv <= 0) return 0;
   const cross::Plan n = cross::plan(batch, heads, kv_heads, seq_q, seq_kv, cross::sm_count());
-  if (n.splits <= 1) return 0;
+  if (n.splits <= 1 || n.clustered) return 0;
   return n.items * n.splits * n.part_rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
@@ -936,7 +985,7 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
   p.splits = n.splits;
   p.units = n.items * n.splits;
   p.part_rows = static_cast<int>(n.part_rows);
-  if (p.splits > 1) {
+  if (need) {
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + p.units * p.part_rows * head_dim);
   }
@@ -962,6 +1011,7 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
     f.mss = mask_stride;
     f.kv_heads = static_cast<int>(kv_heads);
     f.tiles = n.tiles;
+    f.clustered = n.clustered;
     if (bf16)
       return head_dim == 128 ? cross::launch_few<__nv_bfloat16, 128>(p, f, n.items, batch, st)
                              : cross::launch_few<__nv_bfloat16, 64>(p, f, n.items, batch, st);

@@ -614,24 +614,30 @@ int launch(const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
 //   4352 x 1536 x 1536      15.9         17.1      26.6
 //   128 x 16384 x 4096      17.5         14.5      22.6
 //   15845 x 2048 x 2048     52.2         75.3     132.3
+// An epilogue that does more than scale adds to a launch and to every round,
+// most to the pairs, whose warps take 128 columns each.
 // (Pairs on 256 x 128 tiles were slower than one of these at every size.)
 enum Form { kPair256, kSingle128, kSingle64 };
-inline Form pick_form(int64_t m, int64_t width, int64_t k, bool swiglu, int sms) {
+inline Form pick_form(int64_t m, int64_t width, int64_t k, int epilogue, int sms) {
   struct Candidate {
     Form form;
     int rows, cols, slots;
     double start, block, round;
+    double gated_start, gated_round, act_start, act_round;
   };
+  const bool swiglu = epilogue == kSwiGLU;
   const int half = swiglu ? 2 : 1;  // a SwiGLU tile has half as many output columns
-  const Candidate all[3] = {{kPair256, 256, 256 / half, sms / 2, 6.9, 0.31, 1.6},
-                            {kSingle128, 128, 128 / half, sms, 4.5, 0.29, 1.0},
-                            {kSingle64, 128, 64, sms, 3.8, 0.276, 0.6}};
+  const Candidate all[3] = {{kPair256, 256, 256 / half, sms / 2, 6.9, 0.31, 1.6, 4.5, 2.3, 2.8, 0.8},
+                            {kSingle128, 128, 128 / half, sms, 4.5, 0.29, 1.0, 1.3, 0.0, 1.3, 0.4},
+                            {kSingle64, 128, 64, sms, 3.8, 0.276, 0.6, 1.4, 0.3, 1.5, 0.4}};
   Form best = kSingle128;
   double least = 1e300;
   for (const Candidate& c : all) {
     if (c.form == kSingle64 && swiglu) continue;
     const double rounds = static_cast<double>(cdiv(cdiv(m, c.rows) * cdiv(width, c.cols), c.slots));
-    const double cost = c.start + rounds * cdiv(k, kBK) * c.block + (rounds - 1) * c.round;
+    double cost = c.start + rounds * cdiv(k, kBK) * c.block + (rounds - 1) * c.round;
+    if (epilogue == kGated) cost += c.gated_start + (rounds - 1) * c.gated_round;
+    else if (epilogue != kPlain) cost += c.act_start + (rounds - 1) * c.act_round;
     if (cost < least) {
       least = cost;
       best = c.form;
@@ -642,7 +648,7 @@ inline Form pick_form(int64_t m, int64_t width, int64_t k, bool swiglu, int sms)
 
 template <typename T, int kEpi>
 int launch_form(const void* a, const void* w, const Params<T>& p, cudaStream_t st) {
-  const Form f = pick_form(p.M, kEpi == kSwiGLU ? p.N / 2 : p.N, p.K, kEpi == kSwiGLU, sm_count());
+  const Form f = pick_form(p.M, kEpi == kSwiGLU ? p.N / 2 : p.N, p.K, kEpi, sm_count());
   if (f == kPair256) return launch<T, 256, kEpi, true>(a, w, p, st);
   if constexpr (kEpi != kSwiGLU)
     if (f == kSingle64) return launch<T, 64, kEpi, false>(a, w, p, st);
@@ -1032,8 +1038,12 @@ XGB_API int xgb_int8_gemm(const int8_t* a, const int8_t* w, int64_t M, int64_t N
   return dtype == XGB_BF16 ? product<__nv_bfloat16>(c, nullptr, 0) : product<__half>(c, nullptr, 0);
 }
 
-XGB_API int64_t xgb_int8_linear_workspace(int64_t M, int64_t K) {
-  if (M <= 0 || K <= 0) return 0;
+static bool fused(const void* x, int64_t ldx, int64_t M, int64_t K) {
+  return int8::fuses(M, K) && a16(x) && (M == 1 || ldx % 8 == 0);
+}
+
+XGB_API int64_t xgb_int8_linear_workspace(const void* x, int64_t ldx, int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || fused(x, ldx, M, K)) return 0;
   return cdiv(M * K, 16) * 16 + M * static_cast<int64_t>(sizeof(float));
 }
 
@@ -1048,11 +1058,12 @@ XGB_API int xgb_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t
   int rc = check(c);
   if (rc) return rc;
   if (M > 1 && ldx < K) return XGB_ERR_STRIDE;
-  if (!workspace || workspace_bytes < xgb_int8_linear_workspace(M, K)) return XGB_ERR_WORKSPACE;
-  if (!a16(workspace)) return XGB_ERR_ALIGN;
+  const int64_t need = xgb_int8_linear_workspace(x, ldx, M, K);
+  if (need && (!workspace || workspace_bytes < need)) return XGB_ERR_WORKSPACE;
+  if (need && !a16(workspace)) return XGB_ERR_ALIGN;
   if ((rc = check_device())) return rc;
   const bool bf16 = dtype == XGB_BF16;
-  if (int8::fuses(M, K) && a16(x) && (M == 1 || ldx % 8 == 0))
+  if (!need)
     return bf16 ? product<__nv_bfloat16>(c, x, ldx) : product<__half>(c, x, ldx);
   int8_t* codes = static_cast<int8_t*>(workspace);
   float* scales = reinterpret_cast<float*>(codes + cdiv(M * K, 16) * 16);

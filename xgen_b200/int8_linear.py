@@ -12,6 +12,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
+from ._lib import lib
 from .attention import _err_ptr
 from .ops import _DTYPE_CODE, _call_on, _device_of, _refuse_autograd, _row_stride
 
@@ -30,7 +31,7 @@ def quantize_per_channel_int8(value: torch.Tensor):
 def _arguments(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index, residual):
     """Checks what int8_linear and int8_linear_quantized share; `lead` is the
     input's shape without its channels. Returns (rows, weight, weight_scale,
-    arguments of the epilogue, output [rows, width])."""
+    arguments of the epilogue, output)."""
     what = "H3 INT8 Linear"
     if weight.dtype != torch.int8 or weight.ndim != 2 or dtype not in _DTYPE_CODE:
         raise ValueError(f"{what} requires an int8 [out, in] weight and a bf16/fp16 result")
@@ -59,19 +60,24 @@ def _arguments(lead, dtype, weight, weight_scale, bias, activation, gate, gate_i
         if gate_index.dtype != torch.int64 or (m and (index_rows == 0 or m % index_rows)):
             raise ValueError(f"gated {what} needs an int64 index for each token, or one sequence's for every sample")
         gate_index = gate_index.contiguous()
-        rows, residual = gate.shape[0], residual.reshape(m, n)
+        rows, residual = gate.shape[0], residual if residual.ndim == 2 else residual.reshape(m, n)
         if rows > 1 and gate.stride(0) < n:  # broadcast rows
             gate = gate.contiguous()
         if m > 1 and residual.stride(0) < n:
             residual = residual.contiguous()
         ldg, ldr = _row_stride(gate, n), residual.stride(0) if m > 1 else n
-    out = torch.empty((m, width), device=weight.device, dtype=dtype)
+    out = weight.new_empty((*lead, width), dtype=dtype)
     epilogue = (_DTYPE_CODE[dtype], bias, code, out, width, gate, ldg, gate_index, index_rows, rows, residual, ldr)
+    # (tensors that a view or copy above made live on in `epilogue`)
     return m, weight.contiguous(), weight_scale.contiguous(), epilogue, out
 
 
-def _pointers(epilogue):
-    return [t.data_ptr() if isinstance(t, torch.Tensor) else t for t in epilogue]
+def _pointers(e):
+    """The epilogue's arguments with its tensors as addresses."""
+    dtype, bias, code, out, width, gate, ldg, index, index_rows, rows, residual, ldr = e
+    return (dtype, bias.data_ptr() if bias is not None else None, code, out.data_ptr(), width,
+            *((gate.data_ptr(), ldg, index.data_ptr(), index_rows, rows, residual.data_ptr(), ldr) if gate is not None else
+              (None, 0, None, 0, 0, None, 0)))
 
 
 def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
@@ -96,7 +102,7 @@ def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: tor
         flat, scales = codes.reshape(m, k).contiguous(), scales.reshape(m).contiguous()
         _call_on(index, "xgb_int8_gemm", flat.data_ptr(), weight.data_ptr(), m, n, k, scales.data_ptr(), weight_scale.data_ptr(),
                  *_pointers(epilogue), _err_ptr(codes.device))
-    return out.view(*lead, out.shape[1])
+    return out
 
 
 def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias=None, *,
@@ -121,15 +127,17 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
                                                         residual)
     n, k = weight.shape
     if m:
-        matrix = x.reshape(m, k)
-        if matrix.stride(1) != 1 or (m > 1 and matrix.stride(0) < k):
+        matrix = x if x.ndim == 2 else x.reshape(m, k)
+        ldx, unit = matrix.stride()
+        if unit != 1 or (m > 1 and ldx < k):
             matrix = matrix.contiguous()
-        # codes and scales, laid out as xgb_int8_linear_workspace() says
-        ws_bytes = (m * k + 15) // 16 * 16 + 4 * m
-        ws = torch.empty(ws_bytes, device=x.device, dtype=torch.uint8)
-        _call_on(index, "xgb_int8_linear", matrix.data_ptr(), matrix.stride(0), weight.data_ptr(), m, n, k,
-                 weight_scale.data_ptr(), *_pointers(epilogue), ws.data_ptr(), ws_bytes, _err_ptr(x.device))
-    return out.view(*lead, out.shape[1])
+            ldx = k
+        ptr = matrix.data_ptr()
+        ws_bytes = lib().xgb_int8_linear_workspace(ptr, ldx, m, k)
+        ws = x.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+        _call_on(index, "xgb_int8_linear", ptr, ldx, weight.data_ptr(), m, n, k, weight_scale.data_ptr(), *_pointers(epilogue),
+                 ws.data_ptr() if ws_bytes else None, ws_bytes, _err_ptr(x.device))
+    return out
 
 
 class H3Int8Linear(nn.Module):

@@ -49,6 +49,11 @@ def _refuse_autograd(what: str, *tensors) -> None:
                 raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
 
 
+def _like(t: torch.Tensor, shape) -> torch.Tensor:
+    """An empty contiguous tensor of t's type and device."""
+    return torch.empty_like(t) if t.shape == shape and t.is_contiguous() else t.new_empty(shape)
+
+
 def _call_on(index: int, name: str, *args) -> None:
     """call(name, *args, stream) with device `index` current (launches go to
     the current device, whatever their stream) and on its current stream."""
@@ -307,7 +312,7 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
         raise ValueError(f"{what}: positions must be integers or 32/64-bit floats of shape [S, A] or [B, S, A]")
     if axes > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    q_out = torch.empty((b, s, h, d), device=query.device, dtype=query.dtype)
+    q_out = _like(query, (b, s, h, d))
     k_out = k_ptr = k_out_ptr = k_strides = None
     kh = 0
     if key is not None:
@@ -316,7 +321,7 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
         kh = key.shape[2]
         if key.shape != (b, s, kh, d):
             raise ValueError(f"{what}: query and key differ in batch, sequence or head dim")
-        k_out = torch.empty((b, s, kh, d), device=key.device, dtype=key.dtype)
+        k_out = _like(key, (b, s, kh, d))
         k_ptr, k_out_ptr, k_strides = key.data_ptr(), k_out.data_ptr(), _I64x3(*key.stride()[:3])
     if not b * s * d or not h or (key is not None and not kh):
         if b * s * d and (h or kh):
@@ -413,14 +418,14 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
             raise ValueError(f"{what}: indices must be int64 [S] or [B, S]")
         index_batch = s if indices.ndim == 2 else 0
         indices = indices.contiguous()
-    x_out = torch.empty((b, s, w), device=branch.device, dtype=dtype)
+    x_out = _like(branch, (b, s, w))
     quant_code, code_type = _QUANT_CODE[quant]
     h_out = codes = scales = None
     if quant_code:
-        codes = torch.empty((b, s, w), device=branch.device, dtype=code_type)
-        scales = torch.empty((b, s), device=branch.device, dtype=torch.float32)
+        codes = branch.new_empty((b, s, w), dtype=code_type)
+        scales = branch.new_empty((b, s), dtype=torch.float32)
     elif pre_norm is not None:
-        h_out = torch.empty((b, s, w), device=branch.device, dtype=dtype)
+        h_out = torch.empty_like(x_out)
     if b * s:
         _call_on(index, "xgb_sandwich_norm", branch.data_ptr(), _I64x2(bs[0], bs[1]), residual.data_ptr(), _I64x2(rs[0], rs[1]),
                  code, b, s, w, _NORM_CODE[post_norm], _ptr(post_weight), _NORM_CODE[pre_norm], _ptr(pre_weight), eps,
