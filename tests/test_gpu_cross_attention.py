@@ -126,6 +126,41 @@ def test_masks(cuda_device, sq, skv, d):
     check(got, q, kk, vv, valid[3:4].expand(5, -1))
 
 
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+@pytest.mark.parametrize("skv", [1, 60, 64, 200, 520])
+def test_many_units_for_each_cta(cuda_device, d, dtype, skv):
+    """Long query sequences: every CTA walks several units, of one key tile and
+    of many, and of samples without keys in between."""
+    from xgen_b200.attention import cross_attention
+
+    b, h, sq = 4, 6, 10000  # 960 units
+    q, k, v = inputs(b, h, 3, sq, skv, d, dtype, cuda_device, seed=skv)
+    lens = torch.tensor([skv, 0, max(1, skv // 3), skv], dtype=torch.int32)
+    for n in (None, lens):
+        got = cross_attention(q, k, v, kv_lens=n.to(cuda_device) if n is not None else None)
+        valid = torch.ones(b, skv, dtype=torch.bool) if n is None else torch.arange(skv)[None] < n[:, None]
+        at = torch.cat([torch.arange(0, sq, 97), torch.arange(sq - 20, sq)])  # rows of all units
+        check(got[:, :, at], q[:, :, at], k, v, valid)
+        if n is not None:
+            assert not got[1].any()
+
+
+def test_later_tiles_far_above_the_first(cuda_device):
+    """The first 64 keys set a row's reference value; later scores exceed it by
+    2^20 to 2^400, in some rows only, once or again and again."""
+    from xgen_b200.attention import cross_attention
+
+    for dtype, steps in ((torch.bfloat16, (0, 60, 70, 300, 310, 50)), (torch.float16, (0, 12, 30, 60, 61, 3))):
+        skv = 64 * len(steps) + 5
+        q, k, v = inputs(1, 2, 2, 150, skv, 64, dtype, cuda_device, seed=3)
+        q, k = q * 0.25, k * 0.25
+        q[..., 0] = torch.where(torch.arange(150, device=cuda_device) % 3 == 0, 1.0, 0.0).to(dtype)
+        raise_by = torch.tensor(steps, device=cuda_device).repeat_interleave(64)
+        k[..., 0] = torch.cat([raise_by, raise_by[:5]]).to(dtype) / 4
+        got = cross_attention(q, k, v, sm_scale=math.log(2) * 4)  # scores in log2 units: steps
+        check(got, q, k, v, torch.ones(1, skv, dtype=torch.bool), math.log(2) * 4)
+
+
 def test_large_scores_and_infinities(cuda_device):
     """Scores far apart (the running maximum rises many times), rows of -inf
     scores, and a value of infinity where it is attended to."""

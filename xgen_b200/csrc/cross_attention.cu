@@ -19,13 +19,35 @@
 // loads and first scores of the next unit overlap the last tiles and the
 // epilogue of this one:
 //   warps 0-3, 4-7  softmax and epilogue of query tile 0, 1 (a thread a row)
-//   warp 8          TMA producer: Q tiles, a ring of 64-key K/V tiles
+//   warp 8          TMA producer: Q tiles, a ring of 64-key K tiles, one of V tiles
 //   warps 9, 10     MMA issuers of query tile 0, 1
 //   warp 11         clears the value rows behind the last key of a sample
 // TMEM (512 columns): two S buffers of 64 fp32 columns for each query tile
-// (P overwrites its S), O0, O1. Softmax as in the self-attention kernel: exp2
-// domain, 32-bit statistics, O rescaled only when the running maximum rises by
-// more than 8, P rounded to the type of V for the second product.
+// (P overwrites its S), O0, O1. Q has two buffers, so the next unit's queries
+// are there when its first scores are due; a unit's output is staged in the
+// one that held its queries.
+//
+// What bounds a step of 64 keys for both query tiles is the tensor pipe and
+// the threads that feed it. Measured back to back on one SM: a 128 x 64 x 16
+// product from shared memory takes 49 cycles (its 6 KB of operands at 128 bytes
+// a cycle; the arithmetic alone 32), a 128 x 128 x 16 one with P from TMEM 64,
+// and one thread sends out at most one product in 51 cycles: 16 x 49 + 8 x 64 =
+// 1,296 cycles a step. (The one product in 51 cycles holds for a thread picked
+// as lane 0; one picked by elect.sync sends out one in 16, its operands being
+// uniform for the compiler.) So an issuer has nothing to compute between the last
+// probabilities of a tile and its products: descriptors, flags and the waits
+// that can be early are behind it, indexes are kept by increments, a step has a
+// single commit (S(t)'s, sent behind P V(t - 2); the softmax warps, which see
+// it, pass on which K and V tiles that frees), and warps, not threads, arrive.
+//
+// Softmax in the exp2 domain with 32-bit sums. The reference value m of a row
+// is the maximum of its first key tile. A later score may exceed it by 2^40
+// (bf16; 2^15 in fp16) before a probability or a sum could overflow, and being
+// larger than one costs no digits, so later tiles take no maximum: the tile's
+// own sum shows whether one came near the limit, and only then is the maximum
+// taken, O rescaled and the tile repeated. Without the maximum's instructions
+// and their place in the chain from scores to probabilities a step is a third
+// shorter. P is rounded to the type of V for the second product.
 //
 // Parts of a unit leave 32-bit O, m and l rows in a workspace of the call;
 // a second small kernel joins them.
@@ -47,10 +69,15 @@ constexpr int kThreads = 384;
 constexpr int kTmaWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kFixWarp = 11;
-constexpr float kTau = 8.0f;
 constexpr float kNegInf = -__builtin_huge_valf();
-
-constexpr int kOutBytes = 32 * 128;
+#ifndef XGB_CROSS_POLY
+#define XGB_CROSS_POLY 0
+#endif
+constexpr int kPoly = XGB_CROSS_POLY;
+template <int kShare>
+__device__ __forceinline__ constexpr bool poly_pair(int pair) {
+  return kShare > 0 && pair % (kShare > 0 ? kShare : 1) == kShare - 1;
+}
 
 template <typename T, int kD>
 struct Cfg {
@@ -59,14 +86,15 @@ struct Cfg {
   static constexpr int kQBytes = kSubs * kQSub;
   static constexpr int kKVSub = kBN * 128;
   static constexpr int kKVBytes = kSubs * kKVSub;
-  static constexpr int kStages = kD == 128 ? 4 : 8;
-  static constexpr int kKOff = 2 * kQBytes;
+  static constexpr int kStages = kD == 128 ? 3 : 6;
+  static constexpr int kKOff = 4 * kQBytes;  // [query tile][buffer]
   static constexpr int kVOff = kKOff + kStages * kKVBytes;
-  static constexpr int kOutOff = kVOff + kStages * kKVBytes;  // 32 rows x 64 channels of each softmax warp
-  static constexpr int kBarOff = kOutOff + 8 * kOutBytes;
+  static constexpr int kBarOff = kVOff + kStages * kKVBytes;
   static constexpr int kSmem = kBarOff + 512 + 1024;  // + barriers + alignment slack
   static constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-  static constexpr uint32_t kIdescQK = instr_desc(1, kFmt, kFmt, false, false, kBM, kBN);
+  static constexpr uint32_t kIdescQK = instr_desc(1, kFmt, kFmt, false, false, kBM, 0);  // + keys
+  // Sum of a tile's 64 probabilities above which its maximum is looked at.
+  static constexpr float kLimit = std::is_same<T, __nv_bfloat16>::value ? 1.0995116e12f /* 2^40 */ : 32768.0f;
   static constexpr uint32_t kIdescPV = instr_desc(1, kFmt, kFmt, false, true, kBM, kD);
 };
 
@@ -81,7 +109,8 @@ struct Params {
   int qb, qh, kb, kh, vb, vh;
   int n_qt;      // units of 256 rows of a (batch, head)
   int splits;    // parts of a unit's keys
-  int64_t units;  // batch * heads * n_qt * splits
+  uint32_t units;  // batch * heads * n_qt * splits, below 2^31
+  FastDiv div_splits, div_qt, div_heads, div_group;
   int part_rows;  // rows of a part in the workspace
   float* part_o;  // [units][part_rows][D]
   float2* part_ml;  // [units][part_rows]
@@ -89,49 +118,52 @@ struct Params {
 };
 
 struct Barriers {
-  uint64_t q_full[2], q_empty[2];
-  uint64_t k_full[8], v_full[8], v_ready[8], kv_empty[8];
+  uint64_t q_full[2][2], q_empty[2][2];  // [query tile][buffer]
+  uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
   uint64_t s_full[2][2], p_full[2][2];
-  uint64_t pv_done[2];
   uint64_t o_full[2], o_empty[2];
   uint64_t end[2];
   uint32_t tmem_base;
 };
 
-// A CTA's walk over its non-empty units. Units without keys are visited by the
-// softmax warps only.
+// A unit of a CTA's walk. Every role finds its units by itself, some of them
+// on one thread in the products' critical path, so the divisions are 32-bit
+// multiplications.
 struct Unit {
-  int64_t id;
+  uint32_t id;
   int b, h, m0;
   int kv0, n_kv;  // key tiles [kv0, kv0 + n_kv)
   int len;
 };
 
-__device__ __forceinline__ Unit unit_at(const Params& p, int64_t id) {
+__device__ __forceinline__ Unit unit_at(const Params& p, uint32_t id) {
   Unit u;
   u.id = id;
-  const int64_t item = id / p.splits;
-  const int part = static_cast<int>(id - item * p.splits);
-  const int64_t bh = item / p.n_qt;
-  u.m0 = static_cast<int>(item - bh * p.n_qt) * kRows;
-  u.b = static_cast<int>(bh / p.heads);
-  u.h = static_cast<int>(bh - static_cast<int64_t>(u.b) * p.heads);
+  const uint32_t item = fast_div(id, p.div_splits), bh = fast_div(item, p.div_qt), b = fast_div(bh, p.div_heads);
+  const int part = static_cast<int>(id - item * p.div_splits.d);
+  u.m0 = static_cast<int>(item - bh * p.div_qt.d) * kRows;
+  u.b = static_cast<int>(b);
+  u.h = static_cast<int>(bh - b * p.div_heads.d);
   u.len = p.lens ? min(max(__ldg(p.lens + u.b), 0), p.seq_kv) : p.seq_kv;
   const int n_all = (u.len + kBN - 1) / kBN;
-  const int per = (n_all + p.splits - 1) / p.splits;
+  const int per = static_cast<int>(fast_div(n_all + p.splits - 1, p.div_splits));
   u.kv0 = min(part * per, n_all);
   u.n_kv = min(per, n_all - u.kv0);
   return u;
 }
 
-// Position in the stream of key tiles that the CTA's non-empty units make up.
+// Position in the stream of key tiles that the CTA's non-empty units make up
+// (units without keys are visited by the softmax warps only).
+template <int kStages>
 struct Cursor {
   Unit u;
   int t;      // tile within the unit
   int g;      // tile within the stream
   int n;      // non-empty units before this one
+  int stage;  // g % kStages
+  uint32_t lap;  // g / kStages, its parity
   bool more;
-  __device__ __forceinline__ void seek(const Params& p, int64_t id) {
+  __device__ __forceinline__ void seek(const Params& p, uint32_t id) {
     more = false;
     for (; id < p.units; id += gridDim.x) {
       u = unit_at(p, id);
@@ -143,11 +175,18 @@ struct Cursor {
     t = 0;
   }
   __device__ __forceinline__ void start(const Params& p) {
-    g = n = 0;
+    g = n = stage = 0;
+    lap = 0;
     seek(p, blockIdx.x);
   }
+  __device__ __forceinline__ int keys() const { return min(kBN, u.len - (u.kv0 + t) * kBN); }
+  __device__ __forceinline__ int steps() const { return (keys() + 15) >> 4; }  // products' key extents are multiples of 16
   __device__ __forceinline__ void next(const Params& p) {
     ++g;
+    if (++stage == kStages) {
+      stage = 0;
+      lap ^= 1;
+    }
     if (++t == u.n_kv) {
       ++n;
       seek(p, u.id + gridDim.x);
@@ -178,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Barriers* bars = reinterpret_cast<Barriers*>(smem + C::kBarOff);
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // the same register for the warp
   const int lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -186,18 +225,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->k_full[s], 1);
       mbar_init(&bars->v_full[s], 1);
       mbar_init(&bars->v_ready[s], 1);
-      mbar_init(&bars->kv_empty[s], 2);  // released by both issuers
+      mbar_init(&bars->k_empty[s], 2);  // released by both softmax warpgroups
+      mbar_init(&bars->v_empty[s], 2);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars->q_full[i], 1);
-      mbar_init(&bars->q_empty[i], 1);
       for (int b = 0; b < 2; ++b) {
+        mbar_init(&bars->q_full[i][b], 1);
+        mbar_init(&bars->q_empty[i][b], 4);  // by the softmax warps, once their output has left
         mbar_init(&bars->s_full[i][b], 1);
-        mbar_init(&bars->p_full[i][b], kBM);
+        mbar_init(&bars->p_full[i][b], 4);  // one arrival a warp: 32 lanes' would queue
       }
-      mbar_init(&bars->pv_done[i], 1);
       mbar_init(&bars->o_full[i], 1);
-      mbar_init(&bars->o_empty[i], kBM);
+      mbar_init(&bars->o_empty[i], 4);
       mbar_init(&bars->end[i], 1);
     }
     fence_barrier_init();
@@ -215,86 +254,110 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == kTmaWarp) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
+    if (elect_one()) {
       bool ok = true;
-      Cursor c;
-      int q_loaded[2] = {0, 0};
+      Cursor<kStages> c;
+      int k_loaded = 0, q_loaded[2] = {0, 0};
       for (c.start(p); c.more && ok; c.next(p)) {
         if (c.t == 0) {
-          for (int i = 0; i < 2 && ok; ++i) {
-            if (c.n > 0) ok = mbar_wait(&bars->q_empty[i], (c.n - 1) & 1, p.err);
+          const int b = c.n & 1;
+          for (int i = 0; i < 2; ++i) {
+            if (c.n > 1) ok = mbar_wait(&bars->q_empty[i][b], ((c.n >> 1) - 1) & 1, p.err);
             if (!ok) break;
-            mbar_arrive_expect_tx(&bars->q_full[i], C::kQBytes);
+            mbar_arrive_expect_tx(&bars->q_full[i][b], C::kQBytes);
             for (int j = 0; j < C::kSubs; ++j)
-              tma_load_4d(smem + i * C::kQBytes + j * C::kQSub, &q_map, &bars->q_full[i], j * 64, c.u.m0 + i * kBM,
-                          c.u.h * p.qh, c.u.b * p.qb);
+              tma_load_4d(smem + (2 * i + b) * C::kQBytes + j * C::kQSub, &q_map, &bars->q_full[i][b], j * 64,
+                          c.u.m0 + i * kBM, c.u.h * p.qh, c.u.b * p.qb);
             ++q_loaded[i];
           }
           if (!ok) break;
         }
-        const int s = c.g % kStages, row = (c.u.kv0 + c.t) * kBN, kvh = c.u.h / p.group;
-        if (c.g >= kStages) ok = mbar_wait(&bars->kv_empty[s], ((c.g / kStages) - 1) & 1, p.err);
+        const int s = c.stage, row = (c.u.kv0 + c.t) * kBN, kvh = static_cast<int>(fast_div(c.u.h, p.div_group));
+        if (c.g >= kStages) ok = mbar_wait(&bars->k_empty[s], c.lap ^ 1, p.err);
         if (!ok) break;
         mbar_arrive_expect_tx(&bars->k_full[s], C::kKVBytes);
         for (int j = 0; j < C::kSubs; ++j)
           tma_load_4d(smem + C::kKOff + s * C::kKVBytes + j * C::kKVSub, &k_map, &bars->k_full[s], j * 64, row, kvh * p.kh,
                       c.u.b * p.kb);
+        ++k_loaded;
+        if (c.g >= kStages) ok = mbar_wait(&bars->v_empty[s], c.lap ^ 1, p.err);
+        if (!ok) break;
         mbar_arrive_expect_tx(&bars->v_full[s], C::kKVBytes);
         for (int j = 0; j < C::kSubs; ++j)
           tma_load_4d(smem + C::kVOff + s * C::kKVBytes + j * C::kKVSub, &v_map, &bars->v_full[s], j * 64, row, kvh * p.vh,
                       c.u.b * p.vb);
       }
       // Never leave with copies in flight: wait (bounded) for the last ones.
-      for (int g = max(0, c.g - kStages); g < c.g; ++g) {
+      for (int g = max(0, k_loaded - kStages); g < k_loaded; ++g)
         mbar_wait(&bars->k_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
+      for (int g = max(0, c.g - kStages); g < c.g; ++g)
         mbar_wait(&bars->v_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
-      }
       for (int i = 0; i < 2; ++i)
-        if (q_loaded[i]) mbar_wait(&bars->q_full[i], (q_loaded[i] - 1) & 1, p.err, 100000000ull);
+        for (int n = max(0, q_loaded[i] - 2); n < q_loaded[i]; ++n)
+          mbar_wait(&bars->q_full[i][n & 1], (n >> 1) & 1, p.err, 100000000ull);
     }
   } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // ------------------------------------------------------------ MMA issuers
     const int i = warp - kMmaWarp;
-    if (lane == 0) {
-      const uint32_t qa = smem_u32(smem) + i * C::kQBytes;
-      const uint32_t k_saddr = smem_u32(smem + C::kKOff), v_saddr = smem_u32(smem + C::kVOff);
+    if (elect_one()) {
+      // Descriptors differ in their address alone (in 16-byte units, from bit 0).
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(smem) + 2 * i * C::kQBytes, 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(smem_u32(smem + C::kKOff), 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + C::kVOff), C::kKVSub, 1024);
       uint64_t* v_bar = p.lens ? bars->v_ready : bars->v_full;
       bool ok = true;
-      Cursor sc, pc;  // scores run two tiles ahead of the second product
+      Cursor<kStages> sc, pc;  // scores run two tiles ahead of the second product
       sc.start(p);
       pc = sc;
+      auto wait_s = [&]() {  // operands of the score cursor's tile
+        if (sc.t == 0) ok = ok && mbar_wait(&bars->q_full[i][sc.n & 1], (sc.n >> 1) & 1, p.err);
+        ok = ok && mbar_wait(&bars->k_full[sc.stage], sc.lap, p.err);
+      };
       auto issue_s = [&]() {
-        const int s = sc.g % kStages;
-        if (sc.t == 0) ok = mbar_wait(&bars->q_full[i], sc.n & 1, p.err);
-        ok = ok && mbar_wait(&bars->k_full[s], (sc.g / kStages) & 1, p.err);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t ka = k_saddr + s * C::kKVBytes;
+        const uint64_t qa = q_desc + (sc.n & 1) * (C::kQBytes / 16), ka = k_desc + sc.stage * (C::kKVBytes / 16);
+        // keys in multiples of 16: N >> 3 at bit 17 of the descriptor
+        const uint32_t idesc = C::kIdescQK | static_cast<uint32_t>(sc.steps() * 2) << 17;
 #pragma unroll
         for (int k = 0; k < kD / 16; ++k)
-          mma_ss<Kind::kF16>(tmem + s_col(i, sc.g & 1), smem_desc_sw128(qa + (k >> 2) * C::kQSub + (k & 3) * 32, 16, 1024),
-                             smem_desc_sw128(ka + (k >> 2) * C::kKVSub + (k & 3) * 32, 16, 1024), C::kIdescQK, k > 0);
+          mma_ss<Kind::kF16>(tmem + s_col(i, sc.g & 1), qa + ((k >> 2) * C::kQSub + (k & 3) * 32) / 16,
+                             ka + ((k >> 2) * C::kKVSub + (k & 3) * 32) / 16, idesc, k > 0);
         tc_commit(&bars->s_full[i][sc.g & 1]);
-        if (sc.t == sc.u.n_kv - 1) tc_commit(&bars->q_empty[i]);
-        sc.next(p);
       };
-      for (int k = 0; k < 2 && sc.more && ok; ++k) issue_s();
-      for (; pc.more && ok; pc.next(p)) {
-        const int s = pc.g % kStages;
-        ok = mbar_wait(&v_bar[s], (pc.g / kStages) & 1, p.err) &&
-             mbar_wait(&bars->p_full[i][pc.g & 1], (pc.g >> 1) & 1, p.err);
-        if (ok && pc.t == 0 && pc.n > 0) ok = mbar_wait(&bars->o_empty[i], (pc.n - 1) & 1, p.err);
+      for (int k = 0; k < 2 && sc.more && ok; ++k) {
+        wait_s();
         if (!ok) break;
         tc_fence_after();
-        const uint32_t va = v_saddr + s * C::kKVBytes;
+        issue_s();
+        sc.next(p);
+      }
+      while (pc.more && ok) {
+        // A unit's first scores wait for its queries, whose buffer the softmax
+        // may free only behind this tile's product: late. All others: early.
+        const bool scores = sc.more, late = sc.t == 0;
+        if (scores && !late) wait_s();
+        const uint64_t va = v_desc + pc.stage * (C::kKVBytes / 16);
+        const uint32_t s_tmem = tmem + s_col(i, pc.g & 1);
+        const int steps = pc.steps();
+        const bool first = pc.t == 0, last = pc.t == pc.u.n_kv - 1;
+        ok = ok && mbar_wait(&v_bar[pc.stage], pc.lap, p.err);
+        if (ok && first && pc.n > 0) ok = mbar_wait(&bars->o_empty[i], (pc.n - 1) & 1, p.err);
+        ok = ok && mbar_wait(&bars->p_full[i][pc.g & 1], (pc.g >> 1) & 1, p.err);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
         for (int k = 0; k < kBN / 16; ++k)
-          mma_ts<Kind::kF16>(tmem + o_col(i), tmem + s_col(i, pc.g & 1) + k * 8,
-                             smem_desc_sw128(va + k * 16 * 128, C::kKVSub, 1024), C::kIdescPV, pc.t > 0 || k > 0);
-        tc_commit(&bars->pv_done[i]);
-        tc_commit(&bars->kv_empty[s]);
-        if (pc.t == pc.u.n_kv - 1) tc_commit(&bars->o_full[i]);
-        if (sc.more) issue_s();
+          if (k < steps) mma_ts<Kind::kF16>(tmem + o_col(i), s_tmem + k * 8, va + k * 16 * 128 / 16, C::kIdescPV, !first || k > 0);
+        if (last) tc_commit(&bars->o_full[i]);
+        if (scores && late) {
+          wait_s();
+          if (!ok) break;
+          tc_fence_after();
+        }
+        // behind the last scores the two phases that would follow still end
+        if (scores) issue_s();
+        else tc_commit(&bars->s_full[i][pc.g & 1]);
+        if (scores) sc.next(p);
+        pc.next(p);
       }
       tc_commit(&bars->end[i]);
       mbar_wait(&bars->end[i], 0, p.err, 100000000ull);
@@ -302,16 +365,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kFixWarp) {
     // ------------------------------------------------------------ value rows behind the last key
     if (p.lens) {
-      Cursor c;
+      Cursor<kStages> c;
       for (c.start(p); c.more; c.next(p)) {
-        const int s = c.g % kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars->v_full[s], (c.g / kStages) & 1, p.err))) break;
-        const int valid = c.u.len - (c.u.kv0 + c.t) * kBN;
-        if (valid < kBN) {
+        const int s = c.stage;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->v_full[s], c.lap, p.err))) break;
+        const int valid = c.keys(), read = (valid + 15) / 16 * 16;
+        if (valid < read) {
           // rows of 128 bytes; the swizzle moves 16-byte pieces within a row
           for (int j = 0; j < C::kSubs; ++j) {
             uint4* rows = reinterpret_cast<uint4*>(smem + C::kVOff + s * C::kKVBytes + j * C::kKVSub);
-            for (int e = valid * 8 + lane; e < kBN * 8; e += 32) rows[e] = make_uint4(0, 0, 0, 0);
+            for (int e = valid * 8 + lane; e < read * 8; e += 32) rows[e] = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
@@ -329,29 +392,115 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float comb = p.scale_log2;
     bool ok = true;
     int g = 0, n = 0;
-    for (int64_t id = blockIdx.x; id < p.units && ok; id += gridDim.x) {
+    int leaving = -1;  // buffer whose output this warp's last store still reads
+    auto release_q = [&]() {
+      if (leaving >= 0 && lane == 0) {
+        bulk_wait_read<0>();
+        mbar_arrive(&bars->q_empty[i][leaving]);
+      }
+      leaving = -1;
+    };
+    int ks = 0, vs = kStages - 2;  // stages of g and of g - 2
+    // A unit's epilogue runs behind the first tile of the next one, whose scores
+    // are there before this one's last product has ended.
+    struct Pending {
+      Unit u;
+      float m, l;
+      int n;  // -1: none
+    } done;
+    done.n = -1;
+    auto epilogue = [&]() {
+      const Unit& v = done.u;
+      const int buf = done.n & 1, row = v.m0 + r;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[i], buf, p.err));
+      done.n = -1;
+      if (!ok) return;
+      tc_fence_after();
+      if (p.splits > 1) {
+        const int64_t part = static_cast<int64_t>(v.id) * p.part_rows + r;
+#pragma unroll 1
+        for (int c = 0; c < kD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_ld_wait();
+          if (row >= p.seq_q) continue;
+          float4* po = reinterpret_cast<float4*>(p.part_o + part * kD) + c * 8;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            po[e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]), __uint_as_float(o[4 * e + 2]),
+                                __uint_as_float(o[4 * e + 3]));
+        }
+        if (row < p.seq_q) p.part_ml[part] = make_float2(done.m, done.l);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bars->o_empty[i]);
+          mbar_arrive(&bars->q_empty[i][buf]);
+        }
+        return;
+      }
+      // The rows take the place of their queries (every product with those has
+      // ended) and leave by TMA, which does not write rows behind the last query.
+      const float inv_l = done.l != 0.f ? 1.0f / done.l : 0.f;
+      uint8_t* stage = smem + (2 * i + buf) * C::kQBytes + lane_base * 128;
+#pragma unroll 1
+      for (int c = 0; c < C::kSubs; ++c) {
+        uint32_t o[2][32];
+        tmem_ld64(o_addr + c * 64, o);
+        tmem_ld_wait();
+        if (c == C::kSubs - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->o_empty[i]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t* y = &o[e >> 2][(e & 3) * 8];
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(y[2 * k]) * inv_l, __uint_as_float(y[2 * k + 1]) * inv_l);
+          *reinterpret_cast<uint4*>(stage + c * C::kQSub + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        for (int c = 0; c < C::kSubs; ++c)
+          tma_store_4d(&o_map, stage + c * C::kQSub, c * 64, v.m0 + i * kBM + lane_base, v.h, v.b);
+        bulk_commit();
+      }
+      leaving = buf;
+    };
+    for (uint32_t id = blockIdx.x; id < p.units && ok; id += gridDim.x) {
       const Unit u = unit_at(p, id);
-      const int row = u.m0 + r;
-      T* dst = static_cast<T*>(p.out) + u.b * p.osb + u.h * p.osh + row * p.oss;
-      const int64_t part = id * p.part_rows + r;
       if (u.n_kv == 0) {
+        const int row = u.m0 + r;
         if (row < p.seq_q) {
           if (p.splits > 1) {
-            p.part_ml[part] = make_float2(kNegInf, 0.f);
+            p.part_ml[static_cast<int64_t>(id) * p.part_rows + r] = make_float2(kNegInf, 0.f);
           } else {
+            uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out) + u.b * p.osb + u.h * p.osh + row * p.oss);
 #pragma unroll
-            for (int c = 0; c < kD / 8; ++c) reinterpret_cast<uint4*>(dst)[c] = make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < kD / 8; ++c) dst[c] = make_uint4(0, 0, 0, 0);
           }
         }
         continue;
       }
       float m_used = kNegInf;
-      float rsa[4] = {0.f, 0.f, 0.f, 0.f}, rsb[4] = {0.f, 0.f, 0.f, 0.f};
+      float sum[2] = {0.f, 0.f};
       for (int t = 0; t < u.n_kv; ++t, ++g) {
         const uint32_t s_addr = lane_addr + s_col(i, g & 1);
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[i][g & 1], (g >> 1) & 1, p.err));
         if (!ok) break;
         tc_fence_after();
+        // S(g) is there, so its K tile is done with, and so is V of g - 2, whose
+        // product the issuer sent out before S(g)
+        if ((warp & 3) == 0 && lane == 0) {
+          mbar_arrive(&bars->k_empty[ks]);
+          if (g >= 2) mbar_arrive(&bars->v_empty[vs]);
+        }
+        ks = ks + 1 == kStages ? 0 : ks + 1;
+        vs = vs + 1 == kStages ? 0 : vs + 1;
         uint32_t x[2][32];
         tmem_ld64(s_addr, x);
         tmem_ld_wait();
@@ -363,122 +512,96 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 32; ++e)
               if (c * 32 + e >= valid) x[c][e] = 0xFF800000u;
         }
-        float m4[4];
+        auto tile_max = [&]() {
+          float m4[4];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          m4[2 * c] = fmax3(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
-          m4[2 * c + 1] = fmax3(__uint_as_float(x[c][3]), __uint_as_float(x[c][4]), __uint_as_float(x[c][5]));
+          for (int c = 0; c < 2; ++c) {
+            m4[2 * c] = fmax3(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]), __uint_as_float(x[c][2]));
+            m4[2 * c + 1] = fmax3(__uint_as_float(x[c][3]), __uint_as_float(x[c][4]), __uint_as_float(x[c][5]));
 #pragma unroll
-          for (int e = 6; e < 30; e += 4) {
-            m4[2 * c] = fmax3(m4[2 * c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
-            m4[2 * c + 1] = fmax3(m4[2 * c + 1], __uint_as_float(x[c][e + 2]), __uint_as_float(x[c][e + 3]));
+            for (int e = 6; e < 30; e += 4) {
+              m4[2 * c] = fmax3(m4[2 * c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+              m4[2 * c + 1] = fmax3(m4[2 * c + 1], __uint_as_float(x[c][e + 2]), __uint_as_float(x[c][e + 3]));
+            }
+            m4[2 * c] = fmax3(m4[2 * c], __uint_as_float(x[c][30]), __uint_as_float(x[c][31]));
           }
-          m4[2 * c] = fmax3(m4[2 * c], __uint_as_float(x[c][30]), __uint_as_float(x[c][31]));
-        }
-        const float mt = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * comb;
-        const float m_new = fmaxf(m_used, mt);
-        const bool need = m_new > m_used + kTau;
-        if (t == 0) {
-          m_used = m_new;
-        } else if (__any_sync(0xffffffffu, need)) {
-          // O must hold the second product of the tile before this one
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->pv_done[i], (g - 1) & 1, p.err));
+          return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * comb;
+        };
+        // P = 2^(comb s - m) over the S buffer; returns its sum in two lanes
+        auto probabilities = [&](float (&ts)[2]) {
+          // a row whose scores are all -inf has its maximum there: p = 2^-inf
+          const float off = m_used == kNegInf ? 0.f : -m_used;
+          float ra[4] = {0.f, 0.f, 0.f, 0.f}, rb[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t packed[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float a, b;
+              ffma2(a, b, __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]), comb, comb, off, off);
+              if (poly_pair<kPoly>(c * 16 + e / 2)) {
+                ex2_poly2<3>(a, b, a, b);
+              } else {
+                a = ex2_approx(a);
+                b = ex2_approx(b);
+              }
+              const int ch = (e / 2) & 3;
+              if (c == 0 && e < 8) {
+                ra[ch] = a;
+                rb[ch] = b;
+              } else {
+                fadd2(ra[ch], rb[ch], ra[ch], rb[ch], a, b);
+              }
+              packed[e / 2] = pack2<T>(a, b);
+            }
+            tmem_st16(s_addr + c * 16, packed);
+          }
+          fadd2(ra[0], rb[0], ra[0], rb[0], ra[1], rb[1]);
+          fadd2(ra[2], rb[2], ra[2], rb[2], ra[3], rb[3]);
+          fadd2(ts[0], ts[1], ra[0], rb[0], ra[2], rb[2]);
+        };
+        if (t == 0) m_used = tile_max();
+        float ts[2];
+        probabilities(ts);
+        if (t > 0 && __any_sync(0xffffffffu, !(ts[0] + ts[1] <= C::kLimit) || m_used == kNegInf)) {
+          // Too large, not a number, or no finite score so far: take the
+          // maximum after all, with O (complete up to the tile before) rescaled.
+          const float m_new = fmaxf(m_used, tile_max());
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[i][(g + 1) & 1], ((g + 1) >> 1) & 1, p.err));
           if (!ok) break;
           tc_fence_after();
-          const float alpha = need ? ex2_approx(m_used - m_new) : 1.0f;
-          if (need) m_used = m_new;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            rsa[j] *= alpha;
-            rsb[j] *= alpha;
-          }
+          const float alpha = m_new > m_used ? ex2_approx(m_used - m_new) : 1.0f;
+          m_used = m_new;
+          sum[0] *= alpha;
+          sum[1] *= alpha;
 #pragma unroll 1
-          for (int c = 0; c < kD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(o_addr + c * 32, o);
+          for (int c = 0; c < kD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + c * 16, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(o_addr + c * 32, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16(o_addr + c * 16, o);
           }
-          tmem_st_wait();
+          probabilities(ts);
         }
-        // a row whose scores are all -inf keeps its maximum there: p = 2^-inf
-        const float off = m_used == kNegInf ? 0.f : -m_used;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float xa, xb;
-            ffma2(xa, xb, __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]), comb, comb, off, off);
-            const float a = ex2_approx(xa), b = ex2_approx(xb);
-            const int ch = (e / 2) & 3;
-            fadd2(rsa[ch], rsb[ch], rsa[ch], rsb[ch], a, b);
-            packed[e / 2] = pack2<T>(a, b);
-          }
-          tmem_st16(s_addr + c * 16, packed);
-        }
+        fadd2(sum[0], sum[1], sum[0], sum[1], ts[0], ts[1]);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&bars->p_full[i][g & 1]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[i][g & 1]);
+        if (t == 0 && done.n >= 0) epilogue();
+        if (!ok) break;
+        if (t == 1) release_q();
       }
       if (!ok) break;
-      const float l = ((rsa[0] + rsb[0]) + (rsa[1] + rsb[1])) + ((rsa[2] + rsb[2]) + (rsa[3] + rsb[3]));
-      // ------------------------------------------------------------ epilogue
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[i], n & 1, p.err));
-      ++n;
-      if (!ok) break;
-      tc_fence_after();
-      if (p.splits > 1) {
-#pragma unroll 1
-        for (int c = 0; c < kD / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(o_addr + c * 32, o);
-          tmem_ld_wait();
-          if (row >= p.seq_q) continue;
-          float4* po = reinterpret_cast<float4*>(p.part_o + part * kD) + c * 8;
-#pragma unroll
-          for (int v = 0; v < 8; ++v)
-            po[v] = make_float4(__uint_as_float(o[4 * v]), __uint_as_float(o[4 * v + 1]), __uint_as_float(o[4 * v + 2]),
-                                __uint_as_float(o[4 * v + 3]));
-        }
-        if (row < p.seq_q) p.part_ml[part] = make_float2(m_used, l);
-        tc_fence_before();
-        mbar_arrive(&bars->o_empty[i]);
-        continue;
-      }
-      // 64 channels at a time through shared memory, so that rows leave as whole
-      // lines; rows behind the last query are not written by the store.
-      const float inv_l = l != 0.f ? 1.0f / l : 0.f;
-      uint8_t* stage = smem + C::kOutOff + warp * kOutBytes;
-#pragma unroll 1
-      for (int c = 0; c < C::kSubs; ++c) {
-        uint32_t o[2][32];
-        tmem_ld64(o_addr + c * 64, o);
-        if (lane == 0) bulk_wait_read<0>();  // the store before this one has left the buffer
-        __syncwarp();
-        tmem_ld_wait();
-        if (c == C::kSubs - 1) {
-          tc_fence_before();
-          mbar_arrive(&bars->o_empty[i]);
-        }
-#pragma unroll
-        for (int v = 0; v < 8; ++v) {
-          const uint32_t* x = &o[v >> 2][(v & 3) * 8];
-          uint32_t w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = pack2<T>(__uint_as_float(x[2 * e]) * inv_l, __uint_as_float(x[2 * e + 1]) * inv_l);
-          *reinterpret_cast<uint4*>(stage + lane * 128 + ((v ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_4d(&o_map, stage, c * 64, u.m0 + i * kBM + lane_base, u.h, u.b);
-          bulk_commit();
-        }
-      }
+      release_q();  // the unit after next loads its queries there
+      done.u = u;
+      done.m = m_used;
+      done.l = sum[0] + sum[1];
+      done.n = n++;
     }
+    if (ok && done.n >= 0) epilogue();
     if (lane == 0) bulk_wait_all();
   }
   tc_fence_before();
@@ -556,11 +679,11 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
   __shared__ float2 sml[kFewWarps][kFewRows];
   __shared__ float2 part_ml[kFewRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int64_t unit = blockIdx.x / p.splits;  // (batch, key head, row tile)
+  const uint32_t unit = blockIdx.x / p.splits;  // (batch, key head, row tile)
   const int part = static_cast<int>(blockIdx.x - unit * p.splits);
-  const int64_t bh = unit / f.tiles;
+  const uint32_t bh = unit / f.tiles;
   const int first_row = static_cast<int>(unit - bh * f.tiles) * kFewRows;
-  const int b = static_cast<int>(bh / f.kv_heads), hk = static_cast<int>(bh - static_cast<int64_t>(b) * f.kv_heads);
+  const int b = static_cast<int>(bh / f.kv_heads), hk = static_cast<int>(bh) - b * f.kv_heads;
   const int rows = p.group * p.seq_q;
   const int len = p.lens ? min(max(__ldg(p.lens + b), 0), p.seq_kv) : p.seq_kv;
   const int steps_all = (len + kFewKeys - 1) / kFewKeys;
@@ -690,7 +813,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
         sum = fmaf(wt, ld_cluster_f32(map_to_rank(&so[0][r][d], q)), sum);
       }
     } else if (p.splits > 1) {
-      const int64_t slot = (unit * p.splits + part) * kFewRows + r;
+      const int64_t slot = (static_cast<int64_t>(unit) * p.splits + part) * kFewRows + r;
       p.part_o[slot * kD + d] = sum;
       if (d == 0) p.part_ml[slot] = part_ml[r];
       continue;
@@ -806,7 +929,7 @@ int launch(const CUtensorMap (&map)[4], const Params& p, int64_t batch, int sms,
   auto kernel = cross_attention_kernel<T, kD>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
     return XGB_ERR_LAUNCH;
-  const int grid = static_cast<int>(std::min<int64_t>(p.units, sms));
+  const int grid = std::min(static_cast<int>(p.units), sms);
   kernel<<<grid, kThreads, C::kSmem, st>>>(map[0], map[1], map[2], map[3], p);
   const int rc = launch_status();
   if (rc || p.splits == 1) return rc;
@@ -983,11 +1106,16 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
   p.oss = out_strides[2];
   p.n_qt = static_cast<int>(cdiv(seq_q, cross::kRows));
   p.splits = n.splits;
-  p.units = n.items * n.splits;
+  if (n.items * n.splits > INT32_MAX - 65536) return XGB_ERR_SHAPE;  // room for a walk's last step
+  p.units = static_cast<uint32_t>(n.items * n.splits);
+  p.div_splits = make_fastdiv(static_cast<uint32_t>(n.splits));
+  p.div_qt = make_fastdiv(static_cast<uint32_t>(p.n_qt));
+  p.div_heads = make_fastdiv(static_cast<uint32_t>(heads));
+  p.div_group = make_fastdiv(static_cast<uint32_t>(p.group));
   p.part_rows = static_cast<int>(n.part_rows);
   if (need) {
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + p.units * p.part_rows * head_dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + n.items * n.splits * p.part_rows * head_dim);
   }
   p.err = error_flag;
   cudaStream_t st = as_stream(stream);
