@@ -36,9 +36,8 @@
 // as lane 0; one picked by elect.sync sends out one in 16, its operands being
 // uniform for the compiler.) So an issuer has nothing to compute between the last
 // probabilities of a tile and its products: descriptors, flags and the waits
-// that can be early are behind it, indexes are kept by increments, a step has a
-// single commit (S(t)'s, sent behind P V(t - 2); the softmax warps, which see
-// it, pass on which K and V tiles that frees), and warps, not threads, arrive.
+// that can be early are behind it, indexes are kept by increments, and warps,
+// not threads, arrive.
 //
 // Softmax in the exp2 domain with 32-bit sums. The reference value m of a row
 // is the maximum of its first key tile. A later score may exceed it by 2^40
@@ -225,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars->k_full[s], 1);
       mbar_init(&bars->v_full[s], 1);
       mbar_init(&bars->v_ready[s], 1);
-      mbar_init(&bars->k_empty[s], 2);  // released by both softmax warpgroups
+      mbar_init(&bars->k_empty[s], 2);  // released by both issuers
       mbar_init(&bars->v_empty[s], 2);
     }
     for (int i = 0; i < 2; ++i) {
@@ -255,42 +254,53 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kTmaWarp) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
+      // K runs two tiles ahead of V, as the scores do of the second product, so
+      // that neither waits for the other's buffer to be free.
       bool ok = true;
-      Cursor<kStages> c;
-      int k_loaded = 0, q_loaded[2] = {0, 0};
-      for (c.start(p); c.more && ok; c.next(p)) {
-        if (c.t == 0) {
-          const int b = c.n & 1;
+      int q_loaded[2] = {0, 0};
+      Cursor<kStages> kc, vc;
+      kc.start(p);
+      vc = kc;
+      auto load_k = [&]() {
+        const Unit& u = kc.u;
+        if (kc.t == 0) {
+          const int b = kc.n & 1;
           for (int i = 0; i < 2; ++i) {
-            if (c.n > 1) ok = mbar_wait(&bars->q_empty[i][b], ((c.n >> 1) - 1) & 1, p.err);
-            if (!ok) break;
+            if (kc.n > 1) ok = ok && mbar_wait(&bars->q_empty[i][b], ((kc.n >> 1) - 1) & 1, p.err);
+            if (!ok) return;
             mbar_arrive_expect_tx(&bars->q_full[i][b], C::kQBytes);
             for (int j = 0; j < C::kSubs; ++j)
               tma_load_4d(smem + (2 * i + b) * C::kQBytes + j * C::kQSub, &q_map, &bars->q_full[i][b], j * 64,
-                          c.u.m0 + i * kBM, c.u.h * p.qh, c.u.b * p.qb);
+                          u.m0 + i * kBM, u.h * p.qh, u.b * p.qb);
             ++q_loaded[i];
           }
-          if (!ok) break;
         }
-        const int s = c.stage, row = (c.u.kv0 + c.t) * kBN, kvh = static_cast<int>(fast_div(c.u.h, p.div_group));
-        if (c.g >= kStages) ok = mbar_wait(&bars->k_empty[s], c.lap ^ 1, p.err);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&bars->k_full[s], C::kKVBytes);
+        if (kc.g >= kStages) ok = ok && mbar_wait(&bars->k_empty[kc.stage], kc.lap ^ 1, p.err);
+        if (!ok) return;
+        mbar_arrive_expect_tx(&bars->k_full[kc.stage], C::kKVBytes);
+        const int kvh = static_cast<int>(fast_div(u.h, p.div_group));
         for (int j = 0; j < C::kSubs; ++j)
-          tma_load_4d(smem + C::kKOff + s * C::kKVBytes + j * C::kKVSub, &k_map, &bars->k_full[s], j * 64, row, kvh * p.kh,
-                      c.u.b * p.kb);
-        ++k_loaded;
-        if (c.g >= kStages) ok = mbar_wait(&bars->v_empty[s], c.lap ^ 1, p.err);
+          tma_load_4d(smem + C::kKOff + kc.stage * C::kKVBytes + j * C::kKVSub, &k_map, &bars->k_full[kc.stage], j * 64,
+                      (u.kv0 + kc.t) * kBN, kvh * p.kh, u.b * p.kb);
+        kc.next(p);
+      };
+      for (int e = 0; e < 2 && kc.more && ok; ++e) load_k();
+      while (vc.more && ok) {
+        const Unit& u = vc.u;
+        if (vc.g >= kStages) ok = mbar_wait(&bars->v_empty[vc.stage], vc.lap ^ 1, p.err);
         if (!ok) break;
-        mbar_arrive_expect_tx(&bars->v_full[s], C::kKVBytes);
+        mbar_arrive_expect_tx(&bars->v_full[vc.stage], C::kKVBytes);
+        const int kvh = static_cast<int>(fast_div(u.h, p.div_group));
         for (int j = 0; j < C::kSubs; ++j)
-          tma_load_4d(smem + C::kVOff + s * C::kKVBytes + j * C::kKVSub, &v_map, &bars->v_full[s], j * 64, row, kvh * p.vh,
-                      c.u.b * p.vb);
+          tma_load_4d(smem + C::kVOff + vc.stage * C::kKVBytes + j * C::kKVSub, &v_map, &bars->v_full[vc.stage], j * 64,
+                      (u.kv0 + vc.t) * kBN, kvh * p.vh, u.b * p.vb);
+        vc.next(p);
+        if (kc.more) load_k();
       }
       // Never leave with copies in flight: wait (bounded) for the last ones.
-      for (int g = max(0, k_loaded - kStages); g < k_loaded; ++g)
+      for (int g = max(0, kc.g - kStages); g < kc.g; ++g)
         mbar_wait(&bars->k_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
-      for (int g = max(0, c.g - kStages); g < c.g; ++g)
+      for (int g = max(0, vc.g - kStages); g < vc.g; ++g)
         mbar_wait(&bars->v_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
       for (int i = 0; i < 2; ++i)
         for (int n = max(0, q_loaded[i] - 2); n < q_loaded[i]; ++n)
@@ -322,6 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_ss<Kind::kF16>(tmem + s_col(i, sc.g & 1), qa + ((k >> 2) * C::kQSub + (k & 3) * 32) / 16,
                              ka + ((k >> 2) * C::kKVSub + (k & 3) * 32) / 16, idesc, k > 0);
         tc_commit(&bars->s_full[i][sc.g & 1]);
+        tc_commit(&bars->k_empty[sc.stage]);
       };
       for (int k = 0; k < 2 && sc.more && ok; ++k) {
         wait_s();
@@ -347,6 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < kBN / 16; ++k)
           if (k < steps) mma_ts<Kind::kF16>(tmem + o_col(i), s_tmem + k * 8, va + k * 16 * 128 / 16, C::kIdescPV, !first || k > 0);
+        tc_commit(&bars->v_empty[pc.stage]);
         if (last) tc_commit(&bars->o_full[i]);
         if (scores && late) {
           wait_s();
@@ -400,7 +412,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       leaving = -1;
     };
-    int ks = 0, vs = kStages - 2;  // stages of g and of g - 2
     // A unit's epilogue runs behind the first tile of the next one, whose scores
     // are there before this one's last product has ended.
     struct Pending {
@@ -442,26 +453,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       // The rows take the place of their queries (every product with those has
       // ended) and leave by TMA, which does not write rows behind the last query.
       const float inv_l = done.l != 0.f ? 1.0f / done.l : 0.f;
-      uint8_t* stage = smem + (2 * i + buf) * C::kQBytes + lane_base * 128;
-#pragma unroll 1
-      for (int c = 0; c < C::kSubs; ++c) {
-        uint32_t o[2][32];
-        tmem_ld64(o_addr + c * 64, o);
-        tmem_ld_wait();
-        if (c == C::kSubs - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars->o_empty[i]);
-        }
+      uint8_t* stage = smem + (2 * i + buf) * C::kQBytes + lane_base * 128 + lane * 128;
+      uint32_t o[C::kSubs][2][32];
+#pragma unroll
+      for (int c = 0; c < C::kSubs; ++c) tmem_ld64(o_addr + c * 64, o[c]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->o_empty[i]);
+#pragma unroll
+      for (int c = 0; c < C::kSubs; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const uint32_t* y = &o[e >> 2][(e & 3) * 8];
+          const uint32_t* y = &o[c][e >> 2][(e & 3) * 8];
           uint32_t w[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(y[2 * k]) * inv_l, __uint_as_float(y[2 * k + 1]) * inv_l);
-          *reinterpret_cast<uint4*>(stage + c * C::kQSub + lane * 128 + ((e ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          *reinterpret_cast<uint4*>(stage + c * C::kQSub + ((e ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
@@ -493,14 +502,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[i][g & 1], (g >> 1) & 1, p.err));
         if (!ok) break;
         tc_fence_after();
-        // S(g) is there, so its K tile is done with, and so is V of g - 2, whose
-        // product the issuer sent out before S(g)
-        if ((warp & 3) == 0 && lane == 0) {
-          mbar_arrive(&bars->k_empty[ks]);
-          if (g >= 2) mbar_arrive(&bars->v_empty[vs]);
-        }
-        ks = ks + 1 == kStages ? 0 : ks + 1;
-        vs = vs + 1 == kStages ? 0 : vs + 1;
         uint32_t x[2][32];
         tmem_ld64(s_addr, x);
         tmem_ld_wait();
