@@ -23,9 +23,10 @@
 //   warps 9, 10     MMA issuers of query tile 0, 1
 //   warp 11         clears the value rows behind the last key of a sample
 // TMEM (512 columns): two S buffers of 64 fp32 columns for each query tile
-// (P overwrites its S), O0, O1. Q has two buffers, so the next unit's queries
-// are there when its first scores are due; a unit's output is staged in the
-// one that held its queries.
+// (P overwrites its S), O0, O1. Shared memory at D = 128: three 32 KB places
+// for query tiles, so that the next unit's first one is there long before its
+// scores are due and its second one two key tiles before, three K and V tiles,
+// and 4 KB a softmax warp in which output rows wait for their TMA store.
 //
 // What bounds a step of 64 keys for both query tiles is the tensor pipe and
 // the threads that feed it. Measured back to back on one SM: a 128 x 64 x 16
@@ -78,6 +79,9 @@ __device__ __forceinline__ constexpr bool poly_pair(int pair) {
   return kShare > 0 && pair % (kShare > 0 ? kShare : 1) == kShare - 1;
 }
 
+constexpr int kQPlaces = 3;
+constexpr int kOutBytes = 32 * 128;  // 32 rows x 64 channels
+
 template <typename T, int kD>
 struct Cfg {
   static constexpr int kSubs = kD / 64;                // 128-byte-wide sub-tiles of a row
@@ -86,9 +90,10 @@ struct Cfg {
   static constexpr int kKVSub = kBN * 128;
   static constexpr int kKVBytes = kSubs * kKVSub;
   static constexpr int kStages = kD == 128 ? 3 : 6;
-  static constexpr int kKOff = 4 * kQBytes;  // [query tile][buffer]
+  static constexpr int kKOff = kQPlaces * kQBytes;
   static constexpr int kVOff = kKOff + kStages * kKVBytes;
-  static constexpr int kBarOff = kVOff + kStages * kKVBytes;
+  static constexpr int kOutOff = kVOff + kStages * kKVBytes;
+  static constexpr int kBarOff = kOutOff + 8 * kOutBytes;
   static constexpr int kSmem = kBarOff + 512 + 1024;  // + barriers + alignment slack
   static constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   static constexpr uint32_t kIdescQK = instr_desc(1, kFmt, kFmt, false, false, kBM, 0);  // + keys
@@ -117,8 +122,13 @@ struct Params {
 };
 
 struct Barriers {
-  uint64_t q_full[2][2], q_empty[2][2];  // [query tile][buffer]
-  uint64_t k_full[6], k_empty[6], v_full[6], v_ready[6], v_empty[6];
+  // Query tiles 2n + i go round the places; the barriers go round twice as many
+  // tiles, so that each is only ever waited for by one query tile's issuer, a
+  // phase after the other.
+  uint64_t q_full[2 * kQPlaces], q_empty[2 * kQPlaces];
+  // V(g) and K(g + 2) come and go together: an issuer uses them in one step.
+  uint64_t kv_full[6], v_ready[6], kv_empty[6];
+  uint64_t first_full[2], first_empty[2];  // K(0), K(1)
   uint64_t s_full[2][2], p_full[2][2];
   uint64_t o_full[2], o_empty[2];
   uint64_t end[2];
@@ -153,14 +163,10 @@ __device__ __forceinline__ Unit unit_at(const Params& p, uint32_t id) {
 
 // Position in the stream of key tiles that the CTA's non-empty units make up
 // (units without keys are visited by the softmax warps only).
-template <int kStages>
 struct Cursor {
   Unit u;
-  int t;      // tile within the unit
-  int g;      // tile within the stream
-  int n;      // non-empty units before this one
-  int stage;  // g % kStages
-  uint32_t lap;  // g / kStages, its parity
+  int t;  // tile within the unit
+  int n;  // non-empty units before this one
   bool more;
   __device__ __forceinline__ void seek(const Params& p, uint32_t id) {
     more = false;
@@ -174,21 +180,28 @@ struct Cursor {
     t = 0;
   }
   __device__ __forceinline__ void start(const Params& p) {
-    g = n = stage = 0;
-    lap = 0;
+    n = 0;
     seek(p, blockIdx.x);
   }
+  __device__ __forceinline__ bool last() const { return t == u.n_kv - 1; }
   __device__ __forceinline__ int keys() const { return min(kBN, u.len - (u.kv0 + t) * kBN); }
-  __device__ __forceinline__ int steps() const { return (keys() + 15) >> 4; }  // products' key extents are multiples of 16
   __device__ __forceinline__ void next(const Params& p) {
-    ++g;
-    if (++stage == kStages) {
-      stage = 0;
-      lap ^= 1;
-    }
     if (++t == u.n_kv) {
       ++n;
       seek(p, u.id + gridDim.x);
+    }
+  }
+};
+
+// Place of tile g in a ring of kStages: g % kStages and the parity of g / kStages.
+template <int kStages>
+struct Ring {
+  int stage = 0;
+  uint32_t lap = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) {
+      stage = 0;
+      lap ^= 1;
     }
   }
 };
@@ -221,16 +234,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&bars->k_full[s], 1);
-      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->kv_full[s], 1);
       mbar_init(&bars->v_ready[s], 1);
-      mbar_init(&bars->k_empty[s], 2);  // released by both issuers
-      mbar_init(&bars->v_empty[s], 2);
+      mbar_init(&bars->kv_empty[s], 2);  // released by both issuers
+    }
+    for (int e = 0; e < 2 * kQPlaces; ++e) {
+      mbar_init(&bars->q_full[e], 1);
+      mbar_init(&bars->q_empty[e], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars->first_full[i], 1);
+      mbar_init(&bars->first_empty[i], 2);
       for (int b = 0; b < 2; ++b) {
-        mbar_init(&bars->q_full[i][b], 1);
-        mbar_init(&bars->q_empty[i][b], 4);  // by the softmax warps, once their output has left
         mbar_init(&bars->s_full[i][b], 1);
         mbar_init(&bars->p_full[i][b], 4);  // one arrival a warp: 32 lanes' would queue
       }
@@ -254,122 +269,158 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kTmaWarp) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
-      // K runs two tiles ahead of V, as the scores do of the second product, so
-      // that neither waits for the other's buffer to be free.
+      // K runs two tiles ahead of V, as the scores do of the second product.
       bool ok = true;
-      int q_loaded[2] = {0, 0};
-      Cursor<kStages> kc, vc;
+      int k_loaded = 0, v_loaded = 0, q_loaded = 0;
+      Cursor kc, vc;
       kc.start(p);
       vc = kc;
-      auto load_k = [&]() {
+      auto load_q = [&]() {  // a unit's two query tiles, with its first keys
         const Unit& u = kc.u;
-        if (kc.t == 0) {
-          const int b = kc.n & 1;
-          for (int i = 0; i < 2; ++i) {
-            if (kc.n > 1) ok = ok && mbar_wait(&bars->q_empty[i][b], ((kc.n >> 1) - 1) & 1, p.err);
-            if (!ok) return;
-            mbar_arrive_expect_tx(&bars->q_full[i][b], C::kQBytes);
-            for (int j = 0; j < C::kSubs; ++j)
-              tma_load_4d(smem + (2 * i + b) * C::kQBytes + j * C::kQSub, &q_map, &bars->q_full[i][b], j * 64,
-                          u.m0 + i * kBM, u.h * p.qh, u.b * p.qb);
-            ++q_loaded[i];
-          }
+        for (int i = 0; i < 2; ++i, ++q_loaded) {
+          const int place = q_loaded % kQPlaces, before = q_loaded - kQPlaces;  // the place's last tile
+          if (before >= 0)
+            ok = ok && mbar_wait(&bars->q_empty[before % (2 * kQPlaces)], (before / (2 * kQPlaces)) & 1, p.err);
+          if (!ok) return;
+          uint64_t* bar = &bars->q_full[q_loaded % (2 * kQPlaces)];
+          mbar_arrive_expect_tx(bar, C::kQBytes);
+          for (int j = 0; j < C::kSubs; ++j)
+            tma_load_4d(smem + place * C::kQBytes + j * C::kQSub, &q_map, bar, j * 64, u.m0 + i * kBM, u.h * p.qh, u.b * p.qb);
         }
-        if (kc.g >= kStages) ok = ok && mbar_wait(&bars->k_empty[kc.stage], kc.lap ^ 1, p.err);
-        if (!ok) return;
-        mbar_arrive_expect_tx(&bars->k_full[kc.stage], C::kKVBytes);
-        const int kvh = static_cast<int>(fast_div(u.h, p.div_group));
-        for (int j = 0; j < C::kSubs; ++j)
-          tma_load_4d(smem + C::kKOff + kc.stage * C::kKVBytes + j * C::kKVSub, &k_map, &bars->k_full[kc.stage], j * 64,
-                      (u.kv0 + kc.t) * kBN, kvh * p.kh, u.b * p.kb);
-        kc.next(p);
       };
-      for (int e = 0; e < 2 && kc.more && ok; ++e) load_k();
-      while (vc.more && ok) {
-        const Unit& u = vc.u;
-        if (vc.g >= kStages) ok = mbar_wait(&bars->v_empty[vc.stage], vc.lap ^ 1, p.err);
-        if (!ok) break;
-        mbar_arrive_expect_tx(&bars->v_full[vc.stage], C::kKVBytes);
+      auto load_k = [&](uint64_t* bar, int stage) {
+        const Unit& u = kc.u;
         const int kvh = static_cast<int>(fast_div(u.h, p.div_group));
         for (int j = 0; j < C::kSubs; ++j)
-          tma_load_4d(smem + C::kVOff + vc.stage * C::kKVBytes + j * C::kKVSub, &v_map, &bars->v_full[vc.stage], j * 64,
+          tma_load_4d(smem + C::kKOff + stage * C::kKVBytes + j * C::kKVSub, &k_map, bar, j * 64, (u.kv0 + kc.t) * kBN,
+                      kvh * p.kh, u.b * p.kb);
+        ++k_loaded;
+      };
+      for (int e = 0; e < 2 && kc.more && ok; ++e) {
+        if (kc.t == 0) load_q();
+        if (!ok) break;
+        mbar_arrive_expect_tx(&bars->first_full[e], C::kKVBytes);
+        load_k(&bars->first_full[e], e);
+        kc.next(p);
+      }
+      Ring<kStages> ring;
+      int k_stage = 2 % kStages;
+      while (vc.more && ok) {
+        if (v_loaded >= kStages) ok = mbar_wait(&bars->kv_empty[ring.stage], ring.lap ^ 1, p.err);
+        // the first keys' places become free by their own barriers
+        else if (kc.more && v_loaded + 2 >= kStages)
+          ok = mbar_wait(&bars->first_empty[v_loaded + 2 - kStages], 0, p.err);
+        if (!ok) break;
+        uint64_t* bar = &bars->kv_full[ring.stage];
+        mbar_arrive_expect_tx(bar, kc.more ? 2 * C::kKVBytes : C::kKVBytes);
+        const Unit& u = vc.u;
+        const int kvh = static_cast<int>(fast_div(u.h, p.div_group));
+        for (int j = 0; j < C::kSubs; ++j)
+          tma_load_4d(smem + C::kVOff + ring.stage * C::kKVBytes + j * C::kKVSub, &v_map, bar, j * 64,
                       (u.kv0 + vc.t) * kBN, kvh * p.vh, u.b * p.vb);
+        ++v_loaded;
         vc.next(p);
-        if (kc.more) load_k();
+        ring.next();
+        if (kc.more) {
+          load_k(bar, k_stage);
+          k_stage = k_stage + 1 == kStages ? 0 : k_stage + 1;
+          if (kc.t == 0) load_q();
+          if (!ok) break;
+          kc.next(p);
+        }
       }
       // Never leave with copies in flight: wait (bounded) for the last ones.
-      for (int g = max(0, kc.g - kStages); g < kc.g; ++g)
-        mbar_wait(&bars->k_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
-      for (int g = max(0, vc.g - kStages); g < vc.g; ++g)
-        mbar_wait(&bars->v_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
-      for (int i = 0; i < 2; ++i)
-        for (int n = max(0, q_loaded[i] - 2); n < q_loaded[i]; ++n)
-          mbar_wait(&bars->q_full[i][n & 1], (n >> 1) & 1, p.err, 100000000ull);
+      for (int g = 0; g < min(2, k_loaded); ++g) mbar_wait(&bars->first_full[g], 0, p.err, 100000000ull);
+      for (int g = max(0, v_loaded - kStages); g < v_loaded; ++g)
+        mbar_wait(&bars->kv_full[g % kStages], (g / kStages) & 1, p.err, 100000000ull);
+      for (int n = max(0, q_loaded - kQPlaces); n < q_loaded; ++n)
+        mbar_wait(&bars->q_full[n % (2 * kQPlaces)], (n / (2 * kQPlaces)) & 1, p.err, 100000000ull);
     }
   } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
     // ------------------------------------------------------------ MMA issuers
     const int i = warp - kMmaWarp;
     if (elect_one()) {
       // Descriptors differ in their address alone (in 16-byte units, from bit 0).
-      const uint64_t q_desc = smem_desc_sw128(smem_u32(smem) + 2 * i * C::kQBytes, 16, 1024);
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(smem), 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(smem_u32(smem + C::kKOff), 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(smem_u32(smem + C::kVOff), C::kKVSub, 1024);
-      uint64_t* v_bar = p.lens ? bars->v_ready : bars->v_full;
+      uint64_t* kv_bar = p.lens ? bars->v_ready : bars->kv_full;
       bool ok = true;
-      Cursor<kStages> sc, pc;  // scores run two tiles ahead of the second product
+      Cursor sc;  // tile of the next scores, two ahead of the second product's
       sc.start(p);
-      pc = sc;
-      auto wait_s = [&]() {  // operands of the score cursor's tile
-        if (sc.t == 0) ok = ok && mbar_wait(&bars->q_full[i][sc.n & 1], (sc.n >> 1) & 1, p.err);
-        ok = ok && mbar_wait(&bars->k_full[sc.stage], sc.lap, p.err);
+      // What the second product of a tile has to know: products' key extents are
+      // multiples of 16.
+      struct Tile {
+        int steps, n;
+        bool there, first, last;
       };
-      auto issue_s = [&]() {
-        const uint64_t qa = q_desc + (sc.n & 1) * (C::kQBytes / 16), ka = k_desc + sc.stage * (C::kKVBytes / 16);
-        // keys in multiples of 16: N >> 3 at bit 17 of the descriptor
-        const uint32_t idesc = C::kIdescQK | static_cast<uint32_t>(sc.steps() * 2) << 17;
+      auto tile = [&]() { return Tile{(sc.keys() + 15) >> 4, sc.n, sc.more, sc.t == 0, sc.last()}; };
+      int k_stage = 0;
+      Ring<2 * kQPlaces> q_ring;  // of query tiles i, i + 2, ...
+      if (i == 1) q_ring.next();
+      auto issue_s = [&](int steps, int buffer, bool last) {
+        const int place = q_ring.stage >= kQPlaces ? q_ring.stage - kQPlaces : q_ring.stage;
+        const uint64_t qa = q_desc + place * (C::kQBytes / 16), ka = k_desc + k_stage * (C::kKVBytes / 16);
+        // keys: N >> 3 at bit 17 of the descriptor
+        const uint32_t idesc = C::kIdescQK | static_cast<uint32_t>(steps * 2) << 17;
 #pragma unroll
         for (int k = 0; k < kD / 16; ++k)
-          mma_ss<Kind::kF16>(tmem + s_col(i, sc.g & 1), qa + ((k >> 2) * C::kQSub + (k & 3) * 32) / 16,
+          mma_ss<Kind::kF16>(tmem + s_col(i, buffer), qa + ((k >> 2) * C::kQSub + (k & 3) * 32) / 16,
                              ka + ((k >> 2) * C::kKVSub + (k & 3) * 32) / 16, idesc, k > 0);
-        tc_commit(&bars->s_full[i][sc.g & 1]);
-        tc_commit(&bars->k_empty[sc.stage]);
+        tc_commit(&bars->s_full[i][buffer]);
+        if (last) {
+          tc_commit(&bars->q_empty[q_ring.stage]);
+          q_ring.next();
+          q_ring.next();
+        }
+        k_stage = k_stage + 1 == kStages ? 0 : k_stage + 1;
       };
-      for (int k = 0; k < 2 && sc.more && ok; ++k) {
-        wait_s();
-        if (!ok) break;
-        tc_fence_after();
-        issue_s();
-        sc.next(p);
+      Tile now{0, 0, false, false, false}, after = now;
+      for (int e = 0; e < 2; ++e) {
+        const Tile t = tile();
+        if (t.there && ok) {
+          if (t.first) ok = mbar_wait(&bars->q_full[q_ring.stage], q_ring.lap, p.err);
+          ok = ok && mbar_wait(&bars->first_full[e], 0, p.err);
+          if (ok) {
+            tc_fence_after();
+            issue_s(t.steps, e, t.last);
+            tc_commit(&bars->first_empty[e]);
+            sc.next(p);
+          }
+        }
+        (e == 0 ? now : after) = t;
       }
-      while (pc.more && ok) {
-        // A unit's first scores wait for its queries, whose buffer the softmax
-        // may free only behind this tile's product: late. All others: early.
-        const bool scores = sc.more, late = sc.t == 0;
-        if (scores && !late) wait_s();
-        const uint64_t va = v_desc + pc.stage * (C::kKVBytes / 16);
-        const uint32_t s_tmem = tmem + s_col(i, pc.g & 1);
-        const int steps = pc.steps();
-        const bool first = pc.t == 0, last = pc.t == pc.u.n_kv - 1;
-        ok = ok && mbar_wait(&v_bar[pc.stage], pc.lap, p.err);
-        if (ok && first && pc.n > 0) ok = mbar_wait(&bars->o_empty[i], (pc.n - 1) & 1, p.err);
-        ok = ok && mbar_wait(&bars->p_full[i][pc.g & 1], (pc.g >> 1) & 1, p.err);
+      Ring<kStages> ring;
+      for (int buffer = 0, lap = 0; now.there && ok; buffer ^= 1, lap ^= buffer ^ 1) {
+        const Tile next = tile();
+        const uint64_t va = v_desc + ring.stage * (C::kKVBytes / 16);
+        const uint32_t s_tmem = tmem + s_col(i, buffer);
+        ok = mbar_wait(&kv_bar[ring.stage], ring.lap, p.err);
+        if (ok && now.first && now.n > 0) ok = mbar_wait(&bars->o_empty[i], (now.n - 1) & 1, p.err);
+        ok = ok && mbar_wait(&bars->p_full[i][buffer], lap, p.err);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < kBN / 16; ++k)
-          if (k < steps) mma_ts<Kind::kF16>(tmem + o_col(i), s_tmem + k * 8, va + k * 16 * 128 / 16, C::kIdescPV, !first || k > 0);
-        tc_commit(&bars->v_empty[pc.stage]);
-        if (last) tc_commit(&bars->o_full[i]);
-        if (scores && late) {
-          wait_s();
-          if (!ok) break;
-          tc_fence_after();
+          if (k < now.steps)
+            mma_ts<Kind::kF16>(tmem + o_col(i), s_tmem + k * 8, va + k * 16 * 128 / 16, C::kIdescPV, !now.first || k > 0);
+        if (now.last) tc_commit(&bars->o_full[i]);
+        if (next.there) {
+          // a unit's queries may wait for what this product sets free
+          if (next.first) {
+            ok = mbar_wait(&bars->q_full[q_ring.stage], q_ring.lap, p.err);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          issue_s(next.steps, buffer, next.last);
+        } else {
+          tc_commit(&bars->s_full[i][buffer]);  // the two phases behind the last scores still end
         }
-        // behind the last scores the two phases that would follow still end
-        if (scores) issue_s();
-        else tc_commit(&bars->s_full[i][pc.g & 1]);
-        if (scores) sc.next(p);
-        pc.next(p);
+        tc_commit(&bars->kv_empty[ring.stage]);
+        if (next.there) sc.next(p);
+        ring.next();
+        now = after;
+        after = next;
       }
       tc_commit(&bars->end[i]);
       mbar_wait(&bars->end[i], 0, p.err, 100000000ull);
@@ -377,10 +428,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kFixWarp) {
     // ------------------------------------------------------------ value rows behind the last key
     if (p.lens) {
-      Cursor<kStages> c;
-      for (c.start(p); c.more; c.next(p)) {
-        const int s = c.stage;
-        if (!__all_sync(0xffffffffu, mbar_wait(&bars->v_full[s], c.lap, p.err))) break;
+      Cursor c;
+      Ring<kStages> ring;
+      for (c.start(p); c.more; c.next(p), ring.next()) {
+        const int s = ring.stage;
+        if (!__all_sync(0xffffffffu, mbar_wait(&bars->kv_full[s], ring.lap, p.err))) break;
         const int valid = c.keys(), read = (valid + 15) / 16 * 16;
         if (valid < read) {
           // rows of 128 bytes; the swizzle moves 16-byte pieces within a row
@@ -404,14 +456,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float comb = p.scale_log2;
     bool ok = true;
     int g = 0, n = 0;
-    int leaving = -1;  // buffer whose output this warp's last store still reads
-    auto release_q = [&]() {
-      if (leaving >= 0 && lane == 0) {
-        bulk_wait_read<0>();
-        mbar_arrive(&bars->q_empty[i][leaving]);
-      }
-      leaving = -1;
-    };
     // A unit's epilogue runs behind the first tile of the next one, whose scores
     // are there before this one's last product has ended.
     struct Pending {
@@ -422,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     done.n = -1;
     auto epilogue = [&]() {
       const Unit& v = done.u;
-      const int buf = done.n & 1, row = v.m0 + r;
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[i], buf, p.err));
+      const int row = v.m0 + r;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->o_full[i], done.n & 1, p.err));
       done.n = -1;
       if (!ok) return;
       tc_fence_after();
@@ -444,16 +488,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (row < p.seq_q) p.part_ml[part] = make_float2(done.m, done.l);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars->o_empty[i]);
-          mbar_arrive(&bars->q_empty[i][buf]);
-        }
+        if (lane == 0) mbar_arrive(&bars->o_empty[i]);
         return;
       }
-      // The rows take the place of their queries (every product with those has
-      // ended) and leave by TMA, which does not write rows behind the last query.
+      // 64 channels at a time through shared memory, so that rows leave as whole
+      // lines by TMA, which does not write rows behind the last query.
       const float inv_l = done.l != 0.f ? 1.0f / done.l : 0.f;
-      uint8_t* stage = smem + (2 * i + buf) * C::kQBytes + lane_base * 128 + lane * 128;
+      uint8_t* stage = smem + C::kOutOff + warp * kOutBytes;
       uint32_t o[C::kSubs][2][32];
 #pragma unroll
       for (int c = 0; c < C::kSubs; ++c) tmem_ld64(o_addr + c * 64, o[c]);
@@ -462,23 +503,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->o_empty[i]);
 #pragma unroll
-      for (int c = 0; c < C::kSubs; ++c)
+      for (int c = 0; c < C::kSubs; ++c) {
+        uint4 w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const uint32_t* y = &o[c][e >> 2][(e & 3) * 8];
-          uint32_t w[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] = pack2<T>(__uint_as_float(y[2 * k]) * inv_l, __uint_as_float(y[2 * k + 1]) * inv_l);
-          *reinterpret_cast<uint4*>(stage + c * C::kQSub + ((e ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          auto two = [&](int k) { return pack2<T>(__uint_as_float(y[2 * k]) * inv_l, __uint_as_float(y[2 * k + 1]) * inv_l); };
+          w[e] = make_uint4(two(0), two(1), two(2), two(3));
         }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        for (int c = 0; c < C::kSubs; ++c)
-          tma_store_4d(&o_map, stage + c * C::kQSub, c * 64, v.m0 + i * kBM + lane_base, v.h, v.b);
-        bulk_commit();
+        if (lane == 0) bulk_wait_read<0>();  // the store before this one has left the buffer
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) = w[e];
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_4d(&o_map, stage, c * 64, v.m0 + i * kBM + lane_base, v.h, v.b);
+          bulk_commit();
+        }
       }
-      leaving = buf;
     };
     for (uint32_t id = blockIdx.x; id < p.units && ok; id += gridDim.x) {
       const Unit u = unit_at(p, id);
@@ -593,10 +636,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bars->p_full[i][g & 1]);
         if (t == 0 && done.n >= 0) epilogue();
         if (!ok) break;
-        if (t == 1) release_q();
       }
       if (!ok) break;
-      release_q();  // the unit after next loads its queries there
       done.u = u;
       done.m = m_used;
       done.l = sum[0] + sum[1];
