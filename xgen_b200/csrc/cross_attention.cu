@@ -70,14 +70,7 @@ constexpr int kTmaWarp = 8;
 constexpr int kMmaWarp = 9;
 constexpr int kFixWarp = 11;
 constexpr float kNegInf = -__builtin_huge_valf();
-#ifndef XGB_CROSS_POLY
-#define XGB_CROSS_POLY 0
-#endif
-constexpr int kPoly = XGB_CROSS_POLY;
-template <int kShare>
-__device__ __forceinline__ constexpr bool poly_pair(int pair) {
-  return kShare > 0 && pair % (kShare > 0 ? kShare : 1) == kShare - 1;
-}
+constexpr int kTurnBar = 1;  // named barriers 1, 2: the exponentials' turn of query tile 0, 1
 
 constexpr int kQPlaces = 3;
 constexpr int kOutBytes = 32 * 128;  // 32 rows x 64 channels
@@ -456,6 +449,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float comb = p.scale_log2;
     bool ok = true;
     int g = 0, n = 0;
+    // The two query tiles take turns with the exponentials. Without, both run
+    // in step: 64 exponentials a row take 1,150 cycles for the two of them at
+    // once, the SFU's rate, and what comes before and after, 700 cycles, leaves
+    // it idle. A turn passes by named barriers: one wait and one arrival for
+    // each tile, tile 1 hands tile 0 the first turn and tile 0 takes the last.
+    const int own_turn = kTurnBar + i, other_turn = kTurnBar + (i ^ 1);
+    int turns = 0;
+    if (i == 1) named_arrive(other_turn, 2 * kBM);
     // A unit's epilogue runs behind the first tile of the next one, whose scores
     // are there before this one's last product has ended.
     struct Pending {
@@ -583,12 +584,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 32; e += 2) {
               float a, b;
               ffma2(a, b, __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]), comb, comb, off, off);
-              if (poly_pair<kPoly>(c * 16 + e / 2)) {
-                ex2_poly2<3>(a, b, a, b);
-              } else {
-                a = ex2_approx(a);
-                b = ex2_approx(b);
-              }
+              a = ex2_approx(a);
+              b = ex2_approx(b);
               const int ch = (e / 2) & 3;
               if (c == 0 && e < 8) {
                 ra[ch] = a;
@@ -606,7 +603,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         if (t == 0) m_used = tile_max();
         float ts[2];
+        named_sync(own_turn, 2 * kBM);
         probabilities(ts);
+        named_arrive(other_turn, 2 * kBM);
+        ++turns;
         if (t > 0 && __any_sync(0xffffffffu, !(ts[0] + ts[1] <= C::kLimit) || m_used == kNegInf)) {
           // Too large, not a number, or no finite score so far: take the
           // maximum after all, with O (complete up to the tile before) rescaled.
@@ -643,6 +643,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       done.l = sum[0] + sum[1];
       done.n = n++;
     }
+    if (!ok) {
+      // After a failed wait the other tile still gets its turns.
+      int all = 0;
+      for (uint32_t id = blockIdx.x; id < p.units; id += gridDim.x) all += unit_at(p, id).n_kv;
+      for (; turns < all; ++turns) {
+        named_sync(own_turn, 2 * kBM);
+        named_arrive(other_turn, 2 * kBM);
+      }
+    }
+    if (i == 0) named_sync(own_turn, 2 * kBM);
     if (ok && done.n >= 0) epilogue();
     if (lane == 0) bulk_wait_all();
   }
