@@ -25,8 +25,10 @@
 // TMEM (512 columns): two S buffers of 64 fp32 columns for each query tile
 // (P overwrites its S), O0, O1. Shared memory at D = 128: three 32 KB places
 // for query tiles, so that the next unit's first one is there long before its
-// scores are due and its second one two key tiles before, three K and V tiles,
-// and 4 KB a softmax warp in which output rows wait for their TMA store.
+// scores are due and its second one two key tiles before, two K and V tiles (a
+// third gave nothing), and 8 KB a softmax warp in which its output rows wait
+// for their TMA store (with 4 KB, half of the channels after the other,
+// 124,992 x 77 takes 305 us instead of 282).
 //
 // What bounds a step of 64 keys for both query tiles is the tensor pipe and
 // the threads that feed it. Measured back to back on one SM: a 128 x 64 x 16
@@ -73,7 +75,7 @@ constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kTurnBar = 1;  // named barriers 1, 2: the exponentials' turn of query tile 0, 1
 
 constexpr int kQPlaces = 3;
-constexpr int kOutBytes = 32 * 128;  // 32 rows x 64 channels
+constexpr int kOutBytes = 32 * 128;  // 32 rows x 64 channels of a softmax warp
 
 template <typename T, int kD>
 struct Cfg {
@@ -82,11 +84,11 @@ struct Cfg {
   static constexpr int kQBytes = kSubs * kQSub;
   static constexpr int kKVSub = kBN * 128;
   static constexpr int kKVBytes = kSubs * kKVSub;
-  static constexpr int kStages = kD == 128 ? 3 : 6;
+  static constexpr int kStages = kD == 128 ? 2 : 4;
   static constexpr int kKOff = kQPlaces * kQBytes;
   static constexpr int kVOff = kKOff + kStages * kKVBytes;
   static constexpr int kOutOff = kVOff + kStages * kKVBytes;
-  static constexpr int kBarOff = kOutOff + 8 * kOutBytes;
+  static constexpr int kBarOff = kOutOff + 8 * kSubs * kOutBytes;
   static constexpr int kSmem = kBarOff + 512 + 1024;  // + barriers + alignment slack
   static constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   static constexpr uint32_t kIdescQK = instr_desc(1, kFmt, kFmt, false, false, kBM, 0);  // + keys
@@ -492,13 +494,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&bars->o_empty[i]);
         return;
       }
-      // 64 channels at a time through shared memory, so that rows leave as whole
-      // lines by TMA, which does not write rows behind the last query.
+      // Through shared memory, so that rows leave as whole lines by TMA, which
+      // does not write rows behind the last query.
       const float inv_l = done.l != 0.f ? 1.0f / done.l : 0.f;
-      uint8_t* stage = smem + C::kOutOff + warp * kOutBytes;
+      uint8_t* stage = smem + C::kOutOff + warp * C::kSubs * kOutBytes;
       uint32_t o[C::kSubs][2][32];
 #pragma unroll
       for (int c = 0; c < C::kSubs; ++c) tmem_ld64(o_addr + c * 64, o[c]);
+      if (lane == 0) bulk_wait_read<0>();  // the last unit's stores have left the buffer
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
@@ -512,14 +515,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           auto two = [&](int k) { return pack2<T>(__uint_as_float(y[2 * k]) * inv_l, __uint_as_float(y[2 * k + 1]) * inv_l); };
           w[e] = make_uint4(two(0), two(1), two(2), two(3));
         }
-        if (lane == 0) bulk_wait_read<0>();  // the store before this one has left the buffer
-        __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) = w[e];
+        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(stage + c * kOutBytes + lane * 128 + ((e ^ (lane & 7)) << 4)) = w[e];
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          tma_store_4d(&o_map, stage, c * 64, v.m0 + i * kBM + lane_base, v.h, v.b);
+          tma_store_4d(&o_map, stage + c * kOutBytes, c * 64, v.m0 + i * kBM + lane_base, v.h, v.b);
           bulk_commit();
         }
       }
