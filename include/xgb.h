@@ -351,7 +351,7 @@ int xgb_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t M, int6
  * (0 for most sizes), 16-byte aligned, its contents need no initialisation. */
 int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv,
                                       int64_t head_dim);
-int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int64_t seq_q);
+int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv);
 int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                         const void* v, const int64_t* v_strides, int dtype, int64_t batch, int64_t heads,
                         int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int* kv_lens,

@@ -107,7 +107,9 @@ def test_cross_attention_arguments():
     assert call(qst=i64([512, 64, 128, 2])) == -3 and call(qst=i64([512, 64, 132, 1])) == -3
     assert call(kst=i64([1024, 64, 0, 1])) == -3 and call(ost=i64([0, 64, 128, 1])) == -3 and call(qst=i64([512, 64, -128, 1])) == -3
     assert call(q=ODD) == -4
-    assert call(sq=33, mask=D) == -2 and h.xgb_cross_attention_takes_mask(2, 2, 32) and not h.xgb_cross_attention_takes_mask(4, 2, 17)
+    takes = h.xgb_cross_attention_takes_mask
+    assert call(sq=9, mask=D) == -2 and takes(2, 2, 8, 8) and not takes(2, 2, 9, 4096)
+    assert takes(4, 2, 12, 1024) and not takes(4, 2, 12, 1023) and not takes(4, 2, 13, 1024) and not takes(3, 2, 1, 8)
     need = h.xgb_cross_attention_workspace(1, 2, 2, 1, 4096, 64)  # few rows, many keys: split
     assert need > 0
     assert call(b=1, sq=1, skv=4096) == -7 and call(b=1, sq=1, skv=4096, ws=D, wsb=need - 1) == -7

@@ -69,7 +69,8 @@ def no_timeouts(cuda_device):
 
 @pytest.mark.parametrize("b,h,hk,sq,skv", [
     (1, 1, 1, 1, 1), (1, 2, 2, 128, 64), (1, 2, 1, 129, 65), (2, 3, 3, 300, 77), (1, 4, 2, 257, 512), (2, 2, 2, 1000, 333),
-    (1, 1, 1, 5, 1000), (3, 2, 1, 64, 63), (1, 24, 24, 700, 226), (1, 6, 2, 1, 4099), (1, 1, 1, 3000, 2), (5, 8, 8, 17, 129)])
+    (1, 1, 1, 5, 1000), (3, 2, 1, 64, 63), (1, 24, 24, 700, 226), (1, 6, 2, 1, 4099), (1, 1, 1, 3000, 2), (5, 8, 8, 17, 129),
+    (2, 6, 2, 8, 1030), (1, 2, 2, 8, 600), (1, 1, 1, 1, 9000), (1, 2, 2, 9, 2000), (40, 4, 1, 2, 300)])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_matches_softmax(cuda_device, b, h, hk, sq, skv, d, dtype):

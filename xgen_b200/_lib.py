@@ -99,7 +99,7 @@ SIGNATURES = {
     "xgb_int8_linear": (c_int, [c_vp, c_i64, c_vp, c_i64, c_i64, c_i64, c_vp, c_int, c_vp, c_int, c_vp, c_i64,
                                 c_vp, c_i64, c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, c_vp]),
     "xgb_cross_attention_workspace": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
-    "xgb_cross_attention_takes_mask": (c_int, [c_i64, c_i64, c_i64]),
+    "xgb_cross_attention_takes_mask": (c_int, [c_i64, c_i64, c_i64, c_i64]),
     "xgb_cross_attention": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_int, c_i64, c_i64, c_i64,
                                     c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i64, c_float, c_vp,
                                     c_i64p, c_vp, c_i64, c_vp, c_vp]),

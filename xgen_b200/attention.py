@@ -20,6 +20,7 @@ import torch.nn.functional as F
 
 from . import _lib, trace
 from ._lib import call, i64_array
+from .ops import _DTYPE_CODE, _call_on, _device_of, _refuse_autograd
 
 HEAD_DIM = 128
 _err_flags: dict[int, torch.Tensor] = {}
@@ -34,13 +35,15 @@ def _err_flag(device: torch.device) -> torch.Tensor:
     return flag
 
 
-def _err_ptr(device: torch.device):
-    """The error word's address; None when the first call on a device is being
-    captured (the word would then live in the graph's own memory)."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    if idx not in _err_flags and torch.cuda.is_current_stream_capturing():
-        return None
-    return _err_flag(device).data_ptr()
+def _err_ptr(index: int):
+    """The error word's address on GPU `index`; None when the first call there
+    is being captured (the word would then live in the graph's own memory)."""
+    flag = _err_flags.get(index)
+    if flag is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        flag = _err_flag(torch.device("cuda", index))
+    return flag.data_ptr()
 
 
 _split_workspaces: dict[int, torch.Tensor] = {}
@@ -234,8 +237,6 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     without keys gives zeros. out: a [B, H, Sq, D] view of the query's type,
     which must not overlap the inputs. Nothing is shared between calls: the
     workspace of a call comes from the caching allocator."""
-    from .ops import _DTYPE_CODE, _call_on, _device_of, _refuse_autograd
-
     what = "cross attention"
     index = _device_of(what, query, key, value, kv_lens, key_mask, out)
     _refuse_autograd(what, query, key, value)
@@ -274,7 +275,7 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     lib = _lib.lib()
     mask = (None, 0, 0)
     if key_mask is not None:
-        if lib.xgb_cross_attention_takes_mask(h, hk, sq):
+        if lib.xgb_cross_attention_takes_mask(h, hk, sq, skv):
             mask = (key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1))
         else:
             kv_lens = key.new_empty((b,), dtype=torch.int32)
@@ -291,7 +292,7 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     ws = query.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
     _call_on(index, "xgb_cross_attention", query.data_ptr(), _steps(query), key.data_ptr(), _steps(key), value.data_ptr(),
              _steps(value), code, b, h, hk, sq, skv, d, kv_lens.data_ptr() if kv_lens is not None else None, *mask, sm_scale,
-             out.data_ptr(), _steps(out), ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(query.device))
+             out.data_ptr(), _steps(out), ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(index))
     return out
 
 

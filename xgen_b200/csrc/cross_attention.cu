@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // 8, whose members each join some of the rows over distributed shared memory;
 // only few units with many keys need more parts than that, and join in the
 // second kernel.
-// Keys that are not there are not loaded: zeros, with scores of -inf.
+// Keys behind a sample's last one are not loaded: zeros, with scores of -inf.
 constexpr int kFewRows = 8;
 constexpr int kFewWarps = 4;
 constexpr int kFewKeys = 16;  // keys of a warp's step
@@ -751,41 +751,47 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
     load_row<kChunks>(f.q, b * f.qsb + h * f.qsh + s * f.qss + 8 * c, r < rows, q);
   }
   const int64_t kbase = b * f.ksb + hk * f.ksh + 8 * c, vbase = b * f.vsb + hk * f.vsh + 8 * c;
-  auto there = [&](int key) { return key < len && (!f.mask || __ldg(f.mask + b * f.msb + key * f.mss) != 0); };
+  auto unmasked = [&](int key) { return !f.mask || (key < len && __ldg(f.mask + b * f.msb + key * f.mss) != 0); };
 
   float o[2 * kChunks][4] = {};
   float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};  // rows 2c, 2c + 1
-  uint4 k0[kChunks], k1[kChunks], v0[kChunks], v1[kChunks];
+  // Keys and values of this step and the next: both are requested a step ahead,
+  // so that a step costs its arithmetic, not a memory access. (With V requested
+  // in its own step 4 tokens against 4,099 keys took 12.3 us.)
+  uint4 k0[kChunks], k1[kChunks], v0[kChunks], v1[kChunks], vn0[kChunks], vn1[kChunks];
+  bool keep0 = false, keep1 = false, next0 = false, next1 = false;
+  auto request = [&](int at) {
+    const int64_t key = static_cast<int64_t>(at) * kFewKeys + g;
+    const bool in0 = at < step1 && key < len, in1 = at < step1 && key + 8 < len;
+    load_row<kChunks>(f.k, kbase + key * f.kss, in0, k0);
+    load_row<kChunks>(f.k, kbase + (key + 8) * f.kss, in1, k1);
+    load_row<kChunks>(f.v, vbase + key * f.vss, in0, vn0);
+    load_row<kChunks>(f.v, vbase + (key + 8) * f.vss, in1, vn1);
+    next0 = in0 && unmasked(static_cast<int>(key));
+    next1 = in1 && unmasked(static_cast<int>(key) + 8);
+  };
   int step = step0 + warp;
-  bool go0 = false, go1 = false;
-  if (step < step1) {
-    go0 = there(step * kFewKeys + g);
-    go1 = there(step * kFewKeys + g + 8);
-    load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(step) * kFewKeys + g) * f.kss, go0, k0);
-    load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(step) * kFewKeys + g + 8) * f.kss, go1, k1);
-  }
+  if (step < step1) request(step);
   for (; step < step1; step += kFewWarps) {
-    const int64_t key = static_cast<int64_t>(step) * kFewKeys + g;
-    load_row<kChunks>(f.v, vbase + key * f.vss, go0, v0);
-    load_row<kChunks>(f.v, vbase + (key + 8) * f.vss, go1, v1);
+    keep0 = next0;
+    keep1 = next1;
+    const uint4 none = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {  // what a mask leaves out may hold anything
+      v0[j] = keep0 ? vn0[j] : none;
+      v1[j] = keep1 ? vn1[j] : none;
+    }
     float st[4] = {0.f, 0.f, 0.f, 0.f};  // keys g (0, 1) and g + 8 (2, 3), rows 2c, 2c + 1
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
       mma16816<T>(st, k0[j].x, k1[j].x, k0[j].y, k1[j].y, q[j].x, q[j].y);
       mma16816<T>(st, k0[j].z, k1[j].z, k0[j].w, k1[j].w, q[j].z, q[j].w);
     }
-    const bool was0 = go0, was1 = go1;
-    const int next = step + kFewWarps;
-    if (next < step1) {
-      go0 = there(next * kFewKeys + g);
-      go1 = there(next * kFewKeys + g + 8);
-      load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(next) * kFewKeys + g) * f.kss, go0, k0);
-      load_row<kChunks>(f.k, kbase + (static_cast<int64_t>(next) * kFewKeys + g + 8) * f.kss, go1, k1);
-    }
+    request(step + kFewWarps);
     float pr[4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float a = was0 ? st[e] * p.scale_log2 : kNegInf, d = was1 ? st[e + 2] * p.scale_log2 : kNegInf;
+      const float a = keep0 ? st[e] * p.scale_log2 : kNegInf, d = keep1 ? st[e + 2] * p.scale_log2 : kNegInf;
       float top = fmaxf(a, d);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
@@ -881,16 +887,17 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
 }
 
 // Joins the parts of a row: M = max m, o = sum 2^(m - M) O / sum 2^(m - M) l.
-// One warp a row; a part without keys (l = 0) left no O.
-template <typename T, int kD>
-__global__ void __launch_bounds__(256) join_kernel(const Params p, int64_t rows, int few_tiles) {
-  const int lane = threadIdx.x & 31;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);  // (batch, head, row)
-  if (at >= rows) return;
-  const int64_t bh = at / p.seq_q;
-  const int row = static_cast<int>(at - bh * p.seq_q);
-  const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh - static_cast<int64_t>(b) * p.heads);
-  int64_t item = bh * p.n_qt + row / kRows;
+// A block a row; its warps share the parts, of which there may be hundreds. A
+// part without keys (l = 0) left no O.
+constexpr int kMostParts = 512;
+template <typename T, int kD, int kJoinWarps>
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p, int few_tiles) {
+  __shared__ float so[kJoinWarps][kD], sl[kJoinWarps], sm[kJoinWarps], weight[kMostParts];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t bh = blockIdx.x / static_cast<uint32_t>(p.seq_q);  // (batch, head)
+  const int row = static_cast<int>(blockIdx.x - bh * p.seq_q);
+  const int b = static_cast<int>(bh / p.heads), h = static_cast<int>(bh) - b * p.heads;
+  int64_t item = static_cast<int64_t>(bh) * p.n_qt + row / kRows;
   int r = row % kRows;
   if (few_tiles) {  // rows of a key head in tiles of 8
     const int in_head = h % p.group * p.seq_q + row;
@@ -898,39 +905,59 @@ __global__ void __launch_bounds__(256) join_kernel(const Params p, int64_t rows,
     r = in_head % kFewRows;
   }
   const int64_t first = item * p.splits * p.part_rows + r;
-  // m and l of 32 parts at a time, a lane each; then the O of the parts with
-  // keys, whose loads do not wait for one another
+  auto at = [&](int q) { return first + static_cast<int64_t>(q) * p.part_rows; };
   float mx = kNegInf;
-  for (int q = lane; q < p.splits; q += 32) mx = fmaxf(mx, __ldg(&p.part_ml[first + static_cast<int64_t>(q) * p.part_rows]).x);
+  for (int q = threadIdx.x; q < p.splits; q += kJoinWarps * 32) mx = fmaxf(mx, __ldg(&p.part_ml[at(q)]).x);
   mx = warp_max(mx);
-  const float base = mx == kNegInf ? 0.f : mx;
-  float l = 0.f, o[kD / 32] = {};
-  for (int q0 = 0; q0 < p.splits; q0 += 32) {
-    float w = 0.f, lq = 0.f;
-    if (q0 + lane < p.splits) {
-      const float2 ml = __ldg(&p.part_ml[first + static_cast<int64_t>(q0 + lane) * p.part_rows]);
-      lq = ml.y;
-      w = ex2_approx(ml.x - base);
-      l = fmaf(w, lq, l);
-    }
-    const int n = min(32, p.splits - q0);
-#pragma unroll 4
-    for (int q = 0; q < n; ++q) {
-      const float wq = __shfl_sync(0xffffffffu, w, q), has = __shfl_sync(0xffffffffu, lq, q);
-      if (has == 0.f) continue;
-      const float* po = p.part_o + (first + static_cast<int64_t>(q0 + q) * p.part_rows) * kD + lane;
+  if (lane == 0) sm[warp] = mx;
+  __syncthreads();
 #pragma unroll
-      for (int c = 0; c < kD / 32; ++c) o[c] = fmaf(wq, __ldg(po + c * 32), o[c]);
-    }
+  for (int w = 0; w < kJoinWarps; ++w) mx = fmaxf(mx, sm[w]);
+  const float base = mx == kNegInf ? 0.f : mx;
+  float l = 0.f;
+  for (int q = threadIdx.x; q < p.splits; q += kJoinWarps * 32) {
+    const float2 ml = __ldg(&p.part_ml[at(q)]);
+    const float w = ml.y != 0.f ? ex2_approx(ml.x - base) : 0.f;
+    weight[q] = ml.y != 0.f ? w : -1.f;  // no O to read
+    l = fmaf(w, ml.y, l);
   }
   l = warp_sum(l);
+  __syncthreads();
+  // predicated loads, so that eight parts are on their way at once
+  float o[kD / 32] = {};
+#pragma unroll 8
+  for (int q = warp; q < p.splits; q += kJoinWarps) {
+    const float w = weight[q];
+    const float* po = p.part_o + at(q) * kD + lane;
+#pragma unroll
+    for (int c = 0; c < kD / 32; ++c) o[c] = fmaf(w, w != -1.f ? __ldg(po + c * 32) : 0.f, o[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < kD / 32; ++c) so[warp][c * 32 + lane] = o[c];
+  if (lane == 0) sl[warp] = l;
+  __syncthreads();
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) l += sl[w];
   const float inv_l = l != 0.f ? 1.0f / l : 0.f;
   T* dst = static_cast<T*>(p.out) + b * p.osb + h * p.osh + row * p.oss;
+  for (int d = threadIdx.x; d < kD; d += kJoinWarps * 32) {
+    float v = 0.f;
 #pragma unroll
-  for (int c = 0; c < kD / 32; ++c) {
-    if constexpr (std::is_same<T, __half>::value) dst[c * 32 + lane] = __float2half_rn(o[c] * inv_l);
-    else dst[c * 32 + lane] = __float2bfloat16_rn(o[c] * inv_l);
+    for (int w = 0; w < kJoinWarps; ++w) v += so[w][d];
+    if constexpr (std::is_same<T, __half>::value) dst[d] = __float2half_rn(v * inv_l);
+    else dst[d] = __float2bfloat16_rn(v * inv_l);
   }
+}
+
+// 4 warps a row, 16 where there are more parts than those take at once (444
+// parts: 29 us with 4).
+template <typename T, int kD>
+int join(const Params& p, int64_t rows, int few_tiles, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>(rows);
+  if (p.splits > 64) join_kernel<T, kD, 16><<<grid, 512, 0, st>>>(p, few_tiles);
+  else join_kernel<T, kD, 4><<<grid, 128, 0, st>>>(p, few_tiles);
+  return launch_status();
 }
 
 int sm_count() {
@@ -940,9 +967,17 @@ int sm_count() {
   return n > 0 ? n : 148;
 }
 
-// How a call is laid out: the few-row form for up to kFewMost query rows of a
-// key head, and the parts of a unit's keys.
-constexpr int64_t kFewMost = 32;
+// How a call is laid out. The few-row form takes up to 8 query rows of a key
+// head; up to 24 where several query heads share long keys, which the tiled
+// kernel would read once for each of them. Measured, few / tiled, D = 128:
+//   24 heads, rows 8, 512 keys: 6 / 10 us       rows 16: 13.8 / 10.4 us
+//   rows 16, 4,096 keys, own keys: 28 / 19 us
+//   rows 12 of 3 shared heads, batch 4: 512 keys 16 / 12 us, 4,096 keys 37 / 57 us
+//   rows 30 of 3 shared heads, batch 4, 4,096 keys: 61 / 56 us
+inline bool takes_few(int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv) {
+  const int64_t rows = heads / kv_heads * seq_q;
+  return rows <= kFewRows || (heads > kv_heads && rows <= 3 * kFewRows && seq_kv >= 1024);
+}
 struct Plan {
   bool few;
   int tiles;  // few: row tiles of a key head
@@ -954,7 +989,7 @@ struct Plan {
 inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int sms) {
   Plan n{};
   const int64_t rows = heads / kv_heads * seq_q;
-  n.few = rows <= kFewMost;
+  n.few = takes_few(heads, kv_heads, seq_q, seq_kv);
   if (n.few) {
     n.tiles = static_cast<int>(cdiv(rows, kFewRows));
     n.items = batch * kv_heads * n.tiles;
@@ -962,7 +997,7 @@ inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, 
     // warps. A cluster of up to 8 parts needs no second kernel; it is taken as
     // soon as it gives every SM a CTA.
     const int64_t most = cdiv(seq_kv, kFewKeys * kFewWarps);
-    n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(3 * sms / n.items, most)));
+    n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({3 * sms / n.items, most, kMostParts})));
     n.clustered = n.splits > 1 && (n.splits <= 8 || n.items * 8 >= sms);
     if (n.clustered) n.splits = std::min(n.splits, 8);
     n.part_rows = kFewRows;
@@ -971,7 +1006,7 @@ inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, 
   n.items = batch * heads * cdiv(seq_q, kRows);
   n.splits = 1;
   // parts only where whole units would leave more than half of the SMs idle
-  if (n.items * 2 <= sms) n.splits = static_cast<int>(std::min<int64_t>(sms / n.items, cdiv(seq_kv, kBN)));
+  if (n.items * 2 <= sms) n.splits = static_cast<int>(std::min<int64_t>({sms / n.items, cdiv(seq_kv, kBN), kMostParts}));
   n.part_rows = std::min<int64_t>(seq_q, kRows);
   return n;
 }
@@ -986,9 +1021,7 @@ int launch(const CUtensorMap (&map)[4], const Params& p, int64_t batch, int sms,
   kernel<<<grid, kThreads, C::kSmem, st>>>(map[0], map[1], map[2], map[3], p);
   const int rc = launch_status();
   if (rc || p.splits == 1) return rc;
-  const int64_t rows = batch * p.heads * p.seq_q;
-  join_kernel<T, kD><<<static_cast<unsigned>(cdiv(rows, 8)), 256, 0, st>>>(p, rows, 0);
-  return launch_status();
+  return join<T, kD>(p, batch * p.heads * p.seq_q, 0, st);
 }
 
 template <typename T, int kD>
@@ -1011,9 +1044,7 @@ int launch_few(const Params& p, const FewParams& f, int64_t items, int64_t batch
   }
   const int rc = launch_status();
   if (rc || p.splits == 1 || f.clustered) return rc;
-  const int64_t rows = batch * p.heads * p.seq_q;
-  join_kernel<T, kD><<<static_cast<unsigned>(cdiv(rows, 8)), 256, 0, st>>>(p, rows, f.tiles);
-  return launch_status();
+  return join<T, kD>(p, batch * p.heads * p.seq_q, f.tiles, st);
 }
 
 // ---------------------------------------------------------------- masked keys
@@ -1110,8 +1141,9 @@ XGB_API int64_t xgb_cross_attention_workspace(int64_t batch, int64_t heads, int6
   return n.items * n.splits * n.part_rows * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-XGB_API int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int64_t seq_q) {
-  return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads / kv_heads * seq_q <= cross::kFewMost;
+XGB_API int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv) {
+  return heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && seq_q > 0 && seq_kv > 0 &&
+         cross::takes_few(heads, kv_heads, seq_q, seq_kv);
 }
 
 XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -1136,7 +1168,7 @@ XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const v
     }
   }
   if (!cross::aligned16(q) || !cross::aligned16(k) || !cross::aligned16(v) || !cross::aligned16(out)) return XGB_ERR_ALIGN;
-  if (mask && !xgb_cross_attention_takes_mask(heads, kv_heads, seq_q)) return XGB_ERR_SHAPE;
+  if (mask && !xgb_cross_attention_takes_mask(heads, kv_heads, seq_q, seq_kv)) return XGB_ERR_SHAPE;
   const int sms = cross::sm_count();
   const cross::Plan n = cross::plan(batch, heads, kv_heads, seq_q, seq_kv, sms);
   const int64_t need = xgb_cross_attention_workspace(batch, heads, kv_heads, seq_q, seq_kv, head_dim);

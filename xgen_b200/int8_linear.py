@@ -101,7 +101,7 @@ def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: tor
     if m:
         flat, scales = codes.reshape(m, k).contiguous(), scales.reshape(m).contiguous()
         _call_on(index, "xgb_int8_gemm", flat.data_ptr(), weight.data_ptr(), m, n, k, scales.data_ptr(), weight_scale.data_ptr(),
-                 *_pointers(epilogue), _err_ptr(codes.device))
+                 *_pointers(epilogue), _err_ptr(index))
     return out
 
 
@@ -136,7 +136,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         ws_bytes = lib().xgb_int8_linear_workspace(ptr, ldx, m, k)
         ws = x.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
         _call_on(index, "xgb_int8_linear", ptr, ldx, weight.data_ptr(), m, n, k, weight_scale.data_ptr(), *_pointers(epilogue),
-                 ws.data_ptr() if ws_bytes else None, ws_bytes, _err_ptr(x.device))
+                 ws.data_ptr() if ws_bytes else None, ws_bytes, _err_ptr(index))
     return out
 
 
