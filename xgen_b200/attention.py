@@ -218,9 +218,7 @@ _I64x4 = _lib.c_i64 * 4
 
 
 def _steps(t: torch.Tensor):
-    """Element strides with 0 for dimensions of one entry (never stepped over)."""
-    n, st = t.shape, t.stride()
-    return _I64x4(st[0] if n[0] > 1 else 0, st[1] if n[1] > 1 else 0, st[2] if n[2] > 1 else 0, 1)
+    return _I64x4(*t.stride())
 
 
 def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, kv_lens=None, key_mask=None,
@@ -241,14 +239,15 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     index = _device_of(what, query, key, value, kv_lens, key_mask, out)
     _refuse_autograd(what, query, key, value)
     code = _DTYPE_CODE.get(query.dtype)
-    if (code is None or query.ndim != 4 or key.ndim != 4 or value.ndim != 4 or key.dtype != query.dtype
+    qn, kn = query.shape, key.shape
+    if (code is None or len(qn) != 4 or len(kn) != 4 or value.ndim != 4 or key.dtype != query.dtype
             or value.dtype != query.dtype or query.stride(3) != 1 or key.stride(3) != 1 or value.stride(3) != 1):
         raise ValueError(f"{what} requires bf16/fp16 [B, H, S, D] views of one type with unit channel stride")
-    b, h, sq, d = query.shape
-    hk, skv = key.shape[1], key.shape[2]
+    b, h, sq, d = qn
+    kb, hk, skv, kd = kn
     if d not in CROSS_HEAD_DIMS:
         raise ValueError(f"{what} requires head dim 64 or 128")
-    if key.shape != value.shape or key.shape[0] != b or key.shape[3] != d or hk == 0 or h % hk:
+    if kn != value.shape or kb != b or kd != d or hk == 0 or h % hk:
         raise ValueError(f"{what}: key and value must match, have the query's batch and head dim and divide its heads")
     sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
     if not 0.0 < sm_scale < math.inf:
@@ -265,8 +264,8 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
             raise ValueError(f"{what}: key_mask must be bool [B, Skv], [1, Skv] or [B, 1, 1, Skv]")
         key_mask = key_mask.expand(b, skv)
     if out is None:
-        out = query.new_empty((b, h, sq, d))
-    elif out.shape != query.shape or out.dtype != query.dtype or out.stride(-1) != 1:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    elif out.shape != qn or out.dtype != query.dtype or out.stride(-1) != 1:
         raise ValueError(f"{what} output must be a [B, H, Sq, D] view of the query's type with unit channel stride")
     if not b * h * sq:
         return out

@@ -1114,8 +1114,9 @@ XGB_API int xgb_pack_keys(const uint8_t* mask, int64_t mask_batch_stride, int64_
   if (batch <= 0 || batch > 65535 || heads <= 0 || heads > 65535 || seq <= 0 || seq > (1 << 30) ||
       (head_dim != 64 && head_dim != 128))
     return XGB_ERR_SHAPE;
+  const int64_t extent[3] = {batch, heads, seq};
   for (int d = 0; d < 3; ++d)
-    if (k_strides[d] % 8 || v_strides[d] % 8) return XGB_ERR_STRIDE;
+    if (extent[d] > 1 && (k_strides[d] % 8 || v_strides[d] % 8)) return XGB_ERR_STRIDE;
   if (k_strides[3] != 1 || v_strides[3] != 1) return XGB_ERR_STRIDE;
   if (!cross::aligned16(k) || !cross::aligned16(v) || !cross::aligned16(k_out) || !cross::aligned16(v_out))
     return XGB_ERR_ALIGN;

@@ -11,6 +11,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.nn import RMSNorm as _RMSNorm
 
 from . import _lib
 from ._lib import call, f64_array, i64_array
@@ -18,7 +19,8 @@ from ._lib import call, f64_array, i64_array
 _DTYPE_CODE = {torch.bfloat16: _lib.XGB_BF16, torch.float16: _lib.XGB_F16}
 _DTYPE_CODE_F32 = {**_DTYPE_CODE, torch.float32: _lib.XGB_F32}
 _raw_stream = torch._C._cuda_getCurrentRawStream  # the current stream's handle, without a Stream object
-_I64x2, _I64x3 = _lib.c_i64 * 2, _lib.c_i64 * 3
+_current_device = torch._C._cuda_getDevice
+_I64x3, _I64x4 = _lib.c_i64 * 3, _lib.c_i64 * 4
 
 
 def _stream(t: torch.Tensor) -> int:
@@ -49,19 +51,22 @@ def _refuse_autograd(what: str, *tensors) -> None:
                 raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
 
 
-def _like(t: torch.Tensor, shape) -> torch.Tensor:
-    """An empty contiguous tensor of t's type and device."""
-    return torch.empty_like(t) if t.shape == shape and t.is_contiguous() else t.new_empty(shape)
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An empty contiguous tensor of t's shape, type and device."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _call_on(index: int, name: str, *args) -> None:
     """call(name, *args, stream) with device `index` current (launches go to
     the current device, whatever their stream) and on its current stream."""
-    if index == torch.cuda.current_device():
-        call(name, *args, _raw_stream(index))
+    fn = getattr(_lib.lib(), name)
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            call(name, *args, _raw_stream(index))
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _lib.check(name, status)
 
 
 def try_h3_partial_rope(query: torch.Tensor, key: torch.Tensor, cos: torch.Tensor,
@@ -302,6 +307,9 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     qs = query.stride()
     if qs[3] != 1 and d > 1:
         raise ValueError(f"{what} need views with unit channel stride")
+    for w in (w_q, w_k):
+        if w is not None and (w.shape != (d,) or w.dtype != query.dtype or not w.is_contiguous()):
+            raise ValueError(f"{what}: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
     axes, channels, thetas, rotary = _axes_of(axes if type(axes) is tuple else tuple(axes),
                                               tuple(theta) if type(theta) is list else theta)
     if rotary > d:
@@ -312,22 +320,22 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
         raise ValueError(f"{what}: positions must be integers or 32/64-bit floats of shape [S, A] or [B, S, A]")
     if axes > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
-    q_out = _like(query, (b, s, h, d))
+    q_out = _like(query)
     k_out = k_ptr = k_out_ptr = k_strides = None
     kh = 0
     if key is not None:
         if key.ndim != 4 or key.dtype != query.dtype or (key.stride(-1) != 1 and d > 1):
             raise ValueError(f"{what} need [B, S, H, D] views of one type with unit channel stride")
-        kh = key.shape[2]
-        if key.shape != (b, s, kh, d):
+        kb, ks, kh, kd = key.shape
+        if kb != b or ks != s or kd != d:
             raise ValueError(f"{what}: query and key differ in batch, sequence or head dim")
-        k_out = _like(key, (b, s, kh, d))
-        k_ptr, k_out_ptr, k_strides = key.data_ptr(), k_out.data_ptr(), _I64x3(*key.stride()[:3])
+        k_out = _like(key)
+        k_ptr, k_out_ptr, k_strides = key.data_ptr(), k_out.data_ptr(), _I64x4(*key.stride())
     if not b * s * d or not h or (key is not None and not kh):
         if b * s * d and (h or kh):
             raise ValueError(f"{what} need at least one head of query and key")
         return q_out, k_out
-    _call_on(index, "xgb_rope_axes", query.data_ptr(), _I64x3(qs[0], qs[1], qs[2]), k_ptr, k_strides, code, b, s, h, kh, d,
+    _call_on(index, "xgb_rope_axes", query.data_ptr(), _I64x4(*qs), k_ptr, k_strides, code, b, s, h, kh, d,
              positions.data_ptr(), at, positions.stride(0) if len(ps) == 3 else 0, positions.stride(-2), axes, channels,
              thetas, int(interleaved), w_q.data_ptr() if w_q is not None else None,
              w_k.data_ptr() if w_k is not None else None, eps_q, eps_k, q_out.data_ptr(), k_out_ptr)
@@ -349,10 +357,11 @@ def _norm_of(norm, query):
     """(weight, eps) of a Q/K norm module, (None, 0) without one."""
     if norm is None:
         return None, 0.0
-    weight = norm.weight if type(norm) is torch.nn.RMSNorm else None
-    if weight is None or weight.shape != query.shape[-1:] or weight.dtype != query.dtype or not weight.is_contiguous():
-        raise ValueError("rotary positions: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
-    return weight, float(norm.eps if norm.eps is not None else torch.finfo(query.dtype).eps)
+    weight = norm.weight if type(norm) is _RMSNorm else None
+    if weight is None:
+        raise ValueError("rotary positions: norms must be torch.nn.RMSNorm with a weight")
+    eps = norm.eps
+    return weight, eps if eps is not None else torch.finfo(query.dtype).eps
 
 
 _NORM_CODE = {None: 0, "layernorm": 1, "rmsnorm": 2}
@@ -418,16 +427,16 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
             raise ValueError(f"{what}: indices must be int64 [S] or [B, S]")
         index_batch = s if indices.ndim == 2 else 0
         indices = indices.contiguous()
-    x_out = _like(branch, (b, s, w))
+    x_out = _like(branch)
     quant_code, code_type = _QUANT_CODE[quant]
     h_out = codes = scales = None
     if quant_code:
         codes = branch.new_empty((b, s, w), dtype=code_type)
         scales = branch.new_empty((b, s), dtype=torch.float32)
     elif pre_norm is not None:
-        h_out = torch.empty_like(x_out)
+        h_out = _like(branch)
     if b * s:
-        _call_on(index, "xgb_sandwich_norm", branch.data_ptr(), _I64x2(bs[0], bs[1]), residual.data_ptr(), _I64x2(rs[0], rs[1]),
+        _call_on(index, "xgb_sandwich_norm", branch.data_ptr(), _I64x3(*bs), residual.data_ptr(), _I64x3(*rs),
                  code, b, s, w, _NORM_CODE[post_norm], _ptr(post_weight), _NORM_CODE[pre_norm], _ptr(pre_weight), eps,
                  _ptr(gate), _row_stride(gate, w), residual_scale, _ptr(scale), _row_stride(scale, w), _ptr(shift),
                  _row_stride(shift, w), _ptr(indices), index_batch, table_rows, x_out.data_ptr(), _ptr(h_out), quant_code,
