@@ -59,9 +59,9 @@ __device__ __forceinline__ double load_position(const Params& p, int64_t at) {
   }
 }
 
-__device__ __forceinline__ float2 cos_sin(const Params& p, int64_t token, double per_unit, int axis) {
-  const int64_t b = token / p.seq, s = token - b * p.seq;
-  const double turns = load_position(p, b * p.pb + s * p.ps + axis) * per_unit;
+// `at`: where the token's positions start.
+__device__ __forceinline__ float2 cos_sin(const Params& p, int64_t at, double per_unit, int axis) {
+  const double turns = load_position(p, at + axis) * per_unit;
   float sn, cs;
   sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sn, &cs);
   return make_float2(cs, sn);
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) rope_axes_scalar_kernel(const Params
     }
     const int half = p.rotary / 2;
     for (int i = lane; i < half; i += 32) {
-      const float2 cs = cos_sin(p, token, turns.per_unit[i], turns.axis[i]);
+      const float2 cs = cos_sin(p, b * p.pb + s * p.ps, turns.per_unit[i], turns.axis[i]);
       const int ca = interleaved ? 2 * i : i, cb = interleaved ? 2 * i + 1 : i + half;
       float a = to_float(src[ca]), d = to_float(src[cb]);
       if (w) {
@@ -121,56 +121,129 @@ __global__ void __launch_bounds__(kThreads) rope_axes_scalar_kernel(const Params
   }
 }
 
-// Eight consecutive channels.
-__device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
-  unpack_bf16x8(__ldg(reinterpret_cast<const uint4*>(p)), f);
-}
-__device__ __forceinline__ void load8(const __half* p, float (&f)[8]) {
-  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+constexpr int kN = 8;  // channels of a piece, pairs of a thread
+
+// A piece as it lies in memory.
+template <typename T>
+struct Raw {
+  static constexpr int kWords = kN * static_cast<int>(sizeof(T)) / 4;
+  uint32_t w[kWords];
+};
+template <typename T>
+__device__ __forceinline__ void load(const T* p, Raw<T>& r) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+  for (int i = 0; i < Raw<T>::kWords; i += 4) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i / 4);
+    r.w[i] = v.x;
+    r.w[i + 1] = v.y;
+    r.w[i + 2] = v.z;
+    r.w[i + 3] = v.w;
+  }
+}
+__device__ __forceinline__ void unpack(const Raw<float>& r, float (&f)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN; ++i) f[i] = __uint_as_float(r.w[i]);
+}
+__device__ __forceinline__ void unpack(const Raw<__nv_bfloat16>& r, float (&f)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    f[2 * i] = __uint_as_float(r.w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(r.w[i] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void unpack(const Raw<__half>& r, float (&f)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
     f[2 * i] = v.x;
     f[2 * i + 1] = v.y;
   }
 }
-__device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&f)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(round_bf16x2(f[0], f[1]), round_bf16x2(f[2], f[3]), round_bf16x2(f[4], f[5]),
-                                            round_bf16x2(f[6], f[7]));
-}
-__device__ __forceinline__ void store8(__half* p, const float (&f)[8]) {
-  uint32_t w[4];
+__device__ __forceinline__ void pack(const float (&f)[kN], Raw<float>& r) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&v);
-  }
-  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < kN; ++i) r.w[i] = __float_as_uint(f[i]);
 }
+__device__ __forceinline__ void pack(const float (&f)[kN], Raw<__nv_bfloat16>& r) {
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) r.w[i] = round_bf16x2(f[2 * i], f[2 * i + 1]);
+}
+__device__ __forceinline__ void pack(const float (&f)[kN], Raw<__half>& r) {
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    r.w[i] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store(T* p, const Raw<T>& r) {
+#pragma unroll
+  for (int i = 0; i < Raw<T>::kWords; i += 4)
+    reinterpret_cast<uint4*>(p)[i / 4] = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
+}
+
+// Two pieces of kN channels as kN pairs (a, d), two pairs a register pair:
+// channel i of both pieces, or neighbours when interleaved.
+template <bool kInterleaved, typename T>
+__device__ __forceinline__ void to_pairs(const Raw<T> (&r)[2], float2 (&a)[kN / 2], float2 (&d)[kN / 2]) {
+  float f[2][kN];
+  unpack(r[0], f[0]);
+  unpack(r[1], f[1]);
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    if constexpr (kInterleaved) {
+      const int at = i / (kN / 4), o = 4 * (i % (kN / 4));
+      a[i] = make_float2(f[at][o], f[at][o + 2]);
+      d[i] = make_float2(f[at][o + 1], f[at][o + 3]);
+    } else {
+      a[i] = make_float2(f[0][2 * i], f[0][2 * i + 1]);
+      d[i] = make_float2(f[1][2 * i], f[1][2 * i + 1]);
+    }
+  }
+}
+template <bool kInterleaved, typename T>
+__device__ __forceinline__ void from_pairs(const float2 (&a)[kN / 2], const float2 (&d)[kN / 2], Raw<T> (&r)[2]) {
+  float f[2][kN];
+#pragma unroll
+  for (int i = 0; i < kN / 2; ++i) {
+    if constexpr (kInterleaved) {
+      const int at = i / (kN / 4), o = 4 * (i % (kN / 4));
+      f[at][o] = a[i].x;
+      f[at][o + 1] = d[i].x;
+      f[at][o + 2] = a[i].y;
+      f[at][o + 3] = d[i].y;
+    } else {
+      f[0][2 * i] = a[i].x;
+      f[0][2 * i + 1] = a[i].y;
+      f[1][2 * i] = d[i].x;
+      f[1][2 * i + 1] = d[i].y;
+    }
+  }
+  pack(f[0], r[0]);
+  pack(f[1], r[1]);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.y); }
 
 // Vector form: width and rotary multiples of 16, 16-byte aligned rows. Threads
 // are (token, head step, lane): 2^lane_bits lanes a head, 2^head_bits heads at
 // a time, the rest of the 256 threads tokens. A block walks over groups of
 // tokens; a group's cos/sin go through one of two shared buffers, so one
-// barrier a group is enough.
+// barrier a group is enough. With a norm the instructions weigh as much as the
+// bytes, so the arithmetic is packed (two values an instruction) and nothing
+// is divided in the walk; 64 registers keep 32 warps on an SM, whose loads are
+// what hides the sum between a head's loads and its stores (85 registers and
+// 24 warps: a sixth slower; factors with the weights multiplied in, held in 118
+// registers: a third). 126,754 tokens, Q and K of 24 heads of 128 in bf16:
+// 490 us (6.4 TB/s), with the norms 582 us.
 template <typename T, bool kInterleaved, bool kNorm>
-__global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const Params p, const __grid_constant__ Turns turns,
-                                                                 int lane_bits, int head_bits) {
+__global__ void __launch_bounds__(kThreads, 4) rope_axes_vec_kernel(const Params p, const __grid_constant__ Turns turns,
+                                                                 int lane_bits, int head_bits, FastDiv div_seq,
+                                                                 FastDiv div_pairs) {
   __shared__ double per_unit[kMaxPairs];
   __shared__ uint8_t axis[kMaxPairs];
-  // at most 256 / lanes tokens of 8 * lanes pairs each
-  __shared__ __align__(16) float cos_buf[2][kThreads * 8];
-  __shared__ __align__(16) float sin_buf[2][kThreads * 8];
+  // at most 256 / lanes tokens of kN * lanes pairs each
+  __shared__ __align__(16) float cos_buf[2][kThreads * kN];
+  __shared__ __align__(16) float sin_buf[2][kThreads * kN];
   const int pairs = p.rotary / 2;
   for (int i = threadIdx.x; i < pairs; i += kThreads) {
     per_unit[i] = turns.per_unit[i];
@@ -181,98 +254,126 @@ __global__ void __launch_bounds__(kThreads) rope_axes_vec_kernel(const Params p,
   const int first_head = (threadIdx.x >> lane_bits) & ((1 << head_bits) - 1);
   const int t = threadIdx.x >> (lane_bits + head_bits);
   const int per_group = kThreads >> (lane_bits + head_bits);
-  const int heads = p.heads[0] + p.heads[1];
-  const bool active = j < p.width / 16, turned = j < p.rotary / 16;
-  const int ca = kInterleaved || !turned ? 16 * j : 8 * j;
-  const int cb = kInterleaved || !turned ? ca + 8 : ca + pairs;
-  const int64_t groups = (p.tokens + per_group - 1) / per_group;
+  const bool active = 2 * kN * j < p.width, turned = 2 * kN * j < p.rotary;
+  const int ca = kInterleaved || !turned ? 2 * kN * j : kN * j;
+  const int cb = kInterleaved || !turned ? ca + kN : ca + pairs;
+  const float inv_width = 1.f / p.width;
+  const uint32_t tokens = static_cast<uint32_t>(p.tokens), step = per_group * gridDim.x;
   int buf = 0;
-  for (int64_t group = blockIdx.x; group < groups; group += gridDim.x, buf ^= 1) {
-    const int64_t first = group * per_group;
-    for (int i = threadIdx.x; i < per_group * pairs; i += kThreads) {
-      const int tt = i / pairs, pair = i - tt * pairs;
-      if (first + tt < p.tokens) {
-        const float2 cs = cos_sin(p, first + tt, per_unit[pair], axis[pair]);
+  for (uint32_t first = blockIdx.x * per_group; first < tokens; first += step, buf ^= 1) {
+    for (uint32_t i = threadIdx.x; i < per_group * pairs; i += kThreads) {
+      const uint32_t tt = fast_div(i, div_pairs), pair = i - tt * pairs;
+      if (first + tt < tokens) {
+        const uint32_t b = fast_div(first + tt, div_seq), at = first + tt - b * div_seq.d;
+        const float2 cs = cos_sin(p, b * p.pb + at * p.ps, per_unit[pair], axis[pair]);
         cos_buf[buf][i] = cs.x;
         sin_buf[buf][i] = cs.y;
       }
     }
     __syncthreads();
-    const int64_t token = first + t;
-    const bool here = active && token < p.tokens;
-    float c[8], s[8];
+    const uint32_t token = first + t;
+    const bool here = active && token < tokens;
+    const uint32_t b = fast_div(token, div_seq), at = token - b * div_seq.d;
+    float2 c[kN / 2], s[kN / 2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = 1.f;
-      s[i] = 0.f;
+    for (int i = 0; i < kN / 2; ++i) {
+      c[i] = both(1.f);
+      s[i] = both(0.f);
     }
     if (here && turned) {
 #pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const float4 cv = *reinterpret_cast<const float4*>(&cos_buf[buf][t * pairs + 8 * j + i]);
-        const float4 sv = *reinterpret_cast<const float4*>(&sin_buf[buf][t * pairs + 8 * j + i]);
-        c[i] = cv.x; c[i + 1] = cv.y; c[i + 2] = cv.z; c[i + 3] = cv.w;
-        s[i] = sv.x; s[i + 1] = sv.y; s[i + 2] = sv.z; s[i + 3] = sv.w;
+      for (int i = 0; i < kN / 2; i += 2) {
+        const float4 cv = *reinterpret_cast<const float4*>(&cos_buf[buf][t * pairs + kN * j + 2 * i]);
+        const float4 sv = *reinterpret_cast<const float4*>(&sin_buf[buf][t * pairs + kN * j + 2 * i]);
+        c[i] = make_float2(cv.x, cv.y);
+        c[i + 1] = make_float2(cv.z, cv.w);
+        s[i] = make_float2(sv.x, sv.y);
+        s[i + 1] = make_float2(sv.z, sv.w);
       }
     }
-    const int64_t b = token / p.seq, at = token - b * p.seq;
+    const T* q_src = static_cast<const T*>(p.src[0]) + b * p.sb[0] + at * p.ss[0];
+    const T* k_src = static_cast<const T*>(p.src[1]) + b * p.sb[1] + at * p.ss[1];
+    T* q_dst = static_cast<T*>(p.dst[0]) + static_cast<int64_t>(token) * (p.heads[0] * p.width);
+    T* k_dst = static_cast<T*>(p.dst[1]) + static_cast<int64_t>(token) * (p.heads[1] * p.width);
+    const int heads = p.heads[0] + p.heads[1];
 #pragma unroll 2
     for (int h0 = 0; h0 < heads; h0 += 1 << head_bits) {
       int h = h0 + first_head;
       const bool go = here && h < heads;
-      const int which = h >= p.heads[0];
-      if (which) h -= p.heads[0];
-      float x[8], y[8];
+      const bool key = h >= p.heads[0];
+      if (key) h -= p.heads[0];
+      const T* src = key ? k_src + h * p.sh[1] : q_src + h * p.sh[0];
+      Raw<T> raw[2];
+      float2 a[kN / 2], d[kN / 2];
       if (go) {
-        const T* src = static_cast<const T*>(p.src[which]) + b * p.sb[which] + at * p.ss[which] + h * p.sh[which];
-        load8(src + ca, x);
-        load8(src + cb, y);
+        load(src + ca, raw[0]);
+        load(src + cb, raw[1]);
+        to_pairs<kInterleaved>(raw, a, d);
       }
       if constexpr (kNorm) {
+        const T* w = static_cast<const T*>(key ? p.weight[1] : p.weight[0]);
         // every lane takes part; a tensor without a norm keeps its values
-        float sq = 0.f;
+        float2 sq = both(0.f);
         if (go) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], fmaf(y[i], y[i], sq));
+          for (int i = 0; i < kN / 2; ++i) sq = __ffma2_rn(a[i], a[i], __ffma2_rn(d[i], d[i], sq));
         }
-        for (int o = (1 << lane_bits) >> 1; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-        const T* w = static_cast<const T*>(p.weight[which]);
+        float sum = sq.x + sq.y;
+        for (int o = (1 << lane_bits) >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (go && w) {
-          const float rstd = rsqrtf(sq / p.width + p.eps[which]);
-          float wa[8], wb[8];
-          load8(w + ca, wa);
-          load8(w + cb, wb);
+          const float2 r = both(rsqrtf(fmaf(sum, inv_width, key ? p.eps[1] : p.eps[0])));
+          Raw<T> wr[2];
+          float2 wa[kN / 2], wd[kN / 2];
+          load(w + ca, wr[0]);
+          load(w + cb, wr[1]);
+          to_pairs<kInterleaved>(wr, wa, wd);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            x[i] *= rstd * wa[i];
-            y[i] *= rstd * wb[i];
+          for (int i = 0; i < kN / 2; ++i) {
+            a[i] = __fmul2_rn(a[i], __fmul2_rn(wa[i], r));
+            d[i] = __fmul2_rn(d[i], __fmul2_rn(wd[i], r));
           }
         }
       }
       if (go) {
-        T* dst = static_cast<T*>(p.dst[which]) + (token * p.heads[which] + h) * p.width;
-        if constexpr (kInterleaved) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float a = x[2 * i], d = y[2 * i];
-            x[2 * i] = a * c[i] - x[2 * i + 1] * s[i];
-            x[2 * i + 1] = x[2 * i + 1] * c[i] + a * s[i];
-            y[2 * i] = d * c[4 + i] - y[2 * i + 1] * s[4 + i];
-            y[2 * i + 1] = y[2 * i + 1] * c[4 + i] + d * s[4 + i];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float a = x[i];
-            x[i] = a * c[i] - y[i] * s[i];
-            y[i] = y[i] * c[i] + a * s[i];
-          }
+        for (int i = 0; i < kN / 2; ++i) {
+          const float2 turned_a = __ffma2_rn(a[i], c[i], __fmul2_rn(d[i], minus(s[i])));
+          d[i] = __ffma2_rn(d[i], c[i], __fmul2_rn(a[i], s[i]));
+          a[i] = turned_a;
         }
-        store8(dst + ca, x);
-        store8(dst + cb, y);
+        from_pairs<kInterleaved>(a, d, raw);
+        T* dst = (key ? k_dst : q_dst) + h * p.width;
+        store(dst + ca, raw[0]);
+        store(dst + cb, raw[1]);
       }
     }
   }
+}
+
+// The turns of these axes. A thread keeps those of its last axes: 64 powers
+// take about 2 us, as long as the launch.
+const Turns& turns_of(int axes, const int64_t* channels, const double* thetas) {
+  struct Last {
+    int axes = 0;
+    int64_t channels[kMaxAxes];
+    double thetas[kMaxAxes];
+    Turns turns;
+  };
+  static thread_local Last last;
+  if (last.axes == axes && std::equal(channels, channels + axes, last.channels) &&
+      std::equal(thetas, thetas + axes, last.thetas))
+    return last.turns;
+  constexpr double kTwoPi = 6.283185307179586476925286766559;
+  int pairs = 0;
+  for (int a = 0; a < axes; ++a)
+    for (int64_t i = 0; i < channels[a] / 2; ++i, ++pairs) {
+      last.turns.per_unit[pairs] = pow(thetas[a], -2.0 * static_cast<double>(i) / static_cast<double>(channels[a])) / kTwoPi;
+      last.turns.axis[pairs] = static_cast<uint8_t>(a);
+    }
+  std::copy(channels, channels + axes, last.channels);
+  std::copy(thetas, thetas + axes, last.thetas);
+  last.axes = axes;
+  return last.turns;
 }
 
 int bits_for(int n) {  // smallest b with 2^b >= n
@@ -296,18 +397,21 @@ int launch(const Params& p, const Turns& turns, bool interleaved, cudaStream_t s
     rope_axes_scalar_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p, turns, interleaved);
     return launch_status();
   }
-  const int lane_bits = bits_for(p.width / 16);
+  const int lane_bits = bits_for(p.width / (2 * kN));
   // Few tokens: all heads of a token at once, so that more blocks have work.
-  // Many: 8 heads at a time, so that a group has enough angles for its threads.
-  const int most = p.tokens <= 2 * 148 ? 8 - lane_bits : std::min(3, 8 - lane_bits);
-  const int head_bits = std::min(bits_for(heads), most);
+  // Many: up to 8 heads at a time, 4 where 8 would leave more than an eighth
+  // of the threads without a head.
+  const bool few = p.tokens <= 2 * 148;
+  int head_bits = std::min(bits_for(heads), few ? 8 - lane_bits : std::min(3, 8 - lane_bits));
+  if (!few && head_bits == 3 && (cdiv(heads, 8) * 8 - heads) * 8 > heads) head_bits = 2;
   const int64_t groups = cdiv(p.tokens, kThreads >> (lane_bits + head_bits));
-  const int64_t blocks = std::min<int64_t>(groups, 148 * 8);
-  const bool norm = p.weight[0] || p.weight[1];
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(groups, 148 * 8));
+  const FastDiv div_seq = make_fastdiv(static_cast<uint32_t>(p.seq)), div_pairs = make_fastdiv(static_cast<uint32_t>(p.rotary / 2));
   auto run = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(p, turns, lane_bits, head_bits);
+    kernel<<<grid, kThreads, 0, st>>>(p, turns, lane_bits, head_bits, div_seq, div_pairs);
     return launch_status();
   };
+  const bool norm = p.weight[0] || p.weight[1];
   if (interleaved) return norm ? run(rope_axes_vec_kernel<T, true, true>) : run(rope_axes_vec_kernel<T, true, false>);
   return norm ? run(rope_axes_vec_kernel<T, false, true>) : run(rope_axes_vec_kernel<T, false, false>);
 }
@@ -330,19 +434,15 @@ XGB_API int xgb_rope_axes(const void* q, const int64_t* q_strides, const void* k
       axes > kMaxAxes || q_heads > 65535 || k_heads > 65535)
     return XGB_ERR_SHAPE;
   if ((q_weight && !(q_eps >= 0.f)) || (k_weight && !(k_eps >= 0.f))) return XGB_ERR_ARG;
-  Turns turns;
-  int pairs = 0;
-  constexpr double kTwoPi = 6.283185307179586476925286766559;
+  int64_t rotary = 0;
   for (int64_t a = 0; a < axes; ++a) {
-    const int64_t d = axis_channels[a];
-    if (d <= 0 || d % 2 || 2 * pairs + d > width) return XGB_ERR_SHAPE;
+    if (axis_channels[a] <= 0 || axis_channels[a] % 2 || axis_channels[a] > width - rotary) return XGB_ERR_SHAPE;
     if (!(thetas[a] > 0.0)) return XGB_ERR_ARG;
-    for (int64_t i = 0; i < d / 2; ++i, ++pairs) {
-      turns.per_unit[pairs] = pow(thetas[a], -2.0 * static_cast<double>(i) / static_cast<double>(d)) / kTwoPi;
-      turns.axis[pairs] = static_cast<uint8_t>(a);
-    }
+    rotary += axis_channels[a];
   }
   if (batch == 0 || seq == 0) return XGB_OK;
+  if (seq > INT32_MAX || batch > INT32_MAX / seq) return XGB_ERR_SHAPE;
+  const Turns& turns = turns_of(static_cast<int>(axes), axis_channels, thetas);
   Params p{};
   const void* src[2] = {q, k};
   void* dst[2] = {q_out, k_out};
@@ -370,7 +470,7 @@ XGB_API int xgb_rope_axes(const void* q, const int64_t* q_strides, const void* k
   p.tokens = batch * seq;
   p.seq = seq;
   p.width = static_cast<int>(width);
-  p.rotary = 2 * pairs;
+  p.rotary = static_cast<int>(rotary);
   cudaStream_t st = as_stream(stream);
   if (dtype == XGB_BF16) return launch<__nv_bfloat16>(p, turns, interleaved != 0, st);
   if (dtype == XGB_F16) return launch<__half>(p, turns, interleaved != 0, st);
