@@ -70,7 +70,8 @@ def arguments(w, rows, dtype, dev, g, post, pre, seq, *, weights=True, gate=True
 
 
 @pytest.mark.parametrize("b,s,w", [(1, 1, 1), (1, 3, 8), (2, 5, 33), (1, 7, 1536), (2, 33, 257), (1, 4, 5120), (3, 2, 2048),
-                                   (1, 2, 16384), (1, 3, 9999), (1, 130, 64), (1, 5, 8192), (2, 3, 776)])
+                                   (1, 2, 16384), (1, 3, 9999), (1, 130, 64), (1, 5, 8192), (2, 3, 776),
+                                   (1, 300, 1536), (3, 101, 2040), (1, 297, 5120), (2, 150, 512), (1, 9, 400), (1, 299, 8184)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("post,pre", [("rmsnorm", "layernorm"), ("layernorm", "rmsnorm"), (None, "rmsnorm"), ("rmsnorm", None)])
 def test_matches_formula(cuda_device, b, s, w, dtype, post, pre):

@@ -223,12 +223,19 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // constant because every address is then a base and an immediate: with both
 // as run-time values the addresses, index divisions and joins of the sums took
 // more instructions than the arithmetic (55 a channel at width 5120).
+// At two bytes a value 64 registers a thread, 32 warps an SM, hold a row's
+// loads and hide the joins of its sums: 31,689 rows of 5120 take 219 us
+// (5.9 TB/s), with as many registers as the compiler likes 253 us, with 51
+// 258 us. At four bytes the loads need the registers (44 us either way for
+// 8,704 rows of 1536).
 template <int kThreads>
 constexpr int kRowsOf = kThreads == 32 ? 4 : 1;  // rows of a block
+template <typename T, int kThreads>
+constexpr int kBlocksOf = sizeof(T) == 2 && kThreads <= 512 ? 1024 / (kThreads * kRowsOf<kThreads>) : 1;
 
 template <typename T, int kThreads, int kChunks>
-__global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>) sandwich_norm_vec_kernel(const Params p, uint32_t rows,
-                                                                                         FastDiv div_seq) {
+__global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kThreads>)
+    sandwich_norm_vec_kernel(const Params p, uint32_t rows, FastDiv div_seq) {
   constexpr int kWarps = kThreads / 32;
   __shared__ float red[5][kWarps];
   const uint32_t r = kWarps == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
@@ -412,10 +419,21 @@ int launch_vec(const Params& p, int64_t rows, cudaStream_t st) {
   return launch_status();
 }
 
-// The fewest threads that hold a row at up to four pieces a thread.
+// The fewest threads that hold a row at up to four pieces a thread. Few rows,
+// which leave the GPU's threads idle: a piece a thread (64 rows of 1536: 3.6
+// us, with three pieces 5.3 us; at 8,704 rows 25 and 21 us).
 template <typename T>
 int pick_vec(const Params& p, int64_t rows, cudaStream_t st) {
   const int chunks = p.width / 8;
+  if (rows <= 2 * 148 && chunks > 32 && chunks <= 1024) {
+    if (chunks <= 64) return launch_vec<T, 64, 1>(p, rows, st);
+    if (chunks <= 128) return launch_vec<T, 128, 1>(p, rows, st);
+    if (chunks <= 192) return launch_vec<T, 192, 1>(p, rows, st);
+    if (chunks <= 256) return launch_vec<T, 256, 1>(p, rows, st);
+    if (chunks <= 384) return launch_vec<T, 384, 1>(p, rows, st);
+    if (chunks <= 640) return launch_vec<T, 640, 1>(p, rows, st);
+    return launch_vec<T, 1024, 1>(p, rows, st);
+  }
   if (chunks <= 32) return launch_vec<T, 32, 1>(p, rows, st);
   if (chunks <= 64) return launch_vec<T, 32, 2>(p, rows, st);
   if (chunks <= 128) return launch_vec<T, 32, 4>(p, rows, st);
