@@ -454,8 +454,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     // The two query tiles take turns with the exponentials. Without, both run
     // in step: 64 exponentials a row take 1,150 cycles for the two of them at
     // once, the SFU's rate, and what comes before and after, 700 cycles, leaves
-    // it idle. A turn passes by named barriers: one wait and one arrival for
-    // each tile, tile 1 hands tile 0 the first turn and tile 0 takes the last.
+    // it idle. A turn passes half way through a tile (at its end: 2 to 3%
+    // slower), by named barriers: one wait and one arrival for each tile, tile 1
+    // hands tile 0 the first turn and tile 0 takes the last. (A share of the
+    // exponentials by polynomials in packed arithmetic made a step longer, with
+    // a sixth of them 6 to 17% and with half 20%: a turn is a chain of one warp
+    // on each scheduler.)
     const int own_turn = kTurnBar + i, other_turn = kTurnBar + (i ^ 1);
     int turns = 0;
     if (i == 1) named_arrive(other_turn, 2 * kBM);
@@ -574,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * comb;
         };
         // P = 2^(comb s - m) over the S buffer; returns its sum in two lanes
-        auto probabilities = [&](float (&ts)[2]) {
+        auto probabilities = [&](float (&ts)[2], bool pass_turn) {
           // a row whose scores are all -inf has its maximum there: p = 2^-inf
           const float off = m_used == kNegInf ? 0.f : -m_used;
           float ra[4] = {0.f, 0.f, 0.f, 0.f}, rb[4] = {0.f, 0.f, 0.f, 0.f};
@@ -597,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               packed[e / 2] = pack2<T>(a, b);
             }
             tmem_st16(s_addr + c * 16, packed);
+            if (c == 0 && pass_turn) named_arrive(other_turn, 2 * kBM);
           }
           fadd2(ra[0], rb[0], ra[0], rb[0], ra[1], rb[1]);
           fadd2(ra[2], rb[2], ra[2], rb[2], ra[3], rb[3]);
@@ -605,8 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (t == 0) m_used = tile_max();
         float ts[2];
         named_sync(own_turn, 2 * kBM);
-        probabilities(ts);
-        named_arrive(other_turn, 2 * kBM);
+        probabilities(ts, true);
         ++turns;
         if (t > 0 && __any_sync(0xffffffffu, !(ts[0] + ts[1] <= C::kLimit) || m_used == kNegInf)) {
           // Too large, not a number, or no finite score so far: take the
@@ -628,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
             tmem_st16(o_addr + c * 16, o);
           }
-          probabilities(ts);
+          probabilities(ts, false);
         }
         fadd2(sum[0], sum[1], sum[0], sum[1], ts[0], ts[1]);
         tmem_st_wait();
