@@ -12,6 +12,7 @@ does at x_base/x_base/operator/attention.py:357-362).
 """
 from __future__ import annotations
 
+import functools
 import math
 import os
 
@@ -20,7 +21,7 @@ import torch.nn.functional as F
 
 from . import _lib, trace
 from ._lib import call, i64_array
-from .ops import _DTYPE_CODE, _call_on, _device_of, _refuse_autograd
+from .ops import _DTYPE_CODE, _call_on, _device_of, _form, _refuse_autograd
 
 HEAD_DIM = 128
 _err_flags: dict[int, torch.Tensor] = {}
@@ -212,13 +213,7 @@ def dense_attention(q, k, v, sm_scale: float | None = None, out=None) -> torch.T
 
 
 CROSS_HEAD_DIMS = (64, 128)
-
-
 _I64x4 = _lib.c_i64 * 4
-
-
-def _steps(t: torch.Tensor):
-    return _I64x4(*t.stride())
 
 
 def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, *, kv_lens=None, key_mask=None,
@@ -237,17 +232,53 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     workspace of a call comes from the caching allocator."""
     what = "cross attention"
     index = _device_of(what, query, key, value, kv_lens, key_mask, out)
-    _refuse_autograd(what, query, key, value)
-    code = _DTYPE_CODE.get(query.dtype)
-    qn, kn = query.shape, key.shape
-    if (code is None or len(qn) != 4 or len(kn) != 4 or value.ndim != 4 or key.dtype != query.dtype
-            or value.dtype != query.dtype or query.stride(3) != 1 or key.stride(3) != 1 or value.stride(3) != 1):
+    _refuse_autograd(what, query, key, value, out)
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    plan = _cross_plan(index, _form(query), _form(key), _form(value), _form(kv_lens), _form(key_mask), _form(out), sm_scale)
+    q_strides, k_strides, v_strides, out_strides, sizes, sm_scale, takes_mask, ws_bytes, convert_lens = plan
+    if not sizes[1] * sizes[2] * sizes[4]:
+        return out
+    if not sizes[5]:
+        return out.zero_()
+    mask = (None, 0, 0)
+    if key_mask is not None:
+        _, b, _, hk, _, skv, d = sizes
+        key_mask = (key_mask[:, 0, 0] if key_mask.ndim == 4 else key_mask).expand(b, skv)
+        if takes_mask:
+            mask = (key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1))
+        else:
+            kv_lens = key.new_empty((b,), dtype=torch.int32)
+            packed = key.new_empty((2, b, hk, skv, d))
+            _call_on(index, "xgb_pack_keys", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), key.data_ptr(),
+                     k_strides, value.data_ptr(), v_strides, b, hk, skv, d, packed[0].data_ptr(), packed[1].data_ptr(),
+                     kv_lens.data_ptr())
+            key, value = packed[0], packed[1]
+            k_strides = v_strides = _I64x4(*key.stride())
+    elif convert_lens:
+        kv_lens = kv_lens.clamp(0, sizes[5]).to(torch.int32).contiguous()
+    ws = query.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    _call_on(index, "xgb_cross_attention", query.data_ptr(), q_strides, key.data_ptr(), k_strides, value.data_ptr(), v_strides,
+             *sizes, kv_lens.data_ptr() if kv_lens is not None else None, *mask, sm_scale, out.data_ptr(), out_strides,
+             ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(index))
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _cross_plan(index, query, key, value, kv_lens, key_mask, out, sm_scale):
+    """Checks a cross_attention call by its tensors' forms; what follows from
+    them: the C call's arguments, whether its kernel reads the mask, the
+    workspace's bytes, whether kv_lens has to be converted."""
+    what = "cross attention"
+    shape, strides, dtype = query
+    code = _DTYPE_CODE.get(dtype)
+    if code is None or any(len(t[0]) != 4 or t[2] != dtype or t[1][3] != 1 for t in (query, key, value)):
         raise ValueError(f"{what} requires bf16/fp16 [B, H, S, D] views of one type with unit channel stride")
-    b, h, sq, d = qn
-    kb, hk, skv, kd = kn
+    b, h, sq, d = shape
+    kb, hk, skv, kd = key[0]
     if d not in CROSS_HEAD_DIMS:
         raise ValueError(f"{what} requires head dim 64 or 128")
-    if kn != value.shape or kb != b or kd != d or hk == 0 or h % hk:
+    if key[0] != value[0] or kb != b or kd != d or hk == 0 or h % hk:
         raise ValueError(f"{what}: key and value must match, have the query's batch and head dim and divide its heads")
     sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
     if not 0.0 < sm_scale < math.inf:
@@ -255,44 +286,22 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     if kv_lens is not None:
         if key_mask is not None:
             raise ValueError(f"{what} takes kv_lens or key_mask, not both")
-        if kv_lens.shape != (b,) or kv_lens.dtype not in (torch.int32, torch.int64):
+        if kv_lens[0] != (b,) or kv_lens[2] not in (torch.int32, torch.int64):
             raise ValueError(f"{what}: kv_lens must be int32 or int64 [B]")
     if key_mask is not None:
-        if key_mask.ndim == 4 and key_mask.shape[1:3] == (1, 1):
-            key_mask = key_mask[:, 0, 0]
-        if key_mask.dtype != torch.bool or key_mask.ndim != 2 or key_mask.shape[0] not in (1, b) or key_mask.shape[1] != skv:
+        n = key_mask[0]
+        if len(n) == 4 and n[1:3] == (1, 1):
+            n = (n[0], n[3])
+        if key_mask[2] != torch.bool or len(n) != 2 or n[0] not in (1, b) or n[1] != skv:
             raise ValueError(f"{what}: key_mask must be bool [B, Skv], [1, Skv] or [B, 1, 1, Skv]")
-        key_mask = key_mask.expand(b, skv)
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    elif out.shape != qn or out.dtype != query.dtype or out.stride(-1) != 1:
+    if out[0] != shape or out[2] != dtype or out[1][3] != 1:
         raise ValueError(f"{what} output must be a [B, H, Sq, D] view of the query's type with unit channel stride")
-    if not b * h * sq:
-        return out
-    if not skv:
-        return out.zero_()
     lib = _lib.lib()
-    mask = (None, 0, 0)
-    if key_mask is not None:
-        if lib.xgb_cross_attention_takes_mask(h, hk, sq, skv):
-            mask = (key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1))
-        else:
-            kv_lens = key.new_empty((b,), dtype=torch.int32)
-            packed = key.new_empty((2, b, hk, skv, d))
-            _call_on(index, "xgb_pack_keys", key_mask.data_ptr(), key_mask.stride(0), key_mask.stride(1), key.data_ptr(),
-                     _steps(key), value.data_ptr(), _steps(value), b, hk, skv, d, packed[0].data_ptr(), packed[1].data_ptr(),
-                     kv_lens.data_ptr())
-            key, value = packed[0], packed[1]
-    elif kv_lens is not None:
-        if kv_lens.dtype != torch.int32:
-            kv_lens = kv_lens.clamp(0, skv).to(torch.int32)
-        kv_lens = kv_lens.contiguous()
-    ws_bytes = lib.xgb_cross_attention_workspace(b, h, hk, sq, skv, d)
-    ws = query.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    _call_on(index, "xgb_cross_attention", query.data_ptr(), _steps(query), key.data_ptr(), _steps(key), value.data_ptr(),
-             _steps(value), code, b, h, hk, sq, skv, d, kv_lens.data_ptr() if kv_lens is not None else None, *mask, sm_scale,
-             out.data_ptr(), _steps(out), ws.data_ptr() if ws is not None else None, ws_bytes, _err_ptr(index))
-    return out
+    with torch.cuda.device(index):
+        ws_bytes = lib.xgb_cross_attention_workspace(b, h, hk, sq, skv, d)
+    return (_I64x4(*strides), _I64x4(*key[1]), _I64x4(*value[1]), _I64x4(*out[1]), (code, b, h, hk, sq, skv, d), sm_scale,
+            bool(lib.xgb_cross_attention_takes_mask(h, hk, sq, skv)), ws_bytes,
+            kv_lens is not None and (kv_lens[2] != torch.int32 or (b > 1 and kv_lens[1] != (1,))))
 
 
 class H3AttentionBackendB200:

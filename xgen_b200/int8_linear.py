@@ -9,12 +9,15 @@ and `int8_linear_quantized` are the same on a caller's own tensors.
 """
 from __future__ import annotations
 
+import functools
+import math
+
 import torch
 from torch import nn
 
 from ._lib import lib
 from .attention import _err_ptr
-from .ops import _DTYPE_CODE, _call_on, _device_of, _refuse_autograd, _row_stride
+from .ops import _DTYPE_CODE, _call_on, _device_of, _form, _refuse_autograd
 
 ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "swiglu": 3}
 MAX_IN_FEATURES = 131056  # sums of 128 * 128 * K stay within 32-bit integers
@@ -28,56 +31,66 @@ def quantize_per_channel_int8(value: torch.Tensor):
     return (value.float() / scale[:, None]).round().clamp(-127, 127).to(torch.int8), scale
 
 
-def _arguments(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index, residual):
-    """Checks what int8_linear and int8_linear_quantized share; `lead` is the
-    input's shape without its channels. Returns (rows, weight, weight_scale,
-    arguments of the epilogue, output)."""
+@functools.lru_cache(maxsize=1024)
+def _plan(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index, residual):
+    """Checks what int8_linear and int8_linear_quantized share by the tensors'
+    forms; `lead` is the input's shape without its channels. Returns the rows,
+    channels, the C call's numbers and what has to be copied first."""
     what = "H3 INT8 Linear"
-    if weight.dtype != torch.int8 or weight.ndim != 2 or dtype not in _DTYPE_CODE:
+    if weight[2] != torch.int8 or len(weight[0]) != 2 or dtype not in _DTYPE_CODE:
         raise ValueError(f"{what} requires an int8 [out, in] weight and a bf16/fp16 result")
-    n, k = weight.shape
+    n, k = weight[0]
     if n % 16 or k % 16 or not n or not k or k > MAX_IN_FEATURES:
         raise ValueError(f"{what} requires projection dimensions divisible by 16 (in <= {MAX_IN_FEATURES})")
-    if weight_scale.dtype != torch.float32 or weight_scale.shape != (n,):
+    if weight_scale[2] != torch.float32 or weight_scale[0] != (n,):
         raise ValueError(f"{what} requires an fp32 scale for each output channel")
     code = ACTIVATIONS.get(activation, -1)
     if code < 0:
         raise ValueError(f"Unknown {what} activation: {activation}")
     width = n // 2 if code == 3 else n
-    if bias is not None:
-        if bias.shape != (n,) or bias.dtype != dtype:
-            raise ValueError(f"{what} requires a bias [out] of the result's type")
-        bias = bias.contiguous()
-    m = lead.numel()
+    if bias is not None and (bias[0] != (n,) or bias[2] != dtype):
+        raise ValueError(f"{what} requires a bias [out] of the result's type")
+    m = math.prod(lead)
     ldg = ldr = rows = index_rows = 0
+    copy_gate = copy_residual = False
     if gate is not None or gate_index is not None or residual is not None:
         if gate is None or gate_index is None or residual is None or code:
             raise ValueError(f"gated {what} needs gate rows, their index and a residual, and no activation")
-        if (gate.ndim != 2 or gate.shape[1] != n or gate.shape[0] == 0 or gate.dtype != dtype or gate.stride(1) != 1
-                or residual.dtype != dtype or residual.shape != (*lead, n) or residual.stride(-1) != 1):
+        if (len(gate[0]) != 2 or gate[0][1] != n or gate[0][0] == 0 or gate[2] != dtype or gate[1][1] != 1
+                or residual[2] != dtype or residual[0] != (*lead, n) or residual[1][-1] != 1):
             raise ValueError(f"gated {what} needs [M, out] gate rows and a residual of the result's shape and type")
-        index_rows = gate_index.numel()
-        if gate_index.dtype != torch.int64 or (m and (index_rows == 0 or m % index_rows)):
+        index_rows = math.prod(gate_index[0])
+        if gate_index[2] != torch.int64 or (m and (index_rows == 0 or m % index_rows)):
             raise ValueError(f"gated {what} needs an int64 index for each token, or one sequence's for every sample")
-        gate_index = gate_index.contiguous()
-        rows, residual = gate.shape[0], residual if residual.ndim == 2 else residual.reshape(m, n)
-        if rows > 1 and gate.stride(0) < n:  # broadcast rows
-            gate = gate.contiguous()
-        if m > 1 and residual.stride(0) < n:
+        rows = gate[0][0]
+        copy_gate = rows > 1 and gate[1][0] < n  # broadcast rows
+        ldg = gate[1][0] if rows > 1 and not copy_gate else n
+        # rows of the residual a stride apart
+        copy_residual = len(lead) != 1 or (m > 1 and residual[1][0] < n)
+        ldr = residual[1][0] if m > 1 and not copy_residual else n
+    return (m, n, k, (*lead, width), (_DTYPE_CODE[dtype], code, width), (ldg, index_rows, rows, ldr), copy_gate, copy_residual)
+
+
+def _epilogue(plan, dtype, weight, bias, gate, gate_index, residual):
+    """The C call's arguments behind the scales, and its output. (The tensors
+    that a copy makes live until the call has been queued: the last item.)"""
+    m, n, _, shape, (dtype_code, code, width), (ldg, index_rows, rows, ldr), copy_gate, copy_residual = plan
+    out = weight.new_empty(shape, dtype=dtype)
+    if bias is not None:
+        bias = bias.contiguous()
+    head = (dtype_code, bias.data_ptr() if bias is not None else None, code, out.data_ptr(), width)
+    if gate is None:
+        return (*head, None, 0, None, 0, 0, None, 0), out, bias
+    gate_index = gate_index.contiguous()
+    if copy_gate:
+        gate = gate.contiguous()
+    if copy_residual:
+        residual = residual.reshape(m, n)
+        if m > 1 and (residual.stride(0) < n or residual.stride(1) != 1):
             residual = residual.contiguous()
-        ldg, ldr = _row_stride(gate, n), residual.stride(0) if m > 1 else n
-    out = weight.new_empty((*lead, width), dtype=dtype)
-    epilogue = (_DTYPE_CODE[dtype], bias, code, out, width, gate, ldg, gate_index, index_rows, rows, residual, ldr)
-    # (tensors that a view or copy above made live on in `epilogue`)
-    return m, weight.contiguous(), weight_scale.contiguous(), epilogue, out
-
-
-def _pointers(e):
-    """The epilogue's arguments with its tensors as addresses."""
-    dtype, bias, code, out, width, gate, ldg, index, index_rows, rows, residual, ldr = e
-    return (dtype, bias.data_ptr() if bias is not None else None, code, out.data_ptr(), width,
-            *((gate.data_ptr(), ldg, index.data_ptr(), index_rows, rows, residual.data_ptr(), ldr) if gate is not None else
-              (None, 0, None, 0, 0, None, 0)))
+        ldr = residual.stride(0) if m > 1 else n
+    return ((*head, gate.data_ptr(), ldg, gate_index.data_ptr(), index_rows, rows, residual.data_ptr(), ldr), out,
+            (bias, gate, gate_index, residual))
 
 
 def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: torch.Tensor,
@@ -95,13 +108,15 @@ def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: tor
     lead = codes.shape[:-1]
     if scales.dtype != torch.float32 or scales.shape != lead:
         raise ValueError(f"{what} requires an fp32 scale for each row of codes")
-    m, weight, weight_scale, epilogue, out = _arguments(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index,
-                                                        residual)
-    n, k = weight.shape
+    plan = _plan(lead, dtype, _form(weight), _form(weight_scale), _form(bias), activation, _form(gate), _form(gate_index),
+                 _form(residual))
+    m, n, k = plan[:3]
+    epilogue, out, _held = _epilogue(plan, dtype, weight, bias, gate, gate_index, residual)
     if m:
+        weight, weight_scale = weight.contiguous(), weight_scale.contiguous()
         flat, scales = codes.reshape(m, k).contiguous(), scales.reshape(m).contiguous()
         _call_on(index, "xgb_int8_gemm", flat.data_ptr(), weight.data_ptr(), m, n, k, scales.data_ptr(), weight_scale.data_ptr(),
-                 *_pointers(epilogue), _err_ptr(index))
+                 *epilogue, _err_ptr(index))
     return out
 
 
@@ -120,14 +135,16 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
     what = "H3 INT8 Linear"
     index = _device_of(what, x, weight, weight_scale, bias, gate, gate_index, residual)
     _refuse_autograd(what, x, weight_scale, bias, gate, residual)
-    if x.dtype not in _DTYPE_CODE or x.ndim < 1 or weight.ndim != 2 or x.shape[-1] != weight.shape[1]:
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _DTYPE_CODE or not shape or weight.ndim != 2 or shape[-1] != weight.shape[1]:
         raise ValueError(f"{what} requires BF16/FP16 input of its weight's width")
-    lead = x.shape[:-1]
-    m, weight, weight_scale, epilogue, out = _arguments(lead, x.dtype, weight, weight_scale, bias, activation, gate, gate_index,
-                                                        residual)
-    n, k = weight.shape
+    plan = _plan(shape[:-1], dtype, _form(weight), _form(weight_scale), _form(bias), activation, _form(gate), _form(gate_index),
+                 _form(residual))
+    m, n, k = plan[:3]
+    epilogue, out, _held = _epilogue(plan, dtype, weight, bias, gate, gate_index, residual)
     if m:
-        matrix = x if x.ndim == 2 else x.reshape(m, k)
+        weight, weight_scale = weight.contiguous(), weight_scale.contiguous()
+        matrix = x if len(shape) == 2 else x.reshape(m, k)
         ldx, unit = matrix.stride()
         if unit != 1 or (m > 1 and ldx < k):
             matrix = matrix.contiguous()
@@ -135,7 +152,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         ptr = matrix.data_ptr()
         ws_bytes = lib().xgb_int8_linear_workspace(ptr, ldx, m, k)
         ws = x.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-        _call_on(index, "xgb_int8_linear", ptr, ldx, weight.data_ptr(), m, n, k, weight_scale.data_ptr(), *_pointers(epilogue),
+        _call_on(index, "xgb_int8_linear", ptr, ldx, weight.data_ptr(), m, n, k, weight_scale.data_ptr(), *epilogue,
                  ws.data_ptr() if ws_bytes else None, ws_bytes, _err_ptr(index))
     return out
 

@@ -51,6 +51,13 @@ def _refuse_autograd(what: str, *tensors) -> None:
                 raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
 
 
+def _form(t):
+    """Shape, strides and type: what the checks of a call go by. They are made
+    once for each set of forms (lru_cache) and not again: a third of a small
+    call's time on the host."""
+    return None if t is None else (t.shape, t.stride(), t.dtype)
+
+
 def _like(t: torch.Tensor) -> torch.Tensor:
     """An empty contiguous tensor of t's shape, type and device."""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
@@ -300,57 +307,66 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     w_k, eps_k = _norm_of(norm_k, query) if key is not None else (None, 0.0)
     index = _device_of(what, query, key, positions, w_q, w_k)
     _refuse_autograd(what, query, key, w_q, w_k)
-    code = _DTYPE_CODE_F32.get(query.dtype)
-    if code is None or query.ndim != 4:
-        raise ValueError(f"{what} need bf16, fp16 or fp32 queries [B, S, H, D]")
-    b, s, h, d = query.shape
-    qs = query.stride()
-    if qs[3] != 1 and d > 1:
-        raise ValueError(f"{what} need views with unit channel stride")
-    for w in (w_q, w_k):
-        if w is not None and (w.shape != (d,) or w.dtype != query.dtype or not w.is_contiguous()):
-            raise ValueError(f"{what}: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
-    axes, channels, thetas, rotary = _axes_of(axes if type(axes) is tuple else tuple(axes),
-                                              tuple(theta) if type(theta) is list else theta)
-    if rotary > d:
-        raise ValueError(f"{what} need axis channels within the head dim")
-    at = _POSITION_CODE.get(positions.dtype)
-    ps = positions.shape
-    if at is None or not (ps == (s, axes) or ps == (b, s, axes)):
-        raise ValueError(f"{what}: positions must be integers or 32/64-bit floats of shape [S, A] or [B, S, A]")
-    if axes > 1 and positions.stride(-1) != 1:
+    plan = _rope_plan(_form(query), _form(key), _form(positions), axes if type(axes) is tuple else tuple(axes),
+                      tuple(theta) if type(theta) is list else theta, _form(w_q), _form(w_k))
+    q_strides, k_strides, sizes, copy_positions, position_args, rotation = plan
+    if copy_positions:
         positions = positions.contiguous()
     q_out = _like(query)
-    k_out = k_ptr = k_out_ptr = k_strides = None
-    kh = 0
+    k_out = k_ptr = k_out_ptr = None
     if key is not None:
-        if key.ndim != 4 or key.dtype != query.dtype or (key.stride(-1) != 1 and d > 1):
-            raise ValueError(f"{what} need [B, S, H, D] views of one type with unit channel stride")
-        kb, ks, kh, kd = key.shape
-        if kb != b or ks != s or kd != d:
-            raise ValueError(f"{what}: query and key differ in batch, sequence or head dim")
         k_out = _like(key)
-        k_ptr, k_out_ptr, k_strides = key.data_ptr(), k_out.data_ptr(), _I64x4(*key.stride())
-    if not b * s * d or not h or (key is not None and not kh):
-        if b * s * d and (h or kh):
-            raise ValueError(f"{what} need at least one head of query and key")
-        return q_out, k_out
-    _call_on(index, "xgb_rope_axes", query.data_ptr(), _I64x4(*qs), k_ptr, k_strides, code, b, s, h, kh, d,
-             positions.data_ptr(), at, positions.stride(0) if len(ps) == 3 else 0, positions.stride(-2), axes, channels,
-             thetas, int(interleaved), w_q.data_ptr() if w_q is not None else None,
-             w_k.data_ptr() if w_k is not None else None, eps_q, eps_k, q_out.data_ptr(), k_out_ptr)
+        k_ptr, k_out_ptr = key.data_ptr(), k_out.data_ptr()
+    if sizes is not None:
+        _call_on(index, "xgb_rope_axes", query.data_ptr(), q_strides, k_ptr, k_strides, *sizes, positions.data_ptr(),
+                 *position_args, *rotation, int(interleaved), w_q.data_ptr() if w_q is not None else None,
+                 w_k.data_ptr() if w_k is not None else None, eps_q, eps_k, q_out.data_ptr(), k_out_ptr)
     return q_out, k_out
 
 
-@functools.lru_cache(maxsize=256)
-def _axes_of(axes: tuple, theta):
-    """(number, channels and thetas as C arrays, sum) of the axes."""
+@functools.lru_cache(maxsize=1024)
+def _rope_plan(query, key, positions, axes, theta, w_q, w_k):
+    """Checks a rope_axes call by its tensors' forms; the arguments of the C
+    call that follow from them (sizes None: nothing to do)."""
+    what = "rotary positions"
+    shape, strides, dtype = query
+    code = _DTYPE_CODE_F32.get(dtype)
+    if code is None or len(shape) != 4:
+        raise ValueError(f"{what} need bf16, fp16 or fp32 queries [B, S, H, D]")
+    b, s, h, d = shape
+    if strides[3] != 1 and d > 1:
+        raise ValueError(f"{what} need views with unit channel stride")
+    for w in (w_q, w_k):
+        if w is not None and (w[0] != (d,) or w[2] != dtype or (w[1] != (1,) and d > 1)):
+            raise ValueError(f"{what}: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
     axes = tuple(int(a) for a in axes)
     thetas = tuple(float(t) for t in theta) if isinstance(theta, tuple) else (float(theta),) * len(axes)
     if not axes or any(a <= 0 or a % 2 for a in axes) or len(thetas) != len(axes) or not all(
             0 < t < float("inf") for t in thetas):
-        raise ValueError("rotary positions need positive even axis channels and a positive theta for each axis")
-    return len(axes), i64_array(axes), f64_array(thetas), sum(axes)
+        raise ValueError(f"{what} need positive even axis channels and a positive theta for each axis")
+    if sum(axes) > d:
+        raise ValueError(f"{what} need axis channels within the head dim")
+    p_shape, p_strides, p_type = positions
+    n = len(axes)
+    at = _POSITION_CODE.get(p_type)
+    if at is None or not (p_shape == (s, n) or p_shape == (b, s, n)):
+        raise ValueError(f"{what}: positions must be integers or 32/64-bit floats of shape [S, A] or [B, S, A]")
+    copy = n > 1 and p_strides[-1] != 1
+    if copy:
+        p_strides = (s * n, n, 1)[-len(p_shape):]
+    kh, k_strides = 0, None
+    if key is not None:
+        if len(key[0]) != 4 or key[2] != dtype or (key[1][3] != 1 and d > 1):
+            raise ValueError(f"{what} need [B, S, H, D] views of one type with unit channel stride")
+        kb, ks, kh, kd = key[0]
+        if kb != b or ks != s or kd != d:
+            raise ValueError(f"{what}: query and key differ in batch, sequence or head dim")
+        k_strides = _I64x4(*key[1])
+    empty = not b * s * d or not h or (key is not None and not kh)
+    if empty and b * s * d and (h or kh):
+        raise ValueError(f"{what} need at least one head of query and key")
+    return (_I64x4(*strides), k_strides, None if empty else (code, b, s, h, kh, d), copy,
+            (at, p_strides[0] if len(p_shape) == 3 else 0, p_strides[-2]), (n, i64_array(axes), f64_array(thetas)))
 
 
 def _norm_of(norm, query):
@@ -392,12 +408,39 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
     what = "sandwich norm"
     index = _device_of(what, branch, residual, post_weight, pre_weight, gate, scale, shift, indices)
     _refuse_autograd(what, branch, residual, post_weight, pre_weight, gate, scale, shift)
-    dtype = branch.dtype
+    plan = _sandwich_plan(_form(branch), _form(residual), post_norm, pre_norm, _form(post_weight), _form(pre_weight), _form(gate),
+                          _form(scale), _form(shift), _form(indices), quant)
+    y_strides, x_strides, sizes, norms, strides, index_batch, table_rows, quant_code, code_type = plan
+    if indices is not None:
+        indices = indices.contiguous()
+    x_out = _like(branch)
+    h_out = codes = scales = None
+    if quant_code:
+        codes = branch.new_empty(branch.shape, dtype=code_type)
+        scales = branch.new_empty(branch.shape[:2], dtype=torch.float32)
+    elif pre_norm is not None:
+        h_out = _like(branch)
+    if sizes is not None:
+        _call_on(index, "xgb_sandwich_norm", branch.data_ptr(), y_strides, residual.data_ptr(), x_strides, *sizes, norms[0],
+                 _ptr(post_weight), norms[1], _ptr(pre_weight), eps, _ptr(gate), strides[0], residual_scale, _ptr(scale),
+                 strides[1], _ptr(shift), strides[2], _ptr(indices), index_batch, table_rows, x_out.data_ptr(), _ptr(h_out),
+                 quant_code, _ptr(codes), _ptr(scales))
+    if pre_norm is None:
+        return x_out
+    return (x_out, codes, scales) if quant_code else (x_out, h_out)
+
+
+@functools.lru_cache(maxsize=1024)
+def _sandwich_plan(branch, residual, post_norm, pre_norm, post_weight, pre_weight, gate, scale, shift, indices, quant):
+    """Checks a sandwich_norm call by its tensors' forms; the arguments of the
+    C call that follow from them (sizes None: nothing to do)."""
+    what = "sandwich norm"
+    shape, bs, dtype = branch
     code = _DTYPE_CODE_F32.get(dtype)
-    if code is None or branch.ndim != 3 or branch.shape != residual.shape or residual.dtype != dtype:
+    if code is None or len(shape) != 3 or shape != residual[0] or residual[2] != dtype:
         raise ValueError(f"{what} needs [B, S, W] branch and residual of one 16- or 32-bit float type")
-    b, s, w = branch.shape
-    bs, rs = branch.stride(), residual.stride()
+    b, s, w = shape
+    rs = residual[1]
     if (bs[2] != 1 or rs[2] != 1) and w > 1:
         raise ValueError(f"{what} needs views with unit channel stride")
     if w > 16384 or w == 0:
@@ -411,50 +454,26 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
     if post_norm is None and post_weight is not None:
         raise ValueError(f"{what} without a norm after the block has no weight for it")
     for t in (post_weight, pre_weight):
-        if t is not None and (t.shape != (w,) or t.dtype != dtype or not t.is_contiguous()):
+        if t is not None and (t[0] != (w,) or t[2] != dtype or (t[1] != (1,) and w > 1)):
             raise ValueError(f"{what}: weights must be contiguous [W] of the branch's type")
-    table_rows = 0
+    table_rows, strides = 0, []
     for t in (gate, scale, shift):
         if t is not None:
-            table_rows = table_rows or t.shape[0]
-            if t.ndim != 2 or t.shape != (table_rows, w) or t.dtype != dtype or (t.stride(1) != 1 and w > 1) or not table_rows:
+            table_rows = table_rows or (t[0][0] if len(t[0]) == 2 else 0)
+            if t[0] != (table_rows, w) or t[2] != dtype or (t[1][1] != 1 and w > 1) or not table_rows:
                 raise ValueError(f"{what}: gate, scale and shift must be [M, W] rows of the branch's type")
+        # one row is never stepped over
+        strides.append(0 if t is None else t[1][0] if table_rows > 1 else w)
     if (table_rows > 0) != (indices is not None):
         raise ValueError(f"{what}: indices come with gate or scale and shift")
-    index_batch = 0
-    if indices is not None:
-        if indices.dtype != torch.int64 or not (indices.shape == (s,) or indices.shape == (b, s)):
-            raise ValueError(f"{what}: indices must be int64 [S] or [B, S]")
-        index_batch = s if indices.ndim == 2 else 0
-        indices = indices.contiguous()
-    x_out = _like(branch)
-    quant_code, code_type = _QUANT_CODE[quant]
-    h_out = codes = scales = None
-    if quant_code:
-        codes = branch.new_empty((b, s, w), dtype=code_type)
-        scales = branch.new_empty((b, s), dtype=torch.float32)
-    elif pre_norm is not None:
-        h_out = _like(branch)
-    if b * s:
-        _call_on(index, "xgb_sandwich_norm", branch.data_ptr(), _I64x3(*bs), residual.data_ptr(), _I64x3(*rs),
-                 code, b, s, w, _NORM_CODE[post_norm], _ptr(post_weight), _NORM_CODE[pre_norm], _ptr(pre_weight), eps,
-                 _ptr(gate), _row_stride(gate, w), residual_scale, _ptr(scale), _row_stride(scale, w), _ptr(shift),
-                 _row_stride(shift, w), _ptr(indices), index_batch, table_rows, x_out.data_ptr(), _ptr(h_out), quant_code,
-                 _ptr(codes), _ptr(scales))
-    if pre_norm is None:
-        return x_out
-    return (x_out, codes, scales) if quant_code else (x_out, h_out)
+    if indices is not None and (indices[2] != torch.int64 or not (indices[0] == (s,) or indices[0] == (b, s))):
+        raise ValueError(f"{what}: indices must be int64 [S] or [B, S]")
+    return (_I64x3(*bs), _I64x3(*rs), (code, b, s, w) if b * s else None, (_NORM_CODE[post_norm], _NORM_CODE[pre_norm]), strides,
+            s if indices is not None and len(indices[0]) == 2 else 0, table_rows, *_QUANT_CODE[quant])
 
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
-
-
-def _row_stride(t, width: int) -> int:
-    """Elements between the rows of a table; one row is never stepped over."""
-    if t is None:
-        return 0
-    return t.stride(0) if t.shape[0] > 1 else width
 
 
 def quantize_per_token_int8(x: torch.Tensor):
