@@ -955,7 +955,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const Params p, i
 }
 
 // 4 warps a row, 16 where there are more parts than those take at once (444
-// parts: 29 us with 4).
+// parts: 29 us with 4 warps, 12 us with 16).
 template <typename T, int kD>
 int join(const Params& p, int64_t rows, int few_tiles, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>(rows);
@@ -997,11 +997,13 @@ inline Plan plan(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, 
   if (n.few) {
     n.tiles = static_cast<int>(cdiv(rows, kFewRows));
     n.items = batch * kv_heads * n.tiles;
-    // Three CTAs an SM are resident, each should have a step for each of its
-    // warps. A cluster of up to 8 parts needs no second kernel; it is taken as
-    // soon as it gives every SM a CTA.
+    // Two CTAs an SM (as many as are resident at D = 128), each with a step for
+    // each of its warps. A cluster of up to 8 parts needs no second kernel; it
+    // is taken as soon as it gives every SM a CTA. With one, two and three CTAs
+    // an SM: 100,000 keys of one head 17, 19 and 25 us, 16,384 of 8 heads 18,
+    // 17 and 22 us, 512 of 24 heads 7.4, 6.5 and 6.6 us.
     const int64_t most = cdiv(seq_kv, kFewKeys * kFewWarps);
-    n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({3 * sms / n.items, most, kMostParts})));
+    n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({2 * sms / n.items, most, kMostParts})));
     n.clustered = n.splits > 1 && (n.splits <= 8 || n.items * 8 >= sms);
     if (n.clustered) n.splits = std::min(n.splits, 8);
     n.part_rows = kFewRows;
