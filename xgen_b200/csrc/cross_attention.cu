@@ -760,8 +760,8 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
   float o[2 * kChunks][4] = {};
   float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};  // rows 2c, 2c + 1
   // Keys and values of this step and the next: both are requested a step ahead,
-  // so that a step costs its arithmetic, not a memory access. (With V requested
-  // in its own step 4 tokens against 4,099 keys took 12.3 us.)
+  // so that a step costs its arithmetic, not a memory access. One token of 4
+  // samples with 24 / 8 heads against 4,099 keys each: 14.7 us (4.6 TB/s).
   uint4 k0[kChunks], k1[kChunks], v0[kChunks], v1[kChunks], vn0[kChunks], vn1[kChunks];
   bool keep0 = false, keep1 = false, next0 = false, next1 = false;
   auto request = [&](int at) {
