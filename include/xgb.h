@@ -279,7 +279,8 @@ int xgb_norm_modulate_quant(const void* x, int64_t ldx, int64_t rows, int64_t wi
  * `interleaved` (2i, 2i + 1). positions [batch, seq, axes] (element strides
  * position_batch_stride, 0 when shared, and position_stride; axis stride 1),
  * position_type 0 int32, 1 int64, 2 float, 3 double; angles are formed in 64
- * bits. axis_channels and thetas are host arrays of `axes` entries. */
+ * bits. axis_channels and thetas are host arrays of `axes` entries. batch * seq
+ * is below 2^31. */
 int xgb_rope_axes(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
                   int64_t batch, int64_t seq, int64_t q_heads, int64_t k_heads, int64_t width,
                   const void* positions, int position_type, int64_t position_batch_stride,
@@ -355,8 +356,9 @@ int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int64_t seq_
 int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                         const void* v, const int64_t* v_strides, int dtype, int64_t batch, int64_t heads,
                         int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int* kv_lens,
-                        const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, float sm_scale, void* out, const int64_t* out_strides, void* workspace,
-                        int64_t workspace_bytes, int* error_flag, void* stream);
+                        const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, float sm_scale,
+                        void* out, const int64_t* out_strides, void* workspace, int64_t workspace_bytes,
+                        int* error_flag, void* stream);
 
 /* The keys and values that `mask` (bytes [batch, seq], 0 = left out) keeps, in
  * order, at the front of contiguous k_out/v_out [batch, heads, seq, head_dim],

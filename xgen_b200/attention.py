@@ -21,7 +21,7 @@ import torch.nn.functional as F
 
 from . import _lib, trace
 from ._lib import call, i64_array
-from .ops import _DTYPE_CODE, _call_on, _device_of, _form, _refuse_autograd
+from .ops import _DTYPE_CODE, _call_on, _device_in, _form, _like, _refuse_autograd
 
 HEAD_DIM = 128
 _err_flags: dict[int, torch.Tensor] = {}
@@ -231,12 +231,11 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     which must not overlap the inputs. Nothing is shared between calls: the
     workspace of a call comes from the caching allocator."""
     what = "cross attention"
-    index = _device_of(what, query, key, value, kv_lens, key_mask, out)
     _refuse_autograd(what, query, key, value, out)
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    plan = _cross_plan(index, _form(query), _form(key), _form(value), _form(kv_lens), _form(key_mask), _form(out), sm_scale)
-    q_strides, k_strides, v_strides, out_strides, sizes, sm_scale, takes_mask, ws_bytes, convert_lens = plan
+        out = _like(query)
+    plan = _cross_plan(_form(query), _form(key), _form(value), _form(kv_lens), _form(key_mask), _form(out), sm_scale)
+    index, q_strides, k_strides, v_strides, out_strides, sizes, sm_scale, takes_mask, ws_bytes, convert_lens = plan
     if not sizes[1] * sizes[2] * sizes[4]:
         return out
     if not sizes[5]:
@@ -265,12 +264,13 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
 
 
 @functools.lru_cache(maxsize=1024)
-def _cross_plan(index, query, key, value, kv_lens, key_mask, out, sm_scale):
+def _cross_plan(query, key, value, kv_lens, key_mask, out, sm_scale):
     """Checks a cross_attention call by its tensors' forms; what follows from
     them: the C call's arguments, whether its kernel reads the mask, the
     workspace's bytes, whether kv_lens has to be converted."""
     what = "cross attention"
-    shape, strides, dtype = query
+    index = _device_in(what, query, key, value, kv_lens, key_mask, out)
+    shape, strides, dtype, _ = query
     code = _DTYPE_CODE.get(dtype)
     if code is None or any(len(t[0]) != 4 or t[2] != dtype or t[1][3] != 1 for t in (query, key, value)):
         raise ValueError(f"{what} requires bf16/fp16 [B, H, S, D] views of one type with unit channel stride")
@@ -299,7 +299,7 @@ def _cross_plan(index, query, key, value, kv_lens, key_mask, out, sm_scale):
     lib = _lib.lib()
     with torch.cuda.device(index):
         ws_bytes = lib.xgb_cross_attention_workspace(b, h, hk, sq, skv, d)
-    return (_I64x4(*strides), _I64x4(*key[1]), _I64x4(*value[1]), _I64x4(*out[1]), (code, b, h, hk, sq, skv, d), sm_scale,
+    return (index, _I64x4(*strides), _I64x4(*key[1]), _I64x4(*value[1]), _I64x4(*out[1]), (code, b, h, hk, sq, skv, d), sm_scale,
             bool(lib.xgb_cross_attention_takes_mask(h, hk, sq, skv)), ws_bytes,
             kv_lens is not None and (kv_lens[2] != torch.int32 or (b > 1 and kv_lens[1] != (1,))))
 

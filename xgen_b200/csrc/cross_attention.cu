@@ -1156,8 +1156,9 @@ XGB_API int xgb_cross_attention_takes_mask(int64_t heads, int64_t kv_heads, int6
 XGB_API int xgb_cross_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                 const void* v, const int64_t* v_strides, int dtype, int64_t batch, int64_t heads,
                                 int64_t kv_heads, int64_t seq_q, int64_t seq_kv, int64_t head_dim, const int* kv_lens,
-                                const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, float sm_scale, void* out, const int64_t* out_strides, void* workspace,
-                                int64_t workspace_bytes, int* error_flag, void* stream) {
+                                const uint8_t* mask, int64_t mask_batch_stride, int64_t mask_stride, float sm_scale,
+                                void* out, const int64_t* out_strides, void* workspace, int64_t workspace_bytes,
+                                int* error_flag, void* stream) {
   if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides || !out_strides) return XGB_ERR_ARG;
   if (dtype != XGB_BF16 && dtype != XGB_F16) return XGB_ERR_ARG;
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || seq_q <= 0 || seq_kv <= 0 || seq_q > (1 << 30) ||

@@ -17,7 +17,7 @@ from torch import nn
 
 from ._lib import lib
 from .attention import _err_ptr
-from .ops import _DTYPE_CODE, _call_on, _device_of, _form, _refuse_autograd
+from .ops import _DTYPE_CODE, _call_on, _device_in, _form, _refuse_autograd
 
 ACTIVATIONS = {None: 0, "gelu": 1, "gelu_tanh": 2, "swiglu": 3}
 MAX_IN_FEATURES = 131056  # sums of 128 * 128 * K stay within 32-bit integers
@@ -32,11 +32,12 @@ def quantize_per_channel_int8(value: torch.Tensor):
 
 
 @functools.lru_cache(maxsize=1024)
-def _plan(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index, residual):
+def _plan(x, lead, dtype, scales, weight, weight_scale, bias, activation, gate, gate_index, residual):
     """Checks what int8_linear and int8_linear_quantized share by the tensors'
     forms; `lead` is the input's shape without its channels. Returns the rows,
-    channels, the C call's numbers and what has to be copied first."""
+    channels, the C call's numbers and what has to be copied first, the device."""
     what = "H3 INT8 Linear"
+    index = _device_in(what, x, scales, weight, weight_scale, bias, gate, gate_index, residual)
     if weight[2] != torch.int8 or len(weight[0]) != 2 or dtype not in _DTYPE_CODE:
         raise ValueError(f"{what} requires an int8 [out, in] weight and a bf16/fp16 result")
     n, k = weight[0]
@@ -68,19 +69,24 @@ def _plan(lead, dtype, weight, weight_scale, bias, activation, gate, gate_index,
         # rows of the residual a stride apart
         copy_residual = len(lead) != 1 or (m > 1 and residual[1][0] < n)
         ldr = residual[1][0] if m > 1 and not copy_residual else n
-    return (m, n, k, (*lead, width), (_DTYPE_CODE[dtype], code, width), (ldg, index_rows, rows, ldr), copy_gate, copy_residual)
+    return (m, n, k, (*lead, width), (_DTYPE_CODE[dtype], code, width), (ldg, index_rows, rows, ldr), copy_gate, copy_residual, index)
 
 
-def _epilogue(plan, dtype, weight, bias, gate, gate_index, residual):
-    """The C call's arguments behind the scales, and its output. (The tensors
-    that a copy makes live until the call has been queued: the last item.)"""
-    m, n, _, shape, (dtype_code, code, width), (ldg, index_rows, rows, ldr), copy_gate, copy_residual = plan
-    out = weight.new_empty(shape, dtype=dtype)
+@functools.lru_cache(maxsize=1024)
+def _workspace(offset, ldx, m, k):
+    """Bytes for an input that starts `offset` bytes behind a 16-byte boundary."""
+    return lib().xgb_int8_linear_workspace(16 + offset, ldx, m, k)
+
+
+def _epilogue(plan, out, bias, gate, gate_index, residual):
+    """The C call's arguments behind the scales, and the tensors that a copy
+    made: they live until the call has been queued."""
+    m, n, _, _, (dtype_code, code, width), (ldg, index_rows, rows, ldr), copy_gate, copy_residual, _ = plan
     if bias is not None:
         bias = bias.contiguous()
     head = (dtype_code, bias.data_ptr() if bias is not None else None, code, out.data_ptr(), width)
     if gate is None:
-        return (*head, None, 0, None, 0, 0, None, 0), out, bias
+        return (*head, None, 0, None, 0, 0, None, 0), bias
     gate_index = gate_index.contiguous()
     if copy_gate:
         gate = gate.contiguous()
@@ -89,7 +95,7 @@ def _epilogue(plan, dtype, weight, bias, gate, gate_index, residual):
         if m > 1 and (residual.stride(0) < n or residual.stride(1) != 1):
             residual = residual.contiguous()
         ldr = residual.stride(0) if m > 1 else n
-    return ((*head, gate.data_ptr(), ldg, gate_index.data_ptr(), index_rows, rows, residual.data_ptr(), ldr), out,
+    return ((*head, gate.data_ptr(), ldg, gate_index.data_ptr(), index_rows, rows, residual.data_ptr(), ldr),
             (bias, gate, gate_index, residual))
 
 
@@ -101,17 +107,17 @@ def int8_linear_quantized(codes: torch.Tensor, scales: torch.Tensor, weight: tor
     quant="int8"). dtype: bf16 or fp16, the type of the result and of bias,
     gate and residual."""
     what = "H3 INT8 Linear"
-    index = _device_of(what, codes, scales, weight, weight_scale, bias, gate, gate_index, residual)
     _refuse_autograd(what, scales, weight_scale, bias, gate, residual)
     if codes.dtype != torch.int8 or codes.ndim < 1 or weight.ndim != 2 or codes.shape[-1] != weight.shape[1]:
         raise ValueError(f"{what} requires int8 codes of its weight's width")
     lead = codes.shape[:-1]
     if scales.dtype != torch.float32 or scales.shape != lead:
         raise ValueError(f"{what} requires an fp32 scale for each row of codes")
-    plan = _plan(lead, dtype, _form(weight), _form(weight_scale), _form(bias), activation, _form(gate), _form(gate_index),
+    plan = _plan(_form(codes), lead, dtype, _form(scales), _form(weight), _form(weight_scale), _form(bias), activation, _form(gate), _form(gate_index),
                  _form(residual))
-    m, n, k = plan[:3]
-    epilogue, out, _held = _epilogue(plan, dtype, weight, bias, gate, gate_index, residual)
+    m, n, k, index = *plan[:3], plan[-1]
+    out = weight.new_empty(plan[3], dtype=dtype)
+    epilogue, _held = _epilogue(plan, out, bias, gate, gate_index, residual)
     if m:
         weight, weight_scale = weight.contiguous(), weight_scale.contiguous()
         flat, scales = codes.reshape(m, k).contiguous(), scales.reshape(m).contiguous()
@@ -133,15 +139,15 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
 
     Each token's largest magnitude becomes 127; sums are exact, one rounding."""
     what = "H3 INT8 Linear"
-    index = _device_of(what, x, weight, weight_scale, bias, gate, gate_index, residual)
     _refuse_autograd(what, x, weight_scale, bias, gate, residual)
     dtype, shape = x.dtype, x.shape
     if dtype not in _DTYPE_CODE or not shape or weight.ndim != 2 or shape[-1] != weight.shape[1]:
         raise ValueError(f"{what} requires BF16/FP16 input of its weight's width")
-    plan = _plan(shape[:-1], dtype, _form(weight), _form(weight_scale), _form(bias), activation, _form(gate), _form(gate_index),
+    plan = _plan(_form(x), shape[:-1], dtype, None, _form(weight), _form(weight_scale), _form(bias), activation, _form(gate), _form(gate_index),
                  _form(residual))
-    m, n, k = plan[:3]
-    epilogue, out, _held = _epilogue(plan, dtype, weight, bias, gate, gate_index, residual)
+    m, n, k, index = *plan[:3], plan[-1]
+    out = x.new_empty(plan[3])
+    epilogue, _held = _epilogue(plan, out, bias, gate, gate_index, residual)
     if m:
         weight, weight_scale = weight.contiguous(), weight_scale.contiguous()
         matrix = x if len(shape) == 2 else x.reshape(m, k)
@@ -150,7 +156,7 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
             matrix = matrix.contiguous()
             ldx = k
         ptr = matrix.data_ptr()
-        ws_bytes = lib().xgb_int8_linear_workspace(ptr, ldx, m, k)
+        ws_bytes = _workspace(ptr % 16, ldx, m, k)
         ws = x.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
         _call_on(index, "xgb_int8_linear", ptr, ldx, weight.data_ptr(), m, n, k, weight_scale.data_ptr(), *epilogue,
                  ws.data_ptr() if ws_bytes else None, ws_bytes, _err_ptr(index))

@@ -33,17 +33,6 @@ def _require_cuda(*tensors: torch.Tensor, what: str) -> None:
             raise ValueError(f"{what} requires CUDA tensors")
 
 
-def _device_of(what: str, *tensors) -> int:
-    """Index of the one GPU that all tensors (None: not given) are on."""
-    index = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != index or index < 0:
-            if any(x is not None and not x.is_cuda for x in tensors):
-                raise ValueError(f"{what} requires CUDA tensors")
-            raise ValueError(f"{what} needs its tensors on one device")
-    return index
-
-
 def _refuse_autograd(what: str, *tensors) -> None:
     if torch.is_grad_enabled():
         for t in tensors:
@@ -52,10 +41,20 @@ def _refuse_autograd(what: str, *tensors) -> None:
 
 
 def _form(t):
-    """Shape, strides and type: what the checks of a call go by. They are made
-    once for each set of forms (lru_cache) and not again: a third of a small
-    call's time on the host."""
-    return None if t is None else (t.shape, t.stride(), t.dtype)
+    """Shape, strides, type and device: what the checks of a call go by. They
+    are made once for each set of forms (lru_cache) and not again: a third of a
+    small call's time on the host."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _device_in(what: str, *forms) -> int:
+    """Index of the one GPU that all tensors (None: not given) are on."""
+    at = {f[3] for f in forms if f is not None}
+    if min(at) < 0:
+        raise ValueError(f"{what} requires CUDA tensors")
+    if len(at) > 1:
+        raise ValueError(f"{what} needs its tensors on one device")
+    return at.pop()
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
@@ -305,11 +304,10 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     what = "rotary positions"
     w_q, eps_q = _norm_of(norm_q, query)
     w_k, eps_k = _norm_of(norm_k, query) if key is not None else (None, 0.0)
-    index = _device_of(what, query, key, positions, w_q, w_k)
     _refuse_autograd(what, query, key, w_q, w_k)
     plan = _rope_plan(_form(query), _form(key), _form(positions), axes if type(axes) is tuple else tuple(axes),
                       tuple(theta) if type(theta) is list else theta, _form(w_q), _form(w_k))
-    q_strides, k_strides, sizes, copy_positions, position_args, rotation = plan
+    index, q_strides, k_strides, sizes, copy_positions, position_args, rotation = plan
     if copy_positions:
         positions = positions.contiguous()
     q_out = _like(query)
@@ -329,7 +327,8 @@ def _rope_plan(query, key, positions, axes, theta, w_q, w_k):
     """Checks a rope_axes call by its tensors' forms; the arguments of the C
     call that follow from them (sizes None: nothing to do)."""
     what = "rotary positions"
-    shape, strides, dtype = query
+    index = _device_in(what, query, key, positions, w_q, w_k)
+    shape, strides, dtype, _ = query
     code = _DTYPE_CODE_F32.get(dtype)
     if code is None or len(shape) != 4:
         raise ValueError(f"{what} need bf16, fp16 or fp32 queries [B, S, H, D]")
@@ -346,7 +345,7 @@ def _rope_plan(query, key, positions, axes, theta, w_q, w_k):
         raise ValueError(f"{what} need positive even axis channels and a positive theta for each axis")
     if sum(axes) > d:
         raise ValueError(f"{what} need axis channels within the head dim")
-    p_shape, p_strides, p_type = positions
+    p_shape, p_strides, p_type, _ = positions
     n = len(axes)
     at = _POSITION_CODE.get(p_type)
     if at is None or not (p_shape == (s, n) or p_shape == (b, s, n)):
@@ -365,7 +364,7 @@ def _rope_plan(query, key, positions, axes, theta, w_q, w_k):
     empty = not b * s * d or not h or (key is not None and not kh)
     if empty and b * s * d and (h or kh):
         raise ValueError(f"{what} need at least one head of query and key")
-    return (_I64x4(*strides), k_strides, None if empty else (code, b, s, h, kh, d), copy,
+    return (index, _I64x4(*strides), k_strides, None if empty else (code, b, s, h, kh, d), copy,
             (at, p_strides[0] if len(p_shape) == 3 else 0, p_strides[-2]), (n, i64_array(axes), f64_array(thetas)))
 
 
@@ -406,11 +405,10 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
     32-bit arithmetic; x and h are rounded once each, h from the x before its
     rounding."""
     what = "sandwich norm"
-    index = _device_of(what, branch, residual, post_weight, pre_weight, gate, scale, shift, indices)
     _refuse_autograd(what, branch, residual, post_weight, pre_weight, gate, scale, shift)
     plan = _sandwich_plan(_form(branch), _form(residual), post_norm, pre_norm, _form(post_weight), _form(pre_weight), _form(gate),
                           _form(scale), _form(shift), _form(indices), quant)
-    y_strides, x_strides, sizes, norms, strides, index_batch, table_rows, quant_code, code_type = plan
+    index, y_strides, x_strides, sizes, norms, strides, index_batch, table_rows, quant_code, code_type = plan
     if indices is not None:
         indices = indices.contiguous()
     x_out = _like(branch)
@@ -435,7 +433,8 @@ def _sandwich_plan(branch, residual, post_norm, pre_norm, post_weight, pre_weigh
     """Checks a sandwich_norm call by its tensors' forms; the arguments of the
     C call that follow from them (sizes None: nothing to do)."""
     what = "sandwich norm"
-    shape, bs, dtype = branch
+    index = _device_in(what, branch, residual, post_weight, pre_weight, gate, scale, shift, indices)
+    shape, bs, dtype, _ = branch
     code = _DTYPE_CODE_F32.get(dtype)
     if code is None or len(shape) != 3 or shape != residual[0] or residual[2] != dtype:
         raise ValueError(f"{what} needs [B, S, W] branch and residual of one 16- or 32-bit float type")
@@ -468,7 +467,7 @@ def _sandwich_plan(branch, residual, post_norm, pre_norm, post_weight, pre_weigh
         raise ValueError(f"{what}: indices come with gate or scale and shift")
     if indices is not None and (indices[2] != torch.int64 or not (indices[0] == (s,) or indices[0] == (b, s))):
         raise ValueError(f"{what}: indices must be int64 [S] or [B, S]")
-    return (_I64x3(*bs), _I64x3(*rs), (code, b, s, w) if b * s else None, (_NORM_CODE[post_norm], _NORM_CODE[pre_norm]), strides,
+    return (index, _I64x3(*bs), _I64x3(*rs), (code, b, s, w) if b * s else None, (_NORM_CODE[post_norm], _NORM_CODE[pre_norm]), strides,
             s if indices is not None and len(indices[0]) == 2 else 0, table_rows, *_QUANT_CODE[quant])
 
 
@@ -481,7 +480,7 @@ def quantize_per_token_int8(x: torch.Tensor):
     (codes, scales[rows]) with scale = max(amax/127, FLT_MIN) and codes the
     nearest integers to x / scale, ties to even."""
     what = "H3 INT8 quantization"
-    index = _device_of(what, x)
+    index = _device_in(what, _form(x))
     _refuse_autograd(what, x)
     if x.dtype not in _DTYPE_CODE or x.ndim != 2 or (x.stride(-1) != 1 and x.shape[1] > 1) or x.shape[1] == 0 or (
             x.shape[0] > 1 and x.stride(0) < x.shape[1]):
