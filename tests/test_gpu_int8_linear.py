@@ -93,7 +93,8 @@ def test_codes_of_ties_zeros_tiny_and_not_finite(cuda_device):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 16, 16), (1, 4608, 1536), (7, 144, 96), (16, 512, 2064), (33, 1536, 1536), (128, 256, 128),
-                                   (129, 272, 1040), (300, 1024, 5120), (1000, 2064, 80), (65, 16, 4096), (513, 768, 656)])
+                                   (129, 272, 1040), (300, 1024, 5120), (1000, 2064, 80), (65, 16, 4096), (513, 768, 656),
+                                   (4, 64, 1536), (13, 48, 1888), (32, 160, 768), (3, 96, 8192), (2, 80, 208), (24, 272, 1024), (5, 32, 4912)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("activation", [None, "gelu", "gelu_tanh", "swiglu", "gated"])
 def test_matches_exact_product(cuda_device, m, n, k, dtype, activation):

@@ -705,12 +705,13 @@ __device__ __forceinline__ uint2 codes8(const float (&f)[8], float s, float inv)
 // rearranging. The integer sums of the warps meet in shared memory: the result
 // does not depend on how K is shared. With kFused every CTA first quantises
 // the tokens itself, a few thousand values, while its first rows of w are on
-// their way: one launch instead of two.
+// their way: one launch instead of two; a warp a token (8 x 1536 -> 4608: 5.5
+// us, with the whole CTA on each token in turn 8.4), up to 3 tokens the CTA.
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kFewAhead = 3;        // pieces of a warp in flight
 constexpr int kFewMost = 32;        // tokens
-constexpr int64_t kFusedMost = 16384;  // values that every CTA quantises for itself
+constexpr int64_t kFusedMost = 24576;  // values that every CTA quantises for itself
 
 __device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
@@ -749,28 +750,52 @@ __global__ void __launch_bounds__(kFewThreads) few_int8_kernel(const int8_t* __r
   if constexpr (!kFused) {
     wait_for_quantiser();
   } else {
-    for (int m = 0; m < p.M; ++m) {
-      const T* xr = x + m * ldx;
-      uint32_t top = 0;
-      for (int k = threadIdx.x; k < p.K / 8; k += kFewThreads) {
-        float f[8];
-        unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
+    if (p.M > 3) {  // a warp a token
+      const int left = p.K / 8;
+      for (int m = warp; m < p.M; m += kFewWarps) {
+        const T* xr = x + m * ldx;
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int k = lane; k < left; k += 32) {
+          float f[8];
+          unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+          for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+        }
+        const float s = scale_of(__reduce_max_sync(0xffffffffu, top)), inv = __frcp_rn(s);
+        if (lane == 0) scales[m] = s;
+#pragma unroll 4
+        for (int k = lane; k < left; k += 32) {
+          float f[8];
+          unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
+          *reinterpret_cast<uint2*>(codes + m * stride + 8 * k) = codes8(f, s, inv);
+        }
       }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) red[warp] = top;
       __syncthreads();
+    } else {
+      for (int m = 0; m < p.M; ++m) {
+        const T* xr = x + m * ldx;
+        uint32_t top = 0;
+        for (int k = threadIdx.x; k < p.K / 8; k += kFewThreads) {
+          float f[8];
+          unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
 #pragma unroll
-      for (int i = 0; i < kFewWarps; ++i) top = max(top, red[i]);
-      const float s = scale_of(top), inv = __frcp_rn(s);
-      if (threadIdx.x == 0) scales[m] = s;
-      for (int k = threadIdx.x; k < p.K / 8; k += kFewThreads) {
-        float f[8];
-        unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
-        *reinterpret_cast<uint2*>(codes + m * stride + 8 * k) = codes8(f, s, inv);
+          for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7FFFFFFFu);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) red[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kFewWarps; ++i) top = max(top, red[i]);
+        const float s = scale_of(top), inv = __frcp_rn(s);
+        if (threadIdx.x == 0) scales[m] = s;
+        for (int k = threadIdx.x; k < p.K / 8; k += kFewThreads) {
+          float f[8];
+          unpack8(xr, __ldg(reinterpret_cast<const uint4*>(xr) + k), f);
+          *reinterpret_cast<uint2*>(codes + m * stride + 8 * k) = codes8(f, s, inv);
+        }
+        __syncthreads();
       }
-      __syncthreads();
     }
   }
   int acc[kTokenTiles][4] = {};
@@ -854,7 +879,10 @@ int launch_few(const void* a, const void* w, const Params<T>& p, const T* x, int
 }
 
 // Tokens that a call may quantise within the product: little work, and codes
-// (M * (K + 64) bytes, 18 KB at most) that fit beside the sums.
+// (M * (K + 64) bytes, 26 KB at most) that fit beside the sums. One launch /
+// two, in a graph and in an eager loop: 8 x 1536 -> 4608 5.5 / 5.9 us and 11.6
+// / 16.5 us, 16 x 1536 -> 4608 7.6 / 5.9 and 15.6 / 16.8, 12 x 2048 -> 2048
+// 6.6 / 6.1 and 13.3 / 16.5, 18 x 1536 -> 8192 15.4 / 9.8 and 16.6 / 16.5.
 inline bool fuses(int64_t m, int64_t k) { return m <= kFewMost && m * k <= kFusedMost; }
 
 // x: the tokens to quantise within the product (null: `a` and p.sa hold their
