@@ -234,7 +234,7 @@ __device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.
 // what hides the sum between a head's loads and its stores (85 registers and
 // 24 warps: a sixth slower; factors with the weights multiplied in, held in 118
 // registers: a third). 126,754 tokens, Q and K of 24 heads of 128 in bf16:
-// 490 us (6.4 TB/s), with the norms 582 us.
+// 490 us (6.4 TB/s), with the norms 569 us.
 template <typename T, bool kInterleaved, bool kNorm>
 __global__ void __launch_bounds__(kThreads, 4) rope_axes_vec_kernel(const Params p, const __grid_constant__ Turns turns,
                                                                  int lane_bits, int head_bits, FastDiv div_seq,
@@ -296,7 +296,8 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_vec_kernel(const Params
     T* q_dst = static_cast<T*>(p.dst[0]) + static_cast<int64_t>(token) * (p.heads[0] * p.width);
     T* k_dst = static_cast<T*>(p.dst[1]) + static_cast<int64_t>(token) * (p.heads[1] * p.width);
     const int heads = p.heads[0] + p.heads[1];
-#pragma unroll 2
+    constexpr int kUnroll = kNorm ? 3 : 2;  // 2 with a norm: 2% slower
+#pragma unroll kUnroll
     for (int h0 = 0; h0 < heads; h0 += 1 << head_bits) {
       int h = h0 + first_head;
       const bool go = here && h < heads;
