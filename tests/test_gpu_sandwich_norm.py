@@ -198,3 +198,64 @@ def test_refusals(cuda_device):
         sandwich_norm(torch.zeros(1, 1, 16385, device=cuda_device), torch.zeros(1, 1, 16385, device=cuda_device))
     with pytest.raises(ValueError, match="autograd"):
         sandwich_norm(x.clone().requires_grad_(), x)
+
+
+def codes_in_64_bits(y, x, a, quant):
+    """(x, codes' values, scales, where the quotient is off a code's border by more than 2^-30 of itself) from the definition."""
+    norm = lambda t, kind, w: (lambda d: d / (d.pow(2).mean(-1, keepdim=True) + a["eps"]).sqrt() * (1.0 if w is None else w.double()))(  # noqa: E731
+        t - t.mean(-1, keepdim=True) if kind == "layernorm" else t) if kind else t
+    at = a.get("indices")
+    v = norm(y.double(), a["post_norm"], a.get("post_weight"))
+    if a.get("gate") is not None:
+        v = v * a["gate"].double()[at]
+    new = x.double() + a["residual_scale"] * v
+    h = norm(new, a["pre_norm"], a.get("pre_weight"))
+    if a.get("scale") is not None:
+        h = h * (1 + a["scale"].double()[at]) + a["shift"].double()[at]
+    s = (h.abs().amax(-1, keepdim=True) / (127 if quant == "int8" else 448)).clamp_min(torch.finfo(torch.float32).tiny)
+    code = (lambda q: q.round()) if quant == "int8" else (lambda q: q.float().to(torch.float8_e4m3fn).double())
+    low, high = (code(h / s * (1 + d)) for d in (-2.0 ** -30, 2.0 ** -30))
+    return new, code(h / s), s[..., 0], low == high
+
+
+@pytest.mark.parametrize("b,s,w", [(1, 16384, 336), (3, 1, 1), (2, 300, 33), (1, 700, 1001), (1, 200, 2001), (2, 60, 4100), (1, 9, 8200),
+                                   (1, 5, 16384), (2, 801, 1536)])
+@pytest.mark.parametrize("quant", ["int8", "e4m3"])
+@pytest.mark.parametrize("post,pre", [("rmsnorm", "layernorm"), ("layernorm", "rmsnorm"), (None, "rmsnorm")])
+def test_codes_of_32_bit_rows_are_the_definitions(cuda_device, b, s, w, quant, post, pre):
+    """Next to a code's border a last bit decides, and the decoded value moves by
+    a whole code: 32-bit rows are computed in 64 bits, and every code but those
+    within 2^-30 of a border, relative, is that of the definition (64-bit errors
+    are a few thousand times smaller). x and the scales are rounded once: half a
+    step, 2^-24, and a 2^-20 part of it for the 64-bit errors."""
+    from xgen_b200.ops import sandwich_norm
+
+    g = torch.Generator().manual_seed(w)
+    base = torch.randn(b, s, w + 1, generator=g).to(cuda_device)
+    y, x = 0.7 * base[..., 1:] + 0.1, 2 * torch.randn(b, s, w, generator=g).to(cuda_device)
+    a = {**arguments(w, 6, torch.float32, cuda_device, g, post, pre, s, modulate=s % 2 == 0), "residual_scale": 0.5, "eps": 2.0 ** -20}
+    got, codes, scales = sandwich_norm(y, x, quant=quant, **a)
+    rx, value, rs, sure = codes_in_64_bits(y, x, a, quant)
+    assert sure.double().mean() > 1 - 1e-5
+    off = (codes.float().double() != value) & sure
+    assert not off.any(), (int(off.sum()), off.numel())
+    assert ((scales.double() - rs).abs() <= 2.0 ** -24 * (1 + 2.0 ** -20) * rs).all()
+    assert ((got.double() - rx).abs() <= 2.0 ** -24 * (1 + 2.0 ** -20) * rx.abs() + 2.0 ** -45).all()  # a sum that cancels: 64-bit errors
+    again = sandwich_norm(base[..., 1:].mul(0.7).add(0.1), x, quant=quant, **a)  # the same rows, aligned
+    assert all(torch.equal(p.view(torch.uint8) if p.dtype == torch.float8_e4m3fn else p, q.view(torch.uint8) if q.dtype == torch.float8_e4m3fn else q)
+               for p, q in zip((got, codes, scales), again))
+
+
+def test_codes_of_32_bit_rows_not_finite_and_tiny(cuda_device):
+    from xgen_b200.ops import sandwich_norm
+
+    x = torch.randn(1, 6, 200, device=cuda_device)
+    x[0, 1, 3], x[0, 2, 4], x[0, 3] = float("nan"), float("inf"), 0.0
+    x[0, 4] *= 1e-30
+    gate, at = torch.ones(2, 200, device=cuda_device), torch.tensor([0, 0, 0, 0, 0, 2], device=cuda_device)
+    got, codes, scales = sandwich_norm(torch.zeros_like(x), x, quant="int8", post_norm=None, pre_norm="rmsnorm", gate=gate, indices=at)
+    assert torch.isnan(scales[0, 1]) and torch.isnan(scales[0, 2]) and torch.isnan(scales[0, 5]) and torch.isnan(got[0, 5]).all()
+    assert not codes[0, 3].any() and scales[0, 3] == torch.finfo(torch.float32).tiny
+    # far below eps the norm is x * 1000
+    assert scales[0, 4] > 0 and codes[0, 4].abs().max() == 127
+    assert torch.isfinite(scales[0, [0, 3, 4]]).all() and torch.equal(got[0, :5].nan_to_num(), x[0, :5].nan_to_num())

@@ -10,7 +10,7 @@
 // Statistics, x' and h are 32-bit in registers; each stored value is rounded
 // once, and h is computed from the x' before its rounding. Variances are sums
 // of squared differences from the mean, so a mean far from zero costs no
-// digits.
+// digits. 32-bit rows with codes are computed in 64 bits (below).
 //
 // Bound by HBM: y and x in, x' and h out. The two norms of the unfused form
 // would read x' twice more and write and read post(y).
@@ -102,7 +102,8 @@ __device__ __forceinline__ uint8_t code_of(float h, float s, int quant) {
 }
 
 // Scalar form for any width, stride and alignment: one block a row, the row in
-// shared memory.
+// shared memory. (32-bit rows come here without codes, here and in the vector
+// form.)
 constexpr int kScalarThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kScalarThreads) sandwich_norm_scalar_kernel(const Params p) {
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kScalarThreads) sandwich_norm_scalar_kernel(co
     top = max(top, __float_as_uint(v) & 0x7FFFFFFFu);
     if (p.h_out) put(static_cast<T*>(p.h_out) + r * p.width + c, v);
   }
-  if (!p.codes) return;
+  if (sizeof(T) == 4 || !p.codes) return;
   const float sc = code_scale_of(block_amax<kScalarThreads>(top, reinterpret_cast<uint32_t*>(red)), p.quant);
   if (threadIdx.x == 0) p.code_scale[r] = sc;
   for (int c = threadIdx.x; c < p.width; c += kScalarThreads) p.codes[r * p.width + c] = code_of(row[c], sc, p.quant);
@@ -372,7 +373,7 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
         top = max(max(top, __float_as_uint(v[j][e].x) & 0x7FFFFFFFu), __float_as_uint(v[j][e].y) & 0x7FFFFFFFu);
     }
   }
-  if (!p.codes) return;
+  if (sizeof(T) == 4 || !p.codes) return;
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (kWarps > 1) {
     if ((threadIdx.x & 31) == 0) red[4][threadIdx.x >> 5] = __uint_as_float(top);
@@ -409,6 +410,143 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
     }
     *reinterpret_cast<uint2*>(codes + j * kThreads * 8) = make_uint2(lo, hi);
   }
+}
+
+// 32-bit rows with codes, in 64 bits. A code whose quotient lies next to the
+// border between two codes goes by its last bits: in 32 bits one to four of a
+// million fall on the other side, and what such a code stands for is then off
+// by a whole code, 2e-5 to 1.2e-4 of the tensor's norm. (16-bit rows keep 32
+// bits: there that is far below the rounding of what the codes stand for.) In
+// 64 bits only a quotient within some 2^-50 of a border can differ from the
+// definition's. An e4m3 code is that of the quotient rounded to 32 bits.
+//
+// Values c, c + kThreads, .. of a row are a thread's, so any stride and
+// alignment will do. Bound by 64-bit arithmetic and the conversions to and from
+// 64 bits (9 a value): 8,704 rows of 1536 to int8 take 103 us with 20 or with 32
+// warps on an SM (41 us in 32 bits), 16,384 of 336 45 us. At 64 registers wide
+// rows fill the SM: 15,844 of 5120 take 714 us, with x requested ahead of its
+// use and 96 registers 1,025 us.
+template <int kThreads, int kValues>
+__global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, 1024 / (kThreads * kRowsOf<kThreads>)) sandwich_norm_codes64_kernel(const Params p, int64_t rows, double inv_width) {
+  constexpr int kWarps = kThreads / 32;
+  __shared__ double red[5][kWarps];
+  const int64_t r = kWarps == 1 ? blockIdx.x * static_cast<int64_t>(kRowsOf<kThreads>) + (threadIdx.x >> 5) : blockIdx.x;
+  if (kWarps == 1 && r >= rows) return;
+  const int64_t b = r / p.seq, s = r - b * p.seq;
+  const int lane = kWarps == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int left = p.width - lane;  // value j exists while j * kThreads < left
+  const float* y = static_cast<const float*>(p.y) + b * p.yb + s * p.ys + lane;
+  const float* x = static_cast<const float*>(p.x) + b * p.xb + s * p.xs + lane;
+  double v[kValues];
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) {
+    v[j] = j * kThreads < left ? __ldg(y + j * kThreads) : 0.f;
+  }
+  int64_t t = 0;
+  bool known = true;
+  if (p.idx) {
+    t = __ldg(p.idx + b * p.idx_batch + s);
+    known = t >= 0 && t < p.table_rows;
+    if (!known) t = 0;
+  }
+  const float* gate = static_cast<const float*>(p.gate) + t * p.ldg + lane;
+  const float* scale = static_cast<const float*>(p.scale) + t * p.lds + lane;
+  const float* shift = static_cast<const float*>(p.shift) + t * p.ldsh + lane;
+  // every reduction has its own slots, as in the vector form
+  auto sum = [&](double a, int slot) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if constexpr (kWarps > 1) {
+      if ((threadIdx.x & 31) == 0) red[slot][threadIdx.x >> 5] = a;
+      __syncthreads();
+      a = 0.0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) a += red[slot][i];
+    }
+    return a;
+  };
+  // The norm without its last factor, which it returns: 1 / deviation.
+  auto centred = [&](int kind, int slot) {
+    if (kind == kNone) return 1.0;
+    double acc = 0.0;
+    if (kind == kLayer) {
+#pragma unroll
+      for (int j = 0; j < kValues; ++j)
+        if (j * kThreads < left) acc += v[j];
+      const double mean = sum(acc, slot) * inv_width;
+      acc = 0.0;
+#pragma unroll
+      for (int j = 0; j < kValues; ++j) v[j] -= mean;
+    }
+#pragma unroll
+    for (int j = 0; j < kValues; ++j)
+      if (j * kThreads < left) acc = fma(v[j], v[j], acc);
+    return rsqrt(fma(sum(acc, slot + 1), inv_width, static_cast<double>(p.eps)));
+  };
+  double rstd = centred(p.post, 0);
+  if (p.gate && !known) rstd = CUDART_NAN;
+  float* x_out = static_cast<float*>(p.x_out) + r * p.width + lane;
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) {
+    if (j * kThreads >= left) continue;
+    v[j] *= rstd;
+    if (p.post_weight) v[j] *= __ldg(static_cast<const float*>(p.post_weight) + lane + j * kThreads);
+    if (p.gate) v[j] *= __ldg(gate + j * kThreads);
+    v[j] = fma(static_cast<double>(p.residual_scale), v[j], static_cast<double>(__ldg(x + j * kThreads)));
+    x_out[j * kThreads] = static_cast<float>(v[j]);
+  }
+  rstd = centred(p.pre, 2);
+  if (p.scale && !known) rstd = CUDART_NAN;
+  unsigned long long top = 0;  // bits of the largest magnitude, so that a NaN stays one
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) {
+    if (j * kThreads >= left) continue;
+    v[j] *= rstd;
+    if (p.pre_weight) v[j] *= __ldg(static_cast<const float*>(p.pre_weight) + lane + j * kThreads);
+    if (p.scale) v[j] = fma(v[j], 1.0 + __ldg(scale + j * kThreads), static_cast<double>(__ldg(shift + j * kThreads)));
+    if (p.h_out) static_cast<float*>(p.h_out)[r * p.width + lane + j * kThreads] = static_cast<float>(v[j]);
+    top = max(top, static_cast<unsigned long long>(__double_as_longlong(fabs(v[j]))));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if constexpr (kWarps > 1) {
+    if ((threadIdx.x & 31) == 0) red[4][threadIdx.x >> 5] = __longlong_as_double(static_cast<long long>(top));
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) top = max(top, static_cast<unsigned long long>(__double_as_longlong(red[4][i])));
+  }
+  const double most = p.quant == kInt8 ? 127.0 : 448.0;
+  double sc = __longlong_as_double(static_cast<long long>(top)) / most;
+  if (sc < FLT_MIN) sc = FLT_MIN;  // a NaN stays one
+  const double inv = __drcp_rn(sc);
+  if (lane == 0) p.code_scale[r] = static_cast<float>(sc);
+  uint8_t* codes = p.codes + r * p.width + lane;
+#pragma unroll
+  for (int j = 0; j < kValues; ++j) {
+    if (j * kThreads >= left) continue;
+    // the correctly rounded quotient, as div_by; of at most `most` and a rounding
+    double q = v[j] * inv;
+    q = fma(fma(q, -sc, v[j]), inv, q);
+    codes[j * kThreads] = p.quant == kInt8 ? static_cast<uint8_t>(__double2int_rn(q)) : f32_to_e4m3(static_cast<float>(q));
+  }
+}
+
+template <int kThreads, int kValues>
+int launch_codes64(const Params& p, int64_t rows, cudaStream_t st) {
+  constexpr int kBlockRows = kRowsOf<kThreads>;
+  sandwich_norm_codes64_kernel<kThreads, kValues>
+      <<<static_cast<unsigned>(cdiv(rows, kBlockRows)), kThreads * kBlockRows, 0, st>>>(p, rows, 1.0 / p.width);
+  return launch_status();
+}
+
+int pick_codes64(const Params& p, int64_t rows, cudaStream_t st) {
+  if (p.width <= 256) return launch_codes64<32, 8>(p, rows, st);
+  if (p.width <= 512) return launch_codes64<32, 16>(p, rows, st);
+  if (p.width <= 1024) return launch_codes64<64, 16>(p, rows, st);
+  if (p.width <= 2048) return launch_codes64<128, 16>(p, rows, st);
+  if (p.width <= 4096) return launch_codes64<256, 16>(p, rows, st);
+  if (p.width <= 8192) return launch_codes64<512, 16>(p, rows, st);
+  return launch_codes64<1024, 16>(p, rows, st);
 }
 
 template <typename T, int kThreads, int kChunks>
@@ -450,6 +588,7 @@ int pick_vec(const Params& p, int64_t rows, cudaStream_t st) {
 
 template <typename T>
 int launch(const Params& p, int64_t rows, cudaStream_t st) {
+  if (sizeof(T) == 4 && p.codes) return pick_codes64(p, rows, st);
   const auto whole = [](const void* q, int64_t strides) {  // 16-byte pieces
     return reinterpret_cast<uintptr_t>(q) % 16 == 0 && strides * static_cast<int64_t>(sizeof(T)) % 16 == 0;
   };

@@ -403,7 +403,10 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
     int8_linear_quantized / H3FP8Linear.forward_quantized take.
 
     32-bit arithmetic; x and h are rounded once each, h from the x before its
-    rounding."""
+    rounding. Codes of fp32 rows are taken in 64 bits, and so are the
+    definition's: in 32 bits a few of a million would fall on the other side of
+    a border between two codes, as they do for 16-bit rows, whose own rounding
+    is larger."""
     what = "sandwich norm"
     _refuse_autograd(what, branch, residual, post_weight, pre_weight, gate, scale, shift)
     plan = _sandwich_plan(_form(branch), _form(residual), post_norm, pre_norm, _form(post_weight), _form(pre_weight), _form(gate),
