@@ -118,3 +118,18 @@ def test_cross_attention_arguments():
     assert h.xgb_pack_keys(D, 0, 1, D, ks, D, ks, 1, 2, 8, 96, D, D, D, None) == -2
     assert h.xgb_pack_keys(D, 0, 1, D, i64([1024, 64, 12, 1]), D, ks, 1, 2, 8, 64, D, D, D, None) == -3
     assert h.xgb_pack_keys(D, 0, 1, ODD, ks, D, ks, 1, 2, 8, 64, D, D, D, None) == -4
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_eps_of_a_norm_that_names_none(dtype):
+    """torch.nn.RMSNorm(d) has eps None, for which the module takes the epsilon
+    of the type that it computes in. At a deviation of 0.02 a wrong one shows."""
+    from xgen_b200.ops import _norm_of
+
+    norm = torch.nn.RMSNorm(128, dtype=dtype)
+    x = (0.02 * torch.randn(64, 128, generator=torch.Generator().manual_seed(0))).to(dtype)
+    _, eps = _norm_of(norm)
+    ref = norm(x).double()
+    y = x.double() * torch.rsqrt(x.double().pow(2).mean(-1, keepdim=True) + eps)
+    # the module's result is rounded at most twice (the type, then the weight of one)
+    assert ((y - ref).abs() <= (torch.finfo(dtype).eps + 2.0 ** -20) * y.abs()).all()

@@ -157,3 +157,20 @@ def test_refusals(cuda_device):
         rope_axes(q.double(), None, pos, axes=(32, 32))
     with pytest.raises(ValueError, match="autograd"):
         rope_axes(q.clone().requires_grad_(), None, pos, axes=(32, 32))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("std", [1.0, 0.02, 1e-4])
+def test_norm_without_an_eps(cuda_device, dtype, std):
+    """torch.nn.RMSNorm's default: the module itself is the definition. At
+    positions of zero nothing turns; the module may round in between, so a step
+    of the type."""
+    from xgen_b200.ops import rope_axes
+
+    g = torch.Generator().manual_seed(7)
+    norm = torch.nn.RMSNorm(64, device=cuda_device, dtype=dtype).requires_grad_(False)
+    q = (std * torch.randn(1, 30, 2, 64, generator=g)).to(cuda_device, dtype)
+    got, _ = rope_axes(q, None, torch.zeros(30, 1, device=cuda_device, dtype=torch.int64), axes=(64,), norm_q=norm)
+    ref = norm(q).double()
+    step = torch.finfo(dtype).eps
+    assert ((got.double() - ref).abs() <= 2 * step * ref.abs() + step * torch.finfo(dtype).smallest_normal).all()

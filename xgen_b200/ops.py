@@ -302,8 +302,8 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     32-bit arithmetic, one rounding at the end (the try_h3_* operators round
     after every step, as the reference does). Returns contiguous (query, key)."""
     what = "rotary positions"
-    w_q, eps_q = _norm_of(norm_q, query)
-    w_k, eps_k = _norm_of(norm_k, query) if key is not None else (None, 0.0)
+    w_q, eps_q = _norm_of(norm_q)
+    w_k, eps_k = _norm_of(norm_k) if key is not None else (None, 0.0)
     _refuse_autograd(what, query, key, w_q, w_k)
     plan = _rope_plan(_form(query), _form(key), _form(positions), axes if type(axes) is tuple else tuple(axes),
                       tuple(theta) if type(theta) is list else theta, _form(w_q), _form(w_k))
@@ -368,15 +368,17 @@ def _rope_plan(query, key, positions, axes, theta, w_q, w_k):
             (at, p_strides[0] if len(p_shape) == 3 else 0, p_strides[-2]), (n, i64_array(axes), f64_array(thetas)))
 
 
-def _norm_of(norm, query):
-    """(weight, eps) of a Q/K norm module, (None, 0) without one."""
+def _norm_of(norm):
+    """(weight, eps) of a Q/K norm module, (None, 0) without one. A module that
+    names no eps takes the epsilon of the type it computes in, which for all
+    three types is fp32."""
     if norm is None:
         return None, 0.0
     weight = norm.weight if type(norm) is _RMSNorm else None
     if weight is None:
         raise ValueError("rotary positions: norms must be torch.nn.RMSNorm with a weight")
     eps = norm.eps
-    return weight, eps if eps is not None else torch.finfo(query.dtype).eps
+    return weight, eps if eps is not None else torch.finfo(torch.float32).eps
 
 
 _NORM_CODE = {None: 0, "layernorm": 1, "rmsnorm": 2}
