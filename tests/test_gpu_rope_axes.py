@@ -174,3 +174,26 @@ def test_norm_without_an_eps(cuda_device, dtype, std):
     ref = norm(q).double()
     step = torch.finfo(dtype).eps
     assert ((got.double() - ref).abs() <= 2 * step * ref.abs() + step * torch.finfo(dtype).smallest_normal).all()
+
+
+@pytest.mark.parametrize("d,axes", [(128, (32, 32, 32)), (128, (16,)), (72, (8, 16, 16)), (96, (30, 20))])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_channels_that_are_not_rotated_are_copied(cuda_device, d, axes, interleaved, dtype):
+    """Bit for bit, infinities, NaN and zeros of either sign among them, in the
+    vector form (d and the axes' sum multiples of 16) and the scalar one."""
+    from xgen_b200.ops import rope_axes
+
+    r = sum(axes)
+    q = torch.randn(1, 40, 3, d, generator=torch.Generator().manual_seed(d)).to(cuda_device, dtype)
+    for n, value in enumerate((float("inf"), -float("inf"), float("nan"), -0.0, 0.0)):
+        q[0, n::7, :, r + n] = value
+        q[0, n::9, :, d - 1 - n] = value
+    positions = torch.arange(40 * len(axes), device=cuda_device).view(40, -1)
+    got, key = rope_axes(q, q, positions, axes=axes, interleaved=interleaved)
+    bits = torch.int32 if dtype == torch.float32 else torch.int16
+    nan = torch.isnan(q[..., r:])
+    assert torch.equal(torch.isnan(got[..., r:]), nan)
+    assert torch.equal(got[..., r:].contiguous().view(bits)[~nan], q[..., r:].contiguous().view(bits)[~nan])
+    check(got[..., :r].contiguous(), q[..., :r], positions, axes, interleaved)
+    assert torch.equal(key.view(bits), got.view(bits))

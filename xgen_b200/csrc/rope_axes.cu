@@ -16,6 +16,7 @@
 // their cos/sin in registers while it walks over the token's heads of Q and K,
 // so a token's angles are computed once, not once a head.
 #include <algorithm>
+#include <type_traits>
 
 #include "xgb_common.cuh"
 
@@ -235,7 +236,10 @@ __device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.
 // 24 warps: a sixth slower; factors with the weights multiplied in, held in 118
 // registers: a third). 126,754 tokens, Q and K of 24 heads of 128 in bf16:
 // 490 us (6.4 TB/s), with the norms 569 us.
-template <typename T, bool kInterleaved, bool kNorm>
+// kPartial: not all channels are rotated. The others are left as they are:
+// turned by an angle of zero, an infinity would make its neighbour a NaN. (The
+// branch in every call: 1% slower where all are rotated.)
+template <typename T, bool kInterleaved, bool kNorm, bool kPartial>
 __global__ void __launch_bounds__(kThreads, 4) rope_axes_vec_kernel(const Params p, const __grid_constant__ Turns turns,
                                                                  int lane_bits, int head_bits, FastDiv div_seq,
                                                                  FastDiv div_pairs) {
@@ -254,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_vec_kernel(const Params
   const int first_head = (threadIdx.x >> lane_bits) & ((1 << head_bits) - 1);
   const int t = threadIdx.x >> (lane_bits + head_bits);
   const int per_group = kThreads >> (lane_bits + head_bits);
-  const bool active = 2 * kN * j < p.width, turned = 2 * kN * j < p.rotary;
+  const bool active = 2 * kN * j < p.width, turned = !kPartial || 2 * kN * j < p.rotary;
   const int ca = kInterleaved || !turned ? 2 * kN * j : kN * j;
   const int cb = kInterleaved || !turned ? ca + kN : ca + pairs;
   const float inv_width = 1.f / p.width;
@@ -337,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_axes_vec_kernel(const Params
       }
       if (go) {
 #pragma unroll
-        for (int i = 0; i < kN / 2; ++i) {
+        for (int i = 0; turned && i < kN / 2; ++i) {
           const float2 turned_a = __ffma2_rn(a[i], c[i], __fmul2_rn(d[i], minus(s[i])));
           d[i] = __ffma2_rn(d[i], c[i], __fmul2_rn(a[i], s[i]));
           a[i] = turned_a;
@@ -412,9 +416,15 @@ int launch(const Params& p, const Turns& turns, bool interleaved, cudaStream_t s
     kernel<<<grid, kThreads, 0, st>>>(p, turns, lane_bits, head_bits, div_seq, div_pairs);
     return launch_status();
   };
-  const bool norm = p.weight[0] || p.weight[1];
-  if (interleaved) return norm ? run(rope_axes_vec_kernel<T, true, true>) : run(rope_axes_vec_kernel<T, true, false>);
-  return norm ? run(rope_axes_vec_kernel<T, false, true>) : run(rope_axes_vec_kernel<T, false, false>);
+  auto pick = [&](auto interleave, auto norm) {
+    constexpr bool kInterleaved = decltype(interleave)::value, kNorm = decltype(norm)::value;
+    if (p.rotary < p.width) return run(rope_axes_vec_kernel<T, kInterleaved, kNorm, true>);
+    return run(rope_axes_vec_kernel<T, kInterleaved, kNorm, false>);
+  };
+  const std::true_type yes{};
+  const std::false_type no{};
+  if (p.weight[0] || p.weight[1]) return interleaved ? pick(yes, yes) : pick(no, yes);
+  return interleaved ? pick(yes, no) : pick(no, no);
 }
 
 }  // namespace
