@@ -133,3 +133,26 @@ def test_eps_of_a_norm_that_names_none(dtype):
     y = x.double() * torch.rsqrt(x.double().pow(2).mean(-1, keepdim=True) + eps)
     # the module's result is rounded at most twice (the type, then the weight of one)
     assert ((y - ref).abs() <= (torch.finfo(dtype).eps + 2.0 ** -20) * y.abs()).all()
+
+
+def test_shapes_of_a_gate_index():
+    """An index is one for each token (in the tokens' shape or flat) or one for
+    the trailing dimensions, repeated before them; others would be read as
+    something else than they say."""
+    from xgen_b200.int8_linear import _plan
+
+    def form(shape, dtype=torch.bfloat16):
+        return torch.Size(shape), torch.empty(shape, device="meta").stride(), dtype, 0
+
+    def plan(lead, index):
+        return _plan(form((*lead, 64)), torch.Size(lead), torch.bfloat16, None, form((64, 64), torch.int8), form((64,), torch.float32), None, None,
+                     form((4, 64)), form(index, torch.int64), form((*lead, 64)))
+
+    for lead, index, rows in (((3, 37), (3, 37), 111), ((3, 37), (37,), 37), ((3, 37), (1, 37), 37), ((3, 37), (111,), 111), ((5,), (5,), 5),
+                              ((2, 3, 7), (3, 7), 21), ((2, 3, 7), (7,), 7), ((2, 3, 7), (1, 1, 7), 7), ((1, 9), (9,), 9), ((3, 1), (3,), 3),
+                              ((3, 37), (1,), 1), ((), (), 1), ((), (1,), 1), ((3, 0), (0,), 0)):
+        assert plan(lead, index)[5][1] == rows, (lead, index)
+    for lead, index in (((3, 37), (3,)), ((3, 37), (3, 1)), ((3, 37), (37, 3)), ((4,), (2,)), ((2, 3, 7), (2,)), ((2, 3, 7), (2, 3)), ((2, 3, 7), (2, 3, 1)),
+                        ((6, 6), (12,)), ((6, 6), (3,)), ((2, 3, 7), (2, 1, 7)), ((4,), (3,)), ((4,), (0,)), ((3, 37), (1, 1, 37, 1))):
+        with pytest.raises(ValueError, match="index"):
+            plan(lead, index)

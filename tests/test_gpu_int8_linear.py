@@ -237,3 +237,37 @@ def test_refusals(cuda_device):
     with pytest.raises(ValueError, match="autograd"):
         int8_linear(x.clone().requires_grad_(), w, ws)
     assert int8_linear(x[:0], w, ws, bias).shape == (0, 64)
+
+
+@pytest.mark.parametrize("m", [2, 130])
+def test_shapes_of_the_index(cuda_device, m):
+    """Every form that is taken names the same rows; one for each sample is not
+    taken for one for each token."""
+    from xgen_b200.int8_linear import int8_linear, int8_linear_quantized
+    from xgen_b200.ops import quantize_per_token_int8
+
+    b, s, n = 3, m, 64
+    x, w, ws, bias = problem(b * s, n, 64, torch.bfloat16, cuda_device)
+    gate, res = torch.randn(4, n, device=cuda_device).bfloat16(), torch.randn(b, s, n, device=cuda_device).bfloat16()
+    one = torch.randint(0, 4, (s,), device=cuda_device)
+    every = torch.randint(0, 4, (b, s), device=cuda_device)
+    codes, scales = quantize_per_token_int8(x)
+
+    def call(at):
+        got = int8_linear(x.view(b, s, 64), w, ws, bias, gate=gate, gate_index=at, residual=res)
+        again = int8_linear_quantized(codes.view(b, s, 64), scales.view(b, s), w, ws, bias, gate=gate, gate_index=at, residual=res)
+        assert torch.equal(got, again)
+        return got
+
+    for forms in ((one, one[None], one.expand(b, s), one.repeat(b)), (every, every.flatten(), every.t().contiguous().t()),
+                  (one[:1], one[:1, None], one[:1].expand(s), one[0])):
+        first = call(forms[0])
+        at = forms[0].expand(b, s).reshape(-1)
+        ref, slack = reference(*codes_of(x), w, ws, bias, None, (gate, at, res.view(b * s, n)))
+        within(first.view(b * s, n), ref, slack)
+        assert all(torch.equal(first, call(f)) for f in forms[1:])
+    for bad in (torch.arange(b, device=cuda_device), torch.arange(b, device=cuda_device)[:, None], every.t(), every[:, :, None], every[:2]):
+        with pytest.raises(ValueError, match="index"):
+            call(bad)
+    with pytest.raises(ValueError, match="index"):
+        int8_linear(x[:4], w, ws, bias, gate=gate, gate_index=one[:2], residual=res.view(b * s, n)[:4])

@@ -31,6 +31,17 @@ def quantize_per_channel_int8(value: torch.Tensor):
     return (value.float() / scale[:, None]).round().clamp(-127, 127).to(torch.int8), scale
 
 
+def _one_for_each(index, lead) -> bool:
+    """Whether an index of this shape names rows for tokens of shape `lead`: one
+    for each token, in their shape or flat, or one for each place of their
+    trailing dimensions, repeated before them (dimensions of one may lead)."""
+    if index == (math.prod(lead),):
+        return True
+    while index and index[0] == 1:
+        index = index[1:]
+    return index == lead[len(lead) - len(index):]
+
+
 @functools.lru_cache(maxsize=1024)
 def _plan(x, lead, dtype, scales, weight, weight_scale, bias, activation, gate, gate_index, residual):
     """Checks what int8_linear and int8_linear_quantized share by the tensors'
@@ -61,7 +72,7 @@ def _plan(x, lead, dtype, scales, weight, weight_scale, bias, activation, gate, 
                 or residual[2] != dtype or residual[0] != (*lead, n) or residual[1][-1] != 1):
             raise ValueError(f"gated {what} needs [M, out] gate rows and a residual of the result's shape and type")
         index_rows = math.prod(gate_index[0])
-        if gate_index[2] != torch.int64 or (m and (index_rows == 0 or m % index_rows)):
+        if gate_index[2] != torch.int64 or not _one_for_each(tuple(gate_index[0]), tuple(lead)):
             raise ValueError(f"gated {what} needs an int64 index for each token, or one sequence's for every sample")
         rows = gate[0][0]
         copy_gate = rows > 1 and gate[1][0] < n  # broadcast rows
@@ -134,8 +145,9 @@ def int8_linear(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tenso
         activation "gelu" (erf), "gelu_tanh", or "swiglu": silu(first half of
         the output channels) * second half, out/2 columns; or
         residual + gate[gate_index] * y: gate [M, out] AdaLN rows, gate_index
-        int64 for each token or for one sequence of a batch (an index outside
-        the rows makes its token NaN), residual [..., out].
+        int64 for each token (of x's shape without its channels, or flat) or for
+        its trailing dimensions, [S] of [B, S, in] for one sequence of a batch
+        (an index outside the rows makes its token NaN), residual [..., out].
 
     Each token's largest magnitude becomes 127; sums are exact, one rounding."""
     what = "H3 INT8 Linear"
