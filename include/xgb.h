@@ -43,6 +43,12 @@ int xgb_version(void);
 /* Human-readable name of a status code (static string). */
 const char* xgb_status_string(int status);
 
+/* A device int of the current device that lives as long as the library does
+ * there and is zero at first, for the error_flag arguments below: allocated by
+ * nobody's stream or graph, so a call captured at any time may be given it.
+ * NULL without a device. */
+int* xgb_error_word(void);
+
 /* ---- Elementwise operators, bit-exact with the reference Triton kernels ---- */
 
 /* Rotate-half RoPE over the first `rotary` channels of contiguous bf16

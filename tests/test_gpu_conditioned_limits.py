@@ -130,3 +130,44 @@ def test_first_call_of_a_process_is_captured(cuda_device):
     run = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], cwd=Path(__file__).resolve().parents[1], capture_output=True,
                          text=True, timeout=240)
     assert run.returncode == 0 and "equal" in run.stdout, run.stdout + run.stderr
+
+
+ERROR_WORD_OF_A_CAPTURED_CALL = """
+import torch
+from xgen_b200 import attention, int8_linear
+
+dev = torch.device("cuda")
+seen, real = [], attention._err_ptr
+
+def spy(index):
+    seen.append(real(index))
+    return seen[-1]
+
+attention._err_ptr = int8_linear._err_ptr = spy
+q, kv = torch.randn(1, 4, 300, 128, device=dev).bfloat16(), torch.randn(1, 4, 300, 128, device=dev).bfloat16()
+x, w, ws = torch.randn(600, 256, device=dev).half(), torch.ones(256, 256, device=dev, dtype=torch.int8), torch.rand(256, device=dev)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = [attention.dense_attention(q, kv, kv), attention.cross_attention(q, kv, kv), int8_linear.int8_linear(x, w, ws)]
+word = attention._err_flag(dev)
+assert len(seen) == 2 and seen[0] and set(seen) == {word.data_ptr()}, seen
+assert attention.kernel_errors(dev) == 0  # nothing has run
+word.fill_(5)  # what a wait that ran out would leave
+graph.replay()
+assert attention.kernel_errors(dev) == 5  # a replay does not clear it
+word.zero_()
+del graph, outs
+torch.cuda.empty_cache()
+again = [attention.cross_attention(q, kv, kv), int8_linear.int8_linear(x, w, ws)]
+assert set(seen) == {word.data_ptr()} and attention.kernel_errors(dev) == 0
+print("word")
+"""
+
+
+def test_a_first_captured_call_has_the_error_word(cuda_device):
+    """A wait that gives up in a replayed graph is recorded where kernel_errors
+    looks, also when the capture was the process's first call."""
+    run = subprocess.run([sys.executable, "-c", ERROR_WORD_OF_A_CAPTURED_CALL], cwd=Path(__file__).resolve().parents[1], capture_output=True,
+                         text=True, timeout=240)
+    assert run.returncode == 0 and "word" in run.stdout, run.stdout + run.stderr

@@ -35,6 +35,7 @@ c_i64p = ctypes.POINTER(ctypes.c_int64)
 SIGNATURES = {
     "xgb_version": (c_int, []),
     "xgb_status_string": (ctypes.c_char_p, [c_int]),
+    "xgb_error_word": (c_vp, []),
     "xgb_partial_rope": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_i64,
                                  c_i64, c_vp]),
     "xgb_qk_rms": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_vp, c_float, c_float, c_vp, c_vp,

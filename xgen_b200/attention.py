@@ -27,24 +27,32 @@ HEAD_DIM = 128
 _err_flags: dict[int, torch.Tensor] = {}
 
 
+class _Word:
+    """One int32 at a device address, as torch.as_tensor takes it."""
+
+    def __init__(self, address: int):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 2}
+
+
 def _err_flag(device: torch.device) -> torch.Tensor:
+    """The error word of the kernels' bounded waits on `device`: the library's
+    own, so that it has one address from the first call on, captured or not."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     flag = _err_flags.get(idx)
     if flag is None:
-        flag = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.cuda.device(idx):
+            address = _lib.lib().xgb_error_word()
+            if not address:
+                raise _lib.XGBError("xgb_error_word", _lib.XGB_ERR_DEVICE)
+            flag = torch.as_tensor(_Word(address), device=torch.device("cuda", idx))
         _err_flags[idx] = flag
     return flag
 
 
-def _err_ptr(index: int):
-    """The error word's address on GPU `index`; None when the first call there
-    is being captured (the word would then live in the graph's own memory)."""
+def _err_ptr(index: int) -> int:
+    """The error word's address on GPU `index`."""
     flag = _err_flags.get(index)
-    if flag is None:
-        if torch.cuda.is_current_stream_capturing():
-            return None
-        flag = _err_flag(torch.device("cuda", index))
-    return flag.data_ptr()
+    return (flag if flag is not None else _err_flag(torch.device("cuda", index))).data_ptr()
 
 
 _split_workspaces: dict[int, torch.Tensor] = {}
