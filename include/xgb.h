@@ -303,9 +303,9 @@ int xgb_rope_axes(const void* q, const int64_t* q_strides, const void* k, const 
  * gate, scale and shift (any may be NULL, scale and shift together) rows of
  * AdaLN tables of table_rows rows; idx = indices[batch * index_batch_stride +
  * seq], where an index outside the table makes its row NaN. x_out contiguous;
- * h to h_out (may be NULL), or as codes with one scale a row: quant 1 int8
- * (scale max(amax/127, FLT_MIN)), 2 e4m3 (amax/448). Rows of XGB_F32 with codes
- * are computed in 64 bits, others in 32. */
+ * h to h_out and as codes with one scale a row, each of which may be NULL:
+ * quant 1 int8 (scale max(amax/127, FLT_MIN)), 2 e4m3 (amax/448), 0 none. Rows
+ * of XGB_F32 with codes are computed in 64 bits, others in 32. */
 int xgb_sandwich_norm(const void* y, const int64_t* y_strides, const void* x, const int64_t* x_strides, int dtype,
                       int64_t batch, int64_t seq, int64_t width, int post_norm, const void* post_weight,
                       int pre_norm, const void* pre_weight, float eps, const void* gate, int64_t ldg,

@@ -259,3 +259,32 @@ def test_codes_of_32_bit_rows_not_finite_and_tiny(cuda_device):
     # far below eps the norm is x * 1000
     assert scales[0, 4] > 0 and codes[0, 4].abs().max() == 127
     assert torch.isfinite(scales[0, [0, 3, 4]]).all() and torch.equal(got[0, :5].nan_to_num(), x[0, :5].nan_to_num())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("w", [33, 64, 1536, 9999])
+@pytest.mark.parametrize("quant", [1, 2])
+def test_values_and_codes_of_one_call(cuda_device, dtype, w, quant):
+    """The C entry may be given h_out and codes together: each is what a call
+    for it alone gives (the codes of 32-bit rows are taken from h in 64 bits,
+    which h_out rounds once)."""
+    from xgen_b200 import _lib
+    from xgen_b200.ops import _DTYPE_CODE_F32
+
+    y, x = (torch.randn(2, 7, w, generator=torch.Generator().manual_seed(w + n)).to(cuda_device, dtype) for n in range(2))
+    strides = (_lib.c_i64 * 3)(*x.stride())
+
+    def call(values, codes):
+        out = [torch.empty_like(x), torch.empty_like(x) if values else None, torch.empty(2, 7, w, dtype=torch.uint8, device=cuda_device) if codes else None,
+               torch.empty(2, 7, device=cuda_device) if codes else None]
+        p = [t.data_ptr() if t is not None else None for t in out]
+        _lib.call("xgb_sandwich_norm", y.data_ptr(), strides, x.data_ptr(), strides, _DTYPE_CODE_F32[dtype], 2, 7, w, 2, None, 1, None, 1e-6, None, 0,
+                  1.0, None, 0, None, 0, None, 0, 0, p[0], p[1], quant if codes else 0, p[2], p[3], torch.cuda.current_stream().cuda_stream)
+        return out
+
+    both, values, codes = call(True, True), call(True, False), call(False, True)
+    assert torch.equal(both[2], codes[2]) and torch.equal(both[3], codes[3])
+    if dtype == torch.float32:
+        torch.testing.assert_close(both[1], values[1], rtol=2.0 ** -18, atol=2.0 ** -18 * values[1].abs().max().item())
+    else:
+        assert torch.equal(both[0], values[0]) and torch.equal(both[1], values[1])

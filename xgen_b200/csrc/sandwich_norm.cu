@@ -365,9 +365,8 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[j][e] = __ffma2_rn(v[j][e], __fadd2_rn(f[e], both(1.f)), g[e]);
     }
-    if (p.h_out) {
-      store8(h_out + j * kThreads * 8, v[j]);
-    } else {
+    if (p.h_out) store8(h_out + j * kThreads * 8, v[j]);
+    if (sizeof(T) == 2 && p.codes) {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         top = max(max(top, __float_as_uint(v[j][e].x) & 0x7FFFFFFFu), __float_as_uint(v[j][e].y) & 0x7FFFFFFFu);
