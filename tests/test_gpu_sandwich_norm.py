@@ -288,3 +288,33 @@ def test_values_and_codes_of_one_call(cuda_device, dtype, w, quant):
         torch.testing.assert_close(both[1], values[1], rtol=2.0 ** -18, atol=2.0 ** -18 * values[1].abs().max().item())
     else:
         assert torch.equal(both[0], values[0]) and torch.equal(both[1], values[1])
+
+
+@pytest.mark.parametrize("w", [100, 129, 1000, 1536, 5120, 10000])
+def test_layernorm_far_from_zero(cuda_device, w):
+    """The mean is taken off before anything is multiplied, and its own rounding
+    error e is summed with the squares and taken off too.
+
+    A constant row c: e is at most 32 roundings, 2^-19 |c|; the difference from
+    the mean is exactly e everywhere, its mean is known to 2^-19 of it, so what
+    is left is 2^-38 |c|, times 1/sqrt(eps).
+    A mean of 1000 deviations: differences are exact (within a factor of two of
+    the mean), their mean is known to 2^-19 of their mean magnitude (one
+    deviation at most), 1/deviation to 2^-19: 2^-19 (1 + |h|) and the last
+    roundings, 2^-22 (1 + |h|)."""
+    from xgen_b200.ops import sandwich_norm
+
+    eps, consts = 1e-5, torch.tensor([3.1415, 1000.3, 30.3, -7e4, 0.1], device=cuda_device)
+    x = consts[None, :, None].expand(1, 5, w).contiguous()
+    zero = torch.zeros_like(x)
+    bound = 2.0 ** -38 * consts.abs() / eps ** 0.5
+    for h in (sandwich_norm(zero, x, post_norm=None, pre_norm="layernorm", eps=eps)[1],
+              sandwich_norm(x, zero, post_norm="layernorm", pre_norm=None, eps=eps)):
+        assert (h[0].abs().amax(-1) <= bound).all(), h[0].abs().amax(-1) / bound
+    x = (1000 + torch.randn(1, 50, w, generator=torch.Generator().manual_seed(w))).to(cuda_device)
+    ref = torch.nn.functional.layer_norm(x.double(), (w,), eps=eps)
+    bound = (2.0 ** -19 + 2.0 ** -22) * (1 + ref.abs())
+    zero = torch.zeros_like(x)
+    for h in (sandwich_norm(zero, x, post_norm=None, pre_norm="layernorm", eps=eps)[1],
+              sandwich_norm(x, zero, post_norm="layernorm", pre_norm=None, eps=eps)):
+        assert ((h.double() - ref).abs() <= bound).all(), ((h.double() - ref).abs() / bound).max()

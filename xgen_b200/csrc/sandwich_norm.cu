@@ -8,9 +8,12 @@
 // tensors' type, or h as int8 / e4m3 codes with one 32-bit scale a row,
 // max(amax / 127 or 448, FLT_MIN): what the next 8-bit linear reads.
 // Statistics, x' and h are 32-bit in registers; each stored value is rounded
-// once, and h is computed from the x' before its rounding. Variances are sums
-// of squared differences from the mean, so a mean far from zero costs no
-// digits. 32-bit rows with codes are computed in 64 bits (below).
+// once, and h is computed from the x' before its rounding. A LayerNorm takes
+// the mean off first; the differences are summed along with their squares, and
+// what their sum shows of the mean's own rounding is taken off as well. So a
+// mean far from zero costs no digits, and a constant row gives zeros to 2^-38
+// of its value over sqrt(eps). 32-bit rows with codes are computed in 64 bits
+// (below).
 //
 // Bound by HBM: y and x in, x' and h out. The two norms of the unfused form
 // would read x' twice more and write and read post(y).
@@ -119,8 +122,9 @@ __global__ void __launch_bounds__(kScalarThreads) sandwich_norm_scalar_kernel(co
     known = t >= 0 && t < p.table_rows;
     if (!known) t = 0;
   }
-  // (mean, 1 / deviation) of the values in `row`, which this thread wrote at
-  // its own places
+  // (what is left of the mean, 1 / deviation) of the values in `row`, which this
+  // thread wrote at its own places; a LayerNorm's are made differences from
+  // their mean
   auto stats = [&](int kind, float& mean, float& rstd) {
     mean = 0.f;
     rstd = 1.f;
@@ -131,11 +135,15 @@ __global__ void __launch_bounds__(kScalarThreads) sandwich_norm_scalar_kernel(co
       mean = block_sum<kScalarThreads>(acc, red) / p.width;
       acc = 0.f;
     }
+    float off = 0.f;
     for (int c = threadIdx.x; c < p.width; c += kScalarThreads) {
       const float d = row[c] - mean;
+      if (kind == kLayer) row[c] = d;
+      off += d;
       acc = fmaf(d, d, acc);
     }
-    rstd = rsqrtf(block_sum<kScalarThreads>(acc, red) / p.width + p.eps);
+    mean = kind == kLayer ? block_sum<kScalarThreads>(off, red) / p.width : 0.f;
+    rstd = rsqrtf(fmaxf(block_sum<kScalarThreads>(acc, red) / p.width - mean * mean, 0.f) + p.eps);
   };
   for (int c = threadIdx.x; c < p.width; c += kScalarThreads) row[c] = to_float(y[c]);
   float mean, rstd;
@@ -238,7 +246,8 @@ template <typename T, int kThreads, int kChunks>
 __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kThreads>)
     sandwich_norm_vec_kernel(const Params p, uint32_t rows, FastDiv div_seq) {
   constexpr int kWarps = kThreads / 32;
-  __shared__ float red[5][kWarps];
+  __shared__ float red[3][kWarps];
+  __shared__ float2 red2[2][kWarps];
   const uint32_t r = kWarps == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;
   if (kWarps == 1 && r >= rows) return;
   const uint32_t b = fast_div(r, div_seq), s = r - b * div_seq.d;
@@ -275,8 +284,25 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
     }
     return v;
   };
+  // Two at once: each half of a warp goes on with one of them.
+  auto two_sums = [&](float a, float c, float2* slots) {
+    const bool upper = threadIdx.x & 16;
+    float v = upper ? c : a;
+    v += __shfl_xor_sync(0xffffffffu, upper ? a : c, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (kWarps > 1) {
+      if ((threadIdx.x & 15) == 0) reinterpret_cast<float*>(slots + (threadIdx.x >> 5))[upper] = v;
+      __syncthreads();
+      float2 both_sums = both(0.f);
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) both_sums = __fadd2_rn(both_sums, slots[i]);
+      return both_sums;
+    }
+    return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
+  };
   float2 v[kChunks][4];
-  // The norm as v * rstd + shift.
+  // The norm as v * rstd + shift, of a LayerNorm's values less their mean.
   auto stats = [&](int kind, int slot, float& rstd, float& shift) {
     rstd = 1.f;
     shift = 0.f;
@@ -288,26 +314,29 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
         if (j * kThreads < left)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc = __fadd2_rn(acc, v[j][e]);
-      const float mean = sum(acc.x + acc.y, slot) * inv_width;
-      const float2 minus = both(-mean);
+      const float2 minus = both(-sum(acc.x + acc.y, slot) * inv_width);
       acc = both(0.f);
+      float2 off = both(0.f);
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
         if (j * kThreads < left)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 d = __fadd2_rn(v[j][e], minus);
-            acc = __ffma2_rn(d, d, acc);
+            v[j][e] = __fadd2_rn(v[j][e], minus);
+            off = __fadd2_rn(off, v[j][e]);
+            acc = __ffma2_rn(v[j][e], v[j][e], acc);
           }
-      rstd = rsqrtf(fmaf(sum(acc.x + acc.y, slot + 1), inv_width, p.eps));
-      shift = -mean * rstd;
+      const float2 sums = two_sums(acc.x + acc.y, off.x + off.y, red2[slot]);
+      const float rest = sums.y * inv_width;
+      rstd = rsqrtf(fmaxf(fmaf(sums.x, inv_width, -rest * rest), 0.f) + p.eps);
+      shift = -rest * rstd;
     } else {
 #pragma unroll
       for (int j = 0; j < kChunks; ++j)
         if (j * kThreads < left)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc = __ffma2_rn(v[j][e], v[j][e], acc);
-      rstd = rsqrtf(fmaf(sum(acc.x + acc.y, slot + 1), inv_width, p.eps));
+      rstd = rsqrtf(fmaf(sum(acc.x + acc.y, slot), inv_width, p.eps));
     }
   };
 #pragma unroll
@@ -340,7 +369,7 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
     store8(x_out + j * kThreads * 8, v[j]);
   }
   if (!p.h_out && !p.codes) return;
-  stats(p.pre, 2, rstd, shift);
+  stats(p.pre, 1, rstd, shift);
   if (p.scale && !known) rstd = CUDART_NAN_F;
   const T* pre_weight = static_cast<const T*>(p.pre_weight) + lane * 8;
   const T* mod_scale = static_cast<const T*>(p.scale) + t * p.lds + lane * 8;
@@ -375,10 +404,10 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
   if (sizeof(T) == 4 || !p.codes) return;
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (kWarps > 1) {
-    if ((threadIdx.x & 31) == 0) red[4][threadIdx.x >> 5] = __uint_as_float(top);
+    if ((threadIdx.x & 31) == 0) red[2][threadIdx.x >> 5] = __uint_as_float(top);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) top = max(top, __float_as_uint(red[4][i]));
+    for (int i = 0; i < kWarps; ++i) top = max(top, __float_as_uint(red[2][i]));
   }
   const float sc = code_scale_of(__uint_as_float(top), p.quant);
   const float inv = __frcp_rn(sc);
