@@ -352,7 +352,9 @@ int xgb_int8_linear(const void* x, int64_t ldx, const int8_t* w, int64_t M, int6
  * elements, multiples of 8; 0 where the batch or the heads are broadcast),
  * heads a multiple of kv_heads. kv_lens (device, [batch], may be NULL): keys
  * that each sample has, clamped to [0, seq_kv]; what lies behind them has no
- * influence, NaN included, and a sample without keys gives zeros. mask (device
+ * influence, NaN included, and a sample without keys gives zeros. Values are
+ * summed in 32 bits before they are divided: magnitudes below 2^126 / seq_kv
+ * cannot overflow, and those from 2^-80 keep their digits. mask (device
  * bytes [batch, seq_kv], may be NULL): 0 leaves a key out as well; taken where
  * xgb_cross_attention_takes_mask() says so (few query rows), elsewhere
  * xgb_pack_keys comes before. workspace: xgb_cross_attention_workspace() bytes

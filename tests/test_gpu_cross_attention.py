@@ -315,3 +315,60 @@ def test_refusals(cuda_device):
         cross_attention(q, k[:, :, :1].expand(-1, -1, 20, -1), v)  # one key for all places
     with pytest.raises(ValueError, match="autograd"):
         cross_attention(q.clone().requires_grad_(), k, v)
+
+
+@pytest.mark.parametrize("sq", [1, 3400])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rise", [7, 9, 20, 39, 60])
+def test_large_values_behind_a_late_high_score(cuda_device, sq, d, rise):
+    """Scores of later tiles that exceed the first's by 2^7 to 2^60, and values
+    up to 2^116: below 2^126 / 330, so the result is finite. One token, and 84
+    units, which are more than half the SMs and so keep all their keys."""
+    from xgen_b200.attention import cross_attention
+
+    q, k, v = inputs(2, 3, 3, sq, 330, d, torch.bfloat16, cuda_device, seed=rise)
+    q, k = 0.05 * q, 0.05 * k
+    q[..., 0] = 1.0
+    k[..., 0] = torch.where(torch.arange(330, device=cuda_device) >= 100, float(rise), 0.0).to(torch.bfloat16)
+    v = (v.float().clamp(-4, 4) * 2.0 ** 114).to(torch.bfloat16)
+    got = cross_attention(q, k, v, sm_scale=math.log(2))
+    assert torch.isfinite(got).all()
+    at = torch.cat([torch.arange(0, sq, 61), torch.arange(max(0, sq - 20), sq)])
+    check(got[:, :, at], q[:, :, at], k, v, torch.ones(2, 330, dtype=torch.bool), math.log(2))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens", [False, True])
+def test_scores_that_rise_within_whole_units(cuda_device, d, dtype, lens):
+    """The row's reference value is raised at some tiles, in some rows, of units
+    that keep all their keys, again and again and by 2^3 to 2^300; the samples
+    differ in their number of tiles."""
+    from xgen_b200.attention import cross_attention
+
+    steps = (0, 3, 60, 61, 70, 300, 310, 50) if dtype == torch.bfloat16 else (0, 3, 12, 30, 60, 61, 75, 3)
+    skv = 64 * len(steps) - 9
+    b, h, sq = 3, 3, 2600  # 99 units
+    q, k, v = inputs(b, h, 3, sq, skv, d, dtype, cuda_device, seed=d)
+    q, k = q * 0.25, k * 0.25
+    q[..., 0] = ((torch.arange(sq, device=cuda_device) // 5) % 3 == 0).to(dtype)
+    k[..., 0] = (torch.tensor(steps, device=cuda_device).repeat_interleave(64)[:skv] / 4).to(dtype)
+    n = torch.tensor([skv, 150, 321], dtype=torch.int32) if lens else None
+    got = cross_attention(q, k, v, sm_scale=math.log(2) * 4, kv_lens=n.to(cuda_device) if lens else None)
+    valid = torch.arange(skv)[None] < n[:, None] if lens else torch.ones(b, skv, dtype=torch.bool)
+    at = torch.cat([torch.arange(0, sq, 37), torch.arange(sq - 20, sq)])
+    check(got[:, :, at], q[:, :, at], k, v, valid, math.log(2) * 4)
+
+
+@pytest.mark.parametrize("sq", [1, 40, 3400])
+def test_small_values(cuda_device, sq):
+    """Magnitudes of 2^-80 keep their digits: the same result as at 1, scaled."""
+    from xgen_b200.attention import cross_attention
+
+    q, k, v = inputs(2, 3, 3, sq, 330, 128, torch.bfloat16, cuda_device, seed=4)
+    v = (v.float().sign() * (1 + v.float().abs())).to(torch.bfloat16)
+    got, small = cross_attention(q, k, v), cross_attention(q, k, (v.float() * 2.0 ** -80).to(torch.bfloat16))
+    # what is lost of a sum where products below 2^-126 are: 330 of them against
+    # a p of at least 2^-24 times 2^-80, 2^-13 of the mean magnitude
+    a = cross_attention(q, k, v.abs()).double()
+    assert ((small.double() * 2.0 ** 80 - got.double()).abs() <= 2.0 ** -8 * got.double().abs() + 2.0 ** -13 * a).all()

@@ -235,7 +235,10 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
         key_mask  bool [B, Skv], [1, Skv] or [B, 1, 1, Skv]: True = attend
 
     Other keys and values have no influence, whatever they hold; a sample
-    without keys gives zeros. out: a [B, H, Sq, D] view of the query's type,
+    without keys gives zeros. Sums are held in 32 bits, probabilities in the
+    inputs' type for the second product; bf16 values from 2^-80 to 2^126 / Skv in
+    magnitude keep their digits and cannot overflow, in fp16 all do. out: a
+    [B, H, Sq, D] view of the query's type,
     which must not overlap the inputs. Nothing is shared between calls: the
     workspace of a call comes from the caching allocator."""
     what = "cross attention"

@@ -3,7 +3,7 @@
 // sample, shared key heads, head dims 64 and 128, bf16 or fp16:
 //
 //   o[b, h, s] = sum_j p_j v[b, h', j] / sum_j p_j,  j < len[b],  h' = h / (H / H')
-//   p_j = 2^(scale log2(e) q.k_j - m),  m >= the row's largest score - 8
+//   p_j = 2^(scale log2(e) q.k_j - m),  m a value for each row, see below
 //
 // A sample without keys gives rows of zeros. Keys and values at j >= len[b]
 // are not read as numbers: their scores are overwritten with -inf and their
@@ -44,13 +44,24 @@
 // not threads, arrive.
 //
 // Softmax in the exp2 domain with 32-bit sums. The reference value m of a row
-// is the maximum of its first key tile. A later score may exceed it by 2^40
-// (bf16; 2^15 in fp16) before a probability or a sum could overflow, and being
-// larger than one costs no digits, so later tiles take no maximum: the tile's
-// own sum shows whether one came near the limit, and only then is the maximum
-// taken, O rescaled and the tile repeated. Without the maximum's instructions
-// and their place in the chain from scores to probabilities a step is a third
-// shorter. P is rounded to the type of V for the second product.
+// comes from its first key tile. Being larger or smaller than others costs a
+// probability no digits, so later tiles take no maximum: the tile's own sum
+// shows whether one came near a limit, and only then is the maximum taken, O
+// rescaled and the tile repeated. Without the maximum's instructions and their
+// place in the chain from scores to probabilities a step is a third shorter.
+//   bf16: m = the largest score + 24, sums up to 2^8. A later probability may be
+//     2^32 times the first tile's before a tile is repeated. O stays finite for
+//     values below 2^126 / seq_kv in magnitude (each tile of 64 keys adds at
+//     most 2^8 of them; with the row's largest score for m: 2^128 / seq_kv), and
+//     keeps its digits for values from 2^-80. (m = the largest score, sums up to
+//     2^40: infinities from values of 2^88. Sums up to 2^8: 43% slower where
+//     scores have a deviation of 4.)
+//   fp16: m = the largest score, sums up to 2^15, which P can hold; values up to
+//     2^16 cannot overflow O.
+// P is rounded to the type of V for the second product, which takes 16-bit
+// operands of one type: up to half a step of every probability, in the result
+// about as much as its own rounding (bf16: 2.3e-3 from 64 bits in place of
+// 1.7e-3, relative). Exponentials are the SFU's, 2^-22.
 //
 // Parts of a unit leave 32-bit O, m and l rows in a workspace of the call;
 // a second small kernel joins them.
@@ -93,8 +104,10 @@ struct Cfg {
   static constexpr int kSmem = kBarOff + 512 + 1024;  // + barriers + alignment slack
   static constexpr uint32_t kFmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   static constexpr uint32_t kIdescQK = instr_desc(1, kFmt, kFmt, false, false, kBM, 0);  // + keys
-  // Sum of a tile's 64 probabilities above which its maximum is looked at.
-  static constexpr float kLimit = std::is_same<T, __nv_bfloat16>::value ? 1.0995116e12f /* 2^40 */ : 32768.0f;
+  // How far a row's reference value is above its largest score, and the sum of a
+  // tile's probabilities above which the largest score is looked for anew.
+  static constexpr float kAbove = std::is_same<T, __nv_bfloat16>::value ? 24.f : 0.f;
+  static constexpr float kLimit = std::is_same<T, __nv_bfloat16>::value ? 256.f : 32768.f;
   static constexpr uint32_t kIdescPV = instr_desc(1, kFmt, kFmt, false, true, kBM, kD);
 };
 
@@ -580,10 +593,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * comb;
         };
-        // P = 2^(comb s - m) over the S buffer; returns its sum in two lanes
+        // P = 2^(comb s - m_used - kAbove) over the S buffer; returns its sum in
+        // two lanes. (kAbove in m_used itself: 4% slower at D = 64.)
         auto probabilities = [&](float (&ts)[2], bool pass_turn) {
           // a row whose scores are all -inf has its maximum there: p = 2^-inf
-          const float off = m_used == kNegInf ? 0.f : -m_used;
+          const float off = m_used == kNegInf ? 0.f : -C::kAbove - m_used;
           float ra[4] = {0.f, 0.f, 0.f, 0.f}, rb[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
