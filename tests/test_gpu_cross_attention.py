@@ -372,3 +372,17 @@ def test_small_values(cuda_device, sq):
     # a p of at least 2^-24 times 2^-80, 2^-13 of the mean magnitude
     a = cross_attention(q, k, v.abs()).double()
     assert ((small.double() * 2.0 ** 80 - got.double()).abs() <= 2.0 ** -8 * got.double().abs() + 2.0 ** -13 * a).all()
+
+
+def test_scale_is_read_at_every_call(cuda_device):
+    """A scale that float() takes, a tensor of one value among them, counts with
+    its value of the time of the call."""
+    from xgen_b200.attention import cross_attention
+
+    q, k, v = inputs(1, 2, 2, 40, 90, 64, torch.bfloat16, cuda_device)
+    scale = torch.tensor(0.25)
+    first = cross_attention(q, k, v, sm_scale=scale)
+    scale.fill_(0.03125)
+    second = cross_attention(q, k, v, sm_scale=scale)
+    assert torch.equal(first, cross_attention(q, k, v, sm_scale=0.25))
+    assert torch.equal(second, cross_attention(q, k, v, sm_scale=0.03125)) and not torch.equal(first, second)

@@ -197,3 +197,22 @@ def test_channels_that_are_not_rotated_are_copied(cuda_device, d, axes, interlea
     assert torch.equal(got[..., r:].contiguous().view(bits)[~nan], q[..., r:].contiguous().view(bits)[~nan])
     check(got[..., :r].contiguous(), q[..., :r], positions, axes, interleaved)
     assert torch.equal(key.view(bits), got.view(bits))
+
+
+def test_bases_are_read_at_every_call(cuda_device):
+    """Bases and axes that float() and int() take count with their values of the
+    time of the call."""
+    from xgen_b200.ops import rope_axes
+
+    q = torch.randn(1, 9, 2, 64, device=cuda_device)
+    positions = torch.arange(18, device=cuda_device).view(9, 2)
+    theta = torch.tensor(100.0)
+    for wrap in (lambda t: t, lambda t: (t, t), lambda t: [t, t]):
+        for value in (100.0, 5000.0):
+            theta.fill_(value)
+            got, _ = rope_axes(q, None, positions, axes=(32, 32), theta=wrap(theta))
+            assert torch.equal(got, rope_axes(q, None, positions, axes=(32, 32), theta=value)[0])
+    axes = torch.tensor([32, 32])
+    rope_axes(q, None, positions, axes=axes)
+    axes.copy_(torch.tensor([16, 48]))
+    assert torch.equal(rope_axes(q, None, positions, axes=axes)[0], rope_axes(q, None, positions, axes=(16, 48))[0])

@@ -245,7 +245,8 @@ def cross_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
     _refuse_autograd(what, query, key, value, out)
     if out is None:
         out = _like(query)
-    plan = _cross_plan(_form(query), _form(key), _form(value), _form(kv_lens), _form(key_mask), _form(out), sm_scale)
+    plan = _cross_plan(_form(query), _form(key), _form(value), _form(kv_lens), _form(key_mask), _form(out),
+                       None if sm_scale is None else float(sm_scale))
     index, q_strides, k_strides, v_strides, out_strides, sizes, sm_scale, takes_mask, ws_bytes, convert_lens = plan
     if not sizes[1] * sizes[2] * sizes[4]:
         return out
@@ -291,7 +292,8 @@ def _cross_plan(query, key, value, kv_lens, key_mask, out, sm_scale):
         raise ValueError(f"{what} requires head dim 64 or 128")
     if key[0] != value[0] or kb != b or kd != d or hk == 0 or h % hk:
         raise ValueError(f"{what}: key and value must match, have the query's batch and head dim and divide its heads")
-    sm_scale = float(sm_scale) if sm_scale is not None else 1.0 / math.sqrt(d)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(d)
     if not 0.0 < sm_scale < math.inf:
         raise ValueError(f"{what} requires a positive scale")
     if kv_lens is not None:

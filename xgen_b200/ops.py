@@ -305,8 +305,9 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     w_q, eps_q = _norm_of(norm_q)
     w_k, eps_k = _norm_of(norm_k) if key is not None else (None, 0.0)
     _refuse_autograd(what, query, key, w_q, w_k)
-    plan = _rope_plan(_form(query), _form(key), _form(positions), axes if type(axes) is tuple else tuple(axes),
-                      tuple(theta) if type(theta) is list else theta, _form(w_q), _form(w_k))
+    # numbers, not what they are taken from: a plan goes by its arguments' values
+    plan = _rope_plan(_form(query), _form(key), _form(positions), tuple(map(int, axes)),
+                      tuple(map(float, theta)) if isinstance(theta, (tuple, list)) else float(theta), _form(w_q), _form(w_k))
     index, q_strides, k_strides, sizes, copy_positions, position_args, rotation = plan
     if copy_positions:
         positions = positions.contiguous()
@@ -338,8 +339,7 @@ def _rope_plan(query, key, positions, axes, theta, w_q, w_k):
     for w in (w_q, w_k):
         if w is not None and (w[0] != (d,) or w[2] != dtype or (w[1] != (1,) and d > 1)):
             raise ValueError(f"{what}: norms must be torch.nn.RMSNorm over the head dim with a weight of the query's type")
-    axes = tuple(int(a) for a in axes)
-    thetas = tuple(float(t) for t in theta) if isinstance(theta, tuple) else (float(theta),) * len(axes)
+    thetas = theta if isinstance(theta, tuple) else (theta,) * len(axes)
     if not axes or any(a <= 0 or a % 2 for a in axes) or len(thetas) != len(axes) or not all(
             0 < t < float("inf") for t in thetas):
         raise ValueError(f"{what} need positive even axis channels and a positive theta for each axis")
