@@ -156,3 +156,24 @@ def test_shapes_of_a_gate_index():
                         ((6, 6), (12,)), ((6, 6), (3,)), ((2, 3, 7), (2, 1, 7)), ((4,), (3,)), ((4,), (0,)), ((3, 37), (1, 1, 37, 1))):
         with pytest.raises(ValueError, match="index"):
             plan(lead, index)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A tangent would be lost: the operators carry no derivative of either mode."""
+    import torch.autograd.forward_ad as forward_ad
+    from xgen_b200.attention import cross_attention
+    from xgen_b200.int8_linear import int8_linear
+    from xgen_b200.ops import rope_axes, sandwich_norm
+
+    x, q = torch.zeros(1, 4, 64, dtype=torch.bfloat16), torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16)
+    w, pos = torch.zeros(64, 64, dtype=torch.int8), torch.zeros(2, 1)
+    with forward_ad.dual_level():
+        xd, qd = forward_ad.make_dual(x, x), forward_ad.make_dual(q, q)
+        for call in (lambda: sandwich_norm(x, xd), lambda: rope_axes(qd, q, pos, axes=(64,)), lambda: cross_attention(q, qd, q),
+                     lambda: int8_linear(xd, w, torch.ones(64))):
+            with pytest.raises(ValueError, match="autograd"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="autograd"):
+                call()  # forward mode goes on under no_grad
+        with pytest.raises(ValueError, match="CUDA"):
+            sandwich_norm(x, x)

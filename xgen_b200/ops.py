@@ -11,6 +11,7 @@ from __future__ import annotations
 import functools
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch.nn import RMSNorm as _RMSNorm
 
 from . import _lib
@@ -34,10 +35,15 @@ def _require_cuda(*tensors: torch.Tensor, what: str) -> None:
 
 
 def _refuse_autograd(what: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
+    """Refuses tensors whose derivatives, of either mode, a call would lose."""
+    backward, forward = torch.is_grad_enabled(), _forward_ad._current_level >= 0
+    if not (backward or forward):
+        return
+    for t in tensors:
+        if t is not None and backward and t.requires_grad:
+            raise ValueError(f"{what} carries no autograd: call it under torch.no_grad()")
+        if t is not None and forward and _forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{what} carries no autograd: its tensors may not have tangents")
 
 
 def _form(t):
