@@ -177,3 +177,13 @@ def test_forward_mode_tangents_are_refused():
                 call()  # forward mode goes on under no_grad
         with pytest.raises(ValueError, match="CUDA"):
             sandwich_norm(x, x)
+
+
+def test_positions_that_need_a_gradient_are_refused():
+    from xgen_b200.ops import rope_axes
+
+    q, pos = torch.zeros(1, 2, 4, 64, dtype=torch.bfloat16), torch.zeros(2, 1, requires_grad=True)
+    with pytest.raises(ValueError, match="autograd"):
+        rope_axes(q, q, pos, axes=(64,))
+    with torch.no_grad(), pytest.raises(ValueError, match="CUDA"):
+        rope_axes(q, q, pos, axes=(64,))

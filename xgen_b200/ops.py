@@ -310,7 +310,7 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     what = "rotary positions"
     w_q, eps_q = _norm_of(norm_q)
     w_k, eps_k = _norm_of(norm_k) if key is not None else (None, 0.0)
-    _refuse_autograd(what, query, key, w_q, w_k)
+    _refuse_autograd(what, query, key, positions, w_q, w_k)
     # numbers, not what they are taken from: a plan goes by its arguments' values
     plan = _rope_plan(_form(query), _form(key), _form(positions), tuple(map(int, axes)),
                       tuple(map(float, theta)) if isinstance(theta, (tuple, list)) else float(theta), _form(w_q), _form(w_k))
