@@ -216,3 +216,7 @@ def test_bases_are_read_at_every_call(cuda_device):
     rope_axes(q, None, positions, axes=axes)
     axes.copy_(torch.tensor([16, 48]))
     assert torch.equal(rope_axes(q, None, positions, axes=axes)[0], rope_axes(q, None, positions, axes=(16, 48))[0])
+    pair = tuple(axes)  # two views of it
+    rope_axes(q, None, positions, axes=pair)
+    axes.copy_(torch.tensor([48, 16]))
+    assert torch.equal(rope_axes(q, None, positions, axes=pair)[0], rope_axes(q, None, positions, axes=(48, 16))[0])

@@ -312,8 +312,10 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     w_k, eps_k = _norm_of(norm_k) if key is not None else (None, 0.0)
     _refuse_autograd(what, query, key, positions, w_q, w_k)
     # numbers, not what they are taken from: a plan goes by its arguments' values
-    plan = _rope_plan(_form(query), _form(key), _form(positions), tuple(map(int, axes)),
-                      tuple(map(float, theta)) if isinstance(theta, (tuple, list)) else float(theta), _form(w_q), _form(w_k))
+    if type(axes) is not tuple or type(sum(axes)) is not int:
+        axes = tuple(map(int, axes))
+    theta = tuple(map(float, theta)) if isinstance(theta, (tuple, list)) else float(theta)
+    plan = _rope_plan(_form(query), _form(key), _form(positions), axes, theta, _form(w_q), _form(w_k))
     index, q_strides, k_strides, sizes, copy_positions, position_args, rotation = plan
     if copy_positions:
         positions = positions.contiguous()
