@@ -28,8 +28,9 @@
 // scores are due and its second one two key tiles before, two K and V tiles (a
 // third gave nothing), and 8 KB a softmax warp in which its output rows wait
 // for their TMA store (with 4 KB, half of the channels after the other,
-// 124,992 x 77 takes 8% longer). 124,992 rows, 24 heads of 128: 700 us with 512
-// keys, 270 us with 77.
+// 124,992 x 77 takes 8% longer). 124,992 rows, 24 heads of 128, replayed from a
+// graph: 681 to 691 us with 512 keys, 269 us with 77; called in a loop, at the
+// clocks of the power cap, 807 us with 512.
 //
 // What bounds a step of 64 keys for both query tiles is the tensor pipe and
 // the threads that feed it. Measured back to back on one SM: a 128 x 64 x 16
@@ -778,7 +779,7 @@ __global__ void __launch_bounds__(kFewWarps * 32) cross_few_kernel(const Params 
   float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f};  // rows 2c, 2c + 1
   // Keys and values of this step and the next: both are requested a step ahead,
   // so that a step costs its arithmetic, not a memory access. One token of 4
-  // samples with 24 / 8 heads against 4,099 keys each: 14.7 us (4.6 TB/s).
+  // samples with 24 / 8 heads against 4,099 keys each: 14.6 us (4.6 TB/s).
   uint4 k0[kChunks], k1[kChunks], v0[kChunks], v1[kChunks], vn0[kChunks], vn1[kChunks];
   bool keep0 = false, keep1 = false, next0 = false, next1 = false;
   auto request = [&](int at) {

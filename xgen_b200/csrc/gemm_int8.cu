@@ -222,7 +222,8 @@ struct Steps {
   template <typename Free>
   __device__ __forceinline__ bool step(uint32_t acc, int c, int n1, int m1, float sa, const T* gate, bool known,
                                        Gates<kEpi>& gates, Free free) {
-    // SwiGLU takes its two accumulators 32 columns at a time, for registers
+    // SwiGLU takes its two accumulators 32 columns at a time, for registers (168;
+    // pairs still spill 4 bytes, single CTAs 28)
     uint32_t r[2][32], rv[kEpi == kSwiGLU ? 32 : 1];
     if constexpr (kEpi == kSwiGLU) {
       tmem_ld32(acc, r[0]);
@@ -707,7 +708,7 @@ __device__ __forceinline__ uint2 codes8(const float (&f)[8], float s, float inv)
 // rearranging. The integer sums of the warps meet in shared memory: the result
 // does not depend on how K is shared. With kFused every CTA first quantises
 // the tokens itself, a few thousand values, while its first rows of w are on
-// their way: one launch instead of two; a warp a token (8 x 1536 -> 4608: 5.5
+// their way: one launch instead of two; a warp a token (8 x 1536 -> 4608: 5.2
 // us, with the whole CTA on each token in turn 8.4), up to 3 tokens the CTA.
 constexpr int kFewThreads = 256;
 constexpr int kFewWarps = kFewThreads / 32;
@@ -897,9 +898,9 @@ int launch_few(const void* a, const void* w, const Params<T>& p, const T* x, int
 
 // Tokens that a call may quantise within the product: little work, and codes
 // (M * (K + 64) bytes, 26 KB at most) that fit beside the sums. One launch /
-// two, in a graph and in an eager loop: 8 x 1536 -> 4608 5.5 / 5.9 us and 11.6
-// / 16.5 us, 16 x 1536 -> 4608 7.6 / 5.9 and 15.6 / 16.8, 12 x 2048 -> 2048
-// 6.6 / 6.1 and 13.3 / 16.5, 18 x 1536 -> 8192 15.4 / 9.8 and 16.6 / 16.5.
+// two, in a graph and in an eager loop: 8 x 1536 -> 4608 5.2 / 4.7 us and 11.9
+// / 16.7 us, 16 x 1536 -> 4608 7.4 / 5.2 and 11.8 / 16.7, 12 x 2048 -> 2048
+// 6.5 / 5.3 and 11.9 / 16.7, 18 x 1280 -> 8192 12.9 / 8.5 and 14.4 / 16.6.
 inline bool fuses(int64_t m, int64_t k) { return m <= kFewMost && m * k <= kFusedMost; }
 
 // x: the tokens to quantise within the product (null: `a` and p.sa hold their

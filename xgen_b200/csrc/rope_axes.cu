@@ -76,7 +76,9 @@ __device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // Scalar form for any width, pairing and alignment: one warp per head row,
-// lane l owns pairs l, l + 32, ... and the unrotated channels likewise.
+// lane l owns pairs l, l + 32, ... and the unrotated channels likewise. It forms
+// the angles for every head anew: 8,000 tokens of 12 + 12 heads of 64, 40 of
+// them rotated, take 89 us, with all of them, in the vector form, 11.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) rope_axes_scalar_kernel(const Params p, const __grid_constant__ Turns turns,
                                                                     bool interleaved) {
@@ -234,8 +236,10 @@ __device__ __forceinline__ float2 minus(float2 v) { return make_float2(-v.x, -v.
 // is divided in the walk; 64 registers keep 32 warps on an SM, whose loads are
 // what hides the sum between a head's loads and its stores (85 registers and
 // 24 warps: a sixth slower; factors with the weights multiplied in, held in 118
-// registers: a third). 126,754 tokens, Q and K of 24 heads of 128 in bf16:
-// 490 us (6.4 TB/s), with the norms 569 us.
+// registers: a third). fp32 with a norm spills 8 to 16 bytes there, except for
+// halves with all channels rotated. 126,754 tokens, Q and K of 24 heads of 128
+// in bf16: 491 us (6.3 TB/s), with the norms 568 us; 40,000 tokens in fp32: 355
+// us (halves, 5.5 TB/s) and 332 us (neighbours), with the norms 311 and 470 us.
 // kPartial: not all channels are rotated. The others are left as they are:
 // turned by an angle of zero, an infinity would make its neighbour a NaN. (The
 // branch in every call: 1% slower where all are rotated.)

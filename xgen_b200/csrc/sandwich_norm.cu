@@ -105,8 +105,9 @@ __device__ __forceinline__ uint8_t code_of(float h, float s, int quant) {
 }
 
 // Scalar form for any width, stride and alignment: one block a row, the row in
-// shared memory. (32-bit rows come here without codes, here and in the vector
-// form.)
+// shared memory, one value an access. 8,704 rows of 1001 in bf16 take 63 us, of
+// 1000, in the vector form, 17; of 100 29 us, which is what a block a row costs.
+// (32-bit rows with codes go to a form of their own, in 64 bits.)
 constexpr int kScalarThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kScalarThreads) sandwich_norm_scalar_kernel(const Params p) {
@@ -233,10 +234,10 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 // as run-time values the addresses, index divisions and joins of the sums took
 // more instructions than the arithmetic (55 a channel at width 5120).
 // At two bytes a value 64 registers a thread, 32 warps an SM, hold a row's
-// loads and hide the joins of its sums: 31,689 rows of 5120 take 219 us
-// (5.9 TB/s), with as many registers as the compiler likes 253 us, with 51
-// 258 us. At four bytes the loads need the registers (44 us either way for
-// 8,704 rows of 1536).
+// loads and hide the joins of its sums (256 and 512 threads a row spill 16
+// bytes): 31,689 rows of 5120 take 216 us (6.0 TB/s), with a LayerNorm 225 us;
+// with as many registers as the compiler likes 15% more, with 51 18%. At four
+// bytes the loads need the registers (44 us either way for 8,704 rows of 1536).
 template <int kThreads>
 constexpr int kRowsOf = kThreads == 32 ? 4 : 1;  // rows of a block
 template <typename T, int kThreads>
@@ -449,9 +450,10 @@ __global__ void __launch_bounds__(kThreads * kRowsOf<kThreads>, kBlocksOf<T, kTh
 // definition's. An e4m3 code is that of the quotient rounded to 32 bits.
 //
 // Values c, c + kThreads, .. of a row are a thread's, so any stride and
-// alignment will do. Bound by 64-bit arithmetic and the conversions to and from
-// 64 bits (9 a value): 8,704 rows of 1536 to int8 take 103 us with 20 or with 32
-// warps on an SM (41 us in 32 bits), 16,384 of 336 45 us. At 64 registers wide
+// alignment will do. Bound by chains of 64-bit arithmetic, with about 120
+// instructions a value (46% of the issue slots; 36% of the conversions' pipe, 9 a
+// value; 14% of the 64-bit units; DRAM 16%): 8,704 rows of 1536 to int8 take 103
+// us (41 us in 32 bits), 16,384 of 336 45 us, one row 9 us. At 64 registers wide
 // rows fill the SM: 15,844 of 5120 take 714 us, with x requested ahead of its
 // use and 96 registers 1,025 us.
 template <int kThreads, int kValues>
