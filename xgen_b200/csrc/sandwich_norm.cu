@@ -5,8 +5,8 @@
 //
 // post and pre are each RMSNorm or LayerNorm times an optional weight, or
 // nothing; gate and modulation are optional. x' and h are stored in the
-// tensors' type, or h as int8 / e4m3 codes with one 32-bit scale a row,
-// max(amax / 127 or 448, FLT_MIN): what the next 8-bit linear reads.
+// tensors' type, h instead or as well as int8 / e4m3 codes with one 32-bit scale
+// a row, max(amax / 127 or 448, FLT_MIN): what the next 8-bit linear reads.
 // Statistics, x' and h are 32-bit in registers; each stored value is rounded
 // once, and h is computed from the x' before its rounding. A LayerNorm takes
 // the mean off first; the differences are summed along with their squares, and

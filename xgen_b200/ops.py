@@ -306,7 +306,9 @@ def rope_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Te
     torch.nn.RMSNorm modules of a model with Q/K norms, applied first.
 
     32-bit arithmetic, one rounding at the end (the try_h3_* operators round
-    after every step, as the reference does). Returns contiguous (query, key)."""
+    after every step, as the reference does). Fast where D and R are multiples
+    of 16 and rows begin on 16 bytes; other forms take about eight times as
+    long. Returns contiguous (query, key)."""
     what = "rotary positions"
     w_q, eps_q = _norm_of(norm_q)
     w_k, eps_k = _norm_of(norm_k) if key is not None else (None, 0.0)
@@ -416,7 +418,9 @@ def sandwich_norm(branch: torch.Tensor, residual: torch.Tensor, *, post_norm: st
     rounding. Codes of fp32 rows are taken in 64 bits, and so are the
     definition's: in 32 bits a few of a million would fall on the other side of
     a border between two codes, as they do for 16-bit rows, whose own rounding
-    is larger."""
+    is larger. Fast where W is a multiple of 8 and rows, weights and table rows
+    begin on 16 bytes; other forms take four times as long or more (fp32 rows
+    with codes have one form)."""
     what = "sandwich norm"
     _refuse_autograd(what, branch, residual, post_weight, pre_weight, gate, scale, shift)
     plan = _sandwich_plan(_form(branch), _form(residual), post_norm, pre_norm, _form(post_weight), _form(pre_weight), _form(gate),
